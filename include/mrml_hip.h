@@ -513,6 +513,85 @@ int mrml_hip_attention_prefill(mrml_hip_ctx *ctx, const float *d_q, int32_t q_st
                                int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, float scale,
                                int32_t sliding_window, int32_t capacity, int32_t k_format, int32_t v_format);
 
+/* ---- a batch of requests over one paged KV cache -----------------------------
+ * The reference serves one sequence from ring caches; these entry points carry
+ * its cache rows, RoPE and attention (cuda.rs:2478-2519, 2658-2770) to several
+ * requests at once.  A paged cache is n_pages pages of page_size rows (1..2048),
+ * a row being one position in the ring caches' layout and format
+ * ([n_kv_heads][head_dim] f16, or Q8_0 / Q4_0 blocks), so a ring cache is also
+ * a paged one.  A place in it is page * page_size + offset.  A request owns the
+ * pages of its row of the page table; all requests of a call stand behind one
+ * shared prefix (a system prompt, say) that has pages of its own and is stored
+ * once.  Its first own token has position prefix_len.
+ *
+ * Per step: mrml_hip_block_tables once, then for every layer the append and the
+ * attention.  Nothing goes through the host, so the step can be captured and its
+ * graph replayed for token after token (run the ops once before, or reserve the
+ * workspace).  Page ids, slots, lengths and row starts are read from device
+ * memory; places that they put outside the cache are left out, and the next
+ * mrml_hip_sync fails with MRML_HIP_E_INVALID.  At most 4096 requests, 2^20
+ * rows a call, 2^21 positions a request and prefix. */
+
+/* Page tables, slots and positions of a step from the requests' lengths; one
+ * launch, no counterpart in the reference.  For request r with d_lens[r] own
+ * tokens in the cache, d_new[r] says what it wants: n > 0 adds n tokens, 0 is
+ * idle, -1 has finished.  In the requests' order:
+ *  - a finished request's pages (of the tokens it holds) return to the free list
+ *    (d_free, a stack of page ids with room for n_pages, *d_n_free of them
+ *    free), its length becomes 0;
+ *  - then every request that adds tokens takes the pages it lacks from the top
+ *    of the list into its row of d_table ([n_seqs][table_stride]), and gets rows
+ *    d_row_start[r] .. d_row_start[r + 1] of the step (n_seqs + 1 entries).
+ * Row i goes to place d_slots[i] at position d_pos[i] = pos0 + its own position
+ * (pos0: the length of the shared prefix); rows past the last request's up to
+ * max_rows get slot -1 and position 0.  d_lens_out and *d_n_free_out are the
+ * lengths and the free pages afterwards (they may be d_lens and d_n_free).
+ * d_status[r]: 0, or why the request was left as it is, without rows: 1 no page
+ * left for it, 2 its table row is too short, 3 no row left for it, 4 a negative
+ * or too large length or d_new below -1.  Rows and pages are counted over all
+ * requests before it that want some, so after one that had to wait for them
+ * (status 3, 1) no later one overtakes it. */
+int mrml_hip_block_tables(mrml_hip_ctx *ctx, const int32_t *d_lens, const int32_t *d_new, int32_t n_seqs,
+                          int32_t *d_table, int32_t table_stride, int32_t page_size, int32_t *d_free,
+                          const int32_t *d_n_free, int32_t n_pages, int32_t *d_lens_out, int32_t *d_n_free_out,
+                          int32_t *d_row_start, int32_t *d_slots, int32_t *d_pos, int32_t max_rows,
+                          int32_t *d_status, int32_t pos0);
+/* mrml_hip_rope_kv_append_f16_batch for rows that each have their own position
+ * and place: n_rows stacked [q | k | v] rows of d_qkv (left as they are), row i
+ * rotated at position d_pos[i], its q to row i of d_q ([n_rows][n_heads *
+ * head_dim]), its k and v to place d_slots[i] of the paged caches in their
+ * formats -- each the bits that entry point gives.  Rows with a negative slot
+ * are left out, their row of d_q too.  Angles as there: d_table (nullable) for
+ * positions below n_table, else evaluated on the device.  No two rows of a call
+ * may have the same slot.  head_dim a multiple of 32 up to 512, groups up to
+ * 16. */
+int mrml_hip_rope_kv_append_paged(mrml_hip_ctx *ctx, const float *d_qkv, float *d_q, uint16_t *d_k_pages,
+                                  uint16_t *d_v_pages, const int32_t *d_slots, const int32_t *d_pos, int32_t n_rows,
+                                  int32_t n_pages, int32_t page_size, int32_t n_heads, int32_t n_kv_heads,
+                                  int32_t head_dim, float freq_base, float freq_scale, int32_t k_format,
+                                  int32_t v_format, const float *d_table, int32_t n_table);
+/* Attention of a step's rows: row i of request r (d_row_start[r] <= i <
+ * d_row_start[r + 1]) stands at own position d_lens[r] - (d_row_start[r + 1] -
+ * i), d_lens the lengths with the step's tokens in; it sees the shared prefix
+ * (prefix_len positions in the pages of d_prefix, nullable when 0) and its
+ * request's own positions up to itself -- with sliding_window > 0 the last
+ * sliding_window of them -- and gives row i of d_out ([max_rows][n_heads *
+ * head_dim]).  The shared prefix is read once for the rows of all requests.  Query
+ * rows are q_stride floats apart (a multiple of 4).  Rows of no request are left
+ * as they are; a row that sees nothing gives zeros.
+ *
+ * The values are those of mrml_hip_attention_causal over the same rows (K in
+ * Q8_0 or Q4_0 multiplied with q as Q8_0 blocks; softmax and sums in f32), added
+ * in another order: within 1e-5 relative to the output's largest magnitude, like
+ * mrml_hip_attention_causal_split.  Values of quantised V rows must be within
+ * f16's range.  Limits as mrml_hip_rope_kv_append_paged. */
+int mrml_hip_attention_paged(mrml_hip_ctx *ctx, const float *d_q, int32_t q_stride, const uint16_t *d_k_pages,
+                             const uint16_t *d_v_pages, float *d_out, int32_t n_pages, int32_t page_size,
+                             const int32_t *d_prefix, int32_t prefix_len, const int32_t *d_table,
+                             int32_t table_stride, const int32_t *d_lens, const int32_t *d_row_start, int32_t n_seqs,
+                             int32_t max_rows, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, float scale,
+                             int32_t sliding_window, int32_t k_format, int32_t v_format);
+
 /* ---- Gemma-2-shape token step (model.rs forward_token, model.rs:1185-2260,
  * and greedy selection, model.rs:2833-2907) ----------------------------------- */
 /* Numerics of the token step.  EXACT (0, the default): every op in the CPU

@@ -189,6 +189,10 @@ _SIGNATURES = {
     "mrml_hip_attention_prefill": [_P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I, _I, _I],
     "mrml_hip_attention_causal": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _I],
     "mrml_hip_attention_causal_split": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _I],
+    "mrml_hip_block_tables": [_P, _P, _P, _I, _P, _I, _I, _P, _P, _I, _P, _P, _P, _P, _P, _I, _P, _I],
+    "mrml_hip_rope_kv_append_paged": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _F, _I, _I, _P, _I],
+    "mrml_hip_attention_paged": [_P, _P, _I, _P, _P, _P, _I, _I, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I,
+                                 _I],
     "mrml_hip_gemma2_create": [_P, _P, _P, _P, _P, ctypes.POINTER(_P)],
     "mrml_hip_gemma2_destroy": [_P, _P],
     "mrml_hip_gemma2_step": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _I],
@@ -625,6 +629,36 @@ class HipDevice:
         self._check(fn(self.ctx, _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), n_past, n_heads, n_kv_heads,
                        head_dim, scale, -1 if sliding_window is None else int(sliding_window), capacity, k_format,
                        v_format))
+
+    # ---- a batch of requests over one paged KV cache --------------------------------
+    def block_tables(self, lens, new, n_seqs: int, table, table_stride: int, page_size: int, free, n_free,
+                     n_pages: int, lens_out, n_free_out, row_start, slots, pos, max_rows: int, status,
+                     pos0: int = 0) -> None:
+        """Page tables, slots and positions of a step from the requests' lengths (mrml_hip_block_tables)."""
+        self._check(self.lib.mrml_hip_block_tables(
+            self.ctx, _ptr(lens), _ptr(new), n_seqs, _ptr(table), table_stride, page_size, _ptr(free), _ptr(n_free),
+            n_pages, _ptr(lens_out), _ptr(n_free_out), _ptr(row_start), _ptr(slots), _ptr(pos), max_rows,
+            _ptr(status), pos0))
+
+    def qkv_postprocess_paged(self, qkv, q, k_pages, v_pages, slots, pos, n_rows: int, n_pages: int, page_size: int,
+                              n_heads: int, n_kv_heads: int, head_dim: int, freq_base: float, k_format: int = 0,
+                              v_format: int = 0, freq_scale: float = 1.0, table=None, n_table: int = 0) -> None:
+        """qkv_postprocess_batch for rows with their own positions and slots of a paged cache; the rotated q goes to
+        rows of its own (mrml_hip_rope_kv_append_paged)."""
+        self._check(self.lib.mrml_hip_rope_kv_append_paged(
+            self.ctx, _ptr(qkv), _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(slots), _ptr(pos), n_rows, n_pages,
+            page_size, n_heads, n_kv_heads, head_dim, freq_base, freq_scale, k_format, v_format, _ptr(table), n_table))
+
+    def attention_paged(self, q, k_pages, v_pages, out, n_pages: int, page_size: int, prefix, prefix_len: int, table,
+                        table_stride: int, lens, row_start, n_seqs: int, max_rows: int, n_heads: int, n_kv_heads: int,
+                        head_dim: int, scale: float, sliding_window=None, k_format: int = 0, v_format: int = 0,
+                        q_stride: int | None = None) -> None:
+        """Attention of a step's rows over the shared prefix and their requests' pages (mrml_hip_attention_paged)."""
+        self._check(self.lib.mrml_hip_attention_paged(
+            self.ctx, _ptr(q), n_heads * head_dim if q_stride is None else q_stride, _ptr(k_pages), _ptr(v_pages),
+            _ptr(out), n_pages, page_size, _ptr(prefix), prefix_len, _ptr(table), table_stride, _ptr(lens),
+            _ptr(row_start), n_seqs, max_rows, n_heads, n_kv_heads, head_dim, scale,
+            -1 if sliding_window is None else int(sliding_window), k_format, v_format))
 
 
 class Gemma2Model:

@@ -5,6 +5,7 @@
 #include <cstddef>
 #include <cstdint>
 #include <string>
+#include <vector>
 
 #include "../../include/mrml_hip.h"
 #include "plans.h"
@@ -17,6 +18,10 @@ struct mrml_hip_ctx {
     size_t ws_bytes = 0;
     void *noalloc_scratch = nullptr;  // the device's copy of the allocation-free GEMM's scratch
     bool rows_loaded = false;         // attn_rows.hip's code is on the device (load_attn_rows)
+    bool captured = false;            // a graph was captured on this context: it may hold the scratch's address
+    std::vector<void *> retired;      // outgrown scratch that such a graph may still use, freed with the context
+    uint32_t *page_faults = nullptr;  // device: places outside a paged cache that kernels met and left out
+    bool paged_used = false;          // a paged op was issued: sync looks at page_faults
     std::string err;
 };
 

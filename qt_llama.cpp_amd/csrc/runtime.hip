@@ -49,6 +49,15 @@ int check_launch(mrml_hip_ctx *ctx, const char *kernel)
     return e == hipSuccess ? 0 : hip_fail(ctx, e, kernel);
 }
 
+// Keeps outgrown scratch that a captured graph may still use until the context ends.
+static void retire(mrml_hip_ctx *ctx, void *p)
+{
+    try {
+        ctx->retired.push_back(p);
+    } catch (...) {  // no room to remember it: it stays allocated
+    }
+}
+
 void *workspace(mrml_hip_ctx *ctx, size_t bytes)
 {
     if (bytes <= ctx->ws_bytes) return ctx->ws;
@@ -57,7 +66,10 @@ void *workspace(mrml_hip_ctx *ctx, size_t bytes)
         // The old scratch may still be read by queued work.
         hipError_t e = hipStreamSynchronize(ctx->stream);
         if (e != hipSuccess) { hip_fail(ctx, e, "hipStreamSynchronize (workspace)"); return nullptr; }
-        (void)hipFree(ctx->ws);
+        if (!ctx->captured)
+            (void)hipFree(ctx->ws);
+        else
+            retire(ctx, ctx->ws);
         ctx->ws = nullptr;
         ctx->ws_bytes = 0;
     }
@@ -170,6 +182,13 @@ int mrml_hip_create(int32_t device, mrml_hip_ctx **out)
         delete ctx;
         return MRML_HIP_E_HIP;
     }
+    if (hipMalloc(&ctx->page_faults, sizeof(uint32_t)) != hipSuccess ||
+        launch_zero(ctx, ctx->page_faults, sizeof(uint32_t)) != MRML_HIP_OK) {
+        (void)hipFree(ctx->page_faults);
+        (void)hipStreamDestroy(ctx->stream);
+        delete ctx;
+        return MRML_HIP_E_ALLOC;
+    }
     *out = ctx;
     return MRML_HIP_OK;
 }
@@ -180,6 +199,8 @@ int mrml_hip_destroy(mrml_hip_ctx *ctx)
     (void)hipSetDevice(ctx->device);
     if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
     if (ctx->ws) (void)hipFree(ctx->ws);
+    for (void *p : ctx->retired) (void)hipFree(p);
+    if (ctx->page_faults) (void)hipFree(ctx->page_faults);
     if (ctx->stream) (void)hipStreamDestroy(ctx->stream);
     delete ctx;
     return MRML_HIP_OK;
@@ -203,7 +224,17 @@ int mrml_hip_sync(mrml_hip_ctx *ctx)
         return fail(ctx, MRML_HIP_E_HIP,
                     "%u bounded LDS-counter waits gave up (%u matvec, %u decode): the results since the last sync "
                     "are wrong", t_gemv + t_decode, t_gemv, t_decode);
-    return MRML_HIP_OK;
+    if (!ctx->paged_used) return MRML_HIP_OK;
+    // Paged ops leave out places that their page tables, lengths or slots put outside the cache.
+    uint32_t faults = 0;
+    if ((e = hipMemcpy(&faults, ctx->page_faults, sizeof faults, hipMemcpyDeviceToHost)) != hipSuccess)
+        return hip_fail(ctx, e, "page faults");
+    if (!faults) return MRML_HIP_OK;
+    if (int rc = launch_zero(ctx, ctx->page_faults, sizeof faults)) return rc;
+    if ((e = hipStreamSynchronize(ctx->stream)) != hipSuccess) return hip_fail(ctx, e, "hipStreamSynchronize");
+    return fail(ctx, MRML_HIP_E_INVALID,
+                "paged ops since the last sync met page ids, slots or lengths outside the cache (%u seen): those places "
+                "were left out", faults);
 }
 
 int mrml_hip_set_wait_limit(mrml_hip_ctx *ctx, int32_t polls)
@@ -265,6 +296,7 @@ int mrml_hip_graph_begin(mrml_hip_ctx *ctx)
 {
     CTX_GUARD(ctx);
     hipError_t e = hipStreamBeginCapture(ctx->stream, hipStreamCaptureModeThreadLocal);
+    if (e == hipSuccess) ctx->captured = true;
     return e == hipSuccess ? 0 : hip_fail(ctx, e, "hipStreamBeginCapture");
 }
 

@@ -504,6 +504,74 @@ impl HipDevice {
         self.inner.expect(st, "rope_kv_append_f16_batch");
     }
 
+    /// Page tables, slots and positions of a step from the requests' lengths
+    /// (`mrml_hip_block_tables`): `lens` and `n_free` are updated in place.
+    #[allow(clippy::too_many_arguments)]
+    pub fn block_tables(&self, lens: &mut HipBuffer<i32>, new: &HipBuffer<i32>, table: &mut HipBuffer<i32>,
+                        page_size: usize, free: &mut HipBuffer<i32>, n_free: &mut HipBuffer<i32>,
+                        row_start: &mut HipBuffer<i32>, slots: &mut HipBuffer<i32>, pos: &mut HipBuffer<i32>,
+                        status: &mut HipBuffer<i32>, pos0: usize) {
+        let n_seqs = lens.len;
+        assert!(n_seqs > 0 && new.len == n_seqs && status.len == n_seqs && row_start.len == n_seqs + 1);
+        assert!(table.len % n_seqs == 0 && slots.len == pos.len && n_free.len >= 1);
+        let st = unsafe {
+            (self.inner.api.block_tables)(self.inner.ctx, lens.ptr, new.ptr, i32_of(n_seqs, "n_seqs"), table.ptr,
+                                          i32_of(table.len / n_seqs, "table_stride"), i32_of(page_size, "page_size"),
+                                          free.ptr, n_free.ptr, i32_of(free.len, "n_pages"), lens.ptr, n_free.ptr,
+                                          row_start.ptr, slots.ptr, pos.ptr, i32_of(slots.len, "max_rows"), status.ptr,
+                                          i32_of(pos0, "pos0"))
+        };
+        self.inner.expect(st, "block_tables");
+    }
+
+    /// `rope_kv_append_f16_batch` for rows with their own positions and slots of a
+    /// paged cache, the rotated q in rows of its own (`mrml_hip_rope_kv_append_paged`).
+    #[allow(clippy::too_many_arguments)]
+    pub fn rope_kv_append_paged(&self, qkv: &HipBuffer<f32>, q: &mut HipBuffer<f32>, k_pages: &mut HipBuffer<u16>,
+                                v_pages: &mut HipBuffer<u16>, slots: &HipBuffer<i32>, pos: &HipBuffer<i32>,
+                                n_pages: usize, page_size: usize, n_heads: usize, n_kv_heads: usize, head_dim: usize,
+                                freq_base: f32, k_format: i32, v_format: i32) {
+        let n_rows = slots.len;
+        assert!(pos.len == n_rows && q.len == n_rows * n_heads * head_dim);
+        assert_eq!(qkv.len, n_rows * (n_heads + 2 * n_kv_heads) * head_dim);
+        let st = unsafe {
+            (self.inner.api.rope_kv_append_paged)(self.inner.ctx, qkv.ptr, q.ptr, k_pages.ptr, v_pages.ptr, slots.ptr,
+                                                  pos.ptr, i32_of(n_rows, "n_rows"), i32_of(n_pages, "n_pages"),
+                                                  i32_of(page_size, "page_size"), i32_of(n_heads, "n_heads"),
+                                                  i32_of(n_kv_heads, "n_kv_heads"), i32_of(head_dim, "head_dim"),
+                                                  freq_base, 1.0, k_format, v_format, std::ptr::null(), 0)
+        };
+        self.inner.expect(st, "rope_kv_append_paged");
+    }
+
+    /// Attention of a step's rows over the shared prefix and their requests' pages
+    /// (`mrml_hip_attention_paged`).
+    #[allow(clippy::too_many_arguments)]
+    pub fn attention_paged(&self, q: &HipBuffer<f32>, k_pages: &HipBuffer<u16>, v_pages: &HipBuffer<u16>,
+                           out: &mut HipBuffer<f32>, n_pages: usize, page_size: usize, prefix: Option<&HipBuffer<i32>>,
+                           prefix_len: usize, table: &HipBuffer<i32>, lens: &HipBuffer<i32>,
+                           row_start: &HipBuffer<i32>, n_heads: usize, n_kv_heads: usize, head_dim: usize, scale: f32,
+                           sliding_window: Option<usize>, k_format: i32, v_format: i32) {
+        let n_seqs = lens.len;
+        let max_rows = out.len / (n_heads * head_dim);
+        assert!(n_seqs > 0 && max_rows > 0 && row_start.len == n_seqs + 1 && table.len % n_seqs == 0);
+        assert!(prefix.map(|p| p.len * page_size >= prefix_len).unwrap_or(prefix_len == 0));
+        let q_stride = q.len / max_rows;
+        let sw = sliding_window.map(|w| i32_of(w, "sliding_window")).unwrap_or(-1);
+        let prefix_ptr: *const i32 = prefix.map(|p| p.ptr as *const i32).unwrap_or(std::ptr::null());
+        let st = unsafe {
+            (self.inner.api.attention_paged)(self.inner.ctx, q.ptr, i32_of(q_stride, "q_stride"), k_pages.ptr,
+                                             v_pages.ptr, out.ptr, i32_of(n_pages, "n_pages"),
+                                             i32_of(page_size, "page_size"), prefix_ptr,
+                                             i32_of(prefix_len, "prefix_len"), table.ptr,
+                                             i32_of(table.len / n_seqs, "table_stride"), lens.ptr, row_start.ptr,
+                                             i32_of(n_seqs, "n_seqs"), i32_of(max_rows, "max_rows"),
+                                             i32_of(n_heads, "n_heads"), i32_of(n_kv_heads, "n_kv_heads"),
+                                             i32_of(head_dim, "head_dim"), scale, sw, k_format, v_format)
+        };
+        self.inner.expect(st, "attention_paged");
+    }
+
     /// `CudaDevice::rope_256k` (cuda.rs:2248-2285): RoPE of `n_heads` heads of
     /// `d_vec` in place at position `pos`.
     pub fn rope_256k(&self, d_vec: &mut HipBuffer<f32>, pos: usize, head_dim: usize, n_heads: usize, freq_base: f32,

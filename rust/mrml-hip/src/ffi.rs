@@ -203,6 +203,9 @@ api! {
     swiglu: fn(Ctx, *const f32, *const f32, *mut f32, i32) -> c_int = "mrml_hip_swiglu";
     add: fn(Ctx, *const f32, *const f32, *mut f32, i32) -> c_int = "mrml_hip_add";
     attention_prefill: fn(Ctx, *const f32, i32, *const u16, *const u16, *mut f32, i32, i32, i32, i32, i32, f32, i32, i32, i32, i32) -> c_int = "mrml_hip_attention_prefill";
+    block_tables: fn(Ctx, *const i32, *const i32, i32, *mut i32, i32, i32, *mut i32, *const i32, i32, *mut i32, *mut i32, *mut i32, *mut i32, *mut i32, i32, *mut i32, i32) -> c_int = "mrml_hip_block_tables";
+    rope_kv_append_paged: fn(Ctx, *const f32, *mut f32, *mut u16, *mut u16, *const i32, *const i32, i32, i32, i32, i32, i32, i32, f32, f32, i32, i32, *const f32, i32) -> c_int = "mrml_hip_rope_kv_append_paged";
+    attention_paged: fn(Ctx, *const f32, i32, *const u16, *const u16, *mut f32, i32, i32, *const i32, i32, *const i32, i32, *const i32, *const i32, i32, i32, i32, i32, i32, f32, i32, i32, i32) -> c_int = "mrml_hip_attention_paged";
     attention_causal: fn(Ctx, *const f32, *const u16, *const u16, *mut f32, i32, i32, i32, i32, f32, i32, i32, i32, i32) -> c_int = "mrml_hip_attention_causal";
     attention_causal_split: fn(Ctx, *const f32, *const u16, *const u16, *mut f32, i32, i32, i32, i32, f32, i32, i32, i32, i32) -> c_int = "mrml_hip_attention_causal_split";
     gemma2_create: fn(Ctx, *const MrmlHipGemma2Config, *const c_void, *const f32, *const MrmlHipGemma2Layer, *mut Model) -> c_int = "mrml_hip_gemma2_create";
