@@ -39,14 +39,19 @@ typedef int int4v __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kShift = 14.0f;   // p is kept as p * 2^14 (below 2^16, f16's end, with the slack below)
 constexpr float kSlack = 1.5f;    // the maximum may grow by this much before o and l are rescaled
-constexpr int kScanT = 256;       // threads of a workgroup
+constexpr float kBroken = -1.0f;  // in place of l: the part is not finite
 constexpr int kRowsA = 16, kUnitA = 32;  // rows and positions of a stream item's tile (one wave)
-constexpr int kRowsB = 128;              // rows of a block item's tile (four waves)
 constexpr int kFewRows = 32;             // groups of at most so many rows are stream items
+constexpr int kMaxT = 512;               // threads of a workgroup at most
 // Relative cost of a unit on one workgroup, for the split of the workgroups:
-// a block unit keeps the MFMA of all four waves busy, four stream units run side by side.
+// a block unit keeps the MFMA of all waves busy, a stream unit's waves run side by side.
 constexpr int kCostA = 1, kCostB = 8;
 
+// Waves of a workgroup, rows of a block item and positions of its tile by padded head size: two waves a SIMD
+// while a wave's q and o fit 256 registers.
+constexpr int waves_of(int dp, bool quant) { return quant || dp > 256 ? 4 : 8; }
+constexpr int tiles_of(int dp) { return dp > 128 ? 1 : 2; }  // row tiles of 16 a wave
+constexpr int rows_b(int dp) { return waves_of(dp, false) * tiles_of(dp) * 16; }
 constexpr int unit_b(int dp) { return 16384 / dp; }
 
 // Device scratch of a call (paged_attn_scratch_bytes).
@@ -56,10 +61,11 @@ struct Parts {
     float *o_a, *o_b;    // later parts, by worker: [worker][16][head_dim], [workgroup][128][head_dim]
     float2 *ml_a, *ml_b;
     int32_t *first, *last;  // workers that hold an item's first and last unit
-    int2 *row_item;         // {the own items' first index, row within the request}, type in bit 30 of y
+    int4 *row_item;         // {the own items' first index, row within the request, block items?, request}
     int32_t *head;          // {rows are sound, first row, rows}
     int items_a;            // index of the first block item
-    int wgs;
+    int wgs, waves;
+    int rows_b;             // rows of a block item (0: none)
 };
 
 // What a wave knows of the piece it works on (uniform).
@@ -80,13 +86,12 @@ struct Dest {
     bool own;
 };
 
-struct Scan {  // per thread's share of the requests: exclusive sums, in LDS
-    int ua[kScanT + 1], ub[kScanT + 1];  // units
-    int ia[kScanT + 1], ib[kScanT + 1];  // items
-    int rs[kScanT + 1];                  // first row
-    int sum[8][4];
-    int bad, low, need_at;
-    float size;
+struct Scan {  // sums over the requests before each thread's share, in LDS
+    int ua[kMaxT + 1], ub[kMaxT + 1];  // units
+    int ia[kMaxT + 1], ib[kMaxT + 1];  // items
+    int rs[kMaxT + 1], len[kMaxT];     // first row; length of the share's first request
+    int sum[8][4], low[8], flags[8];
+    float size[8];
 };
 
 __device__ __forceinline__ float as_f(uint32_t u) { return __builtin_bit_cast(float, u); }
@@ -103,6 +108,29 @@ __device__ __forceinline__ float over_row(float v, F f)
 }
 __device__ __forceinline__ float row_max(float v) { return over_row(v, [](float a, float b) { return fmaxf(a, b); }); }
 __device__ __forceinline__ float row_sum(float v) { return over_row(v, [](float a, float b) { return a + b; }); }
+
+// A value that every lane of the wave holds, as a scalar.
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ float uni(float v) { return as_f((uint32_t)__builtin_amdgcn_readfirstlane((int)as_u(v))); }
+__device__ __forceinline__ size_t uni(size_t v)
+{
+    return (size_t)(uint32_t)uni((int)(v & 0xffffffffu)) | (size_t)(uint32_t)uni((int)(v >> 32)) << 32;
+}
+
+// No memory access is moved past this by the compiler (waits that count loads rely on their order).
+__device__ __forceinline__ void pin()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// v, as a value that the compiler forms anew where it is used: what follows from it is
+// not kept in registers across a loop.
+__device__ __forceinline__ int here(int v)
+{
+    asm volatile("" : "+v"(v));
+    return v;
+}
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -135,13 +163,18 @@ struct Request {
     int rs, n, len;  // first row, rows, own length (within its table row)
 };
 
-__device__ __forceinline__ Request request_at(const PagedAttn &a, int r)
+__device__ __forceinline__ int share(const PagedAttn &a) { return (a.n_seqs + blockDim.x - 1) / blockDim.x; }
+
+__device__ __forceinline__ int clamp_len(const PagedAttn &a, int len)
 {
-    Request q;
-    q.rs = a.row_start[r];
-    q.n = a.row_start[r + 1] - q.rs;
-    q.len = min(max(a.lens[r], 0), a.table_stride * a.map.page_size);
-    return q;
+    return min(max(len, 0), a.table_stride * a.map.page_size);
+}
+
+__device__ __forceinline__ Request request_at(const PagedAttn &a, const Scan &s, int r)
+{
+    if (share(a) == 1) return Request{s.rs[r], s.rs[r + 1] - s.rs[r], s.len[r]};
+    const int rs = a.row_start[r];
+    return Request{rs, a.row_start[r + 1] - rs, clamp_len(a, a.lens[r])};
 }
 
 // Own positions that rows i0..i1 of a request see: [lo, hi).
@@ -160,30 +193,30 @@ __device__ __forceinline__ int own_units_a(const PagedAttn &a, const Request &q)
     return units_of(lo, hi, kUnitA);
 }
 
-__device__ __forceinline__ int own_units_b(const PagedAttn &a, const Request &q, int block, int unit)
+__device__ __forceinline__ int own_units_b(const PagedAttn &a, const Request &q, int block, int unit, int rows)
 {
     int lo, hi;
-    const int last = min(q.n * a.group, (block + 1) * kRowsB) - 1;
-    own_range(a, q, block * kRowsB / a.group, last / a.group, lo, hi);
+    const int last = min(q.n * a.group, (block + 1) * rows) - 1;
+    own_range(a, q, block * rows / a.group, last / a.group, lo, hi);
     return units_of(lo, hi, unit);
 }
 
 // {stream units, block units, stream items, block items} of a request; returns the units as a float, which cannot
 // overflow.
-__device__ __forceinline__ float request_work(const PagedAttn &a, const Request &q, bool blocks, int unit, int w[4])
+__device__ __forceinline__ float request_work(const PagedAttn &a, const Request &q, int rows, int unit, int w[4])
 {
     w[0] = w[1] = w[2] = w[3] = 0;
     if (q.n <= 0) return 0.0f;
     const int m = q.n * a.group;
-    if (!blocks || m <= kFewRows) {
+    if (!rows || m <= kFewRows) {
         w[2] = (m + kRowsA - 1) / kRowsA * a.n_kv_heads;
         w[0] = w[2] * own_units_a(a, q);
         return (float)w[2] * (float)own_units_a(a, q);
     } else {
-        const int nb = (m + kRowsB - 1) / kRowsB;
+        const int nb = (m + rows - 1) / rows;
         float size = 0.0f;
         for (int b = 0; b < nb; ++b) {
-            const int n = own_units_b(a, q, b, unit);
+            const int n = own_units_b(a, q, b, unit, rows);
             w[1] += n;
             size += (float)n;
         }
@@ -194,43 +227,40 @@ __device__ __forceinline__ float request_work(const PagedAttn &a, const Request 
 }
 
 // Every workgroup forms the same sums over all requests (a few loads a thread).
-__device__ void scan_requests(const PagedAttn &a, Scan &s, bool blocks, int unit)
+// False: row starts that do not ascend within the rows.
+struct Totals {
+    bool ok, need_at;  // need_at: some row stands before its request's first position
+    int low;           // the first own position that a row has
+    float size;        // units, as a float
+};
+
+template <int T>
+__device__ Totals scan_requests(const PagedAttn &a, Scan &s, int rows, int unit)
 {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (a.n_seqs + kScanT - 1) / kScanT, r0 = tid * per;
-    if (tid == 0) {
-        s.bad = 0;
-        s.low = INT32_MAX;
-        s.need_at = 0;
-        s.size = 0.0f;
-    }
-    int w[4] = {0, 0, 0, 0}, bad = 0, low = INT32_MAX, neg = 0;
-    for (int r = r0; r < min(r0 + per, a.n_seqs); ++r) {
-        const int rs = a.row_start[r], re = a.row_start[r + 1];
-        bad |= rs < 0 || re < rs || re > a.max_rows;
-        if (blockIdx.x == 0 && (uint32_t)a.lens[r] > (uint32_t)(a.table_stride * a.map.page_size)) page_fault(a.faults);
-    }
-    __syncthreads();
-    if (bad) s.bad = 1;
-    __syncthreads();
-    if (s.bad) return;
+    const int per = share(a), r0 = tid * per, r1 = min(r0 + per, a.n_seqs);
+    int w[4] = {0, 0, 0, 0}, low = INT32_MAX, flags = 0;
     float size = 0.0f;
-    for (int r = r0; r < min(r0 + per, a.n_seqs); ++r) {
-        const Request q = request_at(a, r);
+    s.rs[tid] = a.row_start[min(r0, a.n_seqs)];
+    if (tid == 0) s.rs[T] = a.row_start[a.n_seqs];
+    for (int r = r0; r < r1; ++r) {
+        const int rs = a.row_start[r], re = a.row_start[r + 1], len = a.lens[r];
+        if (rs < 0 || re < rs || re > a.max_rows) {
+            flags |= 1;
+            continue;
+        }
+        const Request q{rs, re - rs, clamp_len(a, len)};
+        if (q.len != len && blockIdx.x == 0) page_fault(a.faults);
+        if (r == r0) s.len[tid] = q.len;
         int x[4];
-        size += request_work(a, q, blocks, unit, x);
+        size += request_work(a, q, rows, unit, x);
 #pragma unroll
         for (int k = 0; k < 4; ++k) w[k] += x[k];
         if (q.n > 0) {
             low = min(low, q.len - q.n);
-            neg |= q.len < q.n;
+            flags |= q.len < q.n ? 2 : 0;
         }
     }
-    s.rs[tid] = a.row_start[min(r0, a.n_seqs)];
-    if (tid == 0) s.rs[kScanT] = a.row_start[a.n_seqs];
-    if (low < INT32_MAX) atomicMin(&s.low, low);
-    if (neg) s.need_at = 1;
-    if (size > 0.0f) atomicAdd(&s.size, size);  // a rough figure, compared with one bound
     int inc[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -243,22 +273,45 @@ __device__ void scan_requests(const PagedAttn &a, Scan &s, bool blocks, int unit
         inc[k] = x;
         if (lane == 63) s.sum[wave][k] = x;
     }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        low = min(low, __shfl_xor(low, d, 64));
+        flags |= __shfl_xor(flags, d, 64);
+        size += __shfl_xor(size, d, 64);
+    }
+    if (lane == 0) {
+        s.low[wave] = low;
+        s.flags[wave] = flags;
+        s.size[wave] = size;
+    }
     __syncthreads();
+    int before[4] = {0, 0, 0, 0};
+    low = INT32_MAX;
+    flags = 0;
+    size = 0.0f;
+#pragma unroll
+    for (int v = 0; v < T / 64; ++v) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) before[k] += v < wave ? s.sum[v][k] : 0;
+        low = min(low, s.low[v]);
+        flags |= s.flags[v];
+        size += s.size[v];
+    }
     int *dst[4] = {s.ua, s.ub, s.ia, s.ib};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        int before = 0;
-        for (int v = 0; v < wave; ++v) before += s.sum[v][k];
-        dst[k][tid] = before + inc[k] - w[k];
-        if (tid == kScanT - 1) dst[k][kScanT] = before + inc[k];
+        dst[k][tid] = before[k] + inc[k] - w[k];
+        if (tid == T - 1) dst[k][T] = before[k] + inc[k];
     }
     __syncthreads();
+    return Totals{(uni(flags) & 1) == 0, (uni(flags) & 2) != 0,
+                  uni(low), uni(size)};
 }
 
-// The thread whose share [from[t], from[t + 1]) holds x (from ascending, from[0] <= x < from[256]).
+// The thread whose share [from[t], from[t + 1]) holds x (from ascending, from[0] <= x < from[threads]).
 __device__ __forceinline__ int share_of(const int *from, int x)
 {
-    int lo = 0, hi = kScanT - 1;
+    int lo = 0, hi = blockDim.x - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (from[mid] <= x)
@@ -272,61 +325,11 @@ __device__ __forceinline__ int share_of(const int *from, int x)
 // The request of a row (the last one that starts at or before it and has rows).
 __device__ __forceinline__ int request_of(const PagedAttn &a, const Scan &s, int row)
 {
-    const int per = (a.n_seqs + kScanT - 1) / kScanT;
+    const int per = share(a);
     int r = share_of(s.rs, row) * per;
+    if (per == 1) return r;
     while (r + 1 < a.n_seqs && a.row_start[r + 1] <= row) ++r;
     return r;
-}
-
-// ---- a row on its own -------------------------------------------------------------
-//
-// The f16 terms of p and q turn an infinite value into NaN, and a weight of 0
-// times an infinity that its row does not see is one too.  So a row whose part
-// came out NaN is formed again, one position after the other in f32, by the
-// wave; a program whose values are finite never gets here.
-__device__ __noinline__ void slow_row(const PagedAttn &a, const Piece &pc, int mi, int vlo, int vhi, float *o_dst,
-                                      float2 *ml_dst)
-{
-    constexpr int E = 8;  // values a lane at most
-    const int lane = threadIdx.x & 63, hd = a.head_dim;
-    const int tok = pc.tok0 + mi / a.group, head = pc.kvh * a.group + mi % a.group;
-    const float *qr = a.q + (size_t)tok * a.q_stride + (size_t)head * hd;
-    float q[E], o[E], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int d = e * 64 + lane;
-        const float x = d < hd ? qr[d] : 0.0f;
-        q[e] = x;
-        o[e] = 0.0f;
-        if (a.k_fmt != 0) {
-            uint32_t db;
-            int qs;
-            q[e] = (float)q8_0_block32(x, db, qs) * f16_bits_to_f32(db);
-        }
-    }
-    const int kb = kv_row_bytes(a.k_fmt, hd), vb = kv_row_bytes(a.v_fmt, hd);
-    for (int t = max(pc.p0, vlo); t < min(pc.p1, vhi); ++t) {
-        const int place = place_at(a, pc.table, t);
-        if (place < 0) continue;
-        const uint8_t *kr = kv_row(a, a.k, kb, place, pc.kvh), *vr = kv_row(a, a.v, vb, place, pc.kvh);
-        float s = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (e * 64 + lane < hd) s = fmaf(q[e], kv_value(kr, a.k_fmt, e * 64 + lane), s);
-        for (int x = 32; x; x >>= 1) s += __shfl_xor(s, x, 64);
-        s *= a.scale * kLog2e;
-        if (s == -INFINITY) continue;  // no weight
-        const float m2 = fmaxf(m, s), f = exp2f(m - m2), w = exp2f(s - m2);
-        l = l * f + w;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (e * 64 + lane < hd) o[e] = o[e] * f + w * kv_value(vr, a.v_fmt, e * 64 + lane);
-        m = m2;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (e * 64 + lane < hd) o_dst[e * 64 + lane] = o[e];
-    if (lane == 0) *ml_dst = make_float2(m, l);
 }
 
 // ---- query rows ------------------------------------------------------------------
@@ -337,7 +340,7 @@ __device__ __forceinline__ size_t part_row(const PagedAttn &a, const Piece &pc, 
 }
 
 // What row mi of a piece's group sees, in the source's positions: [vlo, vhi).
-__device__ __forceinline__ void row_sees(const PagedAttn &a, const Scan &s, const Piece &pc, int mi, int &vlo, int &vhi)
+__device__ __forceinline__ void row_sees(const PagedAttn &a, const Scan &s, bool need_at, const Piece &pc, int mi, int &vlo, int &vhi)
 {
     vlo = 0;
     vhi = INT32_MAX;
@@ -347,8 +350,8 @@ __device__ __forceinline__ void row_sees(const PagedAttn &a, const Scan &s, cons
         const int at = pc.at0 + mi / a.group;
         vhi = at + 1;
         vlo = a.window ? at - a.window + 1 : 0;
-    } else if (s.need_at || a.window) {
-        const Request q = request_at(a, request_of(a, s, tok));
+    } else if (need_at || a.window) {
+        const Request q = request_at(a, s, request_of(a, s, tok));
         const int at = a.prefix_len + q.len - (q.rs + q.n - tok);
         vhi = min(a.prefix_len, at + 1);
         vlo = a.window ? at - a.window + 1 : 0;
@@ -448,13 +451,14 @@ __device__ __forceinline__ bool softmax_step(float *x, float &m, float &l, float
 
 // ---- stream items: a wave, 16 query rows, K and V straight from memory ------------
 //
-// Per tile of 32 positions a lane loads K of position lane % 16 (+ 16) in 16-byte
+// Per tile of 32 positions a lane takes K of position lane % 16 (+ 16) in 16-byte
 // pieces, which are the product's operand as they are, and V of 8 positions in
 // 16-byte pieces of 8 dims.  V's operand wants 8 positions of one dim: an 8 x 8
 // transpose inside the lane's registers, one v_perm a pair; the dims then lie
-// 8 apart over the operand's rows, which only the store of o has to know.  With
-// K of the next tile and V of this one in flight a wave keeps 32 KB on the
-// way (head_dim 256), so one wave a SIMD suffices to be bound by HBM.
+// 8 apart over the operand's rows, which only the store of o has to know.  K of
+// an f16 cache goes through a tile of LDS of the wave's own (global_load_lds), so
+// that the next tile's K is on its way without registers; the next V is loaded as
+// soon as this one is used up.  A wave keeps up to 32 KB in flight (head_dim 256).
 //
 // Quantised K is multiplied as the ring attention does it: q as Q8_0 blocks,
 // each block's integer sum on the int8 MFMA (16x16x32: one block a
@@ -469,7 +473,13 @@ struct __attribute__((packed, aligned(2))) Bytes8 {
 
 constexpr int kTrRow = 36;  // floats a query row of the score tile in LDS
 
+template <int DP, bool KQ>
 struct WaveLds {
+    int place[32];
+    uint4 k[DP * 4];  // 32 positions, as BlockLds::k
+};
+template <int DP>
+struct WaveLds<DP, true> {
     int place[32];
     float scores[16 * kTrRow];
 };
@@ -518,8 +528,8 @@ __device__ __forceinline__ void load_quant_q(const PagedAttn &a, const float *ro
 }
 
 template <int DP, bool KQ, bool VQ>
-__device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan &sc, const Piece &pc, WaveLds &lds,
-                                            const Dest &to)
+__device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan &sc, bool need_at, const Piece &pc,
+                                            WaveLds<DP, KQ> &lds, const Dest &to)
 {
     constexpr int KS = DP / 32, NG = DP < 128 ? 1 : DP / 128;
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, hd = a.head_dim;
@@ -535,7 +545,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan &sc, 
     else
         c *= load_q<KS>(a, q_row, live, g, qh, ql);
     int vlo, vhi;
-    row_sees(a, sc, pc, mi, vlo, vhi);
+    row_sees(a, sc, need_at, pc, mi, vlo, vhi);
     const int full_lo = wave_max(vlo), full_hi = wave_min(vhi);
     const int krb = kv_row_bytes(a.k_fmt, hd), vrb = kv_row_bytes(a.v_fmt, hd);
     const int kblk = a.k_fmt == 1 ? 34 : 18, vblk = a.v_fmt == 1 ? 34 : 18;
@@ -547,46 +557,53 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan &sc, 
 #pragma unroll
         for (int d = 0; d < 8; ++d) o[n][d] = float4v{0, 0, 0, 0};
 
-    auto place_of_lane = [&](int t0) {
+    // A tile's page ids are loaded two tiles ahead and looked at one tile ahead, when they are long there.
+    auto page_ids = [&](int t0) { return t0 + (lane & 31) < pc.p1 ? pc.table[page_of(a.map, t0 + (lane & 31))] : -1; };
+    auto places = [&](int t0, int id) {
         const int pos = t0 + (lane & 31);
-        if (pos >= pc.p1) return -1;
-        const int place = place_at(a, pc.table, pos);
-        if (place < 0 && lane < 32) page_fault(a.faults);
+        const int place = place_of(a.map, pos, page_of(a.map, pos), id);
+        if (place < 0 && pos < pc.p1 && lane < 32) page_fault(a.faults);
         return place;
     };
-    uint4 kf[KQ ? 1 : 2][KQ ? 1 : KS];
     Bytes8 kq[KQ ? 2 : 1][KQ ? KS : 1];
     uint16_t kd[KQ ? 2 : 1][KQ ? KS : 1];
     auto load_k = [&](int place) {
+        if constexpr (KQ) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint8_t *row = kv_row(a, a.k, krb, __shfl(place, 16 * h + i, 64), pc.kvh);
+            for (int h = 0; h < 2; ++h) {
+                const uint8_t *row = kv_row(a, a.k, krb, __shfl(place, 16 * h + i, 64), pc.kvh);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                if constexpr (KQ) {
+                for (int s = 0; s < KS; ++s) {
                     const uint8_t *b = row + (s * 32 < hd ? s * kblk : 0);
                     kd[h][s] = *reinterpret_cast<const uint16_t *>(b);
                     kq[h][s] = *reinterpret_cast<const Bytes8 *>(b + 2 + (a.k_fmt == 1 ? 8 * g : 8 * (g & 1)));
-                } else {
-                    kf[h][s] = *reinterpret_cast<const uint4 *>(row + g * 16 + (s * 32 < hd ? s * 64 : 0));
                 }
+            }
+        } else {
+            constexpr int P = DP / 8, PI = 64 / P;
+            const int ln = here(lane);
+#pragma unroll
+            for (int n = 0; n < 32 / PI; ++n) {
+                const int p = n * PI + ln / P, piece = (ln % P) ^ (p & 7);
+                const uint8_t *src = kv_row(a, a.k, krb, __shfl(place, p, 64), pc.kvh) + (piece * 8 < hd ? piece * 16 : 0);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)src,
+                                                 (__attribute__((address_space(3))) uint32_t *)(lds.k + n * 64), 16, 0, 0);
             }
         }
     };
-    int place = place_of_lane(pc.p0), place_next = place_of_lane(pc.p0 + kUnitA);
-    load_k(place);
-    for (int t0 = pc.p0; t0 < pc.p1; t0 += kUnitA) {
-        const uint32_t there = (uint32_t)__ballot(place >= 0);  // bit p: position t0 + p
+    uint4 v[VQ ? 1 : NG][8];
+    Bytes8 vq[VQ ? NG : 1][8];
+    _Float16 vd[VQ ? NG : 1][8];
+    auto load_v = [&](int place) {
         lds.place[lane & 31] = place;
+        __builtin_amdgcn_wave_barrier();
         const int4 pa = *reinterpret_cast<const int4 *>(lds.place + 4 * g);
         const int4 pb = *reinterpret_cast<const int4 *>(lds.place + 16 + 4 * g);
+        __builtin_amdgcn_wave_barrier();
         const int pl[8] = {pa.x, pa.y, pa.z, pa.w, pb.x, pb.y, pb.z, pb.w};
-        uint4 v[VQ ? 1 : NG][8];
-        Bytes8 vq[VQ ? NG : 1][8];
-        _Float16 vd[VQ ? NG : 1][8];
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
-            const int d0 = n * 128 + 8 * i, dim = d0 < hd ? d0 : 0;  // past the head: the first dims, never stored
+            const int d0 = n * 128 + 8 * (here(lane) & 15), dim = d0 < hd ? d0 : 0;  // past the head: never stored
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const uint8_t *row = kv_row(a, a.v, vrb, pl[j], pc.kvh);
@@ -599,6 +616,16 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan &sc, 
                 }
             }
         }
+    };
+    int id_next = page_ids(pc.p0 + kUnitA);
+    int place = places(pc.p0, page_ids(pc.p0));
+    load_k(place);
+    pin();
+    load_v(place);
+    for (int t0 = pc.p0; t0 < pc.p1; t0 += kUnitA) {
+        const uint32_t there = (uint32_t)__ballot(place >= 0);  // bit p: position t0 + p
+        const int place_next = places(t0 + kUnitA, id_next);
+        id_next = page_ids(t0 + 2 * kUnitA);
         float x[8];
         if constexpr (KQ) {
             float4v acc[2] = {};
@@ -630,12 +657,17 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan &sc, 
             }
             __builtin_amdgcn_wave_barrier();
         } else {
+            // K is in LDS once no more than this tile's V (loaded after it) is on its way
+            constexpr int kLeft = VQ ? 0 : NG * 8;
+            __builtin_amdgcn_s_waitcnt(0x0f70 | (kLeft & 15) | (kLeft >> 4) << 14);
+            pin();
             float4v acc[2][2] = {};
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const half8 kk = __builtin_bit_cast(half8, kf[h][s]);
+                    const int p = 16 * h + i;
+                    const half8 kk = __builtin_bit_cast(half8, lds.k[p * (DP / 8) + ((4 * s + g) ^ (p & 7))]);
                     acc[h][0] = mfma(kk, qh[s], acc[h][0]);
                     acc[h][1] = mfma(kk, ql[s], acc[h][1]);
                 }
@@ -645,8 +677,9 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan &sc, 
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x[4 * h + r] = (acc[h][0][r] + acc[h][1][r]) * c;
         }
-        const int place_2 = place_of_lane(t0 + 2 * kUnitA);
+        pin();  // K's tile has been read, and no later load passes the next one's
         if (t0 + kUnitA < pc.p1) load_k(place_next);
+        pin();
         const bool edge = t0 < full_lo || t0 + kUnitA > full_hi || there != 0xffffffffu;
         if (edge) {
 #pragma unroll
@@ -656,7 +689,8 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan &sc, 
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (pl[j] < 0) {  // nothing is there: whatever was read must not meet a weight of 0
+                if (!((there >> (16 * (j >> 2) + 4 * g + (j & 3))) & 1)) {
+                    // nothing is there: whatever was read must not meet a weight of 0
 #pragma unroll
                     for (int n = 0; n < NG; ++n) {
                         if constexpr (VQ)
@@ -729,8 +763,8 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan &sc, 
                 }
             }
         }
+        if (t0 + kUnitA < pc.p1) load_v(place_next);
         place = place_next;
-        place_next = place_2;
     }
     l = row_sum(l);
     float check = l;
@@ -739,8 +773,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan &sc, 
 #pragma unroll
         for (int d = 0; d < 8; ++d) check += o[n][d][0] + o[n][d][1] + o[n][d][2] + o[n][d][3];
     check = row_sum(check);
-    const bool wrong = live && check - check != 0.0f;  // NaN or infinite
-    if (live && !wrong) {
+    if (live) {
         const size_t at = part_row(a, pc, to, mi);
         float *dst = to.o + at * hd;
 #pragma unroll
@@ -752,28 +785,21 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan &sc, 
                 *reinterpret_cast<float4 *>(dst + dim) = make_float4(o[n][0][r], o[n][1][r], o[n][2][r], o[n][3][r]);
                 *reinterpret_cast<float4 *>(dst + dim + 4) = make_float4(o[n][4][r], o[n][5][r], o[n][6][r], o[n][7][r]);
             }
-        if (g == 0) to.ml[at] = make_float2(m - kShift, l);
-    }
-    uint32_t again = (uint32_t)__ballot(wrong) & 0xffffu;
-    while (again) {
-        const int b = __builtin_ctz(again);
-        again &= again - 1;
-        const size_t at = part_row(a, pc, to, pc.row0 + b);
-        slow_row(a, pc, pc.row0 + b, __shfl(vlo, b, 64), __shfl(vhi, b, 64), to.o + at * hd, to.ml + at);
+        if (g == 0) to.ml[at] = make_float2(m - kShift, check - check == 0.0f ? l : kBroken);
     }
 }
 
-// ---- block items: a workgroup, 128 query rows, K and V through LDS ------------------
+// ---- block items: a workgroup, many query rows, K and V through LDS -----------------
 //
 // Tiles of T = 16384 / DP positions, two in LDS (128 KB): while the waves work on
 // one, the next is under way.  K goes to LDS directly (global_load_lds), 16-byte
 // pieces of a row exchanged by the position's low bits so that a wave's reads of
 // 16 positions meet no bank twice; V is transposed on its way, as in a
-// stream item, by the thread that has loaded 8 positions x 8 dims, and written as
+// stream item, by the thread that has loaded 8 positions of some dims, and written as
 // 16-byte runs of 8 positions, exchanged by the dim's low bits.  A wave holds 16 * R
 // rows; each piece read from LDS feeds 2 * R products.
 
-// K and V row runs of a block tile in LDS, in 16-byte pieces.
+// Where a run of 8 positions of a dim lies in a tile of T positions, in 16-byte pieces.
 template <int T>
 __device__ __forceinline__ int v_piece(int dim, int run)
 {
@@ -785,83 +811,92 @@ __device__ __forceinline__ int v_piece(int dim, int run)
 
 template <int DP>
 struct BlockLds {
-    static constexpr int T = 16384 / DP;
+    static constexpr int T = unit_b(DP);
     uint4 k[2][2048], v[2][2048];
     int place[3][T];
 };
 
-template <int DP, int R>
-__device__ __forceinline__ void block_item(const PagedAttn &a, const Scan &sc, const Piece &pc, BlockLds<DP> &lds,
-                                           const Dest &to)
+template <int DP>
+__device__ __forceinline__ void block_item(const PagedAttn &a, const Scan &sc, bool need_at, const Piece &pc,
+                                           BlockLds<DP> &lds, const Dest &to)
 {
-    constexpr int KS = DP / 32, NF = DP / 16, T = 16384 / DP, SP = T < 64 ? T : 64, NH = SP / 16, P = DP / 8;
+    constexpr int NW = waves_of(DP, false), R = tiles_of(DP), KS = DP / 32, NF = DP / 16, T = unit_b(DP);
+    constexpr int SP = T < 64 ? T : 64, NH = SP / 16, P = DP / 8;
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4, hd = a.head_dim;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rb = hd * 2;
     const int tiles = (pc.p1 - pc.p0 + T - 1) / T;
 
-    auto set_places = [&](int tile) {
+    // A tile's page ids are loaded two tiles ahead, at a tile's start, and put into LDS as places at its end.
+    auto page_ids = [&](int tile) {
+        const int pos = pc.p0 + tile * T + tid;
+        return tid < T && pos < pc.p1 ? pc.table[page_of(a.map, pos)] : -1;
+    };
+    auto set_places = [&](int tile, int id) {
         if (tid < T) {
-            const int pos = pc.p0 + tile * T + tid;
-            int place = -1;
-            if (pos < pc.p1) {
-                place = place_at(a, pc.table, pos);
-                if (place < 0) page_fault(a.faults);
-            }
+            const int pos = pc.p0 + tile * T + tid, place = place_of(a.map, pos, page_of(a.map, pos), id);
+            if (place < 0 && pos < pc.p1) page_fault(a.faults);
             lds.place[tile % 3][tid] = place;
         }
     };
     auto load_k = [&](int tile) {
-        // a wave's share: T / 4 positions, 64 pieces an instruction
-        constexpr int PI = 64 / P > 0 ? 64 / P : 1;  // positions an instruction
+        constexpr int PW = T / NW, PI = 64 / P;  // positions of a wave's share, of an instruction
+        const int ln = here(lane);
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            const int p = wave * (T / 4) + n * PI + lane / P, piece = (lane % P) ^ (p & 7);
+        for (int n = 0; n < PW / PI; ++n) {
+            const int p = wave * PW + n * PI + ln / P, piece = (ln % P) ^ (p & 7);
             const uint8_t *src = kv_row(a, a.k, rb, lds.place[tile % 3][p], pc.kvh) + (piece * 8 < hd ? piece * 16 : 0);
-            uint4 *dst = &lds.k[tile & 1][(wave * (T / 4) + n * PI) * P];
+            uint4 *dst = &lds.k[tile & 1][(wave * PW + n * PI) * P];
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)src,
                                              (__attribute__((address_space(3))) uint32_t *)dst, 16, 0, 0);
         }
     };
-    const int dl = tid % P, run = tid / P;  // this thread's dims 8 dl .. and run of positions
-    constexpr int kTasks = (T / 8) * P;     // 256
-    static_assert(kTasks == 256, "one task a thread");
-    const int run0 = (run >> 2) * 32 + (run & 3) * 4;  // positions run0 + 0..3 and run0 + 16..19
-    uint4 v[8];
-    int vp[8];
+    // this thread's dims (VD of them) and run of positions: run0 + 0..3 and run0 + 16..19
+    constexpr int VD = 32 / NW, VT = DP / VD;
+    static_assert(VT * (T / 8) == 64 * NW, "one task a thread");
+    const int dl = tid % VT, run = tid / VT, run0 = (run >> 2) * 32 + (run & 3) * 4;
+    uint32_t v[8][VD / 2];
     auto load_v = [&](int tile) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            vp[j] = lds.place[tile % 3][run0 + (j >> 2) * 16 + (j & 3)];
-            v[j] = *reinterpret_cast<const uint4 *>(kv_row(a, a.v, rb, vp[j], pc.kvh) + (dl * 8 < hd ? dl * 16 : 0));
+            const int place = lds.place[tile % 3][run0 + (j >> 2) * 16 + (j & 3)];
+            const uint8_t *src = kv_row(a, a.v, rb, place, pc.kvh) + (dl * VD < hd ? dl * VD * 2 : 0);
+            if constexpr (VD == 8) {
+                const uint4 x = *reinterpret_cast<const uint4 *>(src);
+                v[j][0] = x.x, v[j][1] = x.y, v[j][2] = x.z, v[j][3] = x.w;
+            } else {
+                const uint2 x = *reinterpret_cast<const uint2 *>(src);
+                v[j][0] = x.x, v[j][1] = x.y;
+            }
         }
     };
     auto store_v = [&](int tile) {
-        uint32_t w[8][4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t keep = vp[j] < 0 ? 0u : 0xffffffffu;  // nothing there: no weight may meet it
-            w[j][0] = v[j].x & keep, w[j][1] = v[j].y & keep, w[j][2] = v[j].z & keep, w[j][3] = v[j].w & keep;
-        }
+        for (int j = 0; j < 8; ++j)
+            if (lds.place[tile % 3][run0 + (j >> 2) * 16 + (j & 3)] < 0)  // nothing there: no weight may meet it
 #pragma unroll
-        for (int d = 0; d < 8; ++d) {
+                for (int w = 0; w < VD / 2; ++w) v[j][w] = 0;
+#pragma unroll
+        for (int d = 0; d < VD; ++d) {
             const uint32_t sel = d & 1 ? 0x07060302u : 0x05040100u;
             uint32_t t[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) t[e] = __builtin_amdgcn_perm(w[2 * e + 1][d >> 1], w[2 * e][d >> 1], sel);
-            lds.v[tile & 1][v_piece<T>(8 * dl + d, run)] = make_uint4(t[0], t[1], t[2], t[3]);
+            for (int e = 0; e < 4; ++e) t[e] = __builtin_amdgcn_perm(v[2 * e + 1][d >> 1], v[2 * e][d >> 1], sel);
+            lds.v[tile & 1][v_piece<T>(VD * dl + d, run)] = make_uint4(t[0], t[1], t[2], t[3]);
         }
     };
 
     __syncthreads();  // the tiles' LDS is free
-    set_places(0);
-    if (tiles > 1) set_places(1);
+    const int id0 = page_ids(0), id1 = page_ids(1);
+    set_places(0, id0);
+    set_places(1, id1);
     __syncthreads();
     if (tiles > 0) {
         load_k(0);
         load_v(0);
     }
 
+    const bool busy = pc.row0 + wave * R * 16 < pc.rows;  // the wave has rows
     half8 qh[R][KS], ql[R][KS];
     float c[R], m[R], l[R];
     int vlo[R], vhi[R], full_lo = 0, full_hi = INT32_MAX;
@@ -872,7 +907,7 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan &sc, c
         const bool live = mi < pc.rows;
         const int tok = pc.tok0 + mi / a.group, head = pc.kvh * a.group + mi % a.group;
         c[u] = load_q<KS>(a, a.q + (size_t)tok * a.q_stride + (size_t)head * hd, live, g, qh[u], ql[u]) * a.scale * kLog2e;
-        row_sees(a, sc, pc, mi, vlo[u], vhi[u]);
+        row_sees(a, sc, need_at, pc, mi, vlo[u], vhi[u]);
         full_lo = max(full_lo, wave_max(vlo[u]));
         full_hi = min(full_hi, wave_min(vhi[u]));
         m[u] = -INFINITY;
@@ -885,7 +920,7 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan &sc, c
     for (int tile = 0; tile < tiles; ++tile) {
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): K of this tile is in LDS
         __syncthreads();
-        if (tile + 2 < tiles) set_places(tile + 2);
+        const int id2 = page_ids(tile + 2);
         if (tile + 1 < tiles) {
             load_k(tile + 1);
             load_v(tile + 1);
@@ -894,7 +929,7 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan &sc, c
 #pragma unroll 1
         for (int s0 = 0; s0 < T; s0 += SP) {
             const int t0 = pc.p0 + tile * T + s0;
-            if (t0 >= pc.p1) break;
+            if (t0 >= pc.p1 || !busy) break;
             float4v acc[R][NH];
 #pragma unroll
             for (int u = 0; u < R; ++u)
@@ -956,18 +991,18 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan &sc, c
             }
         }
         if (tile + 1 < tiles) store_v(tile + 1);
+        set_places(tile + 2, id2);
     }
 #pragma unroll
     for (int u = 0; u < R; ++u) {
-        const int first = pc.row0 + (wave * R + u) * 16, mi = first + i;
+        const int mi = pc.row0 + (wave * R + u) * 16 + i;
         const bool live = mi < pc.rows;
         const float lu = row_sum(l[u]);
         float check = lu;
 #pragma unroll
         for (int f = 0; f < NF; ++f) check += o[u][f][0] + o[u][f][1] + o[u][f][2] + o[u][f][3];
         check = row_sum(check);
-        const bool wrong = live && check - check != 0.0f;  // NaN or infinite
-        if (live && !wrong) {
+        if (live) {
             const size_t at = part_row(a, pc, to, mi);
             float *dst = to.o + at * hd;
 #pragma unroll
@@ -975,185 +1010,180 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan &sc, c
                 if (f * 16 < hd)
                     *reinterpret_cast<float4 *>(dst + 16 * f + 4 * g) =
                         make_float4(o[u][f][0], o[u][f][1], o[u][f][2], o[u][f][3]);
-            if (g == 0) to.ml[at] = make_float2(m[u] - kShift, lu);
-        }
-        uint32_t again = (uint32_t)__ballot(wrong) & 0xffffu;
-        while (again) {
-            const int b = __builtin_ctz(again);
-            again &= again - 1;
-            const size_t at = part_row(a, pc, to, first + b);
-            slow_row(a, pc, first + b, __shfl(vlo[u], b, 64), __shfl(vhi[u], b, 64), to.o + at * hd, to.ml + at);
+            if (g == 0) to.ml[at] = make_float2(m[u] - kShift, check - check == 0.0f ? lu : kBroken);
         }
     }
 }
 
 // ---- the launch --------------------------------------------------------------------
 
-// The prefix's items: of the batch's rows, in one kind.
+// The prefix's items: of all rows of the batch, in one kind.
 struct Shared {
-    int rows;              // rows x group
-    bool few;              // stream items
-    int lo, hi;            // positions any row sees
-    int units, blocks;     // units an item, row blocks
+    int rows;           // rows x group
+    bool few;           // stream items
+    int lo, hi;         // positions any row sees
+    int units, items;   // units an item
 };
 
-__device__ __forceinline__ Shared shared_work(const PagedAttn &a, const Scan &s, bool blocks, int unit)
+__device__ __forceinline__ Shared shared_work(const PagedAttn &a, const Scan &s, const Totals &t, int rows_b, int unit)
 {
     Shared p;
-    p.rows = (s.rs[kScanT] - s.rs[0]) * a.group;
-    p.few = !blocks || p.rows <= kFewRows;
+    p.rows = uni(s.rs[blockDim.x] - s.rs[0]) * a.group;
+    p.few = !rows_b || p.rows <= kFewRows;
     p.hi = a.prefix_len;
-    p.lo = 0;
-    if (a.window && s.low < INT32_MAX) p.lo = min(max(a.prefix_len + s.low - a.window + 1, 0), p.hi);
-    const int tile = p.few ? kRowsA : kRowsB;
-    p.blocks = a.prefix_len > 0 ? (p.rows + tile - 1) / tile : 0;
+    p.lo = a.window && t.low < INT32_MAX ? min(max(a.prefix_len + t.low - a.window + 1, 0), p.hi) : 0;
+    const int tile = p.few ? kRowsA : rows_b;
+    p.items = a.prefix_len > 0 ? (p.rows + tile - 1) / tile * a.n_kv_heads : 0;
     p.units = units_of(p.lo, p.hi, p.few ? kUnitA : unit);
     return p;
 }
 
 // The piece at unit u of the stream or block items, at most `left` units long;
-// returns the units taken, and the item's index, and whether the piece holds
-// its first and last unit.
-__device__ __forceinline__ int find_piece(const PagedAttn &a, const Scan &s, const Shared &sh, bool blocks, bool block,
+// returns the units taken, the item's index, and whether the piece holds its
+// first and last unit.
+__device__ __forceinline__ int find_piece(const PagedAttn &a, const Scan &s, const Shared &sh, bool block, int rows_b,
                                           int unit, int u, int left, Piece &pc, int &item, bool &is_first, bool &is_last)
 {
-    const int tile = block ? kRowsB : kRowsA, step = block ? unit : kUnitA;
-    const bool sh_here = sh.few != block;
-    const int sh_items = sh_here ? sh.blocks * a.n_kv_heads : 0;
-    const int sh_units = sh_items * sh.units;
-    int lo, hi, units, within, blk;
+    const int tile = block ? rows_b : kRowsA, step = block ? unit : kUnitA;
+    const int sh_items = sh.few != block ? sh.items : 0, sh_units = sh_items * sh.units;
+    int lo, hi, units, within, blk, tab = 0;
     if (u < sh_units) {
         item = u / sh.units;
         within = u - item * sh.units;
         blk = item / a.n_kv_heads;
+        pc.kvh = item - blk * a.n_kv_heads;
         units = sh.units;
         lo = sh.lo;
         hi = sh.hi;
         pc.pre = true;
-        pc.table = a.prefix;
         pc.tok0 = s.rs[0];
         pc.rows = sh.rows;
         pc.at0 = 0;
     } else {
         u -= sh_units;
-        const int per = (a.n_seqs + kScanT - 1) / kScanT;
         const int t = share_of(block ? s.ub : s.ua, u);
-        int r = t * per, at = (block ? s.ub : s.ua)[t], first = (block ? s.ib : s.ia)[t];
-        Request q;
-        int w[4];
-        for (;; ++r) {
-            q = request_at(a, r);
-            request_work(a, q, blocks, unit, w);
-            const int n = block ? w[1] : w[0];
-            if (u < at + n || r + 1 >= a.n_seqs) break;
-            at += n;
-            first += block ? w[3] : w[2];
+        int r = t * share(a), first = (block ? s.ib : s.ia)[t];
+        u -= (block ? s.ub : s.ua)[t];
+        Request q = request_at(a, s, r);
+        if (share(a) > 1) {
+            for (;;) {
+                int w[4];
+                request_work(a, q, rows_b, unit, w);
+                const int n = block ? w[1] : w[0];
+                if (u < n || r + 1 >= a.n_seqs) break;
+                u -= n;
+                first += block ? w[3] : w[2];
+                q = request_at(a, s, ++r);
+            }
         }
-        u -= at;
         if (!block) {
             units = own_units_a(a, q);
             item = u / units;
             within = u - item * units;
             blk = item / a.n_kv_heads;
+            pc.kvh = item - blk * a.n_kv_heads;
             own_range(a, q, 0, q.n - 1, lo, hi);
         } else {
-            blk = 0;
-            for (;; ++blk) {
-                units = own_units_b(a, q, blk, unit);
+            for (blk = 0;; ++blk) {
+                units = own_units_b(a, q, blk, unit, rows_b);
                 if (u < units * a.n_kv_heads) break;
                 u -= units * a.n_kv_heads;
             }
-            const int kv = u / units;
-            item = blk * a.n_kv_heads + kv;
-            within = u - kv * units;
-            const int last = min(q.n * a.group, (blk + 1) * kRowsB) - 1;
-            own_range(a, q, blk * kRowsB / a.group, last / a.group, lo, hi);
+            pc.kvh = u / units;
+            item = blk * a.n_kv_heads + pc.kvh;
+            within = u - pc.kvh * units;
+            const int last = min(q.n * a.group, (blk + 1) * rows_b) - 1;
+            own_range(a, q, blk * rows_b / a.group, last / a.group, lo, hi);
         }
+        item += sh_items + first;
         pc.pre = false;
-        pc.table = a.table + (size_t)r * a.table_stride;
+        tab = r;
         pc.tok0 = q.rs;
         pc.rows = q.n * a.group;
         pc.at0 = q.len - q.n;
-        const int kvh_item = item;
-        item += sh_items + first;
-        pc.kvh = kvh_item % a.n_kv_heads;
-        blk = kvh_item / a.n_kv_heads;
     }
-    if (pc.pre) pc.kvh = item % a.n_kv_heads;
-    pc.row0 = blk * tile;
+    units = uni(units);
+    within = uni(within);
     const int take = min(units - within, left);
-    pc.p0 = lo + within * step;
-    pc.p1 = min(hi, pc.p0 + take * step);
+    item = uni(item);
+    pc.pre = uni(pc.pre);
+    pc.table = pc.pre ? a.prefix : a.table + (size_t)uni(tab) * a.table_stride;
+    pc.tok0 = uni(pc.tok0);
+    pc.rows = uni(pc.rows);
+    pc.at0 = uni(pc.at0);
+    pc.kvh = uni(pc.kvh);
+    pc.row0 = uni(blk) * tile;
+    pc.p0 = uni(lo) + within * step;
+    pc.p1 = min(uni(hi), pc.p0 + take * step);
     is_first = within == 0;
     is_last = within + take == units;
     return take;
 }
 
-template <int DP, bool KQ, bool VQ, int R>
+template <int DP, bool KQ, bool BLOCKS>
 struct KernelLds {
     Scan scan;
     union {
-        WaveLds wave[4];
+        WaveLds<DP, KQ> wave[waves_of(DP, !BLOCKS)];
         BlockLds<DP> block;
     };
 };
-template <int DP, bool KQ, bool VQ>
-struct KernelLds<DP, KQ, VQ, 0> {
+template <int DP, bool KQ>
+struct KernelLds<DP, KQ, false> {
     Scan scan;
-    WaveLds wave[4];
+    WaveLds<DP, KQ> wave[waves_of(DP, true)];
 };
 
-// R: rows of a block item's wave / 16 (0: stream items alone, the quantised caches).
-template <int DP, bool KQ, bool VQ, int R>
-__global__ __launch_bounds__(kScanT, 1) void paged_attn_kernel(PagedAttn a, Parts parts)
+// Quantised caches have stream items alone.
+template <int DP, bool KQ, bool VQ>
+__global__ __launch_bounds__(64 * waves_of(DP, KQ || VQ)) void paged_attn_kernel(PagedAttn a, Parts parts)
 {
-    __shared__ KernelLds<DP, KQ, VQ, R> lds;
-    constexpr bool kBlocks = R > 0;
-    constexpr int kUnitB = unit_b(DP);
+    constexpr bool kBlocks = !KQ && !VQ;
+    constexpr int kWaves = waves_of(DP, KQ || VQ), T = 64 * kWaves;
+    constexpr int kUnitB = unit_b(DP), kRowsB = kBlocks ? rows_b(DP) : 0;
+    __shared__ KernelLds<DP, KQ, kBlocks> lds;
     const Scan &s = lds.scan;
-    scan_requests(a, lds.scan, kBlocks, kUnitB);
     const int wg = blockIdx.x, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Totals totals = scan_requests<T>(a, lds.scan, kRowsB, kUnitB);
     Shared sh{};
     // row starts that do not ascend, or more units than an int counts (days of work): nothing is computed
-    bool bad = s.bad;
-    if (!bad) {
-        sh = shared_work(a, s, kBlocks, kUnitB);
-        bad = s.size + (float)sh.blocks * (float)a.n_kv_heads * (float)sh.units > 1e9f;
+    bool ok = totals.ok;
+    if (ok) {
+        sh = shared_work(a, s, totals, kRowsB, kUnitB);
+        ok = totals.size + (float)sh.items * (float)sh.units < 1e9f;
     }
     if (wg == 0 && tid == 0) {
-        parts.head[0] = !bad;
-        parts.head[1] = bad ? 0 : s.rs[0];
-        parts.head[2] = bad ? 0 : s.rs[kScanT];
-        if (bad) page_fault(a.faults);
+        *reinterpret_cast<int4 *>(parts.head) = make_int4(ok, ok ? s.rs[0] : 0, ok ? s.rs[T] : 0, 0);
+        if (!ok) page_fault(a.faults);
     }
-    if (bad) return;
-    const int sh_units = sh.blocks * a.n_kv_heads * sh.units, sh_items = sh.blocks * a.n_kv_heads;
-    const int ua = s.ua[kScanT] + (sh.few ? sh_units : 0), ub = s.ub[kScanT] + (sh.few ? 0 : sh_units);
+    if (!ok) return;
+    const int sh_units = sh.items * sh.units;
+    const int ua = uni(s.ua[T]) + (sh.few ? sh_units : 0), ub = uni(s.ub[T]) + (sh.few ? 0 : sh_units);
 
     // which items a row's own part is in
-    for (int row = s.rs[0] + wg * kScanT + tid; row < s.rs[kScanT]; row += parts.wgs * kScanT) {
-        const int r = request_of(a, s, row), per = (a.n_seqs + kScanT - 1) / kScanT, t = r / per;
-        int ia = s.ia[t], ib = s.ib[t], w[4];
-        for (int x = t * per; x < r; ++x) {
-            request_work(a, request_at(a, x), kBlocks, kUnitB, w);
+    for (int row = s.rs[0] + wg * T + tid; row < s.rs[T]; row += parts.wgs * T) {
+        const int r = request_of(a, s, row), t = r / share(a);
+        int ia = s.ia[t], ib = s.ib[t];
+        for (int x = t * share(a); x < r; ++x) {
+            int w[4];
+            request_work(a, request_at(a, s, x), kRowsB, kUnitB, w);
             ia += w[2];
             ib += w[3];
         }
-        const Request q = request_at(a, r);
+        const Request q = request_at(a, s, r);
         const bool block = kBlocks && q.n * a.group > kFewRows;
-        const int first = block ? parts.items_a + ib + (sh.few ? 0 : sh_items) : ia + (sh.few ? sh_items : 0);
-        parts.row_item[row] = make_int2(first, (row - q.rs) | (block ? 1 << 30 : 0));
+        const int first = block ? parts.items_a + ib + (sh.few ? 0 : sh.items) : ia + (sh.few ? sh.items : 0);
+        parts.row_item[row] = make_int4(first, row - q.rs, block, r);
     }
 
     int wb = 0;
-    if (ub > 0) {
+    if (kBlocks && ub > 0) {
         wb = parts.wgs;
         if (ua > 0) {
-            const float fb = (float)ub * kCostB, fa = (float)ua * kCostA * 0.25f;
+            const float fb = (float)ub * kCostB, fa = (float)ua * kCostA;
             wb = min(max((int)(parts.wgs * fb / (fa + fb) + 0.5f), 1), parts.wgs - 1);
         }
     }
-    const int n_a = (parts.wgs - wb) * 4;
     Piece pc;
     int item;
     bool first, last;
@@ -1161,106 +1191,236 @@ __global__ __launch_bounds__(kScanT, 1) void paged_attn_kernel(PagedAttn a, Part
         if (wg < wb) {
             const int quota = (ub + wb - 1) / wb, end = min(ub, (wg + 1) * quota);
             for (int u = wg * quota; u < end;) {
-                u += find_piece(a, s, sh, kBlocks, true, kUnitB, u, end - u, pc, item, first, last);
+                u += find_piece(a, s, sh, true, kRowsB, kUnitB, u, end - u, pc, item, first, last);
                 const size_t row = (size_t)wg * kRowsB;
                 const Dest to = first ? Dest{parts.o[!pc.pre], parts.ml[!pc.pre], true}
                                       : Dest{parts.o_b + row * a.head_dim, parts.ml_b + row, false};
                 if (tid == 0 && first) parts.first[parts.items_a + item] = wg;
                 if (tid == 0 && last) parts.last[parts.items_a + item] = wg;
-                block_item<DP, R ? R : 1>(a, s, pc, lds.block, to);
+                block_item<DP>(a, s, totals.need_at, pc, lds.block, to);
             }
             return;
         }
     }
-    const int worker = (wg - wb) + (parts.wgs - wb) * wave;
-    const int quota = (ua + n_a - 1) / n_a, end = min(ua, (worker + 1) * quota);
+    const int worker = (wg - wb) + (parts.wgs - wb) * wave, workers = (parts.wgs - wb) * kWaves;
+    const int quota = (ua + workers - 1) / workers, end = min(ua, (worker + 1) * quota);
     for (int u = worker * quota; u < end;) {
-        u += find_piece(a, s, sh, kBlocks, false, kUnitB, u, end - u, pc, item, first, last);
+        u += find_piece(a, s, sh, false, kRowsB, kUnitB, u, end - u, pc, item, first, last);
         const size_t row = (size_t)worker * kRowsA;
         const Dest to = first ? Dest{parts.o[!pc.pre], parts.ml[!pc.pre], true}
                               : Dest{parts.o_a + row * a.head_dim, parts.ml_a + row, false};
         if ((tid & 63) == 0 && first) parts.first[item] = worker;
         if ((tid & 63) == 0 && last) parts.last[item] = worker;
-        stream_item<DP, KQ, VQ>(a, s, pc, lds.wave[wave], to);
+        stream_item<DP, KQ, VQ>(a, s, totals.need_at, pc, lds.wave[wave], to);
     }
 }
 
-// Joins the parts of each row and head: a workgroup a row and head, waves over
-// the parts, lanes over the dims.
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a, Parts parts, bool blocks)
+// ---- joining the parts ---------------------------------------------------------------
+
+// The f16 terms of p and q turn an infinite value into NaN, and a weight of 0
+// times an infinity that its row does not see is one too.  So a row with a part
+// that is not finite is formed again here, one position after the other in f32
+// (`waves` waves taking turns); a program whose values are finite never gets here.
+__device__ __noinline__ void slow_row(const PagedAttn a, int row, int r, int h, int wave, int waves, float4 o[2],
+                                      float &m, float &l)
 {
-    __shared__ float s_o[4][512], s_m[4], s_l[4];
-    const int row = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hd = a.head_dim;
-    const int row0 = parts.head[1], row1 = parts.head[2];
-    if (!parts.head[0] || row < row0 || row >= row1) return;
+    constexpr int E = 8;  // values a lane: dims 4 lane .. and 256 + 4 lane ..
+    const int lane = threadIdx.x & 63, hd = a.head_dim, kvh = h / a.group;
+    const int len = clamp_len(a, a.lens[r]), at = a.prefix_len + len - (a.row_start[r + 1] - row);
+    const int first = a.window ? max(0, at - a.window + 1) : 0;
+    const int krb = kv_row_bytes(a.k_fmt, hd), vrb = kv_row_bytes(a.v_fmt, hd);
+    float q[E], x[E] = {};
+    int dim[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        dim[e] = (e >> 2) * 256 + 4 * lane + (e & 3);
+        q[e] = dim[e] < hd ? a.q[(size_t)row * a.q_stride + (size_t)h * hd + dim[e]] : 0.0f;
+    }
+    if (a.k_fmt != 0) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            uint32_t db;
+            int sum;
+            const uint32_t w = q8_0_block8x4(make_float4(q[4 * y], q[4 * y + 1], q[4 * y + 2], q[4 * y + 3]), db, sum);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[4 * y + e] = (float)(int8_t)(w >> (8 * e)) * f16_bits_to_f32(db);
+        }
+    }
+    m = -INFINITY;
+    l = 0.0f;
+    for (int t = first + wave; t <= at; t += waves) {
+        const bool pre = t < a.prefix_len;
+        const int place = pre ? place_at(a, a.prefix, t) : place_at(a, a.table + (size_t)r * a.table_stride, t - a.prefix_len);
+        if (place < 0) continue;
+        const uint8_t *kr = kv_row(a, a.k, krb, place, kvh), *vr = kv_row(a, a.v, vrb, place, kvh);
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (dim[e] < hd) s = fmaf(q[e], kv_value(kr, a.k_fmt, dim[e]), s);
+        for (int y = 32; y; y >>= 1) s += __shfl_xor(s, y, 64);
+        s *= a.scale * kLog2e;
+        if (s == -INFINITY) continue;  // no weight
+        const float m2 = fmaxf(m, s), f = exp2f(m - m2), w = exp2f(s - m2);
+        l = l * f + w;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (dim[e] < hd) x[e] = x[e] * f + w * kv_value(vr, a.v_fmt, dim[e]);
+        m = m2;
+    }
+    o[0] = make_float4(x[0], x[1], x[2], x[3]);
+    o[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+
+// Joins the parts of each row and head.  W waves share a row and head (1 where
+// there are many rows, each in few parts; 4 where a few rows are in many),
+// lane groups take a part each, a lane four dims of it.  Three round trips: where
+// the parts are, their (m, l), their values.
+template <int W>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a, Parts parts)
+{
+    constexpr int kAhead = 4;
+    __shared__ float s_o[4][512], s_l[4], s_m[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), hd = a.head_dim;
+    const int pair = blockIdx.x * (4 / W) + wave / W, row = pair / a.n_heads, h = pair - row * a.n_heads;
+    if (row >= a.max_rows) return;  // W == 1: the last workgroup's spare waves (no barrier there)
+    const int4 head = *reinterpret_cast<const int4 *>(parts.head);
+    const int4 ri = parts.row_item[row];
+    if (!head.x || row < head.y || row >= head.z) return;  // W == 4: the whole workgroup
     const int kvh = h / a.group, gq = h - kvh * a.group;
     const size_t base = (size_t)row * a.n_heads + h;
     // the two items of the row: the prefix's, its own
-    int w0[2], n[2], at[2];
-    bool blk[2];
+    int w0[2], n[2], at[2], rows[2];
     {
-        const int m = (row1 - row0) * a.group, mi = (row - row0) * a.group + gq;
-        blk[0] = blocks && m > kFewRows;
-        const int tile = blk[0] ? kRowsB : kRowsA, item = mi / tile * a.n_kv_heads + kvh + (blk[0] ? parts.items_a : 0);
-        at[0] = mi % tile;
+        const int m = (head.z - head.y) * a.group, mi = (row - head.y) * a.group + gq;
+        const bool block = parts.rows_b && m > kFewRows;
+        rows[0] = block ? parts.rows_b : kRowsA;
+        const int item = mi / rows[0] * a.n_kv_heads + kvh + (block ? parts.items_a : 0);
+        at[0] = mi % rows[0];
         w0[0] = a.prefix_len > 0 ? parts.first[item] : 0;
         n[0] = a.prefix_len > 0 ? parts.last[item] - w0[0] + 1 : 0;
     }
     {
-        const int2 ri = parts.row_item[row];
-        blk[1] = ri.y >> 30;
-        const int mi = (ri.y & ~(1 << 30)) * a.group + gq, tile = blk[1] ? kRowsB : kRowsA;
-        const int item = ri.x + mi / tile * a.n_kv_heads + kvh;
-        at[1] = mi % tile;
+        rows[1] = ri.z ? parts.rows_b : kRowsA;
+        const int mi = ri.y * a.group + gq, item = ri.x + mi / rows[1] * a.n_kv_heads + kvh;
+        at[1] = mi % rows[1];
         w0[1] = parts.first[item];
         n[1] = parts.last[item] - w0[1] + 1;
     }
-    float m = -INFINITY, l = 0.0f;
-    float o[8] = {};
-    for (int k = wave; k < n[0] + n[1]; k += 4) {
+    const int total = n[0] + n[1];
+    auto part = [&](int k, const float *&po, const float2 *&pml) {
         const int x = k >= n[0], j = k - (x ? n[0] : 0);
+        const bool block = rows[x] != kRowsA;
+        const size_t r = (size_t)(w0[x] + j) * rows[x] + at[x];
+        po = j == 0 ? parts.o[x] + base * hd : (block ? parts.o_b : parts.o_a) + r * hd;
+        pml = j == 0 ? parts.ml[x] + base : (block ? parts.ml_b : parts.ml_a) + r;
+    };
+    // lanes over dims (four each; heads beyond 256 dims in two turns), lane groups over parts
+    const int lanes = hd <= 32 ? 8 : hd <= 64 ? 16 : hd <= 128 ? 32 : 64, groups = 64 / lanes * W;
+    const int sub = (wave % W) * (64 / lanes) + lane / lanes, d0 = (lane % lanes) * 4;
+    float top = -INFINITY;
+    bool broken = false;
+    for (int k = lane; k < total; k += 64) {  // the largest m of parts that saw something
         const float *po;
-        float2 ml;
-        if (j == 0) {
-            po = parts.o[x] + base * hd;
-            ml = parts.ml[x][base];
-        } else {
-            const size_t r = (size_t)(w0[x] + j) * (blk[x] ? kRowsB : kRowsA) + at[x];
-            po = (blk[x] ? parts.o_b : parts.o_a) + r * hd;
-            ml = (blk[x] ? parts.ml_b : parts.ml_a)[r];
+        const float2 *pml;
+        part(k, po, pml);
+        const float2 ml = *pml;
+        if (ml.y != 0.0f) top = fmaxf(top, ml.x);
+        broken |= ml.y < 0.0f;
+    }
+    float4 o[2] = {};
+    float l = 0.0f;
+#pragma unroll
+    for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+    if (__any(broken)) {
+        slow_row(a, row, ri.w, h, wave % W, W, o, top, l);
+        if constexpr (W == 4) {
+            if (lane == 0) s_m[wave] = top;
+            __syncthreads();
+            top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+            const float f = l == 0.0f ? 0.0f : exp2f(s_m[wave] - top);
+            l = l == 0.0f ? 0.0f : l * f;
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+                if (f != 0.0f) o[y] = make_float4(o[y].x * f, o[y].y * f, o[y].z * f, o[y].w * f);
         }
-        if (ml.y == 0.0f) continue;  // saw nothing
-        const float m2 = fmaxf(m, ml.x), f = m == -INFINITY ? 0.0f : exp2f(m - m2), w = exp2f(ml.x - m2);
-        l = l * f + ml.y * w;
+        // lane's dims are 4 lane ..: the layout below with all lanes over dims
+        if constexpr (W == 4) {
+            if (4 * lane < hd) *reinterpret_cast<float4 *>(&s_o[wave][4 * lane]) = o[0];
+            if (4 * lane + 256 < hd) *reinterpret_cast<float4 *>(&s_o[wave][4 * lane + 256]) = o[1];
+            if (lane == 0) s_l[wave] = l;
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e * 64 + lane < hd) o[e] = o[e] * f + po[e * 64 + lane] * w;
-        m = m2;
+            for (int y = 0; y < 2; ++y)
+                if (4 * lane + 256 * y < hd)
+                    *reinterpret_cast<float4 *>(a.out + base * hd + 4 * lane + 256 * y) =
+                        l == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(o[y].x / l, o[y].y / l, o[y].z / l, o[y].w / l);
+            return;
+        }
+    } else {
+        for (int k0 = sub; k0 < total; k0 += groups * kAhead) {
+            float4 v[kAhead][2];
+            float2 ml[kAhead];
+#pragma unroll
+            for (int e = 0; e < kAhead; ++e) {
+                const float *po;
+                const float2 *pml;
+                const int k = k0 + e * groups;
+                part(min(k, total - 1), po, pml);
+                ml[e] = k < total ? *pml : make_float2(0.0f, 0.0f);
+                v[e][0] = d0 < hd ? *reinterpret_cast<const float4 *>(po + d0) : make_float4(0, 0, 0, 0);
+                v[e][1] = d0 + 256 < hd ? *reinterpret_cast<const float4 *>(po + d0 + 256) : make_float4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < kAhead; ++e) {
+                if (ml[e].y == 0.0f) continue;  // saw nothing
+                const float w = exp2_hw(ml[e].x - top);
+                l += ml[e].y * w;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    o[x].x += v[e][x].x * w;
+                    o[x].y += v[e][x].y * w;
+                    o[x].z += v[e][x].z * w;
+                    o[x].w += v[e][x].w * w;
+                }
+            }
+        }
+        for (int x = lanes; x < 64; x <<= 1) {
+            l += __shfl_xor(l, x, 64);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                o[y].x += __shfl_xor(o[y].x, x, 64);
+                o[y].y += __shfl_xor(o[y].y, x, 64);
+                o[y].z += __shfl_xor(o[y].z, x, 64);
+                o[y].w += __shfl_xor(o[y].w, x, 64);
+            }
+        }
+        if constexpr (W == 4) {
+            if (lane < lanes) {
+                if (d0 < hd) *reinterpret_cast<float4 *>(&s_o[wave][d0]) = o[0];
+                if (d0 + 256 < hd) *reinterpret_cast<float4 *>(&s_o[wave][d0 + 256]) = o[1];
+                if (lane == 0) s_l[wave] = l;
+            }
+        } else {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const int d = d0 + 256 * y;
+                if (lane < lanes && d < hd)
+                    *reinterpret_cast<float4 *>(a.out + base * hd + d) =
+                        l == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(o[y].x / l, o[y].y / l, o[y].z / l, o[y].w / l);
+            }
+        }
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (e * 64 + lane < hd) s_o[wave][e * 64 + lane] = o[e];
-    if (lane == 0) {
-        s_m[wave] = m;
-        s_l[wave] = l;
-    }
-    __syncthreads();
-    const float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    float f[4], sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        f[w] = s_l[w] == 0.0f ? 0.0f : exp2f(s_m[w] - top);
-        sum += s_l[w] == 0.0f ? 0.0f : s_l[w] * f[w];
-    }
-    for (int d = tid; d < hd; d += 256) {
-        float x = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) x += f[w] == 0.0f ? 0.0f : s_o[w][d] * f[w];
-        a.out[base * hd + d] = sum == 0.0f ? 0.0f : x / sum;
+    if constexpr (W == 4) {
+        __syncthreads();
+        const float sum = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+        for (int d = tid; d < hd; d += 256) {
+            const float x = (s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d]);
+            a.out[base * hd + d] = sum == 0.0f ? 0.0f : x / sum;
+        }
     }
 }
 
-bool has_blocks(const PagedAttn &a) { return a.k_fmt == 0 && a.v_fmt == 0; }
+int padded_dim(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : head_dim <= 256 ? 256 : 512; }
 
 Parts layout(const PagedAttn &a, uint8_t *base, size_t &bytes)
 {
@@ -1271,46 +1431,51 @@ Parts layout(const PagedAttn &a, uint8_t *base, size_t &bytes)
         at += align_up(n, 256);
         return x;
     };
-    p.wgs = 256;
+    const bool quant = a.k_fmt != 0 || a.v_fmt != 0;
+    const int dp = padded_dim(a.head_dim);
+    p.wgs = 256;  // one a CU: they hold most of its registers or LDS
+    p.waves = waves_of(dp, quant);
+    p.rows_b = quant ? 0 : rows_b(dp);
     const size_t heads = (size_t)a.max_rows * a.n_heads, hd = a.head_dim;
     const size_t group_rows = (size_t)a.max_rows * a.group;
-    // stream items: the rows of every request and of the prefix in tiles of 16; block items: tiles of 128 of
+    // stream items: the rows of every request and of the prefix in tiles of 16; block items: tiles of rows_b of
     // groups of more than kFewRows
     const size_t seqs = std::min<size_t>(a.n_seqs, a.max_rows);
     const size_t items_a = (group_rows / kRowsA + seqs + group_rows / kRowsA + 1) * a.n_kv_heads;
-    const size_t items_b = has_blocks(a) ? (2 * (group_rows / kRowsB + 1) + std::min(seqs, group_rows / kFewRows)) * a.n_kv_heads : 0;
+    const size_t items_b =
+        p.rows_b ? (2 * (group_rows / p.rows_b + 1) + std::min(seqs, group_rows / kFewRows)) * a.n_kv_heads : 0;
     p.items_a = (int)items_a;
     for (int k = 0; k < 2; ++k) {
         const bool used = k == 1 || a.prefix_len > 0;
         p.o[k] = reinterpret_cast<float *>(take(used ? heads * hd * 4 : 0));
         p.ml[k] = reinterpret_cast<float2 *>(take(used ? heads * 8 : 0));
     }
-    p.o_a = reinterpret_cast<float *>(take((size_t)p.wgs * 4 * kRowsA * hd * 4));
-    p.ml_a = reinterpret_cast<float2 *>(take((size_t)p.wgs * 4 * kRowsA * 8));
-    const size_t rows_b = has_blocks(a) ? (size_t)p.wgs * kRowsB : 0;
-    p.o_b = reinterpret_cast<float *>(take(rows_b * hd * 4));
-    p.ml_b = reinterpret_cast<float2 *>(take(rows_b * 8));
+    const size_t workers = (size_t)p.wgs * p.waves, wg_rows = (size_t)p.wgs * p.rows_b;
+    p.o_a = reinterpret_cast<float *>(take(workers * kRowsA * hd * 4));
+    p.ml_a = reinterpret_cast<float2 *>(take(workers * kRowsA * 8));
+    p.o_b = reinterpret_cast<float *>(take(wg_rows * hd * 4));
+    p.ml_b = reinterpret_cast<float2 *>(take(wg_rows * 8));
     p.first = reinterpret_cast<int32_t *>(take((items_a + items_b) * 4));
     p.last = reinterpret_cast<int32_t *>(take((items_a + items_b) * 4));
-    p.row_item = reinterpret_cast<int2 *>(take((size_t)a.max_rows * 8));
+    p.row_item = reinterpret_cast<int4 *>(take((size_t)a.max_rows * 16));
     p.head = reinterpret_cast<int32_t *>(take(16));
     bytes = at;
     return p;
 }
 
-template <int DP, int R>
+template <int DP>
 void launch_dp(mrml_hip_ctx *ctx, const PagedAttn &a, const Parts &p)
 {
-    const dim3 grid(p.wgs), block(kScanT);
+    const dim3 grid(p.wgs), block(64 * p.waves);
     const bool kq = a.k_fmt != 0, vq = a.v_fmt != 0;
     if (!kq && !vq)
-        hipLaunchKernelGGL((paged_attn_kernel<DP, false, false, R>), grid, block, 0, ctx->stream, a, p);
+        hipLaunchKernelGGL((paged_attn_kernel<DP, false, false>), grid, block, 0, ctx->stream, a, p);
     else if (!kq)
-        hipLaunchKernelGGL((paged_attn_kernel<DP, false, true, 0>), grid, block, 0, ctx->stream, a, p);
+        hipLaunchKernelGGL((paged_attn_kernel<DP, false, true>), grid, block, 0, ctx->stream, a, p);
     else if (!vq)
-        hipLaunchKernelGGL((paged_attn_kernel<DP, true, false, 0>), grid, block, 0, ctx->stream, a, p);
+        hipLaunchKernelGGL((paged_attn_kernel<DP, true, false>), grid, block, 0, ctx->stream, a, p);
     else
-        hipLaunchKernelGGL((paged_attn_kernel<DP, true, true, 0>), grid, block, 0, ctx->stream, a, p);
+        hipLaunchKernelGGL((paged_attn_kernel<DP, true, true>), grid, block, 0, ctx->stream, a, p);
 }
 
 }  // namespace
@@ -1326,16 +1491,18 @@ int launch_paged_attn(mrml_hip_ctx *ctx, const PagedAttn &a, void *scratch)
 {
     size_t bytes;
     const Parts p = layout(a, reinterpret_cast<uint8_t *>(scratch), bytes);
-    if (a.head_dim <= 64)
-        launch_dp<64, 2>(ctx, a, p);
-    else if (a.head_dim <= 128)
-        launch_dp<128, 2>(ctx, a, p);
-    else if (a.head_dim <= 256)
-        launch_dp<256, 2>(ctx, a, p);
-    else
-        launch_dp<512, 1>(ctx, a, p);
+    switch (padded_dim(a.head_dim)) {
+    case 64: launch_dp<64>(ctx, a, p); break;
+    case 128: launch_dp<128>(ctx, a, p); break;
+    case 256: launch_dp<256>(ctx, a, p); break;
+    default: launch_dp<512>(ctx, a, p); break;
+    }
     if (int rc = check_launch(ctx, "paged_attn_kernel")) return rc;
-    hipLaunchKernelGGL(paged_merge_kernel, dim3(a.max_rows, a.n_heads), dim3(256), 0, ctx->stream, a, p, has_blocks(a));
+    const int pairs = a.max_rows * a.n_heads;
+    if (pairs > 4096)
+        hipLaunchKernelGGL(paged_merge_kernel<1>, dim3((pairs + 3) / 4), dim3(256), 0, ctx->stream, a, p);
+    else
+        hipLaunchKernelGGL(paged_merge_kernel<4>, dim3(pairs), dim3(256), 0, ctx->stream, a, p);
     return check_launch(ctx, "paged_merge_kernel");
 }
 
