@@ -42,10 +42,11 @@ constexpr float kSlack = 1.5f;    // the maximum may grow by this much before o 
 constexpr float kBroken = -1.0f;  // in place of l: the part is not finite
 constexpr int kRowsA = 16, kUnitA = 32;  // rows and positions of a stream item's tile (one wave)
 constexpr int kFewRows = 32;             // groups of at most so many rows are stream items
-constexpr int kMaxT = 512;               // threads of a workgroup at most
-// Relative cost of a unit on one workgroup, for the split of the workgroups:
-// a block unit keeps the MFMA of all waves busy, a stream unit's waves run side by side.
-constexpr int kCostA = 1, kCostB = 8;
+// Costs, for the split of the work, in stream units of one wave (about 3.5 us each): what
+// a stream item costs beside its units (q, the first K and V, the part's store: a
+// chain of round trips), and a block unit per 32 rows of it and wave.
+constexpr int kItemCost = 3;
+constexpr float kBlockCost = 0.28f;
 
 // Waves of a workgroup, rows of a block item and positions of its tile by padded head size: two waves a SIMD
 // while a wave's q and o fit 256 registers.
@@ -86,10 +87,11 @@ struct Dest {
     bool own;
 };
 
-struct Scan {  // sums over the requests before each thread's share, in LDS
-    int ua[kMaxT + 1], ub[kMaxT + 1];  // units
-    int ia[kMaxT + 1], ib[kMaxT + 1];  // items
-    int rs[kMaxT + 1], len[kMaxT];     // first row; length of the share's first request
+template <int T>
+struct Scan {  // sums over the requests before each of T threads' share, in LDS
+    int ua[T + 1], ub[T + 1];  // units
+    int ia[T + 1], ib[T + 1];  // items
+    int rs[T + 1], len[T];     // first row; length of the share's first request
     int sum[8][4], low[8], flags[8];
     float size[8];
 };
@@ -170,7 +172,8 @@ __device__ __forceinline__ int clamp_len(const PagedAttn &a, int len)
     return min(max(len, 0), a.table_stride * a.map.page_size);
 }
 
-__device__ __forceinline__ Request request_at(const PagedAttn &a, const Scan &s, int r)
+template <int T>
+__device__ __forceinline__ Request request_at(const PagedAttn &a, const Scan<T> &s, int r)
 {
     if (share(a) == 1) return Request{s.rs[r], s.rs[r + 1] - s.rs[r], s.len[r]};
     const int rs = a.row_start[r];
@@ -201,7 +204,7 @@ __device__ __forceinline__ int own_units_b(const PagedAttn &a, const Request &q,
     return units_of(lo, hi, unit);
 }
 
-// {stream units, block units, stream items, block items} of a request; returns the units as a float, which cannot
+// {stream units with the items' own cost, block units, stream items, block items} of a request; returns the units as a float, which cannot
 // overflow.
 __device__ __forceinline__ float request_work(const PagedAttn &a, const Request &q, int rows, int unit, int w[4])
 {
@@ -210,8 +213,8 @@ __device__ __forceinline__ float request_work(const PagedAttn &a, const Request 
     const int m = q.n * a.group;
     if (!rows || m <= kFewRows) {
         w[2] = (m + kRowsA - 1) / kRowsA * a.n_kv_heads;
-        w[0] = w[2] * own_units_a(a, q);
-        return (float)w[2] * (float)own_units_a(a, q);
+        w[0] = w[2] * (own_units_a(a, q) + kItemCost);
+        return (float)w[2] * (float)(own_units_a(a, q) + kItemCost);
     } else {
         const int nb = (m + rows - 1) / rows;
         float size = 0.0f;
@@ -235,7 +238,7 @@ struct Totals {
 };
 
 template <int T>
-__device__ Totals scan_requests(const PagedAttn &a, Scan &s, int rows, int unit)
+__device__ Totals scan_requests(const PagedAttn &a, Scan<T> &s, int rows, int unit)
 {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int per = share(a), r0 = tid * per, r1 = min(r0 + per, a.n_seqs);
@@ -323,7 +326,8 @@ __device__ __forceinline__ int share_of(const int *from, int x)
 }
 
 // The request of a row (the last one that starts at or before it and has rows).
-__device__ __forceinline__ int request_of(const PagedAttn &a, const Scan &s, int row)
+template <int T>
+__device__ __forceinline__ int request_of(const PagedAttn &a, const Scan<T> &s, int row)
 {
     const int per = share(a);
     int r = share_of(s.rs, row) * per;
@@ -340,7 +344,8 @@ __device__ __forceinline__ size_t part_row(const PagedAttn &a, const Piece &pc, 
 }
 
 // What row mi of a piece's group sees, in the source's positions: [vlo, vhi).
-__device__ __forceinline__ void row_sees(const PagedAttn &a, const Scan &s, bool need_at, const Piece &pc, int mi, int &vlo, int &vhi)
+template <int T>
+__device__ __forceinline__ void row_sees(const PagedAttn &a, const Scan<T> &s, bool need_at, const Piece &pc, int mi, int &vlo, int &vhi)
 {
     vlo = 0;
     vhi = INT32_MAX;
@@ -467,6 +472,38 @@ __device__ __forceinline__ bool softmax_step(float *x, float &m, float &l, float
 // sides through LDS once.  Quantised V enters as f16 terms too: d * q has at most
 // 19 bits, hi = its rounding, lo = fma(d, q, -hi), both exact.
 
+// K of 16 positions in LDS, as 1 KB chunks (what one global_load_lds of a wave
+// writes) 1040 bytes apart.  A chunk holds 64 / P whole rows of P 16-byte pieces;
+// position p lies in chunk p % (P / 4), so that the eight lanes that read
+// together, of eight consecutive positions, meet eight different bank groups, where
+// rows share a chunk by exchanging the pieces of every other one.  A lane's
+// address is then a base plus a constant, one base for even and one for odd steps.
+constexpr int kChunk = 1040;
+
+template <int P>
+struct KTile {
+    static constexpr int kRows = 64 / P, kChunks = 16 / kRows;  // rows a chunk, chunks of 16 positions
+    static constexpr int kBytes16 = kChunks * kChunk;
+    __device__ static __forceinline__ int flip(int sub) { return P == 16 ? (sub & 1) * 4 : P == 8 ? (sub & 3) * 2 : 0; }
+    // chunk c's lane: the position (of its 16) and the piece that it loads
+    __device__ static __forceinline__ int position(int c, int lane) { return c % kChunks + lane / P * kChunks; }
+    __device__ static __forceinline__ int piece(int lane) { return (lane % P) ^ flip(lane / P); }
+    // byte offset of piece 4 s + g of position i, less 64 (s & ~1)
+    __device__ static __forceinline__ int offset(int i, int g, int odd)
+    {
+        const int sub = i / kChunks;
+        return i % kChunks * kChunk + sub * P * 16 + ((4 * odd + g) ^ flip(sub)) * 16;
+    }
+};
+
+__device__ __forceinline__ half8 read16(const uint8_t *p) { return __builtin_bit_cast(half8, *reinterpret_cast<const uint4 *>(p)); }
+
+__device__ __forceinline__ void load_to_lds(const uint8_t *src, uint8_t *dst)
+{
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)src,
+                                     (__attribute__((address_space(3))) uint32_t *)dst, 16, 0, 0);
+}
+
 struct __attribute__((packed, aligned(2))) Bytes8 {
     uint32_t a, b;
 };
@@ -476,7 +513,7 @@ constexpr int kTrRow = 36;  // floats a query row of the score tile in LDS
 template <int DP, bool KQ>
 struct WaveLds {
     int place[32];
-    uint4 k[DP * 4];  // 32 positions, as BlockLds::k
+    alignas(16) uint8_t k[2 * KTile<DP / 8>::kBytes16];  // 32 positions
 };
 template <int DP>
 struct WaveLds<DP, true> {
@@ -528,7 +565,7 @@ __device__ __forceinline__ void load_quant_q(const PagedAttn &a, const float *ro
 }
 
 template <int DP, bool KQ, bool VQ>
-__device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan &sc, bool need_at, const Piece &pc,
+__device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * waves_of(DP, KQ || VQ)> &sc, bool need_at, const Piece &pc,
                                             WaveLds<DP, KQ> &lds, const Dest &to)
 {
     constexpr int KS = DP / 32, NG = DP < 128 ? 1 : DP / 128;
@@ -558,6 +595,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan &sc, 
         for (int d = 0; d < 8; ++d) o[n][d] = float4v{0, 0, 0, 0};
 
     // A tile's page ids are loaded two tiles ahead and looked at one tile ahead, when they are long there.
+    const int kbase[2] = {KTile<DP / 8>::offset(i, g, 0), KTile<DP / 8>::offset(i, g, 1)};
     auto page_ids = [&](int t0) { return t0 + (lane & 31) < pc.p1 ? pc.table[page_of(a.map, t0 + (lane & 31))] : -1; };
     auto places = [&](int t0, int id) {
         const int pos = t0 + (lane & 31);
@@ -580,14 +618,13 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan &sc, 
                 }
             }
         } else {
-            constexpr int P = DP / 8, PI = 64 / P;
-            const int ln = here(lane);
+            using KT = KTile<DP / 8>;
+            const int ln = here(lane), piece = KT::piece(ln);
 #pragma unroll
-            for (int n = 0; n < 32 / PI; ++n) {
-                const int p = n * PI + ln / P, piece = (ln % P) ^ (p & 7);
-                const uint8_t *src = kv_row(a, a.k, krb, __shfl(place, p, 64), pc.kvh) + (piece * 8 < hd ? piece * 16 : 0);
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)src,
-                                                 (__attribute__((address_space(3))) uint32_t *)(lds.k + n * 64), 16, 0, 0);
+            for (int n = 0; n < 2 * KT::kChunks; ++n) {
+                const int p = n / KT::kChunks * 16 + KT::position(n, ln);
+                load_to_lds(kv_row(a, a.k, krb, __shfl(place, p, 64), pc.kvh) + (piece * 8 < hd ? piece * 16 : 0),
+                            lds.k + n * kChunk);
             }
         }
     };
@@ -662,15 +699,27 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan &sc, 
             __builtin_amdgcn_s_waitcnt(0x0f70 | (kLeft & 15) | (kLeft >> 4) << 14);
             pin();
             float4v acc[2][2] = {};
+            half8 kk[2][2][2];  // the next two steps' pieces are on their way while two steps' products run
+            auto read_k = [&](int s0) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
+                for (int e = 0; e < 2; ++e)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int p = 16 * h + i;
-                    const half8 kk = __builtin_bit_cast(half8, lds.k[p * (DP / 8) + ((4 * s + g) ^ (p & 7))]);
-                    acc[h][0] = mfma(kk, qh[s], acc[h][0]);
-                    acc[h][1] = mfma(kk, ql[s], acc[h][1]);
-                }
+                    for (int h = 0; h < 2; ++h)
+                        kk[(s0 / 2) & 1][e][h] = read16(lds.k + kbase[e] + h * KTile<DP / 8>::kBytes16 + 64 * s0);
+            };
+            read_k(0);
+#pragma unroll
+            for (int s = 0; s < KS; s += 2) {
+                if (s + 2 < KS) read_k(s + 2);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        acc[h][0] = mfma(kk[(s / 2) & 1][e][h], qh[s + e], acc[h][0]);
+                        acc[h][1] = mfma(kk[(s / 2) & 1][e][h], ql[s + e], acc[h][1]);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -791,37 +840,27 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan &sc, 
 
 // ---- block items: a workgroup, many query rows, K and V through LDS -----------------
 //
-// Tiles of T = 16384 / DP positions, two in LDS (128 KB): while the waves work on
-// one, the next is under way.  K goes to LDS directly (global_load_lds), 16-byte
-// pieces of a row exchanged by the position's low bits so that a wave's reads of
-// 16 positions meet no bank twice; V is transposed on its way, as in a
-// stream item, by the thread that has loaded 8 positions of some dims, and written as
-// 16-byte runs of 8 positions, exchanged by the dim's low bits.  A wave holds 16 * R
-// rows; each piece read from LDS feeds 2 * R products.
-
-// Where a run of 8 positions of a dim lies in a tile of T positions, in 16-byte pieces.
-template <int T>
-__device__ __forceinline__ int v_piece(int dim, int run)
-{
-    if constexpr (T >= 64)
-        return dim * (T / 8) + (run ^ (dim & 7) ^ ((dim >> 3) & 7));
-    else
-        return dim * (T / 8) + (run ^ ((dim >> 1) & 3) ^ ((dim >> 3) & 3));
-}
+// Tiles of T = 16384 / DP positions, two in LDS (137 KB with padding): while the waves
+// work on one, the next is under way.  K goes to LDS directly (global_load_lds, as in
+// a stream item); V is transposed on its way by the thread that has loaded 8
+// positions of some dims, and written as 16-byte runs of 8 positions, rows of a dim 16
+// bytes longer than the tile.  A wave holds 16 * R rows; each piece read from LDS feeds
+// 2 * R products.
 
 template <int DP>
 struct BlockLds {
-    static constexpr int T = unit_b(DP);
-    uint4 k[2][2048], v[2][2048];
+    static constexpr int T = unit_b(DP), kPitch = 2 * T + 16;  // bytes of a dim's row
+    alignas(16) uint8_t k[2][T / 16 * KTile<DP / 8>::kBytes16];
+    alignas(16) uint8_t v[2][DP * kPitch];
     int place[3][T];
 };
 
 template <int DP>
-__device__ __forceinline__ void block_item(const PagedAttn &a, const Scan &sc, bool need_at, const Piece &pc,
+__device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * waves_of(DP, false)> &sc, bool need_at, const Piece &pc,
                                            BlockLds<DP> &lds, const Dest &to)
 {
     constexpr int NW = waves_of(DP, false), R = tiles_of(DP), KS = DP / 32, NF = DP / 16, T = unit_b(DP);
-    constexpr int SP = T < 64 ? T : 64, NH = SP / 16, P = DP / 8;
+    constexpr int SP = T < 64 || DP == 128 ? 32 : 64, NH = SP / 16, P = DP / 8;
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4, hd = a.head_dim;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rb = hd * 2;
@@ -839,22 +878,22 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan &sc, b
             lds.place[tile % 3][tid] = place;
         }
     };
+    using KT = KTile<P>;
     auto load_k = [&](int tile) {
-        constexpr int PW = T / NW, PI = 64 / P;  // positions of a wave's share, of an instruction
-        const int ln = here(lane);
+        constexpr int N = T / 16 * KT::kChunks / NW;  // chunks a wave
+        const int ln = here(lane), piece = KT::piece(ln);
 #pragma unroll
-        for (int n = 0; n < PW / PI; ++n) {
-            const int p = wave * PW + n * PI + ln / P, piece = (ln % P) ^ (p & 7);
-            const uint8_t *src = kv_row(a, a.k, rb, lds.place[tile % 3][p], pc.kvh) + (piece * 8 < hd ? piece * 16 : 0);
-            uint4 *dst = &lds.k[tile & 1][(wave * PW + n * PI) * P];
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)src,
-                                             (__attribute__((address_space(3))) uint32_t *)dst, 16, 0, 0);
+        for (int n = 0; n < N; ++n) {
+            const int c = wave * N + n, p = c / KT::kChunks * 16 + KT::position(c, ln);
+            load_to_lds(kv_row(a, a.k, rb, lds.place[tile % 3][p], pc.kvh) + (piece * 8 < hd ? piece * 16 : 0),
+                        lds.k[tile & 1] + c * kChunk);
         }
     };
-    // this thread's dims (VD of them) and run of positions: run0 + 0..3 and run0 + 16..19
-    constexpr int VD = 32 / NW, VT = DP / VD;
+    // this thread's dims (VD of them) and run of positions (run0 + 0..3 and run0 + 16..19): four runs of a
+    // dim by neighbouring lanes, whose writes then meet no bank twice, and 16 lanes along a row
+    constexpr int VD = 32 / NW, VT = DP / VD, kPitch = BlockLds<DP>::kPitch;
     static_assert(VT * (T / 8) == 64 * NW, "one task a thread");
-    const int dl = tid % VT, run = tid / VT, run0 = (run >> 2) * 32 + (run & 3) * 4;
+    const int dl = (tid >> 2) % VT, run = (tid & 3) + tid / (4 * VT) * 4, run0 = (run >> 2) * 32 + (run & 3) * 4;
     uint32_t v[8][VD / 2];
     auto load_v = [&](int tile) {
 #pragma unroll
@@ -882,7 +921,7 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan &sc, b
             uint32_t t[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) t[e] = __builtin_amdgcn_perm(v[2 * e + 1][d >> 1], v[2 * e][d >> 1], sel);
-            lds.v[tile & 1][v_piece<T>(VD * dl + d, run)] = make_uint4(t[0], t[1], t[2], t[3]);
+            *reinterpret_cast<uint4 *>(lds.v[tile & 1] + (VD * dl + d) * kPitch + run * 16) = make_uint4(t[0], t[1], t[2], t[3]);
         }
     };
 
@@ -896,6 +935,7 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan &sc, b
         load_v(0);
     }
 
+    const int kbase[2] = {KT::offset(i, g, 0), KT::offset(i, g, 1)}, vbase = i * kPitch + g * 16;
     const bool busy = pc.row0 + wave * R * 16 < pc.rows;  // the wave has rows
     half8 qh[R][KS], ql[R][KS];
     float c[R], m[R], l[R];
@@ -925,7 +965,7 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan &sc, b
             load_k(tile + 1);
             load_v(tile + 1);
         }
-        const uint4 *kt = lds.k[tile & 1], *vt = lds.v[tile & 1];
+        const uint8_t *kt = lds.k[tile & 1], *vt = lds.v[tile & 1] + vbase;
 #pragma unroll 1
         for (int s0 = 0; s0 < T; s0 += SP) {
             const int t0 = pc.p0 + tile * T + s0;
@@ -935,17 +975,32 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan &sc, b
             for (int u = 0; u < R; ++u)
 #pragma unroll
                 for (int h = 0; h < NH; ++h) acc[u][h] = float4v{0, 0, 0, 0};
+            // the next step's pieces are on their way from LDS while a step's products run
+            constexpr int KG = 2, KN = KS * NH;  // pieces a step, pieces in all: (s, h) = (n / NH, n % NH)
+            half8 kk[2][KG];
+            auto read_k = [&](int n0) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-#pragma unroll
-                for (int h = 0; h < NH; ++h) {
-                    const int p = s0 + 16 * h + i;
-                    const half8 kk = __builtin_bit_cast(half8, kt[p * P + ((4 * s + g) ^ (p & 7))]);
-#pragma unroll
-                    for (int u = 0; u < R; ++u) acc[u][h] = mfma(kk, qh[u][s], acc[u][h]);
-#pragma unroll
-                    for (int u = 0; u < R; ++u) acc[u][h] = mfma(kk, ql[u][s], acc[u][h]);
+                for (int e = 0; e < KG; ++e) {
+                    const int s = (n0 + e) / NH, h = (n0 + e) % NH;
+                    kk[(n0 / KG) & 1][e] = read16(kt + kbase[s & 1] + (s0 / 16 + h) * KT::kBytes16 + 64 * (s & ~1));
                 }
+            };
+            read_k(0);
+#pragma unroll
+            for (int n = 0; n < KN; n += KG) {
+                if (n + KG < KN) read_k(n + KG);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < R; ++u)
+#pragma unroll
+                    for (int e = 0; e < KG; ++e)
+                        acc[u][(n + e) % NH] = mfma(kk[(n / KG) & 1][e], qh[u][(n + e) / NH], acc[u][(n + e) % NH]);
+#pragma unroll
+                for (int u = 0; u < R; ++u)
+#pragma unroll
+                    for (int e = 0; e < KG; ++e)
+                        acc[u][(n + e) % NH] = mfma(kk[(n / KG) & 1][e], ql[u][(n + e) / NH], acc[u][(n + e) % NH]);
+                __builtin_amdgcn_sched_barrier(0);
             }
             const uint64_t there = __ballot(lane < SP && lds.place[tile % 3][s0 + (lane & (SP - 1))] >= 0);
             const bool edge = t0 < full_lo || t0 + SP > full_hi || there != (SP == 64 ? ~0ull : (1ull << (SP & 63)) - 1);
@@ -980,13 +1035,27 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan &sc, b
                     p_hi[u] = as_half8(ph[u][2 * b][0], ph[u][2 * b][1], ph[u][2 * b + 1][0], ph[u][2 * b + 1][1]);
                     p_lo[u] = as_half8(pw[u][2 * b][0], pw[u][2 * b][1], pw[u][2 * b + 1][0], pw[u][2 * b + 1][1]);
                 }
+                constexpr int VG = 2;  // pieces a step
+                half8 vv[2][VG];
+                auto read_v = [&](int f0) {
 #pragma unroll
-                for (int f = 0; f < NF; ++f) {
-                    const half8 vv = __builtin_bit_cast(half8, vt[v_piece<T>(16 * f + i, s0 / 8 + 4 * b + g)]);
+                    for (int f = 0; f < VG; ++f)
+                        vv[(f0 / VG) & 1][f] = read16(vt + (f0 + f) * 16 * kPitch + (s0 / 8 + 4 * b) * 16);
+                };
+                read_v(0);
 #pragma unroll
-                    for (int u = 0; u < R; ++u) o[u][f] = mfma(vv, p_hi[u], o[u][f]);
+                for (int f0 = 0; f0 < NF; f0 += VG) {
+                    if (f0 + VG < NF) read_v(f0 + VG);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int u = 0; u < R; ++u) o[u][f] = mfma(vv, p_lo[u], o[u][f]);
+                    for (int u = 0; u < R; ++u)
+#pragma unroll
+                        for (int f = 0; f < VG; ++f) o[u][f0 + f] = mfma(vv[(f0 / VG) & 1][f], p_hi[u], o[u][f0 + f]);
+#pragma unroll
+                    for (int u = 0; u < R; ++u)
+#pragma unroll
+                        for (int f = 0; f < VG; ++f) o[u][f0 + f] = mfma(vv[(f0 / VG) & 1][f], p_lo[u], o[u][f0 + f]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
@@ -1022,10 +1091,11 @@ struct Shared {
     int rows;           // rows x group
     bool few;           // stream items
     int lo, hi;         // positions any row sees
-    int units, items;   // units an item
+    int units, items;   // units an item, with a stream item's own cost
 };
 
-__device__ __forceinline__ Shared shared_work(const PagedAttn &a, const Scan &s, const Totals &t, int rows_b, int unit)
+template <int T>
+__device__ __forceinline__ Shared shared_work(const PagedAttn &a, const Scan<T> &s, const Totals &t, int rows_b, int unit)
 {
     Shared p;
     p.rows = uni(s.rs[blockDim.x] - s.rs[0]) * a.group;
@@ -1034,15 +1104,18 @@ __device__ __forceinline__ Shared shared_work(const PagedAttn &a, const Scan &s,
     p.lo = a.window && t.low < INT32_MAX ? min(max(a.prefix_len + t.low - a.window + 1, 0), p.hi) : 0;
     const int tile = p.few ? kRowsA : rows_b;
     p.items = a.prefix_len > 0 ? (p.rows + tile - 1) / tile * a.n_kv_heads : 0;
-    p.units = units_of(p.lo, p.hi, p.few ? kUnitA : unit);
+    p.units = units_of(p.lo, p.hi, p.few ? kUnitA : unit) + (p.few ? kItemCost : 0);
     return p;
 }
 
 // The piece at unit u of the stream or block items, at most `left` units long;
 // returns the units taken, the item's index, and whether the piece holds its
-// first and last unit.
-__device__ __forceinline__ int find_piece(const PagedAttn &a, const Scan &s, const Shared &sh, bool block, int rows_b,
-                                          int unit, int u, int left, Piece &pc, int &item, bool &is_first, bool &is_last)
+// first and last positions.  A stream item's own cost stands before its
+// first unit: a share that ends there has no piece of it (none).
+template <int T>
+__device__ __forceinline__ int find_piece(const PagedAttn &a, const Scan<T> &s, const Shared &sh, bool block, int rows_b,
+                                          int unit, int u, int left, Piece &pc, int &item, bool &is_first, bool &is_last,
+                                          bool &none)
 {
     const int tile = block ? rows_b : kRowsA, step = block ? unit : kUnitA;
     const int sh_items = sh.few != block ? sh.items : 0, sh_units = sh_items * sh.units;
@@ -1077,7 +1150,7 @@ __device__ __forceinline__ int find_piece(const PagedAttn &a, const Scan &s, con
             }
         }
         if (!block) {
-            units = own_units_a(a, q);
+            units = own_units_a(a, q) + kItemCost;
             item = u / units;
             within = u - item * units;
             blk = item / a.n_kv_heads;
@@ -1104,7 +1177,8 @@ __device__ __forceinline__ int find_piece(const PagedAttn &a, const Scan &s, con
     }
     units = uni(units);
     within = uni(within);
-    const int take = min(units - within, left);
+    const int take = min(units - within, left), cost = block ? 0 : kItemCost;
+    const int from = max(within - cost, 0), to = max(within + take - cost, 0);
     item = uni(item);
     pc.pre = uni(pc.pre);
     pc.table = pc.pre ? a.prefix : a.table + (size_t)uni(tab) * a.table_stride;
@@ -1113,16 +1187,17 @@ __device__ __forceinline__ int find_piece(const PagedAttn &a, const Scan &s, con
     pc.at0 = uni(pc.at0);
     pc.kvh = uni(pc.kvh);
     pc.row0 = uni(blk) * tile;
-    pc.p0 = uni(lo) + within * step;
-    pc.p1 = min(uni(hi), pc.p0 + take * step);
-    is_first = within == 0;
+    pc.p0 = uni(lo) + from * step;
+    pc.p1 = min(uni(hi), uni(lo) + to * step);
+    is_first = from == 0;
     is_last = within + take == units;
+    none = to == from;
     return take;
 }
 
 template <int DP, bool KQ, bool BLOCKS>
 struct KernelLds {
-    Scan scan;
+    Scan<64 * waves_of(DP, !BLOCKS)> scan;
     union {
         WaveLds<DP, KQ> wave[waves_of(DP, !BLOCKS)];
         BlockLds<DP> block;
@@ -1130,7 +1205,7 @@ struct KernelLds {
 };
 template <int DP, bool KQ>
 struct KernelLds<DP, KQ, false> {
-    Scan scan;
+    Scan<64 * waves_of(DP, true)> scan;
     WaveLds<DP, KQ> wave[waves_of(DP, true)];
 };
 
@@ -1142,7 +1217,7 @@ __global__ __launch_bounds__(64 * waves_of(DP, KQ || VQ)) void paged_attn_kernel
     constexpr int kWaves = waves_of(DP, KQ || VQ), T = 64 * kWaves;
     constexpr int kUnitB = unit_b(DP), kRowsB = kBlocks ? rows_b(DP) : 0;
     __shared__ KernelLds<DP, KQ, kBlocks> lds;
-    const Scan &s = lds.scan;
+    const Scan<T> &s = lds.scan;
     const int wg = blockIdx.x, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Totals totals = scan_requests<T>(a, lds.scan, kRowsB, kUnitB);
     Shared sh{};
@@ -1180,18 +1255,18 @@ __global__ __launch_bounds__(64 * waves_of(DP, KQ || VQ)) void paged_attn_kernel
     if (kBlocks && ub > 0) {
         wb = parts.wgs;
         if (ua > 0) {
-            const float fb = (float)ub * kCostB, fa = (float)ua * kCostA;
+            const float fb = (float)ub * (kBlockCost * kWaves * kRowsB / 32), fa = (float)ua;
             wb = min(max((int)(parts.wgs * fb / (fa + fb) + 0.5f), 1), parts.wgs - 1);
         }
     }
     Piece pc;
     int item;
-    bool first, last;
+    bool first, last, none;
     if constexpr (kBlocks) {
         if (wg < wb) {
             const int quota = (ub + wb - 1) / wb, end = min(ub, (wg + 1) * quota);
             for (int u = wg * quota; u < end;) {
-                u += find_piece(a, s, sh, true, kRowsB, kUnitB, u, end - u, pc, item, first, last);
+                u += find_piece(a, s, sh, true, kRowsB, kUnitB, u, end - u, pc, item, first, last, none);
                 const size_t row = (size_t)wg * kRowsB;
                 const Dest to = first ? Dest{parts.o[!pc.pre], parts.ml[!pc.pre], true}
                                       : Dest{parts.o_b + row * a.head_dim, parts.ml_b + row, false};
@@ -1205,7 +1280,8 @@ __global__ __launch_bounds__(64 * waves_of(DP, KQ || VQ)) void paged_attn_kernel
     const int worker = (wg - wb) + (parts.wgs - wb) * wave, workers = (parts.wgs - wb) * kWaves;
     const int quota = (ua + workers - 1) / workers, end = min(ua, (worker + 1) * quota);
     for (int u = worker * quota; u < end;) {
-        u += find_piece(a, s, sh, false, kRowsB, kUnitB, u, end - u, pc, item, first, last);
+        u += find_piece(a, s, sh, false, kRowsB, kUnitB, u, end - u, pc, item, first, last, none);
+        if (none) continue;
         const size_t row = (size_t)worker * kRowsA;
         const Dest to = first ? Dest{parts.o[!pc.pre], parts.ml[!pc.pre], true}
                               : Dest{parts.o_a + row * a.head_dim, parts.ml_a + row, false};
@@ -1220,55 +1296,46 @@ __global__ __launch_bounds__(64 * waves_of(DP, KQ || VQ)) void paged_attn_kernel
 // The f16 terms of p and q turn an infinite value into NaN, and a weight of 0
 // times an infinity that its row does not see is one too.  So a row with a part
 // that is not finite is formed again here, one position after the other in f32
-// (`waves` waves taking turns); a program whose values are finite never gets here.
-__device__ __noinline__ void slow_row(const PagedAttn a, int row, int r, int h, int wave, int waves, float4 o[2],
-                                      float &m, float &l)
+// (`waves` waves taking turns, q and o in LDS); a program whose values are finite never gets here.
+__device__ __forceinline__ void slow_row(const PagedAttn &a, int row, int r, int h, int wave, int waves, float *s_q,
+                                         float *s_o, float &m, float &l)
 {
-    constexpr int E = 8;  // values a lane: dims 4 lane .. and 256 + 4 lane ..
     const int lane = threadIdx.x & 63, hd = a.head_dim, kvh = h / a.group;
     const int len = clamp_len(a, a.lens[r]), at = a.prefix_len + len - (a.row_start[r + 1] - row);
     const int first = a.window ? max(0, at - a.window + 1) : 0;
     const int krb = kv_row_bytes(a.k_fmt, hd), vrb = kv_row_bytes(a.v_fmt, hd);
-    float q[E], x[E] = {};
-    int dim[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        dim[e] = (e >> 2) * 256 + 4 * lane + (e & 3);
-        q[e] = dim[e] < hd ? a.q[(size_t)row * a.q_stride + (size_t)h * hd + dim[e]] : 0.0f;
-    }
-    if (a.k_fmt != 0) {
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-            uint32_t db;
-            int sum;
-            const uint32_t w = q8_0_block8x4(make_float4(q[4 * y], q[4 * y + 1], q[4 * y + 2], q[4 * y + 3]), db, sum);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) q[4 * y + e] = (float)(int8_t)(w >> (8 * e)) * f16_bits_to_f32(db);
+#pragma unroll 1
+    for (int d0 = 0; d0 < hd; d0 += 64) {
+        const int d = d0 + lane;
+        const float x = d < hd ? a.q[(size_t)row * a.q_stride + (size_t)h * hd + d] : 0.0f;
+        uint32_t db;
+        int sum;
+        const float q8 = (float)q8_0_block32(x, db, sum) * f16_bits_to_f32(db);  // blocks of 32 dims, a half wave each
+        if (d < hd) {
+            s_q[d] = a.k_fmt == 0 ? x : q8;
+            s_o[d] = 0.0f;
         }
     }
     m = -INFINITY;
     l = 0.0f;
+#pragma unroll 1
     for (int t = first + wave; t <= at; t += waves) {
         const bool pre = t < a.prefix_len;
         const int place = pre ? place_at(a, a.prefix, t) : place_at(a, a.table + (size_t)r * a.table_stride, t - a.prefix_len);
         if (place < 0) continue;
         const uint8_t *kr = kv_row(a, a.k, krb, place, kvh), *vr = kv_row(a, a.v, vrb, place, kvh);
         float s = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (dim[e] < hd) s = fmaf(q[e], kv_value(kr, a.k_fmt, dim[e]), s);
+#pragma unroll 1
+        for (int d = lane; d < hd; d += 64) s = fmaf(s_q[d], kv_value(kr, a.k_fmt, d), s);
         for (int y = 32; y; y >>= 1) s += __shfl_xor(s, y, 64);
         s *= a.scale * kLog2e;
         if (s == -INFINITY) continue;  // no weight
         const float m2 = fmaxf(m, s), f = exp2f(m - m2), w = exp2f(s - m2);
         l = l * f + w;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (dim[e] < hd) x[e] = x[e] * f + w * kv_value(vr, a.v_fmt, dim[e]);
+#pragma unroll 1
+        for (int d = lane; d < hd; d += 64) s_o[d] = s_o[d] * f + w * kv_value(vr, a.v_fmt, d);
         m = m2;
     }
-    o[0] = make_float4(x[0], x[1], x[2], x[3]);
-    o[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
 
 // Joins the parts of each row and head.  W waves share a row and head (1 where
@@ -1279,7 +1346,7 @@ template <int W>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a, Parts parts)
 {
     constexpr int kAhead = 4;
-    __shared__ float s_o[4][512], s_l[4], s_m[4];
+    __shared__ float s_o[4][512], s_q[4][512], s_l[4], s_m[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), hd = a.head_dim;
     const int pair = blockIdx.x * (4 / W) + wave / W, row = pair / a.n_heads, h = pair - row * a.n_heads;
     if (row >= a.max_rows) return;  // W == 1: the last workgroup's spare waves (no barrier there)
@@ -1332,28 +1399,16 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a, Parts par
 #pragma unroll
     for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
     if (__any(broken)) {
-        slow_row(a, row, ri.w, h, wave % W, W, o, top, l);
+        slow_row(a, row, ri.w, h, wave % W, W, s_q[wave], s_o[wave], top, l);
         if constexpr (W == 4) {
             if (lane == 0) s_m[wave] = top;
             __syncthreads();
-            top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-            const float f = l == 0.0f ? 0.0f : exp2f(s_m[wave] - top);
-            l = l == 0.0f ? 0.0f : l * f;
-#pragma unroll
-            for (int y = 0; y < 2; ++y)
-                if (f != 0.0f) o[y] = make_float4(o[y].x * f, o[y].y * f, o[y].z * f, o[y].w * f);
-        }
-        // lane's dims are 4 lane ..: the layout below with all lanes over dims
-        if constexpr (W == 4) {
-            if (4 * lane < hd) *reinterpret_cast<float4 *>(&s_o[wave][4 * lane]) = o[0];
-            if (4 * lane + 256 < hd) *reinterpret_cast<float4 *>(&s_o[wave][4 * lane + 256]) = o[1];
-            if (lane == 0) s_l[wave] = l;
+            const float most = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+            const float f = l == 0.0f ? 0.0f : exp2f(top - most);
+            for (int d = lane; d < hd; d += 64) s_o[wave][d] = f == 0.0f ? 0.0f : s_o[wave][d] * f;
+            if (lane == 0) s_l[wave] = f == 0.0f ? 0.0f : l * f;
         } else {
-#pragma unroll
-            for (int y = 0; y < 2; ++y)
-                if (4 * lane + 256 * y < hd)
-                    *reinterpret_cast<float4 *>(a.out + base * hd + 4 * lane + 256 * y) =
-                        l == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(o[y].x / l, o[y].y / l, o[y].z / l, o[y].w / l);
+            for (int d = lane; d < hd; d += 64) a.out[base * hd + d] = l == 0.0f ? 0.0f : s_o[wave][d] / l;
             return;
         }
     } else {
