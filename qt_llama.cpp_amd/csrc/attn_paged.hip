@@ -24,6 +24,7 @@
 // lane % 16), so row statistics need no exchange beyond the row maximum.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.h"
 
@@ -153,10 +154,20 @@ __device__ __forceinline__ int place_at(const PagedAttn &a, const int32_t *table
     return place_of(a.map, pos, pg, table[pg]);
 }
 
-__device__ __forceinline__ const uint8_t *kv_row(const PagedAttn &a, const uint8_t *cache, int row_bytes, int place,
-                                                 int kvh)
+// The rows of one kv head in a cache: place p's at base + p * stride.
+struct HeadRows {
+    const uint8_t *base;
+    uint32_t stride;
+    __device__ __forceinline__ const uint8_t *row(int place) const
+    {
+        return base + (uint64_t)(uint32_t)max(place, 0) * stride;  // none: the first, which is there
+    }
+};
+
+__device__ __forceinline__ HeadRows head_rows(const PagedAttn &a, const uint8_t *cache, int fmt, int kvh)
 {
-    return cache + ((size_t)(uint32_t)max(place, 0) * a.n_kv_heads + kvh) * row_bytes;
+    const int bytes = kv_row_bytes(fmt, a.head_dim);
+    return HeadRows{cache + (size_t)kvh * bytes, (uint32_t)(a.n_kv_heads * bytes)};
 }
 
 // ---- the requests' shares of the work --------------------------------------------
@@ -370,7 +381,10 @@ __device__ __forceinline__ int wave_max(int v)
 }
 __device__ __forceinline__ int wave_min(int v) { return -wave_max(-v); }
 
-// q of one row as two f16 terms of q * 2^k, lane group g holding dims 32 s + 8 g ..: 
+// The factor from products to scores in the log2 domain, positive (a negative scale turns q's sign).
+__device__ __forceinline__ float score_factor(const PagedAttn &a) { return fmaxf(fabsf(a.scale) * kLog2e, 0x1p-126f); }
+
+// q of one row (or -q) as two f16 terms of q * 2^k, lane group g holding dims 32 s + 8 g ..:
 // returns 2^-k.
 template <int KS>
 __device__ __forceinline__ float load_q(const PagedAttn &a, const float *row, bool live, int g, half8 *hi, half8 *lo)
@@ -390,7 +404,7 @@ __device__ __forceinline__ float load_q(const PagedAttn &a, const float *row, bo
     top = row_max(top);
     // the largest value into [2^13, 2^14)
     const int ex = min(max((int)(as_u(top) >> 23), 14), 254);
-    const float up = as_f((uint32_t)(267 - ex) << 23);
+    const float up = as_f((uint32_t)(267 - ex) << 23) * (a.scale < 0.0f ? -1.0f : 1.0f);
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -408,7 +422,7 @@ __device__ __forceinline__ float load_q(const PagedAttn &a, const float *row, bo
 __device__ __forceinline__ void split_p(float x, float y, uint32_t &hi, uint32_t &lo)
 {
     const auto h = __builtin_amdgcn_cvt_pkrtz(x, y);
-    const float rx = x - (float)h[0], ry = y - (float)h[1];
+    const float rx = fmaf((float)h[0], -1.0f, x), ry = fmaf((float)h[1], -1.0f, y);
     const auto l = __builtin_amdgcn_cvt_pkrtz(rx, ry);
     hi = __builtin_bit_cast(uint32_t, h);
     lo = __builtin_bit_cast(uint32_t, l);
@@ -424,16 +438,16 @@ __device__ __forceinline__ float4v mfma(half8 a, half8 b, float4v c)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Running softmax of one row: x holds N scores of this lane (log2 domain, -inf
-// where masked), which become p * 2^14; m and l are brought up to date, true if
-// o has to be multiplied by f.
+// Running softmax of one row: x holds N products of this lane (-inf where masked;
+// a score in the log2 domain is x * c, c > 0), which become p * 2^14; m (the largest
+// score) and l are brought up to date, true if o has to be multiplied by f.
 template <int N>
-__device__ __forceinline__ bool softmax_step(float *x, float &m, float &l, float &f)
+__device__ __forceinline__ bool softmax_step(float *x, float c, float &m, float &l, float &f)
 {
     float top = x[0];
 #pragma unroll
     for (int e = 1; e < N; ++e) top = fmaxf(top, x[e]);
-    top = row_max(top);
+    top = row_max(top) * c;
     const bool grow = top > m + kSlack;
     f = 1.0f;
     const bool any = __any(grow);
@@ -443,11 +457,11 @@ __device__ __forceinline__ bool softmax_step(float *x, float &m, float &l, float
         l *= f;
         m = m2;
     }
-    const float base = m == -INFINITY ? 0.0f : m - kShift;
+    const float base = m == -INFINITY ? 0.0f : kShift - m;
     float sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-        x[e] = exp2_hw(x[e] - base);
+        x[e] = exp2_hw(fmaf(x[e], c, base));
         sum += x[e];
     }
     l += sum;
@@ -472,29 +486,20 @@ __device__ __forceinline__ bool softmax_step(float *x, float &m, float &l, float
 // sides through LDS once.  Quantised V enters as f16 terms too: d * q has at most
 // 19 bits, hi = its rounding, lo = fma(d, q, -hi), both exact.
 
-// K of 16 positions in LDS, as 1 KB chunks (what one global_load_lds of a wave
-// writes) 1040 bytes apart.  A chunk holds 64 / P whole rows of P 16-byte pieces;
-// position p lies in chunk p % (P / 4), so that the eight lanes that read
-// together, of eight consecutive positions, meet eight different bank groups, where
-// rows share a chunk by exchanging the pieces of every other one.  A lane's
-// address is then a base plus a constant, one base for even and one for odd steps.
-constexpr int kChunk = 1040;
+// Tiles in LDS are made of 1 KB chunks, each the left operand of one product: 16 rows
+// (positions of K, dims of V) of four 16-byte pieces (8 dims, 8 positions), lane
+// i + 16 g taking piece g of row i.  Row i lies at 64 * (i / 4 + 4 (i % 4)) with its
+// pieces exchanged by i % 4: the 16 lanes that a wave's 16-byte reads serve together
+// (0-3, 12-15, 20-23, 24-27 and so on) then meet 16 different places of the
+// 64 banks, as do the eight of any eight neighbours, and 16 lanes that write one
+// run of 4 x 4 dims.  Padded rows (16 bytes a row) had 4 conflict cycles a read.  A
+// lane's address is one base plus a constant for every chunk.
+constexpr int kChunk = 1024;
 
-template <int P>
-struct KTile {
-    static constexpr int kRows = 64 / P, kChunks = 16 / kRows;  // rows a chunk, chunks of 16 positions
-    static constexpr int kBytes16 = kChunks * kChunk;
-    __device__ static __forceinline__ int flip(int sub) { return P == 16 ? (sub & 1) * 4 : P == 8 ? (sub & 3) * 2 : 0; }
-    // chunk c's lane: the position (of its 16) and the piece that it loads
-    __device__ static __forceinline__ int position(int c, int lane) { return c % kChunks + lane / P * kChunks; }
-    __device__ static __forceinline__ int piece(int lane) { return (lane % P) ^ flip(lane / P); }
-    // byte offset of piece 4 s + g of position i, less 64 (s & ~1)
-    __device__ static __forceinline__ int offset(int i, int g, int odd)
-    {
-        const int sub = i / kChunks;
-        return i % kChunks * kChunk + sub * P * 16 + ((4 * odd + g) ^ flip(sub)) * 16;
-    }
-};
+__device__ __forceinline__ int chunk_offset(int i, int g) { return ((i >> 2) + 4 * (i & 3)) * 64 + (g ^ (i & 3)) * 16; }
+// what a lane of a wave's global_load_lds (which writes 16 bytes a lane, in lane order) loads
+__device__ __forceinline__ int chunk_row(int lane) { return 4 * ((lane >> 2) & 3) + (lane >> 4); }
+__device__ __forceinline__ int chunk_piece(int lane) { return (lane & 3) ^ (lane >> 4); }
 
 __device__ __forceinline__ half8 read16(const uint8_t *p) { return __builtin_bit_cast(half8, *reinterpret_cast<const uint4 *>(p)); }
 
@@ -513,7 +518,7 @@ constexpr int kTrRow = 36;  // floats a query row of the score tile in LDS
 template <int DP, bool KQ>
 struct WaveLds {
     int place[32];
-    alignas(16) uint8_t k[2 * KTile<DP / 8>::kBytes16];  // 32 positions
+    alignas(16) uint8_t k[DP / 16 * kChunk];  // 32 positions: chunks of 32 dims, of 16 positions
 };
 template <int DP>
 struct WaveLds<DP, true> {
@@ -558,7 +563,7 @@ __device__ __forceinline__ void load_quant_q(const PagedAttn &a, const float *ro
         out.q[s] = (long)((uint64_t)w[0] | ((uint64_t)w[1] << 32));
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            out.d[s][r] = __shfl(d, 4 * g + r, 64);
+            out.d[s][r] = __shfl(a.scale < 0.0f ? -d : d, 4 * g + r, 64);
             out.sum8[s][r] = a.k_fmt == 2 ? -8 * __shfl(sum, 4 * g + r, 64) : 0;
         }
     }
@@ -576,15 +581,15 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
     const float *q_row = a.q + (size_t)tok * a.q_stride + (size_t)head * hd;
     half8 qh[KQ ? 1 : KS], ql[KQ ? 1 : KS];
     QuantQ<KQ ? KS : 1> qq;
-    float c = a.scale * kLog2e;
+    float c = score_factor(a);
     if constexpr (KQ)
         load_quant_q<KS>(a, q_row, live, g, qq);
     else
-        c *= load_q<KS>(a, q_row, live, g, qh, ql);
+        c = fmaxf(c * load_q<KS>(a, q_row, live, g, qh, ql), 0x1p-126f);
     int vlo, vhi;
     row_sees(a, sc, need_at, pc, mi, vlo, vhi);
     const int full_lo = wave_max(vlo), full_hi = wave_min(vhi);
-    const int krb = kv_row_bytes(a.k_fmt, hd), vrb = kv_row_bytes(a.v_fmt, hd);
+    const HeadRows k_rows = head_rows(a, a.k, a.k_fmt, pc.kvh), v_rows = head_rows(a, a.v, a.v_fmt, pc.kvh);
     const int kblk = a.k_fmt == 1 ? 34 : 18, vblk = a.v_fmt == 1 ? 34 : 18;
 
     float m = -INFINITY, l = 0.0f;
@@ -595,7 +600,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
         for (int d = 0; d < 8; ++d) o[n][d] = float4v{0, 0, 0, 0};
 
     // A tile's page ids are loaded two tiles ahead and looked at one tile ahead, when they are long there.
-    const int kbase[2] = {KTile<DP / 8>::offset(i, g, 0), KTile<DP / 8>::offset(i, g, 1)};
+    const int base = chunk_offset(i, g);
     auto page_ids = [&](int t0) { return t0 + (lane & 31) < pc.p1 ? pc.table[page_of(a.map, t0 + (lane & 31))] : -1; };
     auto places = [&](int t0, int id) {
         const int pos = t0 + (lane & 31);
@@ -609,7 +614,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
         if constexpr (KQ) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint8_t *row = kv_row(a, a.k, krb, __shfl(place, 16 * h + i, 64), pc.kvh);
+                const uint8_t *row = k_rows.row(__shfl(place, 16 * h + i, 64));
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
                     const uint8_t *b = row + (s * 32 < hd ? s * kblk : 0);
@@ -618,13 +623,13 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
                 }
             }
         } else {
-            using KT = KTile<DP / 8>;
-            const int ln = here(lane), piece = KT::piece(ln);
+            const int ln = here(lane), piece = chunk_piece(ln) * 16;
 #pragma unroll
-            for (int n = 0; n < 2 * KT::kChunks; ++n) {
-                const int p = n / KT::kChunks * 16 + KT::position(n, ln);
-                load_to_lds(kv_row(a, a.k, krb, __shfl(place, p, 64), pc.kvh) + (piece * 8 < hd ? piece * 16 : 0),
-                            lds.k + n * kChunk);
+            for (int h = 0; h < 2; ++h) {
+                const uint8_t *row = k_rows.row(__shfl(place, 16 * h + chunk_row(ln), 64)) + piece;
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+                    load_to_lds(row + (s * 32 < hd ? s * 64 : 0), lds.k + (h * KS + s) * kChunk);
             }
         }
     };
@@ -643,7 +648,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
             const int d0 = n * 128 + 8 * (here(lane) & 15), dim = d0 < hd ? d0 : 0;  // past the head: never stored
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const uint8_t *row = kv_row(a, a.v, vrb, pl[j], pc.kvh);
+                const uint8_t *row = v_rows.row(pl[j]);
                 if constexpr (VQ) {
                     const uint8_t *b = row + (dim >> 5) * vblk;
                     vd[n][j] = *reinterpret_cast<const _Float16 *>(b);
@@ -690,7 +695,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const float4 y = *reinterpret_cast<const float4 *>(lds.scores + i * kTrRow + 16 * h + 4 * g);
-                x[4 * h] = y.x * c, x[4 * h + 1] = y.y * c, x[4 * h + 2] = y.z * c, x[4 * h + 3] = y.w * c;
+                x[4 * h] = y.x, x[4 * h + 1] = y.y, x[4 * h + 2] = y.z, x[4 * h + 3] = y.w;
             }
             __builtin_amdgcn_wave_barrier();
         } else {
@@ -705,7 +710,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
-                        kk[(s0 / 2) & 1][e][h] = read16(lds.k + kbase[e] + h * KTile<DP / 8>::kBytes16 + 64 * s0);
+                        kk[(s0 / 2) & 1][e][h] = read16(lds.k + base + (h * KS + s0 + e) * kChunk);
             };
             read_k(0);
 #pragma unroll
@@ -724,7 +729,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[4 * h + r] = (acc[h][0][r] + acc[h][1][r]) * c;
+                for (int r = 0; r < 4; ++r) x[4 * h + r] = acc[h][0][r] + acc[h][1][r];
         }
         pin();  // K's tile has been read, and no later load passes the next one's
         if (t0 + kUnitA < pc.p1) load_k(place_next);
@@ -750,7 +755,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
                 }
         }
         float f;
-        if (softmax_step<8>(x, m, l, f)) {
+        if (softmax_step<8>(x, c, m, l, f)) {
 #pragma unroll
             for (int n = 0; n < NG; ++n)
 #pragma unroll
@@ -840,18 +845,17 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
 
 // ---- block items: a workgroup, many query rows, K and V through LDS -----------------
 //
-// Tiles of T = 16384 / DP positions, two in LDS (137 KB with padding): while the waves
-// work on one, the next is under way.  K goes to LDS directly (global_load_lds, as in
-// a stream item); V is transposed on its way by the thread that has loaded 8
-// positions of some dims, and written as 16-byte runs of 8 positions, rows of a dim 16
-// bytes longer than the tile.  A wave holds 16 * R rows; each piece read from LDS feeds
-// 2 * R products.
+// Tiles of T = 16384 / DP positions, two in LDS (128 KB): while the waves work on one,
+// the next is under way.  K goes to LDS directly (global_load_lds, as in a stream
+// item); V is transposed on its way by the thread that has loaded 8 positions of some
+// dims, and written as 16-byte runs of 8 positions.  A wave holds 16 * R rows; each
+// chunk read from LDS feeds 2 * R products.
 
 template <int DP>
 struct BlockLds {
-    static constexpr int T = unit_b(DP), kPitch = 2 * T + 16;  // bytes of a dim's row
-    alignas(16) uint8_t k[2][T / 16 * KTile<DP / 8>::kBytes16];
-    alignas(16) uint8_t v[2][DP * kPitch];
+    static constexpr int T = unit_b(DP);
+    alignas(16) uint8_t k[2][T / 16][DP / 32][kChunk];  // [16 positions][32 dims]
+    alignas(16) uint8_t v[2][T / 32][DP / 16][kChunk];  // [32 positions][16 dims]
     int place[3][T];
 };
 
@@ -860,13 +864,13 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
                                            BlockLds<DP> &lds, const Dest &to)
 {
     constexpr int NW = waves_of(DP, false), R = tiles_of(DP), KS = DP / 32, NF = DP / 16, T = unit_b(DP);
-    constexpr int SP = T < 64 || DP == 128 ? 32 : 64, NH = SP / 16, P = DP / 8;
+    constexpr int SP = T < 64 || DP == 128 ? 32 : 64, NH = SP / 16, kAhead = 3;
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4, hd = a.head_dim;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int rb = hd * 2;
+    const HeadRows k_rows = head_rows(a, a.k, 0, pc.kvh), v_rows = head_rows(a, a.v, 0, pc.kvh);
     const int tiles = (pc.p1 - pc.p0 + T - 1) / T;
 
-    // A tile's page ids are loaded two tiles ahead, at a tile's start, and put into LDS as places at its end.
+    // A tile's page ids are loaded two tiles ahead and put into LDS as places at the end of that tile.
     auto page_ids = [&](int tile) {
         const int pos = pc.p0 + tile * T + tid;
         return tid < T && pos < pc.p1 ? pc.table[page_of(a.map, pos)] : -1;
@@ -878,36 +882,37 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
             lds.place[tile % 3][tid] = place;
         }
     };
-    using KT = KTile<P>;
-    auto load_k = [&](int tile) {
-        constexpr int N = T / 16 * KT::kChunks / NW;  // chunks a wave
-        const int ln = here(lane), piece = KT::piece(ln);
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int c = wave * N + n, p = c / KT::kChunks * 16 + KT::position(c, ln);
-            load_to_lds(kv_row(a, a.k, rb, lds.place[tile % 3][p], pc.kvh) + (piece * 8 < hd ? piece * 16 : 0),
-                        lds.k[tile & 1] + c * kChunk);
-        }
+    // K: a wave's share of the chunks, whole 16-position groups or part of one's steps
+    constexpr int GW = T / 16 >= NW ? T / 16 / NW : 1, SW = T / 16 >= NW ? KS : KS * (T / 16) / NW;
+    constexpr int kParts = GW * SW + 8;  // loads of a tile: chunks of K, 8 positions of V
+    auto load_k = [&](int tile, int n) {
+        const int grp = T / 16 >= NW ? wave * GW + n / SW : wave * (T / 16) / NW;
+        const int s = (T / 16 >= NW ? 0 : wave * SW % KS) + n % SW, ln = here(lane);
+        const uint8_t *row = k_rows.row(lds.place[tile % 3][grp * 16 + chunk_row(ln)]);
+        load_to_lds(row + chunk_piece(ln) * 16 + (s * 32 < hd ? s * 64 : 0), lds.k[tile & 1][grp][s]);
     };
     // this thread's dims (VD of them) and run of positions (run0 + 0..3 and run0 + 16..19): four runs of a
-    // dim by neighbouring lanes, whose writes then meet no bank twice, and 16 lanes along a row
-    constexpr int VD = 32 / NW, VT = DP / VD, kPitch = BlockLds<DP>::kPitch;
+    // dim by neighbouring lanes, 16 lanes along a row
+    constexpr int VD = 32 / NW, VT = DP / VD;
     static_assert(VT * (T / 8) == 64 * NW, "one task a thread");
     const int dl = (tid >> 2) % VT, run = (tid & 3) + tid / (4 * VT) * 4, run0 = (run >> 2) * 32 + (run & 3) * 4;
     uint32_t v[8][VD / 2];
-    auto load_v = [&](int tile) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int place = lds.place[tile % 3][run0 + (j >> 2) * 16 + (j & 3)];
-            const uint8_t *src = kv_row(a, a.v, rb, place, pc.kvh) + (dl * VD < hd ? dl * VD * 2 : 0);
-            if constexpr (VD == 8) {
-                const uint4 x = *reinterpret_cast<const uint4 *>(src);
-                v[j][0] = x.x, v[j][1] = x.y, v[j][2] = x.z, v[j][3] = x.w;
-            } else {
-                const uint2 x = *reinterpret_cast<const uint2 *>(src);
-                v[j][0] = x.x, v[j][1] = x.y;
-            }
+    auto load_v = [&](int tile, int j) {
+        const int place = lds.place[tile % 3][run0 + (j >> 2) * 16 + (j & 3)];
+        const uint8_t *src = v_rows.row(place) + (dl * VD < hd ? dl * VD * 2 : 0);
+        if constexpr (VD == 8) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(src);
+            v[j][0] = x.x, v[j][1] = x.y, v[j][2] = x.z, v[j][3] = x.w;
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2 *>(src);
+            v[j][0] = x.x, v[j][1] = x.y;
         }
+    };
+    auto load_part = [&](int tile, int n) {
+        if (n < GW * SW)
+            load_k(tile, n);
+        else
+            load_v(tile, n - GW * SW);
     };
     auto store_v = [&](int tile) {
 #pragma unroll
@@ -921,21 +926,22 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
             uint32_t t[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) t[e] = __builtin_amdgcn_perm(v[2 * e + 1][d >> 1], v[2 * e][d >> 1], sel);
-            *reinterpret_cast<uint4 *>(lds.v[tile & 1] + (VD * dl + d) * kPitch + run * 16) = make_uint4(t[0], t[1], t[2], t[3]);
+            const int dim = VD * dl + d;
+            *reinterpret_cast<uint4 *>(lds.v[tile & 1][run >> 2][dim >> 4] + chunk_offset(dim & 15, run & 3)) =
+                make_uint4(t[0], t[1], t[2], t[3]);
         }
     };
 
-    __syncthreads();  // the tiles' LDS is free
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): of the last item's loads to LDS
+    __syncthreads();                     // the tiles' LDS is free
     const int id0 = page_ids(0), id1 = page_ids(1);
     set_places(0, id0);
     set_places(1, id1);
     __syncthreads();
-    if (tiles > 0) {
-        load_k(0);
-        load_v(0);
-    }
+#pragma unroll
+    for (int n = 0; n < kParts; ++n) load_part(0, n);
 
-    const int kbase[2] = {KT::offset(i, g, 0), KT::offset(i, g, 1)}, vbase = i * kPitch + g * 16;
+    const int base = chunk_offset(i, g);
     const bool busy = pc.row0 + wave * R * 16 < pc.rows;  // the wave has rows
     half8 qh[R][KS], ql[R][KS];
     float c[R], m[R], l[R];
@@ -946,7 +952,8 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
         const int mi = pc.row0 + (wave * R + u) * 16 + i;
         const bool live = mi < pc.rows;
         const int tok = pc.tok0 + mi / a.group, head = pc.kvh * a.group + mi % a.group;
-        c[u] = load_q<KS>(a, a.q + (size_t)tok * a.q_stride + (size_t)head * hd, live, g, qh[u], ql[u]) * a.scale * kLog2e;
+        c[u] = fmaxf(load_q<KS>(a, a.q + (size_t)tok * a.q_stride + (size_t)head * hd, live, g, qh[u], ql[u]) * score_factor(a),
+                     0x1p-126f);
         row_sees(a, sc, need_at, pc, mi, vlo[u], vhi[u]);
         full_lo = max(full_lo, wave_max(vlo[u]));
         full_hi = min(full_hi, wave_min(vhi[u]));
@@ -955,53 +962,58 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
 #pragma unroll
         for (int f = 0; f < NF; ++f) o[u][f] = float4v{0, 0, 0, 0};
     }
-    if (tiles > 0) store_v(0);
+    store_v(0);
 
     for (int tile = 0; tile < tiles; ++tile) {
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): K of this tile is in LDS
         __syncthreads();
-        const int id2 = page_ids(tile + 2);
-        if (tile + 1 < tiles) {
-            load_k(tile + 1);
-            load_v(tile + 1);
-        }
-        const uint8_t *kt = lds.k[tile & 1], *vt = lds.v[tile & 1] + vbase;
-#pragma unroll 1
-        for (int s0 = 0; s0 < T; s0 += SP) {
+        int id2 = -1;
+        const uint8_t *kt = lds.k[tile & 1][0][0] + base, *vt = lds.v[tile & 1][0][0] + base;
+        // The next tile's loads go out one by one between the first products: at once they would wait for
+        // each other's 16 and more cycles of address work.  (Past the last tile: places of none, the first row.)
+        auto chunk = [&](int s0, auto loads) {
+            constexpr bool kLoads = decltype(loads)::value;
             const int t0 = pc.p0 + tile * T + s0;
-            if (t0 >= pc.p1 || !busy) break;
             float4v acc[R][NH];
 #pragma unroll
             for (int u = 0; u < R; ++u)
 #pragma unroll
                 for (int h = 0; h < NH; ++h) acc[u][h] = float4v{0, 0, 0, 0};
-            // the next step's pieces are on their way from LDS while a step's products run
-            constexpr int KG = 2, KN = KS * NH;  // pieces a step, pieces in all: (s, h) = (n / NH, n % NH)
-            half8 kk[2][KG];
+            // the next kAhead - 1 steps' chunks are on their way from LDS while a step's products run
+            constexpr int KG = 2, KN = KS * NH;  // chunks a step, chunks in all: (s, h) = (n / NH, n % NH)
+            half8 kk[kAhead][KG];
             auto read_k = [&](int n0) {
 #pragma unroll
                 for (int e = 0; e < KG; ++e) {
                     const int s = (n0 + e) / NH, h = (n0 + e) % NH;
-                    kk[(n0 / KG) & 1][e] = read16(kt + kbase[s & 1] + (s0 / 16 + h) * KT::kBytes16 + 64 * (s & ~1));
+                    kk[n0 / KG % kAhead][e] = read16(kt + ((s0 / 16 + h) * KS + s) * kChunk);
                 }
             };
-            read_k(0);
+#pragma unroll
+            for (int n = 0; n < (kAhead - 1) * KG && n < KN; n += KG) read_k(n);
 #pragma unroll
             for (int n = 0; n < KN; n += KG) {
-                if (n + KG < KN) read_k(n + KG);
+                if constexpr (kLoads) {
+                    constexpr int kEach = (kParts * KG + KN - 1) / KN;  // loads a step
+#pragma unroll
+                    for (int x = 0; x < kEach; ++x)
+                        if (n / KG * kEach + x < kParts) load_part(tile + 1, n / KG * kEach + x);
+                }
+                if (n + (kAhead - 1) * KG < KN) read_k(n + (kAhead - 1) * KG);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int u = 0; u < R; ++u)
 #pragma unroll
                     for (int e = 0; e < KG; ++e)
-                        acc[u][(n + e) % NH] = mfma(kk[(n / KG) & 1][e], qh[u][(n + e) / NH], acc[u][(n + e) % NH]);
+                        acc[u][(n + e) % NH] = mfma(kk[n / KG % kAhead][e], qh[u][(n + e) / NH], acc[u][(n + e) % NH]);
 #pragma unroll
                 for (int u = 0; u < R; ++u)
 #pragma unroll
                     for (int e = 0; e < KG; ++e)
-                        acc[u][(n + e) % NH] = mfma(kk[(n / KG) & 1][e], ql[u][(n + e) / NH], acc[u][(n + e) % NH]);
+                        acc[u][(n + e) % NH] = mfma(kk[n / KG % kAhead][e], ql[u][(n + e) / NH], acc[u][(n + e) % NH]);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            if constexpr (kLoads) id2 = page_ids(tile + 2);  // after the tile's loads: nothing waits for it alone
             const uint64_t there = __ballot(lane < SP && lds.place[tile % 3][s0 + (lane & (SP - 1))] >= 0);
             const bool edge = t0 < full_lo || t0 + SP > full_hi || there != (SP == 64 ? ~0ull : (1ull << (SP & 63)) - 1);
             uint32_t ph[R][NH][2], pw[R][NH][2];
@@ -1009,7 +1021,7 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
             for (int u = 0; u < R; ++u) {
                 float x[4 * NH];
 #pragma unroll
-                for (int e = 0; e < 4 * NH; ++e) x[e] = acc[u][e >> 2][e & 3] * c[u];
+                for (int e = 0; e < 4 * NH; ++e) x[e] = acc[u][e >> 2][e & 3];
                 if (edge) {
 #pragma unroll
                     for (int e = 0; e < 4 * NH; ++e) {
@@ -1018,7 +1030,7 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
                     }
                 }
                 float f;
-                if (softmax_step<4 * NH>(x, m[u], l[u], f)) {
+                if (softmax_step<4 * NH>(x, c[u], m[u], l[u], f)) {
 #pragma unroll
                     for (int n = 0; n < NF; ++n) o[u][n] *= f;
                 }
@@ -1035,31 +1047,41 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
                     p_hi[u] = as_half8(ph[u][2 * b][0], ph[u][2 * b][1], ph[u][2 * b + 1][0], ph[u][2 * b + 1][1]);
                     p_lo[u] = as_half8(pw[u][2 * b][0], pw[u][2 * b][1], pw[u][2 * b + 1][0], pw[u][2 * b + 1][1]);
                 }
-                constexpr int VG = 2;  // pieces a step
-                half8 vv[2][VG];
+                constexpr int VG = 2;  // chunks a step
+                half8 vv[kAhead][VG];
                 auto read_v = [&](int f0) {
 #pragma unroll
                     for (int f = 0; f < VG; ++f)
-                        vv[(f0 / VG) & 1][f] = read16(vt + (f0 + f) * 16 * kPitch + (s0 / 8 + 4 * b) * 16);
+                        vv[f0 / VG % kAhead][f] = read16(vt + ((s0 / 32 + b) * NF + f0 + f) * kChunk);
                 };
-                read_v(0);
+#pragma unroll
+                for (int f0 = 0; f0 < (kAhead - 1) * VG && f0 < NF; f0 += VG) read_v(f0);
 #pragma unroll
                 for (int f0 = 0; f0 < NF; f0 += VG) {
-                    if (f0 + VG < NF) read_v(f0 + VG);
+                    if (f0 + (kAhead - 1) * VG < NF) read_v(f0 + (kAhead - 1) * VG);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int u = 0; u < R; ++u)
 #pragma unroll
-                        for (int f = 0; f < VG; ++f) o[u][f0 + f] = mfma(vv[(f0 / VG) & 1][f], p_hi[u], o[u][f0 + f]);
+                        for (int f = 0; f < VG; ++f) o[u][f0 + f] = mfma(vv[f0 / VG % kAhead][f], p_hi[u], o[u][f0 + f]);
 #pragma unroll
                     for (int u = 0; u < R; ++u)
 #pragma unroll
-                        for (int f = 0; f < VG; ++f) o[u][f0 + f] = mfma(vv[(f0 / VG) & 1][f], p_lo[u], o[u][f0 + f]);
+                        for (int f = 0; f < VG; ++f) o[u][f0 + f] = mfma(vv[f0 / VG % kAhead][f], p_lo[u], o[u][f0 + f]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
+        };
+        if (busy) {
+            chunk(0, std::true_type{});
+#pragma unroll 1
+            for (int s0 = SP; s0 < T && pc.p0 + tile * T + s0 < pc.p1; s0 += SP) chunk(s0, std::false_type{});
+        } else {
+#pragma unroll
+            for (int n = 0; n < kParts; ++n) load_part(tile + 1, n);
+            id2 = page_ids(tile + 2);
         }
-        if (tile + 1 < tiles) store_v(tile + 1);
+        store_v(tile + 1);
         set_places(tile + 2, id2);
     }
 #pragma unroll
@@ -1303,7 +1325,7 @@ __device__ __forceinline__ void slow_row(const PagedAttn &a, int row, int r, int
     const int lane = threadIdx.x & 63, hd = a.head_dim, kvh = h / a.group;
     const int len = clamp_len(a, a.lens[r]), at = a.prefix_len + len - (a.row_start[r + 1] - row);
     const int first = a.window ? max(0, at - a.window + 1) : 0;
-    const int krb = kv_row_bytes(a.k_fmt, hd), vrb = kv_row_bytes(a.v_fmt, hd);
+    const HeadRows k_rows = head_rows(a, a.k, a.k_fmt, kvh), v_rows = head_rows(a, a.v, a.v_fmt, kvh);
 #pragma unroll 1
     for (int d0 = 0; d0 < hd; d0 += 64) {
         const int d = d0 + lane;
@@ -1323,7 +1345,7 @@ __device__ __forceinline__ void slow_row(const PagedAttn &a, int row, int r, int
         const bool pre = t < a.prefix_len;
         const int place = pre ? place_at(a, a.prefix, t) : place_at(a, a.table + (size_t)r * a.table_stride, t - a.prefix_len);
         if (place < 0) continue;
-        const uint8_t *kr = kv_row(a, a.k, krb, place, kvh), *vr = kv_row(a, a.v, vrb, place, kvh);
+        const uint8_t *kr = k_rows.row(place), *vr = v_rows.row(place);
         float s = 0.0f;
 #pragma unroll 1
         for (int d = lane; d < hd; d += 64) s = fmaf(s_q[d], kv_value(kr, a.k_fmt, d), s);
@@ -1345,7 +1367,7 @@ __device__ __forceinline__ void slow_row(const PagedAttn &a, int row, int r, int
 template <int W>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a, Parts parts)
 {
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 3;
     __shared__ float s_o[4][512], s_q[4][512], s_l[4], s_m[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), hd = a.head_dim;
     const int pair = blockIdx.x * (4 / W) + wave / W, row = pair / a.n_heads, h = pair - row * a.n_heads;
