@@ -63,11 +63,13 @@ struct Parts {
     float *o_a, *o_b;    // later parts, by worker: [worker][16][head_dim], [workgroup][128][head_dim]
     float2 *ml_a, *ml_b;
     int32_t *first, *last;  // workers that hold an item's first and last unit
-    int4 *row_item;         // {the own items' first index, row within the request, block items?, request}
-    int32_t *head;          // {rows are sound, first row, rows}
-    int items_a;            // index of the first block item
+    int4 *row_item;         // of a row: {request, its first row, its rows}
+    int32_t *head;          // {the row starts are sound, first row, end of rows}
+    // Items are numbered with gaps, so that nothing has to count them: a request's row tiles by its first row and
+    // its place in the batch ((first row * group) / tile rows + r + tile), the prefix's behind them; times n_kv_heads.
+    int pre_a, own_b, pre_b;  // the first stream item of the prefix, block item of a request, of the prefix
     int wgs, waves;
-    int rows_b;             // rows of a block item (0: none)
+    int rows_b;               // rows of a block item (0: none)
 };
 
 // What a wave knows of the piece it works on (uniform).
@@ -89,12 +91,10 @@ struct Dest {
 };
 
 template <int T>
-struct Scan {  // sums over the requests before each of T threads' share, in LDS
-    int ua[T + 1], ub[T + 1];  // units
-    int ia[T + 1], ib[T + 1];  // items
-    int rs[T + 1], len[T];     // first row; length of the share's first request
-    int sum[8][4], low[8], flags[8];
-    float size[8];
+struct Scan {  // over the requests, in LDS
+    int ua[T + 1], ub[T + 1];  // stream and block units before each thread's share of the requests
+    int rs[T + 1], len[T];     // the share's first row, its first request's length
+    int sum[8][2], low[8], flags[8];
 };
 
 __device__ __forceinline__ float as_f(uint32_t u) { return __builtin_bit_cast(float, u); }
@@ -172,167 +172,171 @@ __device__ __forceinline__ HeadRows head_rows(const PagedAttn &a, const uint8_t 
 
 // ---- the requests' shares of the work --------------------------------------------
 
+// All workgroups do this first, out of cold instruction caches: what counts is
+// the number of instructions, so divisions are by multiplication and sums over the
+// lanes by DPP.
+
 struct Request {
     int rs, n, len;  // first row, rows, own length (within its table row)
 };
 
-__device__ __forceinline__ int share(const PagedAttn &a) { return (a.n_seqs + blockDim.x - 1) / blockDim.x; }
-
-__device__ __forceinline__ int clamp_len(const PagedAttn &a, int len)
+__device__ __forceinline__ int div_group(const PagedAttn &a, int x)  // x * group < 2^32
 {
-    return min(max(len, 0), a.table_stride * a.map.page_size);
+    return a.group_magic ? (int)__umulhi((uint32_t)x, a.group_magic) : x;
 }
+
+// x / y for 0 <= x < 2^30, y > 0: the reciprocal's quotient, then its remainder's, then what a rounding left.
+__device__ __forceinline__ int div_fast(int x, int y, int &rest)
+{
+    const float inv = __builtin_amdgcn_rcpf((float)y);
+    int q = (int)((float)x * inv);
+    int r = x - q * y;
+    const int d = (int)((float)r * inv);
+    q += d;
+    r -= d * y;
+    if (r < 0) --q, r += y;
+    if (r >= y) ++q, r -= y;
+    rest = r;
+    return q;
+}
+
+template <int T>
+__device__ __forceinline__ int share(const PagedAttn &a) { return (a.n_seqs + T - 1) / T; }
+
+__device__ __forceinline__ int clamp_len(const PagedAttn &a, int len) { return min(max(len, 0), a.longest); }
 
 template <int T>
 __device__ __forceinline__ Request request_at(const PagedAttn &a, const Scan<T> &s, int r)
 {
-    if (share(a) == 1) return Request{s.rs[r], s.rs[r + 1] - s.rs[r], s.len[r]};
+    if (share<T>(a) == 1) return Request{s.rs[r], s.rs[r + 1] - s.rs[r], s.len[r]};
     const int rs = a.row_start[r];
     return Request{rs, a.row_start[r + 1] - rs, clamp_len(a, a.lens[r])};
 }
 
-// Own positions that rows i0..i1 of a request see: [lo, hi).
+// Own positions that the rows of a request up to row i1, from row i0 on, see: [lo, hi).
 __device__ __forceinline__ void own_range(const PagedAttn &a, const Request &q, int i0, int i1, int &lo, int &hi)
 {
     hi = max(q.len - q.n + i1 + 1, 0);
     lo = a.window ? min(max(q.len - q.n + i0 - a.window + 1, 0), hi) : 0;
 }
 
-__device__ __forceinline__ int units_of(int lo, int hi, int unit) { return max(1, (hi - lo + unit - 1) / unit); }
-
-__device__ __forceinline__ int own_units_a(const PagedAttn &a, const Request &q)
+// The same of a row tile of a request.
+template <int TILE>
+__device__ __forceinline__ void tile_range(const PagedAttn &a, const Request &q, int tile, int &lo, int &hi)
 {
-    int lo, hi;
-    own_range(a, q, 0, q.n - 1, lo, hi);
-    return units_of(lo, hi, kUnitA);
+    own_range(a, q, div_group(a, tile * TILE), div_group(a, min(q.n * a.group, (tile + 1) * TILE) - 1), lo, hi);
 }
 
-__device__ __forceinline__ int own_units_b(const PagedAttn &a, const Request &q, int block, int unit, int rows)
-{
-    int lo, hi;
-    const int last = min(q.n * a.group, (block + 1) * rows) - 1;
-    own_range(a, q, block * rows / a.group, last / a.group, lo, hi);
-    return units_of(lo, hi, unit);
-}
+template <int UNIT>
+__device__ __forceinline__ int units_of(int lo, int hi) { return max(1, (hi - lo + UNIT - 1) / UNIT); }
 
-// {stream units with the items' own cost, block units, stream items, block items} of a request; returns the units as a float, which cannot
-// overflow.
-__device__ __forceinline__ float request_work(const PagedAttn &a, const Request &q, int rows, int unit, int w[4])
+// The units of a request: of stream items (with each item's own cost; all its row
+// tiles take the positions that any of its rows sees) or of block items.
+template <int ROWS, int UNIT>
+__device__ __forceinline__ void request_units(const PagedAttn &a, const Request &q, int &ua, int &ub)
 {
-    w[0] = w[1] = w[2] = w[3] = 0;
-    if (q.n <= 0) return 0.0f;
+    ua = ub = 0;
+    if (q.n <= 0) return;
     const int m = q.n * a.group;
-    if (!rows || m <= kFewRows) {
-        w[2] = (m + kRowsA - 1) / kRowsA * a.n_kv_heads;
-        w[0] = w[2] * (own_units_a(a, q) + kItemCost);
-        return (float)w[2] * (float)(own_units_a(a, q) + kItemCost);
-    } else {
-        const int nb = (m + rows - 1) / rows;
-        float size = 0.0f;
-        for (int b = 0; b < nb; ++b) {
-            const int n = own_units_b(a, q, b, unit, rows);
-            w[1] += n;
-            size += (float)n;
+    int lo, hi;
+    if (!ROWS || m <= kFewRows) {
+        own_range(a, q, 0, q.n - 1, lo, hi);
+        ua = (m + kRowsA - 1) / kRowsA * a.n_kv_heads * (units_of<kUnitA>(lo, hi) + kItemCost);
+    } else if constexpr (ROWS != 0) {
+        for (int b = 0; b * ROWS < m; ++b) {
+            tile_range<ROWS>(a, q, b, lo, hi);
+            ub += units_of<UNIT>(lo, hi);
         }
-        w[1] *= a.n_kv_heads;
-        w[3] = nb * a.n_kv_heads;
-        return size * (float)a.n_kv_heads;
+        ub *= a.n_kv_heads;
     }
 }
 
-// Every workgroup forms the same sums over all requests (a few loads a thread).
-// False: row starts that do not ascend within the rows.
+// Inclusive sum over a wave's lanes.
+__device__ __forceinline__ int wave_scan(int x)
+{
+#define SCAN_STEP(CTRL, ROWS) x += __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false)
+    SCAN_STEP(0x111, 0xf);  // row_shr:1, 2, 4, 8
+    SCAN_STEP(0x112, 0xf);
+    SCAN_STEP(0x114, 0xf);
+    SCAN_STEP(0x118, 0xf);
+    SCAN_STEP(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+    SCAN_STEP(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+#undef SCAN_STEP
+    return x;
+}
+
 struct Totals {
-    bool ok, need_at;  // need_at: some row stands before its request's first position
-    int low;           // the first own position that a row has
-    float size;        // units, as a float
+    bool ok, need_at;  // the row starts ascend within the rows; some row stands before its request's first position
+    int low;           // with a window: the first own position that a row has
 };
 
-template <int T>
-__device__ Totals scan_requests(const PagedAttn &a, Scan<T> &s, int rows, int unit)
+template <int T, int ROWS, int UNIT>
+__device__ __forceinline__ Totals scan_requests(const PagedAttn &a, Scan<T> &s)
 {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = share(a), r0 = tid * per, r1 = min(r0 + per, a.n_seqs);
-    int w[4] = {0, 0, 0, 0}, low = INT32_MAX, flags = 0;
-    float size = 0.0f;
-    s.rs[tid] = a.row_start[min(r0, a.n_seqs)];
-    if (tid == 0) s.rs[T] = a.row_start[a.n_seqs];
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const int per = share<T>(a), r0 = min(tid * per, a.n_seqs), r1 = min(r0 + per, a.n_seqs);
+    int w[2] = {0, 0}, low = INT32_MAX;
+    bool bad = false, neg = false;
+    int rs = a.row_start[r0];
+    s.rs[tid] = rs;
+    if (tid == T - 1) s.rs[T] = a.row_start[a.n_seqs];
     for (int r = r0; r < r1; ++r) {
-        const int rs = a.row_start[r], re = a.row_start[r + 1], len = a.lens[r];
+        const int re = a.row_start[r + 1], len = a.lens[r];
         if (rs < 0 || re < rs || re > a.max_rows) {
-            flags |= 1;
-            continue;
+            bad = true;
+        } else {
+            const Request q{rs, re - rs, clamp_len(a, len)};
+            if (q.len != len && blockIdx.x == 0) page_fault(a.faults);
+            if (r == r0) s.len[tid] = q.len;
+            int ua, ub;
+            request_units<ROWS, UNIT>(a, q, ua, ub);
+            w[0] += ua;
+            w[1] += ub;
+            if (q.n > 0) {
+                low = min(low, q.len - q.n);
+                neg |= q.len < q.n;
+            }
         }
-        const Request q{rs, re - rs, clamp_len(a, len)};
-        if (q.len != len && blockIdx.x == 0) page_fault(a.faults);
-        if (r == r0) s.len[tid] = q.len;
-        int x[4];
-        size += request_work(a, q, rows, unit, x);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] += x[k];
-        if (q.n > 0) {
-            low = min(low, q.len - q.n);
-            flags |= q.len < q.n ? 2 : 0;
-        }
+        rs = re;
     }
-    int inc[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        int x = w[k];
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int y = __shfl_up(x, d, 64);
-            if (lane >= d) x += y;
-        }
-        inc[k] = x;
-        if (lane == 63) s.sum[wave][k] = x;
-    }
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        low = min(low, __shfl_xor(low, d, 64));
-        flags |= __shfl_xor(flags, d, 64);
-        size += __shfl_xor(size, d, 64);
-    }
-    if (lane == 0) {
+    const int inc[2] = {wave_scan(w[0]), ROWS ? wave_scan(w[1]) : 0};
+    const int flags = (__any(bad) ? 1 : 0) | (__any(neg) ? 2 : 0);
+    if (a.window)
+        for (int d = 32; d; d >>= 1) low = min(low, __shfl_xor(low, d, 64));
+    if ((tid & 63) == 63) {
+        s.sum[wave][0] = inc[0];
+        s.sum[wave][1] = inc[1];
         s.low[wave] = low;
         s.flags[wave] = flags;
-        s.size[wave] = size;
     }
     __syncthreads();
-    int before[4] = {0, 0, 0, 0};
+    int before[2] = {0, 0}, all = 0;
     low = INT32_MAX;
-    flags = 0;
-    size = 0.0f;
-#pragma unroll
+#pragma unroll 1
     for (int v = 0; v < T / 64; ++v) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) before[k] += v < wave ? s.sum[v][k] : 0;
+        if (v < wave) before[0] += s.sum[v][0], before[1] += s.sum[v][1];
         low = min(low, s.low[v]);
-        flags |= s.flags[v];
-        size += s.size[v];
+        all |= s.flags[v];
     }
-    int *dst[4] = {s.ua, s.ub, s.ia, s.ib};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        dst[k][tid] = before[k] + inc[k] - w[k];
-        if (tid == T - 1) dst[k][T] = before[k] + inc[k];
+    s.ua[tid] = before[0] + inc[0] - w[0];
+    s.ub[tid] = before[1] + inc[1] - w[1];
+    if (tid == T - 1) {
+        s.ua[T] = before[0] + inc[0];
+        s.ub[T] = before[1] + inc[1];
     }
     __syncthreads();
-    return Totals{(uni(flags) & 1) == 0, (uni(flags) & 2) != 0,
-                  uni(low), uni(size)};
+    all = uni(all);
+    return Totals{(all & 1) == 0, (all & 2) != 0, uni(low)};
 }
 
-// The thread whose share [from[t], from[t + 1]) holds x (from ascending, from[0] <= x < from[threads]).
+// The thread whose share [from[t], from[t + 1]) holds x (from ascending, from[0] <= x < from[T]).
+template <int T>
 __device__ __forceinline__ int share_of(const int *from, int x)
 {
-    int lo = 0, hi = blockDim.x - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (from[mid] <= x)
-            lo = mid;
-        else
-            hi = mid - 1;
-    }
+    int lo = 0;
+#pragma unroll 1
+    for (int step = T / 2; step; step >>= 1)
+        if (from[lo + step] <= x) lo += step;
     return lo;
 }
 
@@ -340,10 +344,10 @@ __device__ __forceinline__ int share_of(const int *from, int x)
 template <int T>
 __device__ __forceinline__ int request_of(const PagedAttn &a, const Scan<T> &s, int row)
 {
-    const int per = share(a);
-    int r = share_of(s.rs, row) * per;
-    if (per == 1) return r;
-    while (r + 1 < a.n_seqs && a.row_start[r + 1] <= row) ++r;
+    const int per = share<T>(a);
+    int r = share_of<T>(s.rs, row) * per;
+    if (per > 1)
+        while (r + 1 < a.n_seqs && a.row_start[r + 1] <= row) ++r;
     return r;
 }
 
@@ -351,7 +355,9 @@ __device__ __forceinline__ int request_of(const PagedAttn &a, const Scan<T> &s, 
 
 __device__ __forceinline__ size_t part_row(const PagedAttn &a, const Piece &pc, const Dest &d, int mi)
 {
-    return d.own ? (size_t)(pc.tok0 + mi / a.group) * a.n_heads + pc.kvh * a.group + mi % a.group : (size_t)(mi - pc.row0);
+    if (!d.own) return (size_t)(mi - pc.row0);
+    const int i = div_group(a, mi);
+    return (size_t)(pc.tok0 + i) * a.n_heads + pc.kvh * a.group + (mi - i * a.group);
 }
 
 // What row mi of a piece's group sees, in the source's positions: [vlo, vhi).
@@ -361,9 +367,9 @@ __device__ __forceinline__ void row_sees(const PagedAttn &a, const Scan<T> &s, b
     vlo = 0;
     vhi = INT32_MAX;
     if (mi >= pc.rows) return;
-    const int tok = pc.tok0 + mi / a.group;
+    const int row = div_group(a, mi), tok = pc.tok0 + row;
     if (!pc.pre) {
-        const int at = pc.at0 + mi / a.group;
+        const int at = pc.at0 + row;
         vhi = at + 1;
         vlo = a.window ? at - a.window + 1 : 0;
     } else if (need_at || a.window) {
@@ -577,7 +583,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, hd = a.head_dim;
     const int mi = pc.row0 + i;
     const bool live = mi < pc.rows;
-    const int tok = pc.tok0 + mi / a.group, head = pc.kvh * a.group + mi % a.group;
+    const int i_row = div_group(a, mi), tok = pc.tok0 + i_row, head = pc.kvh * a.group + mi - i_row * a.group;
     const float *q_row = a.q + (size_t)tok * a.q_stride + (size_t)head * hd;
     half8 qh[KQ ? 1 : KS], ql[KQ ? 1 : KS];
     QuantQ<KQ ? KS : 1> qq;
@@ -951,7 +957,7 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
     for (int u = 0; u < R; ++u) {
         const int mi = pc.row0 + (wave * R + u) * 16 + i;
         const bool live = mi < pc.rows;
-        const int tok = pc.tok0 + mi / a.group, head = pc.kvh * a.group + mi % a.group;
+        const int i_row = div_group(a, mi), tok = pc.tok0 + i_row, head = pc.kvh * a.group + mi - i_row * a.group;
         c[u] = fmaxf(load_q<KS>(a, a.q + (size_t)tok * a.q_stride + (size_t)head * hd, live, g, qh[u], ql[u]) * score_factor(a),
                      0x1p-126f);
         row_sees(a, sc, need_at, pc, mi, vlo[u], vhi[u]);
@@ -1116,17 +1122,17 @@ struct Shared {
     int units, items;   // units an item, with a stream item's own cost
 };
 
-template <int T>
-__device__ __forceinline__ Shared shared_work(const PagedAttn &a, const Scan<T> &s, const Totals &t, int rows_b, int unit)
+template <int T, int ROWS, int UNIT>
+__device__ __forceinline__ Shared shared_work(const PagedAttn &a, const Scan<T> &s, const Totals &t)
 {
     Shared p;
-    p.rows = uni(s.rs[blockDim.x] - s.rs[0]) * a.group;
-    p.few = !rows_b || p.rows <= kFewRows;
+    p.rows = uni(s.rs[T] - s.rs[0]) * a.group;
+    p.few = !ROWS || p.rows <= kFewRows;
     p.hi = a.prefix_len;
     p.lo = a.window && t.low < INT32_MAX ? min(max(a.prefix_len + t.low - a.window + 1, 0), p.hi) : 0;
-    const int tile = p.few ? kRowsA : rows_b;
-    p.items = a.prefix_len > 0 ? (p.rows + tile - 1) / tile * a.n_kv_heads : 0;
-    p.units = units_of(p.lo, p.hi, p.few ? kUnitA : unit) + (p.few ? kItemCost : 0);
+    p.items = (p.few ? (p.rows + kRowsA - 1) / kRowsA : (p.rows + ROWS - 1) / (ROWS ? ROWS : 1)) * a.n_kv_heads;
+    p.units = p.few ? units_of<kUnitA>(p.lo, p.hi) + kItemCost : units_of<UNIT>(p.lo, p.hi);
+    if (a.prefix_len == 0) p.items = 0;
     return p;
 }
 
@@ -1134,83 +1140,68 @@ __device__ __forceinline__ Shared shared_work(const PagedAttn &a, const Scan<T> 
 // returns the units taken, the item's index, and whether the piece holds its
 // first and last positions.  A stream item's own cost stands before its
 // first unit: a share that ends there has no piece of it (none).
-template <int T>
-__device__ __forceinline__ int find_piece(const PagedAttn &a, const Scan<T> &s, const Shared &sh, bool block, int rows_b,
-                                          int unit, int u, int left, Piece &pc, int &item, bool &is_first, bool &is_last,
+template <bool BLOCK, int T, int ROWS, int UNIT>
+__device__ __forceinline__ int find_piece(const PagedAttn &a, const Parts &parts, const Scan<T> &s, const Shared &sh,
+                                          int u, int left, Piece &pc, int &item, bool &is_first, bool &is_last,
                                           bool &none)
 {
-    const int tile = block ? rows_b : kRowsA, step = block ? unit : kUnitA;
-    const int sh_items = sh.few != block ? sh.items : 0, sh_units = sh_items * sh.units;
-    int lo, hi, units, within, blk, tab = 0;
-    if (u < sh_units) {
-        item = u / sh.units;
-        within = u - item * sh.units;
-        blk = item / a.n_kv_heads;
-        pc.kvh = item - blk * a.n_kv_heads;
+    constexpr int kTile = BLOCK ? ROWS : kRowsA, kStep = BLOCK ? UNIT : kUnitA;
+    const int sh_units = sh.few != BLOCK ? sh.items * sh.units : 0;
+    int lo, hi, units, within, blk, r = 0;
+    pc.pre = u < sh_units;
+    if (pc.pre) {
+        blk = div_fast(div_fast(u, sh.units, within), a.n_kv_heads, pc.kvh);
         units = sh.units;
         lo = sh.lo;
         hi = sh.hi;
-        pc.pre = true;
-        pc.tok0 = s.rs[0];
+        pc.tok0 = uni(s.rs[0]);
         pc.rows = sh.rows;
         pc.at0 = 0;
+        item = (BLOCK ? parts.pre_b : parts.pre_a) + blk * a.n_kv_heads + pc.kvh;
     } else {
         u -= sh_units;
-        const int t = share_of(block ? s.ub : s.ua, u);
-        int r = t * share(a), first = (block ? s.ib : s.ia)[t];
-        u -= (block ? s.ub : s.ua)[t];
+        const int *from = BLOCK ? s.ub : s.ua;
+        const int t = share_of<T>(from, u);
+        u -= from[t];
+        r = t * share<T>(a);
         Request q = request_at(a, s, r);
-        if (share(a) > 1) {
+        if (share<T>(a) > 1) {
             for (;;) {
-                int w[4];
-                request_work(a, q, rows_b, unit, w);
-                const int n = block ? w[1] : w[0];
-                if (u < n || r + 1 >= a.n_seqs) break;
-                u -= n;
-                first += block ? w[3] : w[2];
+                int w[2];
+                request_units<ROWS, UNIT>(a, q, w[0], w[1]);
+                if (u < w[BLOCK] || r + 1 >= a.n_seqs) break;
+                u -= w[BLOCK];
                 q = request_at(a, s, ++r);
             }
         }
-        if (!block) {
-            units = own_units_a(a, q) + kItemCost;
-            item = u / units;
-            within = u - item * units;
-            blk = item / a.n_kv_heads;
-            pc.kvh = item - blk * a.n_kv_heads;
+        if constexpr (!BLOCK) {
             own_range(a, q, 0, q.n - 1, lo, hi);
+            units = units_of<kUnitA>(lo, hi) + kItemCost;
+            blk = div_fast(div_fast(u, units, within), a.n_kv_heads, pc.kvh);
         } else {
             for (blk = 0;; ++blk) {
-                units = own_units_b(a, q, blk, unit, rows_b);
+                tile_range<ROWS>(a, q, blk, lo, hi);
+                units = units_of<UNIT>(lo, hi);
                 if (u < units * a.n_kv_heads) break;
                 u -= units * a.n_kv_heads;
             }
-            pc.kvh = u / units;
-            item = blk * a.n_kv_heads + pc.kvh;
-            within = u - pc.kvh * units;
-            const int last = min(q.n * a.group, (blk + 1) * rows_b) - 1;
-            own_range(a, q, blk * rows_b / a.group, last / a.group, lo, hi);
+            pc.kvh = div_fast(u, units, within);
         }
-        item += sh_items + first;
-        pc.pre = false;
-        tab = r;
-        pc.tok0 = q.rs;
-        pc.rows = q.n * a.group;
-        pc.at0 = q.len - q.n;
+        item = (BLOCK ? parts.own_b : 0) + (q.rs * a.group / kTile + r + blk) * a.n_kv_heads + pc.kvh;
+        pc.tok0 = uni(q.rs);
+        pc.rows = uni(q.n * a.group);
+        pc.at0 = uni(q.len - q.n);
     }
     units = uni(units);
     within = uni(within);
-    const int take = min(units - within, left), cost = block ? 0 : kItemCost;
+    const int take = min(units - within, left), cost = BLOCK ? 0 : kItemCost;
     const int from = max(within - cost, 0), to = max(within + take - cost, 0);
     item = uni(item);
-    pc.pre = uni(pc.pre);
-    pc.table = pc.pre ? a.prefix : a.table + (size_t)uni(tab) * a.table_stride;
-    pc.tok0 = uni(pc.tok0);
-    pc.rows = uni(pc.rows);
-    pc.at0 = uni(pc.at0);
+    pc.table = pc.pre ? a.prefix : a.table + (size_t)uni(r) * a.table_stride;
     pc.kvh = uni(pc.kvh);
-    pc.row0 = uni(blk) * tile;
-    pc.p0 = uni(lo) + from * step;
-    pc.p1 = min(uni(hi), uni(lo) + to * step);
+    pc.row0 = uni(blk) * kTile;
+    pc.p0 = uni(lo) + from * kStep;
+    pc.p1 = min(uni(hi), uni(lo) + to * kStep);
     is_first = from == 0;
     is_last = within + take == units;
     none = to == from;
@@ -1241,36 +1232,22 @@ __global__ __launch_bounds__(64 * waves_of(DP, KQ || VQ)) void paged_attn_kernel
     __shared__ KernelLds<DP, KQ, kBlocks> lds;
     const Scan<T> &s = lds.scan;
     const int wg = blockIdx.x, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Totals totals = scan_requests<T>(a, lds.scan, kRowsB, kUnitB);
-    Shared sh{};
-    // row starts that do not ascend, or more units than an int counts (days of work): nothing is computed
-    bool ok = totals.ok;
-    if (ok) {
-        sh = shared_work(a, s, totals, kRowsB, kUnitB);
-        ok = totals.size + (float)sh.items * (float)sh.units < 1e9f;
-    }
+    const Totals totals = scan_requests<T, kRowsB, kUnitB>(a, lds.scan);
+    // row starts that do not ascend: nothing is computed
     if (wg == 0 && tid == 0) {
-        *reinterpret_cast<int4 *>(parts.head) = make_int4(ok, ok ? s.rs[0] : 0, ok ? s.rs[T] : 0, 0);
-        if (!ok) page_fault(a.faults);
+        *reinterpret_cast<int4 *>(parts.head) = make_int4(totals.ok, s.rs[0], s.rs[T], 0);
+        if (!totals.ok) page_fault(a.faults);
     }
-    if (!ok) return;
+    if (!totals.ok) return;
+    const Shared sh = shared_work<T, kRowsB, kUnitB>(a, s, totals);
     const int sh_units = sh.items * sh.units;
     const int ua = uni(s.ua[T]) + (sh.few ? sh_units : 0), ub = uni(s.ub[T]) + (sh.few ? 0 : sh_units);
 
-    // which items a row's own part is in
+    // the request of each row, for joining the parts
     for (int row = s.rs[0] + wg * T + tid; row < s.rs[T]; row += parts.wgs * T) {
-        const int r = request_of(a, s, row), t = r / share(a);
-        int ia = s.ia[t], ib = s.ib[t];
-        for (int x = t * share(a); x < r; ++x) {
-            int w[4];
-            request_work(a, request_at(a, s, x), kRowsB, kUnitB, w);
-            ia += w[2];
-            ib += w[3];
-        }
+        const int r = request_of(a, s, row);
         const Request q = request_at(a, s, r);
-        const bool block = kBlocks && q.n * a.group > kFewRows;
-        const int first = block ? parts.items_a + ib + (sh.few ? 0 : sh.items) : ia + (sh.few ? sh.items : 0);
-        parts.row_item[row] = make_int4(first, row - q.rs, block, r);
+        parts.row_item[row] = make_int4(r, q.rs, q.n, 0);
     }
 
     int wb = 0;
@@ -1286,23 +1263,25 @@ __global__ __launch_bounds__(64 * waves_of(DP, KQ || VQ)) void paged_attn_kernel
     bool first, last, none;
     if constexpr (kBlocks) {
         if (wg < wb) {
-            const int quota = (ub + wb - 1) / wb, end = min(ub, (wg + 1) * quota);
+            int rest;
+            const int quota = uni(div_fast(ub + wb - 1, wb, rest)), end = min(ub, (wg + 1) * quota);
             for (int u = wg * quota; u < end;) {
-                u += find_piece(a, s, sh, true, kRowsB, kUnitB, u, end - u, pc, item, first, last, none);
+                u += find_piece<true, T, kRowsB, kUnitB>(a, parts, s, sh, u, end - u, pc, item, first, last, none);
                 const size_t row = (size_t)wg * kRowsB;
                 const Dest to = first ? Dest{parts.o[!pc.pre], parts.ml[!pc.pre], true}
                                       : Dest{parts.o_b + row * a.head_dim, parts.ml_b + row, false};
-                if (tid == 0 && first) parts.first[parts.items_a + item] = wg;
-                if (tid == 0 && last) parts.last[parts.items_a + item] = wg;
+                if (tid == 0 && first) parts.first[item] = wg;
+                if (tid == 0 && last) parts.last[item] = wg;
                 block_item<DP>(a, s, totals.need_at, pc, lds.block, to);
             }
             return;
         }
     }
     const int worker = (wg - wb) + (parts.wgs - wb) * wave, workers = (parts.wgs - wb) * kWaves;
-    const int quota = (ua + workers - 1) / workers, end = min(ua, (worker + 1) * quota);
+    int rest;
+    const int quota = uni(div_fast(ua + workers - 1, workers, rest)), end = min(ua, (worker + 1) * quota);
     for (int u = worker * quota; u < end;) {
-        u += find_piece(a, s, sh, false, kRowsB, kUnitB, u, end - u, pc, item, first, last, none);
+        u += find_piece<false, T, kRowsB, kUnitB>(a, parts, s, sh, u, end - u, pc, item, first, last, none);
         if (none) continue;
         const size_t row = (size_t)worker * kRowsA;
         const Dest to = first ? Dest{parts.o[!pc.pre], parts.ml[!pc.pre], true}
@@ -1322,7 +1301,7 @@ __global__ __launch_bounds__(64 * waves_of(DP, KQ || VQ)) void paged_attn_kernel
 __device__ __forceinline__ void slow_row(const PagedAttn &a, int row, int r, int h, int wave, int waves, float *s_q,
                                          float *s_o, float &m, float &l)
 {
-    const int lane = threadIdx.x & 63, hd = a.head_dim, kvh = h / a.group;
+    const int lane = threadIdx.x & 63, hd = a.head_dim, kvh = div_group(a, h);
     const int len = clamp_len(a, a.lens[r]), at = a.prefix_len + len - (a.row_start[r + 1] - row);
     const int first = a.window ? max(0, at - a.window + 1) : 0;
     const HeadRows k_rows = head_rows(a, a.k, a.k_fmt, kvh), v_rows = head_rows(a, a.v, a.v_fmt, kvh);
@@ -1375,26 +1354,24 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a, Parts par
     const int4 head = *reinterpret_cast<const int4 *>(parts.head);
     const int4 ri = parts.row_item[row];
     if (!head.x || row < head.y || row >= head.z) return;  // W == 4: the whole workgroup
-    const int kvh = h / a.group, gq = h - kvh * a.group;
+    const int kvh = div_group(a, h), gq = h - kvh * a.group;
     const size_t base = (size_t)row * a.n_heads + h;
     // the two items of the row: the prefix's, its own
-    int w0[2], n[2], at[2], rows[2];
-    {
-        const int m = (head.z - head.y) * a.group, mi = (row - head.y) * a.group + gq;
+    int w0[2], n[2], at[2], rows[2], item[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int row0 = x ? ri.y : head.y, m = (x ? ri.z : head.z - head.y) * a.group, mi = (row - row0) * a.group + gq;
         const bool block = parts.rows_b && m > kFewRows;
-        rows[0] = block ? parts.rows_b : kRowsA;
-        const int item = mi / rows[0] * a.n_kv_heads + kvh + (block ? parts.items_a : 0);
-        at[0] = mi % rows[0];
-        w0[0] = a.prefix_len > 0 ? parts.first[item] : 0;
-        n[0] = a.prefix_len > 0 ? parts.last[item] - w0[0] + 1 : 0;
+        rows[x] = block ? parts.rows_b : kRowsA;
+        const int sh = __builtin_ctz(rows[x]), tile = mi >> sh;
+        at[x] = mi - (tile << sh);
+        const int at0 = x ? (block ? parts.own_b : 0) : (block ? parts.pre_b : parts.pre_a);
+        item[x] = at0 + ((x ? (ri.y * a.group >> sh) + ri.x : 0) + tile) * a.n_kv_heads + kvh;
     }
-    {
-        rows[1] = ri.z ? parts.rows_b : kRowsA;
-        const int mi = ri.y * a.group + gq, item = ri.x + mi / rows[1] * a.n_kv_heads + kvh;
-        at[1] = mi % rows[1];
-        w0[1] = parts.first[item];
-        n[1] = parts.last[item] - w0[1] + 1;
-    }
+    w0[0] = a.prefix_len > 0 ? parts.first[item[0]] : 0;
+    w0[1] = parts.first[item[1]];
+    n[0] = a.prefix_len > 0 ? parts.last[item[0]] - w0[0] + 1 : 0;
+    n[1] = parts.last[item[1]] - w0[1] + 1;
     const int total = n[0] + n[1];
     auto part = [&](int k, const float *&po, const float2 *&pml) {
         const int x = k >= n[0], j = k - (x ? n[0] : 0);
@@ -1421,7 +1398,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a, Parts par
 #pragma unroll
     for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
     if (__any(broken)) {
-        slow_row(a, row, ri.w, h, wave % W, W, s_q[wave], s_o[wave], top, l);
+        slow_row(a, row, ri.x, h, wave % W, W, s_q[wave], s_o[wave], top, l);
         if constexpr (W == 4) {
             if (lane == 0) s_m[wave] = top;
             __syncthreads();
@@ -1515,13 +1492,11 @@ Parts layout(const PagedAttn &a, uint8_t *base, size_t &bytes)
     p.rows_b = quant ? 0 : rows_b(dp);
     const size_t heads = (size_t)a.max_rows * a.n_heads, hd = a.head_dim;
     const size_t group_rows = (size_t)a.max_rows * a.group;
-    // stream items: the rows of every request and of the prefix in tiles of 16; block items: tiles of rows_b of
-    // groups of more than kFewRows
-    const size_t seqs = std::min<size_t>(a.n_seqs, a.max_rows);
-    const size_t items_a = (group_rows / kRowsA + seqs + group_rows / kRowsA + 1) * a.n_kv_heads;
-    const size_t items_b =
-        p.rows_b ? (2 * (group_rows / p.rows_b + 1) + std::min(seqs, group_rows / kFewRows)) * a.n_kv_heads : 0;
-    p.items_a = (int)items_a;
+    const size_t tiles_a = group_rows / kRowsA + 1, tiles_b = p.rows_b ? group_rows / p.rows_b + 1 : 0, kv = a.n_kv_heads;
+    p.pre_a = (int)((tiles_a + a.n_seqs) * kv);
+    p.own_b = (int)(p.pre_a + tiles_a * kv);
+    p.pre_b = (int)(p.own_b + (p.rows_b ? tiles_b + a.n_seqs : 0) * kv);
+    const size_t items = p.pre_b + tiles_b * kv;
     for (int k = 0; k < 2; ++k) {
         const bool used = k == 1 || a.prefix_len > 0;
         p.o[k] = reinterpret_cast<float *>(take(used ? heads * hd * 4 : 0));
@@ -1532,8 +1507,8 @@ Parts layout(const PagedAttn &a, uint8_t *base, size_t &bytes)
     p.ml_a = reinterpret_cast<float2 *>(take(workers * kRowsA * 8));
     p.o_b = reinterpret_cast<float *>(take(wg_rows * hd * 4));
     p.ml_b = reinterpret_cast<float2 *>(take(wg_rows * 8));
-    p.first = reinterpret_cast<int32_t *>(take((items_a + items_b) * 4));
-    p.last = reinterpret_cast<int32_t *>(take((items_a + items_b) * 4));
+    p.first = reinterpret_cast<int32_t *>(take(items * 4));
+    p.last = reinterpret_cast<int32_t *>(take(items * 4));
     p.row_item = reinterpret_cast<int4 *>(take((size_t)a.max_rows * 16));
     p.head = reinterpret_cast<int32_t *>(take(16));
     bytes = at;
@@ -1556,6 +1531,19 @@ void launch_dp(mrml_hip_ctx *ctx, const PagedAttn &a, const Parts &p)
 }
 
 }  // namespace
+
+// Stream units: at most two row tiles a request where there are block items, else tiles of 16 of all rows, over
+// the longest table row; and the prefix's.  Block units are fewer than their rows in tiles of 16 would give.
+bool paged_attn_countable(const PagedAttn &a)
+{
+    const double kv = a.n_kv_heads, rows = (double)a.max_rows * a.group, seqs = std::min(a.n_seqs, a.max_rows);
+    const bool quant = a.k_fmt != 0 || a.v_fmt != 0;
+    const double tiles = rows / kRowsA + seqs, own = a.longest / kUnitA + 1 + kItemCost, pre = a.prefix_len / kUnitA + 1 + kItemCost;
+    const double block = quant ? 1.0 : 1.0 / 8;  // a block tile is 64 rows at least and 32 positions
+    const double a_units = quant ? tiles * own : 2 * seqs * own;
+    return kv * (a_units + block * tiles * (own + pre) + 2 * pre) < (double)(1 << 30) &&
+           kv * (2 * tiles + 2.0 * a.n_seqs + 8) < (double)(1 << 30);
+}
 
 size_t paged_attn_scratch_bytes(const PagedAttn &a)
 {

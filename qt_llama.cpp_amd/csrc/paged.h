@@ -46,11 +46,15 @@ struct PagedAttn {
     PageMap map;
     int q_stride, prefix_len, table_stride, n_seqs, max_rows;
     int n_heads, n_kv_heads, head_dim, group;
+    uint32_t group_magic;  // ceil(2^32 / group), 0 for 1
+    int longest;           // positions of a table row
     int window;  // 0: none
     int k_fmt, v_fmt;
     float scale;
 };
 
+// Whether a call's units of work can be counted in 32 bits.
+bool paged_attn_countable(const PagedAttn &a);
 size_t paged_attn_scratch_bytes(const PagedAttn &a);
 int launch_paged_attn(mrml_hip_ctx *ctx, const PagedAttn &a, void *scratch);
 

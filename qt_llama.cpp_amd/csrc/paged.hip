@@ -465,10 +465,15 @@ int mrml_hip_attention_paged(mrml_hip_ctx *ctx, const float *q, int32_t q_stride
     a.n_kv_heads = n_kv_heads;
     a.head_dim = head_dim;
     a.group = n_heads / n_kv_heads;
+    a.group_magic = a.group > 1 ? (uint32_t)((1ull << 32) / a.group) + 1u : 0u;
+    a.longest = table_stride * page_size;
     a.window = sliding_window > 0 ? sliding_window : 0;
     a.k_fmt = k_format;
     a.v_fmt = v_format;
     a.scale = scale;
+    REQUIRE(ctx, paged_attn_countable(a),
+            "%s: n_seqs=%d, max_rows=%d and positions (%d of a table row, prefix %d) are too many for one call", name, n_seqs,
+            max_rows, a.longest, prefix_len);
     void *scratch = workspace(ctx, std::max<size_t>(paged_attn_scratch_bytes(a), 16));
     if (!scratch) return MRML_HIP_E_ALLOC;
     ctx->paged_used = true;
