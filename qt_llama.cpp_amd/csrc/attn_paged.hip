@@ -43,11 +43,12 @@ constexpr float kSlack = 1.5f;    // the maximum may grow by this much before o 
 constexpr float kBroken = -1.0f;  // in place of l: the part is not finite
 constexpr int kRowsA = 16, kUnitA = 32;  // rows and positions of a stream item's tile (one wave)
 constexpr int kFewRows = 32;             // groups of at most so many rows are stream items
-// Costs, for the split of the work, in stream units of one wave (about 3.5 us each): what
+// Costs, for the split of the work, in stream units of one wave (about 7 us each where few workgroups stream): what
 // a stream item costs beside its units (q, the first K and V, the part's store: a
 // chain of round trips), and a block unit per 32 rows of it and wave.
-constexpr int kItemCost = 3;
-constexpr float kBlockCost = 0.28f;
+constexpr int kItemCost = 2;
+constexpr int kBlockItemCost = 2;  // the same of a block item, in its units
+constexpr float kBlockCost = 0.15f;
 
 // Waves of a workgroup, rows of a block item and positions of its tile by padded head size: two waves a SIMD
 // while a wave's q and o fit 256 registers.
@@ -230,7 +231,7 @@ __device__ __forceinline__ void tile_range(const PagedAttn &a, const Request &q,
 template <int UNIT>
 __device__ __forceinline__ int units_of(int lo, int hi) { return max(1, (hi - lo + UNIT - 1) / UNIT); }
 
-// The units of a request: of stream items (with each item's own cost; all its row
+// The units of a request, with each item's own cost: of stream items (all its row
 // tiles take the positions that any of its rows sees) or of block items.
 template <int ROWS, int UNIT>
 __device__ __forceinline__ void request_units(const PagedAttn &a, const Request &q, int &ua, int &ub)
@@ -245,7 +246,7 @@ __device__ __forceinline__ void request_units(const PagedAttn &a, const Request 
     } else if constexpr (ROWS != 0) {
         for (int b = 0; b * ROWS < m; ++b) {
             tile_range<ROWS>(a, q, b, lo, hi);
-            ub += units_of<UNIT>(lo, hi);
+            ub += units_of<UNIT>(lo, hi) + kBlockItemCost;
         }
         ub *= a.n_kv_heads;
     }
@@ -889,52 +890,42 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
         }
     };
     // K: a wave's share of the chunks, whole 16-position groups or part of one's steps
-    constexpr int GW = T / 16 >= NW ? T / 16 / NW : 1, SW = T / 16 >= NW ? KS : KS * (T / 16) / NW;
-    constexpr int kParts = GW * SW + 8;  // loads of a tile: chunks of K, 8 positions of V
+    constexpr int GW = T / 16 >= NW ? T / 16 / NW : 1, SW = T / 16 >= NW ? KS : KS * (T / 16) / NW, kPartsK = GW * SW;
     auto load_k = [&](int tile, int n) {
         const int grp = T / 16 >= NW ? wave * GW + n / SW : wave * (T / 16) / NW;
         const int s = (T / 16 >= NW ? 0 : wave * SW % KS) + n % SW, ln = here(lane);
         const uint8_t *row = k_rows.row(lds.place[tile % 3][grp * 16 + chunk_row(ln)]);
         load_to_lds(row + chunk_piece(ln) * 16 + (s * 32 < hd ? s * 64 : 0), lds.k[tile & 1][grp][s]);
     };
-    // this thread's dims (VD of them) and run of positions (run0 + 0..3 and run0 + 16..19): four runs of a
-    // dim by neighbouring lanes, 16 lanes along a row
-    constexpr int VD = 32 / NW, VT = DP / VD;
-    static_assert(VT * (T / 8) == 64 * NW, "one task a thread");
-    const int dl = (tid >> 2) % VT, run = (tid & 3) + tid / (4 * VT) * 4, run0 = (run >> 2) * 32 + (run & 3) * 4;
-    uint32_t v[8][VD / 2];
+    // V: this thread's 8 dims and NV positions: a run of 8 in the products' order (run0 + 0..3, run0 + 16..19) or
+    // half of one
+    constexpr int NV = 32 / NW, kHalves = 8 / NV;
+    const int dl = (tid / (4 * kHalves)) % (DP / 8), half = NV == 8 ? 0 : tid & 1, run = ((tid / kHalves) & 3) + tid / (DP / 2 * kHalves) * 4;
+    const int run0 = (run >> 2) * 32 + (run & 3) * 4 + half * 16;
+    uint32_t v[NV][4];
     auto load_v = [&](int tile, int j) {
-        const int place = lds.place[tile % 3][run0 + (j >> 2) * 16 + (j & 3)];
-        const uint8_t *src = v_rows.row(place) + (dl * VD < hd ? dl * VD * 2 : 0);
-        if constexpr (VD == 8) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(src);
-            v[j][0] = x.x, v[j][1] = x.y, v[j][2] = x.z, v[j][3] = x.w;
-        } else {
-            const uint2 x = *reinterpret_cast<const uint2 *>(src);
-            v[j][0] = x.x, v[j][1] = x.y;
-        }
-    };
-    auto load_part = [&](int tile, int n) {
-        if (n < GW * SW)
-            load_k(tile, n);
-        else
-            load_v(tile, n - GW * SW);
+        const uint8_t *row = v_rows.row(lds.place[tile % 3][run0 + (j >> 2) * 16 + (j & 3)]);
+        const uint4 x = *reinterpret_cast<const uint4 *>(row + (dl * 8 < hd ? dl * 16 : 0));
+        v[j][0] = x.x, v[j][1] = x.y, v[j][2] = x.z, v[j][3] = x.w;
     };
     auto store_v = [&](int tile) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < NV; ++j)
             if (lds.place[tile % 3][run0 + (j >> 2) * 16 + (j & 3)] < 0)  // nothing there: no weight may meet it
 #pragma unroll
-                for (int w = 0; w < VD / 2; ++w) v[j][w] = 0;
+                for (int w = 0; w < 4; ++w) v[j][w] = 0;
 #pragma unroll
-        for (int d = 0; d < VD; ++d) {
+        for (int d = 0; d < 8; ++d) {
             const uint32_t sel = d & 1 ? 0x07060302u : 0x05040100u;
-            uint32_t t[4];
+            uint32_t t[NV / 2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) t[e] = __builtin_amdgcn_perm(v[2 * e + 1][d >> 1], v[2 * e][d >> 1], sel);
-            const int dim = VD * dl + d;
-            *reinterpret_cast<uint4 *>(lds.v[tile & 1][run >> 2][dim >> 4] + chunk_offset(dim & 15, run & 3)) =
-                make_uint4(t[0], t[1], t[2], t[3]);
+            for (int e = 0; e < NV / 2; ++e) t[e] = __builtin_amdgcn_perm(v[2 * e + 1][d >> 1], v[2 * e][d >> 1], sel);
+            const int dim = 8 * dl + d;
+            uint8_t *dst = lds.v[tile & 1][run >> 2][dim >> 4] + chunk_offset(dim & 15, run & 3) + half * 8;
+            if constexpr (NV == 8)
+                *reinterpret_cast<uint4 *>(dst) = make_uint4(t[0], t[1], t[2], t[3]);
+            else
+                *reinterpret_cast<uint2 *>(dst) = make_uint2(t[0], t[1]);
         }
     };
 
@@ -945,7 +936,9 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
     set_places(1, id1);
     __syncthreads();
 #pragma unroll
-    for (int n = 0; n < kParts; ++n) load_part(0, n);
+    for (int n = 0; n < kPartsK; ++n) load_k(0, n);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) load_v(0, j);
 
     const int base = chunk_offset(i, g);
     const bool busy = pc.row0 + wave * R * 16 < pc.rows;  // the wave has rows
@@ -975,8 +968,9 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
         __syncthreads();
         int id2 = -1;
         const uint8_t *kt = lds.k[tile & 1][0][0] + base, *vt = lds.v[tile & 1][0][0] + base;
-        // The next tile's loads go out one by one between the first products: at once they would wait for
-        // each other's 16 and more cycles of address work.  (Past the last tile: places of none, the first row.)
+        // The next tile's loads go out one by one between the products, V's between those with K (it has to be
+        // there at the tile's end), K's between those with V: at once they would wait for each other's 16
+        // cycles and more of address work.  (Past the last tile: places of none, the first row.)
         auto chunk = [&](int s0, auto loads) {
             constexpr bool kLoads = decltype(loads)::value;
             const int t0 = pc.p0 + tile * T + s0;
@@ -1000,10 +994,10 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
 #pragma unroll
             for (int n = 0; n < KN; n += KG) {
                 if constexpr (kLoads) {
-                    constexpr int kEach = (kParts * KG + KN - 1) / KN;  // loads a step
+                    constexpr int kEach = (NV * KG + KN - 1) / KN;  // loads a step
 #pragma unroll
                     for (int x = 0; x < kEach; ++x)
-                        if (n / KG * kEach + x < kParts) load_part(tile + 1, n / KG * kEach + x);
+                        if (n / KG * kEach + x < NV) load_v(tile + 1, n / KG * kEach + x);
                 }
                 if (n + (kAhead - 1) * KG < KN) read_k(n + (kAhead - 1) * KG);
                 __builtin_amdgcn_sched_barrier(0);
@@ -1064,6 +1058,12 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
                 for (int f0 = 0; f0 < (kAhead - 1) * VG && f0 < NF; f0 += VG) read_v(f0);
 #pragma unroll
                 for (int f0 = 0; f0 < NF; f0 += VG) {
+                    if constexpr (kLoads) {
+                        constexpr int kEach = (kPartsK * VG + NF - 1) / NF;
+#pragma unroll
+                        for (int x = 0; x < kEach; ++x)
+                            if (b == 0 && f0 / VG * kEach + x < kPartsK) load_k(tile + 1, f0 / VG * kEach + x);
+                    }
                     if (f0 + (kAhead - 1) * VG < NF) read_v(f0 + (kAhead - 1) * VG);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -1084,7 +1084,9 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
             for (int s0 = SP; s0 < T && pc.p0 + tile * T + s0 < pc.p1; s0 += SP) chunk(s0, std::false_type{});
         } else {
 #pragma unroll
-            for (int n = 0; n < kParts; ++n) load_part(tile + 1, n);
+            for (int j = 0; j < NV; ++j) load_v(tile + 1, j);
+#pragma unroll
+            for (int n = 0; n < kPartsK; ++n) load_k(tile + 1, n);
             id2 = page_ids(tile + 2);
         }
         store_v(tile + 1);
@@ -1119,7 +1121,7 @@ struct Shared {
     int rows;           // rows x group
     bool few;           // stream items
     int lo, hi;         // positions any row sees
-    int units, items;   // units an item, with a stream item's own cost
+    int units, items;   // units an item, with its own cost
 };
 
 template <int T, int ROWS, int UNIT>
@@ -1131,15 +1133,15 @@ __device__ __forceinline__ Shared shared_work(const PagedAttn &a, const Scan<T> 
     p.hi = a.prefix_len;
     p.lo = a.window && t.low < INT32_MAX ? min(max(a.prefix_len + t.low - a.window + 1, 0), p.hi) : 0;
     p.items = (p.few ? (p.rows + kRowsA - 1) / kRowsA : (p.rows + ROWS - 1) / (ROWS ? ROWS : 1)) * a.n_kv_heads;
-    p.units = p.few ? units_of<kUnitA>(p.lo, p.hi) + kItemCost : units_of<UNIT>(p.lo, p.hi);
+    p.units = p.few ? units_of<kUnitA>(p.lo, p.hi) + kItemCost : units_of<UNIT>(p.lo, p.hi) + kBlockItemCost;
     if (a.prefix_len == 0) p.items = 0;
     return p;
 }
 
 // The piece at unit u of the stream or block items, at most `left` units long;
 // returns the units taken, the item's index, and whether the piece holds its
-// first and last positions.  A stream item's own cost stands before its
-// first unit: a share that ends there has no piece of it (none).
+// first and last positions.  An item's own cost stands before its first
+// unit: a share that ends there has no piece of it (none).
 template <bool BLOCK, int T, int ROWS, int UNIT>
 __device__ __forceinline__ int find_piece(const PagedAttn &a, const Parts &parts, const Scan<T> &s, const Shared &sh,
                                           int u, int left, Piece &pc, int &item, bool &is_first, bool &is_last,
@@ -1181,7 +1183,7 @@ __device__ __forceinline__ int find_piece(const PagedAttn &a, const Parts &parts
         } else {
             for (blk = 0;; ++blk) {
                 tile_range<ROWS>(a, q, blk, lo, hi);
-                units = units_of<UNIT>(lo, hi);
+                units = units_of<UNIT>(lo, hi) + kBlockItemCost;
                 if (u < units * a.n_kv_heads) break;
                 u -= units * a.n_kv_heads;
             }
@@ -1194,7 +1196,7 @@ __device__ __forceinline__ int find_piece(const PagedAttn &a, const Parts &parts
     }
     units = uni(units);
     within = uni(within);
-    const int take = min(units - within, left), cost = BLOCK ? 0 : kItemCost;
+    const int take = min(units - within, left), cost = BLOCK ? kBlockItemCost : kItemCost;
     const int from = max(within - cost, 0), to = max(within + take - cost, 0);
     item = uni(item);
     pc.table = pc.pre ? a.prefix : a.table + (size_t)uni(r) * a.table_stride;
@@ -1267,6 +1269,7 @@ __global__ __launch_bounds__(64 * waves_of(DP, KQ || VQ)) void paged_attn_kernel
             const int quota = uni(div_fast(ub + wb - 1, wb, rest)), end = min(ub, (wg + 1) * quota);
             for (int u = wg * quota; u < end;) {
                 u += find_piece<true, T, kRowsB, kUnitB>(a, parts, s, sh, u, end - u, pc, item, first, last, none);
+                if (none) continue;
                 const size_t row = (size_t)wg * kRowsB;
                 const Dest to = first ? Dest{parts.o[!pc.pre], parts.ml[!pc.pre], true}
                                       : Dest{parts.o_b + row * a.head_dim, parts.ml_b + row, false};
