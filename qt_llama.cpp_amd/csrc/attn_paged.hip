@@ -52,7 +52,7 @@ constexpr float kBlockCost = 0.15f;
 
 // Waves of a workgroup, rows of a block item and positions of its tile by padded head size: two waves a SIMD
 // while a wave's q and o fit 256 registers.
-constexpr int waves_of(int dp, bool quant) { return quant || dp > 256 ? 4 : 8; }
+constexpr int waves_of(int dp, bool quant) { return dp > (quant ? 128 : 256) ? 4 : 8; }
 constexpr int tiles_of(int dp) { return dp > 128 ? 1 : 2; }  // row tiles of 16 a wave
 constexpr int rows_b(int dp) { return waves_of(dp, false) * tiles_of(dp) * 16; }
 constexpr int unit_b(int dp) { return 16384 / dp; }
@@ -510,10 +510,12 @@ __device__ __forceinline__ int chunk_piece(int lane) { return (lane & 3) ^ (lane
 
 __device__ __forceinline__ half8 read16(const uint8_t *p) { return __builtin_bit_cast(half8, *reinterpret_cast<const uint4 *>(p)); }
 
+// ONCE: with the non-temporal hint.
+template <bool ONCE>
 __device__ __forceinline__ void load_to_lds(const uint8_t *src, uint8_t *dst)
 {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)src,
-                                     (__attribute__((address_space(3))) uint32_t *)dst, 16, 0, 0);
+                                     (__attribute__((address_space(3))) uint32_t *)dst, 16, 0, ONCE ? 2 : 0);
 }
 
 struct __attribute__((packed, aligned(2))) Bytes8 {
@@ -581,6 +583,9 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
                                             WaveLds<DP, KQ> &lds, const Dest &to)
 {
     constexpr int KS = DP / 32, NG = DP < 128 ? 1 : DP / 128;
+    // f16 caches are streamed past the caches: at most two row tiles read the same rows there, while all tiles of a
+    // quantised one do (256 x 1000 positions of 256 dims: 211 us against 224; 4 x 32000 of 8 heads of 128: 107 against 116)
+    constexpr bool kOnce = !KQ && !VQ;
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, hd = a.head_dim;
     const int mi = pc.row0 + i;
     const bool live = mi < pc.rows;
@@ -636,7 +641,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
                 const uint8_t *row = k_rows.row(__shfl(place, 16 * h + chunk_row(ln), 64)) + piece;
 #pragma unroll
                 for (int s = 0; s < KS; ++s)
-                    load_to_lds(row + (s * 32 < hd ? s * 64 : 0), lds.k + (h * KS + s) * kChunk);
+                    load_to_lds<kOnce>(row + (s * 32 < hd ? s * 64 : 0), lds.k + (h * KS + s) * kChunk);
             }
         }
     };
@@ -661,7 +666,8 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
                     vd[n][j] = *reinterpret_cast<const _Float16 *>(b);
                     vq[n][j] = *reinterpret_cast<const Bytes8 *>(b + 2 + (a.v_fmt == 1 ? 8 * (i & 3) : 8 * (i & 1)));
                 } else {
-                    v[n][j] = *reinterpret_cast<const uint4 *>(row + dim * 2);
+                    const uint4 *src = reinterpret_cast<const uint4 *>(row + dim * 2);
+                    v[n][j] = kOnce ? load_stream16(src) : *src;
                 }
             }
         }
@@ -895,7 +901,7 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
         const int grp = T / 16 >= NW ? wave * GW + n / SW : wave * (T / 16) / NW;
         const int s = (T / 16 >= NW ? 0 : wave * SW % KS) + n % SW, ln = here(lane);
         const uint8_t *row = k_rows.row(lds.place[tile % 3][grp * 16 + chunk_row(ln)]);
-        load_to_lds(row + chunk_piece(ln) * 16 + (s * 32 < hd ? s * 64 : 0), lds.k[tile & 1][grp][s]);
+        load_to_lds<false>(row + chunk_piece(ln) * 16 + (s * 32 < hd ? s * 64 : 0), lds.k[tile & 1][grp][s]);
     };
     // V: this thread's 8 dims and NV positions: a run of 8 in the products' order (run0 + 0..3, run0 + 16..19) or
     // half of one
@@ -1342,21 +1348,20 @@ __device__ __forceinline__ void slow_row(const PagedAttn &a, int row, int r, int
     }
 }
 
-// Joins the parts of each row and head.  W waves share a row and head (1 where
-// there are many rows, each in few parts; 4 where a few rows are in many),
-// lane groups take a part each, a lane four dims of it.  Three round trips: where
-// the parts are, their (m, l), their values.
+// Joins the parts of each row and head.  W waves share a row and head, lane groups
+// take a part each, a lane four dims of it, with a running maximum of their own; lane groups and waves
+// join as parts do.  Two round trips: where the parts are, then the parts.
 template <int W>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a, Parts parts)
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void paged_merge_kernel(PagedAttn a, Parts parts)
 {
-    constexpr int kAhead = 3;
-    __shared__ float s_o[4][512], s_q[4][512], s_l[4], s_m[4];
+    constexpr int kAhead = 3, kWaves = W == 1 ? 4 : W;
+    __shared__ float s_o[kWaves][512], s_q[kWaves][512], s_l[kWaves], s_m[kWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6), hd = a.head_dim;
-    const int pair = blockIdx.x * (4 / W) + wave / W, row = pair / a.n_heads, h = pair - row * a.n_heads;
+    const int pair = blockIdx.x * (kWaves / W) + wave / W, row = pair / a.n_heads, h = pair - row * a.n_heads;
     if (row >= a.max_rows) return;  // W == 1: the last workgroup's spare waves (no barrier there)
     const int4 head = *reinterpret_cast<const int4 *>(parts.head);
     const int4 ri = parts.row_item[row];
-    if (!head.x || row < head.y || row >= head.z) return;  // W == 4: the whole workgroup
+    if (!head.x || row < head.y || row >= head.z) return;  // W > 1: the whole workgroup
     const int kvh = div_group(a, h), gq = h - kvh * a.group;
     const size_t base = (size_t)row * a.n_heads + h;
     // the two items of the row: the prefix's, its own
@@ -1386,92 +1391,106 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn a, Parts par
     // lanes over dims (four each; heads beyond 256 dims in two turns), lane groups over parts
     const int lanes = hd <= 32 ? 8 : hd <= 64 ? 16 : hd <= 128 ? 32 : 64, groups = 64 / lanes * W;
     const int sub = (wave % W) * (64 / lanes) + lane / lanes, d0 = (lane % lanes) * 4;
-    float top = -INFINITY;
     bool broken = false;
-    for (int k = lane; k < total; k += 64) {  // the largest m of parts that saw something
-        const float *po;
-        const float2 *pml;
-        part(k, po, pml);
-        const float2 ml = *pml;
-        if (ml.y != 0.0f) top = fmaxf(top, ml.x);
-        broken |= ml.y < 0.0f;
-    }
     float4 o[2] = {};
-    float l = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    for (int k0 = sub; k0 < total; k0 += groups * kAhead) {
+        float4 v[kAhead][2];
+        float2 ml[kAhead];
 #pragma unroll
-    for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
-    if (__any(broken)) {
-        slow_row(a, row, ri.x, h, wave % W, W, s_q[wave], s_o[wave], top, l);
-        if constexpr (W == 4) {
-            if (lane == 0) s_m[wave] = top;
-            __syncthreads();
-            const float most = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-            const float f = l == 0.0f ? 0.0f : exp2f(top - most);
-            for (int d = lane; d < hd; d += 64) s_o[wave][d] = f == 0.0f ? 0.0f : s_o[wave][d] * f;
-            if (lane == 0) s_l[wave] = f == 0.0f ? 0.0f : l * f;
-        } else {
+        for (int e = 0; e < kAhead; ++e) {
+            const float *po;
+            const float2 *pml;
+            const int k = k0 + e * groups;
+            part(min(k, total - 1), po, pml);
+            ml[e] = k < total ? *pml : make_float2(0.0f, 0.0f);
+            v[e][0] = d0 < hd ? *reinterpret_cast<const float4 *>(po + d0) : make_float4(0, 0, 0, 0);
+            v[e][1] = d0 + 256 < hd ? *reinterpret_cast<const float4 *>(po + d0 + 256) : make_float4(0, 0, 0, 0);
+        }
+        float m2 = m;
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+            broken |= ml[e].y < 0.0f;
+            if (ml[e].y != 0.0f) m2 = fmaxf(m2, ml[e].x);
+        }
+        if (m2 == -INFINITY) continue;  // nothing seen so far
+        const float f = exp2_hw(m - m2);
+        m = m2;
+        l *= f;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) o[x] = make_float4(o[x].x * f, o[x].y * f, o[x].z * f, o[x].w * f);
+#pragma unroll
+        for (int e = 0; e < kAhead; ++e) {
+            if (ml[e].y == 0.0f) continue;  // saw nothing
+            const float w = exp2_hw(ml[e].x - m);
+            l += ml[e].y * w;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                o[x].x += v[e][x].x * w;
+                o[x].y += v[e][x].y * w;
+                o[x].z += v[e][x].z * w;
+                o[x].w += v[e][x].w * w;
+            }
+        }
+    }
+    broken = __any(broken);
+    if (lanes < 64) {
+        float m2 = m;
+        for (int x = lanes; x < 64; x <<= 1) m2 = fmaxf(m2, __shfl_xor(m2, x, 64));
+        const float f = m == -INFINITY ? 0.0f : exp2_hw(m - m2);
+        m = m2;
+        l *= f;
+        o[0] = make_float4(o[0].x * f, o[0].y * f, o[0].z * f, o[0].w * f);  // o[1]: past 256 dims alone
+        for (int x = lanes; x < 64; x <<= 1) {
+            l += __shfl_xor(l, x, 64);
+            o[0].x += __shfl_xor(o[0].x, x, 64);
+            o[0].y += __shfl_xor(o[0].y, x, 64);
+            o[0].z += __shfl_xor(o[0].z, x, 64);
+            o[0].w += __shfl_xor(o[0].w, x, 64);
+        }
+    }
+    if constexpr (W == 1) {
+        if (broken) {
+            slow_row(a, row, ri.x, h, 0, 1, s_q[wave], s_o[wave], m, l);
             for (int d = lane; d < hd; d += 64) a.out[base * hd + d] = l == 0.0f ? 0.0f : s_o[wave][d] / l;
             return;
         }
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            const int d = d0 + 256 * y;
+            if (lane < lanes && d < hd)
+                *reinterpret_cast<float4 *>(a.out + base * hd + d) =
+                    l == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(o[y].x / l, o[y].y / l, o[y].z / l, o[y].w / l);
+        }
     } else {
-        for (int k0 = sub; k0 < total; k0 += groups * kAhead) {
-            float4 v[kAhead][2];
-            float2 ml[kAhead];
-#pragma unroll
-            for (int e = 0; e < kAhead; ++e) {
-                const float *po;
-                const float2 *pml;
-                const int k = k0 + e * groups;
-                part(min(k, total - 1), po, pml);
-                ml[e] = k < total ? *pml : make_float2(0.0f, 0.0f);
-                v[e][0] = d0 < hd ? *reinterpret_cast<const float4 *>(po + d0) : make_float4(0, 0, 0, 0);
-                v[e][1] = d0 + 256 < hd ? *reinterpret_cast<const float4 *>(po + d0 + 256) : make_float4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int e = 0; e < kAhead; ++e) {
-                if (ml[e].y == 0.0f) continue;  // saw nothing
-                const float w = exp2_hw(ml[e].x - top);
-                l += ml[e].y * w;
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    o[x].x += v[e][x].x * w;
-                    o[x].y += v[e][x].y * w;
-                    o[x].z += v[e][x].z * w;
-                    o[x].w += v[e][x].w * w;
-                }
-            }
+        if (lane < lanes) {
+            if (d0 < hd) *reinterpret_cast<float4 *>(&s_o[wave][d0]) = o[0];
+            if (d0 + 256 < hd) *reinterpret_cast<float4 *>(&s_o[wave][d0 + 256]) = o[1];
         }
-        for (int x = lanes; x < 64; x <<= 1) {
-            l += __shfl_xor(l, x, 64);
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                o[y].x += __shfl_xor(o[y].x, x, 64);
-                o[y].y += __shfl_xor(o[y].y, x, 64);
-                o[y].z += __shfl_xor(o[y].z, x, 64);
-                o[y].w += __shfl_xor(o[y].w, x, 64);
-            }
+        if (lane == 0) {
+            s_m[wave] = m;
+            s_l[wave] = l;
         }
-        if constexpr (W == 4) {
-            if (lane < lanes) {
-                if (d0 < hd) *reinterpret_cast<float4 *>(&s_o[wave][d0]) = o[0];
-                if (d0 + 256 < hd) *reinterpret_cast<float4 *>(&s_o[wave][d0 + 256]) = o[1];
-                if (lane == 0) s_l[wave] = l;
+        if (__syncthreads_or(broken)) {
+            slow_row(a, row, ri.x, h, wave, W, s_q[wave], s_o[wave], m, l);
+            if (lane == 0) {
+                s_m[wave] = m;
+                s_l[wave] = l;
             }
-        } else {
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                const int d = d0 + 256 * y;
-                if (lane < lanes && d < hd)
-                    *reinterpret_cast<float4 *>(a.out + base * hd + d) =
-                        l == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(o[y].x / l, o[y].y / l, o[y].z / l, o[y].w / l);
-            }
+            __syncthreads();
         }
-    }
-    if constexpr (W == 4) {
-        __syncthreads();
-        const float sum = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
-        for (int d = tid; d < hd; d += 256) {
-            const float x = (s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d]);
+        float most = s_m[0], sum = 0.0f, f[W];
+#pragma unroll
+        for (int w = 1; w < W; ++w) most = fmaxf(most, s_m[w]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            f[w] = s_l[w] == 0.0f ? 0.0f : exp2_hw(s_m[w] - most);
+            sum += f[w] == 0.0f ? 0.0f : s_l[w] * f[w];
+        }
+        for (int d = tid; d < hd; d += 64 * W) {
+            float x = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) x += f[w] == 0.0f ? 0.0f : s_o[w][d] * f[w];
             a.out[base * hd + d] = sum == 0.0f ? 0.0f : x / sum;
         }
     }
@@ -1569,8 +1588,10 @@ int launch_paged_attn(mrml_hip_ctx *ctx, const PagedAttn &a, void *scratch)
     const int pairs = a.max_rows * a.n_heads;
     if (pairs > 4096)
         hipLaunchKernelGGL(paged_merge_kernel<1>, dim3((pairs + 3) / 4), dim3(256), 0, ctx->stream, a, p);
-    else
+    else if (pairs > 256)
         hipLaunchKernelGGL(paged_merge_kernel<4>, dim3(pairs), dim3(256), 0, ctx->stream, a, p);
+    else
+        hipLaunchKernelGGL(paged_merge_kernel<16>, dim3(pairs), dim3(1024), 0, ctx->stream, a, p);
     return check_launch(ctx, "paged_merge_kernel");
 }
 
