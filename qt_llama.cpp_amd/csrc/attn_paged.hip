@@ -578,14 +578,11 @@ __device__ __forceinline__ void load_quant_q(const PagedAttn &a, const float *ro
     }
 }
 
-template <int DP, bool KQ, bool VQ>
+template <int DP, bool KQ, bool VQ, bool ONCE>
 __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * waves_of(DP, KQ || VQ)> &sc, bool need_at, const Piece &pc,
                                             WaveLds<DP, KQ> &lds, const Dest &to)
 {
     constexpr int KS = DP / 32, NG = DP < 128 ? 1 : DP / 128;
-    // f16 caches are streamed past the caches: at most two row tiles read the same rows there, while all tiles of a
-    // quantised one do (256 x 1000 positions of 256 dims: 211 us against 224; 4 x 32000 of 8 heads of 128: 107 against 116)
-    constexpr bool kOnce = !KQ && !VQ;
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, hd = a.head_dim;
     const int mi = pc.row0 + i;
     const bool live = mi < pc.rows;
@@ -641,7 +638,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
                 const uint8_t *row = k_rows.row(__shfl(place, 16 * h + chunk_row(ln), 64)) + piece;
 #pragma unroll
                 for (int s = 0; s < KS; ++s)
-                    load_to_lds<kOnce>(row + (s * 32 < hd ? s * 64 : 0), lds.k + (h * KS + s) * kChunk);
+                    load_to_lds<ONCE>(row + (s * 32 < hd ? s * 64 : 0), lds.k + (h * KS + s) * kChunk);
             }
         }
     };
@@ -667,7 +664,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
                     vq[n][j] = *reinterpret_cast<const Bytes8 *>(b + 2 + (a.v_fmt == 1 ? 8 * (i & 3) : 8 * (i & 1)));
                 } else {
                     const uint4 *src = reinterpret_cast<const uint4 *>(row + dim * 2);
-                    v[n][j] = kOnce ? load_stream16(src) : *src;
+                    v[n][j] = ONCE ? load_stream16(src) : *src;
                 }
             }
         }
@@ -1230,8 +1227,12 @@ struct KernelLds<DP, KQ, false> {
     WaveLds<DP, KQ> wave[waves_of(DP, true)];
 };
 
-// Quantised caches have stream items alone.
-template <int DP, bool KQ, bool VQ>
+// Quantised caches have stream items alone.  ONCE: K and V of stream items are
+// loaded with the non-temporal hint, which pays where the requests' own positions are all there is
+// (256 x 1000 positions of 4 heads of 256 dims: 212 us against 223; 4 x 32000 of 8 heads of 128: 107
+// against 116) and not beside a prefix's blocks (256 requests of 300 positions behind 8192: 225 us against 218).
+// At most two row tiles read the same rows of an f16 cache so; of a quantised one all do.
+template <int DP, bool KQ, bool VQ, bool ONCE>
 __global__ __launch_bounds__(64 * waves_of(DP, KQ || VQ)) void paged_attn_kernel(PagedAttn a, Parts parts)
 {
     constexpr bool kBlocks = !KQ && !VQ;
@@ -1297,7 +1298,7 @@ __global__ __launch_bounds__(64 * waves_of(DP, KQ || VQ)) void paged_attn_kernel
                               : Dest{parts.o_a + row * a.head_dim, parts.ml_a + row, false};
         if ((tid & 63) == 0 && first) parts.first[item] = worker;
         if ((tid & 63) == 0 && last) parts.last[item] = worker;
-        stream_item<DP, KQ, VQ>(a, s, totals.need_at, pc, lds.wave[wave], to);
+        stream_item<DP, KQ, VQ, ONCE>(a, s, totals.need_at, pc, lds.wave[wave], to);
     }
 }
 
@@ -1542,14 +1543,16 @@ void launch_dp(mrml_hip_ctx *ctx, const PagedAttn &a, const Parts &p)
 {
     const dim3 grid(p.wgs), block(64 * p.waves);
     const bool kq = a.k_fmt != 0, vq = a.v_fmt != 0;
-    if (!kq && !vq)
-        hipLaunchKernelGGL((paged_attn_kernel<DP, false, false>), grid, block, 0, ctx->stream, a, p);
+    if (!kq && !vq && a.prefix_len == 0)
+        hipLaunchKernelGGL((paged_attn_kernel<DP, false, false, true>), grid, block, 0, ctx->stream, a, p);
+    else if (!kq && !vq)
+        hipLaunchKernelGGL((paged_attn_kernel<DP, false, false, false>), grid, block, 0, ctx->stream, a, p);
     else if (!kq)
-        hipLaunchKernelGGL((paged_attn_kernel<DP, false, true>), grid, block, 0, ctx->stream, a, p);
+        hipLaunchKernelGGL((paged_attn_kernel<DP, false, true, false>), grid, block, 0, ctx->stream, a, p);
     else if (!vq)
-        hipLaunchKernelGGL((paged_attn_kernel<DP, true, false>), grid, block, 0, ctx->stream, a, p);
+        hipLaunchKernelGGL((paged_attn_kernel<DP, true, false, false>), grid, block, 0, ctx->stream, a, p);
     else
-        hipLaunchKernelGGL((paged_attn_kernel<DP, true, true>), grid, block, 0, ctx->stream, a, p);
+        hipLaunchKernelGGL((paged_attn_kernel<DP, true, true, false>), grid, block, 0, ctx->stream, a, p);
 }
 
 }  // namespace
