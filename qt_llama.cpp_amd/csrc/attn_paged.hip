@@ -52,9 +52,12 @@ constexpr float kBlockCost = 0.15f;
 
 // Waves of a workgroup, rows of a block item and positions of its tile by padded head size: two waves a SIMD
 // while a wave's q and o fit 256 registers.
-constexpr int waves_of(int dp, bool quant) { return dp > (quant ? 128 : 256) ? 4 : 8; }
+constexpr int waves_of(int dp, int kf, int vf)
+{
+    return dp > 256 && vf && !kf ? 2 : dp > (kf || vf ? 128 : 256) ? 4 : 8;  // 2: both tiles of 4 would not fit LDS
+}
 constexpr int tiles_of(int dp) { return dp > 128 ? 1 : 2; }  // row tiles of 16 a wave
-constexpr int rows_b(int dp) { return waves_of(dp, false) * tiles_of(dp) * 16; }
+constexpr int rows_b(int dp) { return waves_of(dp, 0, 0) * tiles_of(dp) * 16; }
 constexpr int unit_b(int dp) { return 16384 / dp; }
 
 // Device scratch of a call (paged_attn_scratch_bytes).
@@ -524,15 +527,91 @@ struct __attribute__((packed, aligned(2))) Bytes8 {
 
 constexpr int kTrRow = 36;  // floats a query row of the score tile in LDS
 
-template <int DP, bool KQ>
-struct WaveLds {
-    int place[32];
-    alignas(16) uint8_t k[DP / 16 * kChunk];  // 32 positions: chunks of 32 dims, of 16 positions
+constexpr int block_bytes(int fmt) { return fmt == 1 ? 34 : 18; }
+
+// A tile of a quantised cache: 32 rows as they lie in memory.  A wave fetches them in
+// 16-byte pieces, neighbouring lanes neighbouring pieces, and picks the blocks out of LDS: lanes that
+// fetch their 8 bytes of a block each make an access to the cache each (1578 a tile of 32
+// positions of 128 dims, 94% of the time the caches could take them in).  A row's last piece
+// ends with the row.  Rows are an odd number of 32 bytes apart: 8 of them fill the 64 banks.
+template <int DP, int FMT>
+struct QuantTile {
+    static constexpr int kRow = ((DP / 32 * block_bytes(FMT) + 31) / 32 | 1) * 32;
+    static constexpr int kPieces = (DP / 32 * block_bytes(FMT) + 15) / 16;  // of a row, at most
+    static constexpr int kLoads = (32 * kPieces + 63) / 64;
+    alignas(16) uint8_t b[32 * kRow];
 };
-template <int DP>
-struct WaveLds<DP, true> {
-    int place[32];
-    float scores[16 * kTrRow];
+
+struct __attribute__((packed, aligned(2))) Bytes16 {
+    uint32_t x, y, z, w;
+};
+
+// A wave's pieces of such a tile: where they lie and, on their way, what they hold.
+template <int DP, int FMT>
+struct QuantPieces {
+    using Tile = QuantTile<DP, FMT>;
+    uint32_t at[Tile::kLoads];  // row << 16 | byte in it
+    uint4 x[Tile::kLoads];
+    __device__ __forceinline__ void start(int row_bytes, int lane)
+    {
+        const int pieces = (row_bytes + 15) / 16;
+        int rest;
+        const int step_row = 64 / pieces, step = 64 - step_row * pieces;
+        int row = div_fast(lane, pieces, rest);
+#pragma unroll
+        for (int e = 0; e < Tile::kLoads; ++e) {  // past the tile: its last piece once more
+            at[e] = row < 32 ? (uint32_t)row << 16 | (uint32_t)min(rest * 16, row_bytes - 16) : 31u << 16 | (uint32_t)(row_bytes - 16);
+            row += step_row;
+            rest += step;
+            if (rest >= pieces) rest -= pieces, ++row;
+        }
+    }
+    __device__ __forceinline__ void load(const HeadRows &rows, int place)
+    {
+#pragma unroll
+        for (int e = 0; e < Tile::kLoads; ++e) {
+            const Bytes16 y = *reinterpret_cast<const Bytes16 *>(rows.row(__shfl(place, at[e] >> 16, 64)) + (at[e] & 0xffff));
+            x[e] = make_uint4(y.x, y.y, y.z, y.w);
+        }
+    }
+    // LDS takes an access apart whose address is no multiple of its size (28 cycles each): a last piece that ends
+    // with its row is written in what both share.
+    __device__ __forceinline__ void store(Tile &tile, int row_bytes) const
+    {
+#pragma unroll
+        for (int e = 0; e < Tile::kLoads; ++e) {
+            uint8_t *dst = tile.b + (at[e] >> 16) * Tile::kRow + (at[e] & 0xffff);
+            const uint32_t w[4] = {x[e].x, x[e].y, x[e].z, x[e].w};
+            if ((row_bytes & 15) == 0) {
+                *reinterpret_cast<uint4 *>(dst) = x[e];
+            } else if ((row_bytes & 3) == 0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) ((volatile __attribute__((address_space(3))) uint32_t *)dst)[j] = w[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    ((volatile __attribute__((address_space(3))) uint16_t *)dst)[j] = (uint16_t)(w[j / 2] >> 16 * (j & 1));
+            }
+        }
+    }
+};
+// 8 bytes at p + at, at even: of the words around them.
+__device__ __forceinline__ Bytes8 pick8(const uint8_t *p, int at)
+{
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(p + (at & ~2));
+    const uint32_t w0 = w[0], w1 = w[1], w2 = w[2];
+    return Bytes8{__builtin_amdgcn_alignbyte(w1, w0, at & 2), __builtin_amdgcn_alignbyte(w2, w1, at & 2)};
+}
+
+struct None {};
+
+template <int DP, int KF, int VF>
+struct WaveLds {
+    int place[VF ? 1 : 32];
+    alignas(16) uint8_t k[KF ? 16 : DP / 16 * kChunk];  // 32 positions: chunks of 32 dims, of 16 positions
+    float scores[KF ? 16 * kTrRow : 1];
+    std::conditional_t<KF != 0, QuantTile<DP, KF ? KF : 1>, None> kq;
+    std::conditional_t<VF != 0, QuantTile<DP, VF ? VF : 1>, None> vq;
 };
 
 // Query rows for a quantised K: operand bytes, and scale and sum of each block
@@ -544,7 +623,7 @@ struct QuantQ {
     int4v sum8[KS];  // -8 * sum of the block's quants: what Q4_0's offset takes away
 };
 
-template <int KS>
+template <int KS, int KF>
 __device__ __forceinline__ void load_quant_q(const PagedAttn &a, const float *row, bool live, int g, QuantQ<KS> &out)
 {
 #pragma unroll
@@ -573,15 +652,16 @@ __device__ __forceinline__ void load_quant_q(const PagedAttn &a, const float *ro
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             out.d[s][r] = __shfl(a.scale < 0.0f ? -d : d, 4 * g + r, 64);
-            out.sum8[s][r] = a.k_fmt == 2 ? -8 * __shfl(sum, 4 * g + r, 64) : 0;
+            out.sum8[s][r] = KF == 2 ? -8 * __shfl(sum, 4 * g + r, 64) : 0;
         }
     }
 }
 
-template <int DP, bool KQ, bool VQ, bool ONCE>
-__device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * waves_of(DP, KQ || VQ)> &sc, bool need_at, const Piece &pc,
-                                            WaveLds<DP, KQ> &lds, const Dest &to)
+template <int DP, int KF, int VF, bool ONCE>
+__device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * waves_of(DP, KF, VF)> &sc, bool need_at, const Piece &pc,
+                                            WaveLds<DP, KF, VF> &lds, const Dest &to)
 {
+    constexpr bool KQ = KF != 0, VQ = VF != 0;
     constexpr int KS = DP / 32, NG = DP < 128 ? 1 : DP / 128;
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, hd = a.head_dim;
     const int mi = pc.row0 + i;
@@ -592,14 +672,14 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
     QuantQ<KQ ? KS : 1> qq;
     float c = score_factor(a);
     if constexpr (KQ)
-        load_quant_q<KS>(a, q_row, live, g, qq);
+        load_quant_q<KS, KF>(a, q_row, live, g, qq);
     else
         c = fmaxf(c * load_q<KS>(a, q_row, live, g, qh, ql), 0x1p-126f);
     int vlo, vhi;
     row_sees(a, sc, need_at, pc, mi, vlo, vhi);
     const int full_lo = wave_max(vlo), full_hi = wave_min(vhi);
     const HeadRows k_rows = head_rows(a, a.k, a.k_fmt, pc.kvh), v_rows = head_rows(a, a.v, a.v_fmt, pc.kvh);
-    const int kblk = a.k_fmt == 1 ? 34 : 18, vblk = a.v_fmt == 1 ? 34 : 18;
+    constexpr int kBlkK = block_bytes(KF), kBlkV = block_bytes(VF);
 
     float m = -INFINITY, l = 0.0f;
     float4v o[NG][8];
@@ -617,20 +697,18 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
         if (place < 0 && pos < pc.p1 && lane < 32) page_fault(a.faults);
         return place;
     };
-    Bytes8 kq[KQ ? 2 : 1][KQ ? KS : 1];
-    uint16_t kd[KQ ? 2 : 1][KQ ? KS : 1];
+    std::conditional_t<KQ, QuantPieces<DP, KF ? KF : 1>, None> k_on_way;
+    std::conditional_t<VQ, QuantPieces<DP, VF ? VF : 1>, None> v_on_way;
+    if constexpr (KQ) {
+        k_on_way.start(kv_row_bytes(KF, hd), lane);
+        if (hd < DP)  // blocks past the head: scales and quants of 0
+            for (int x = kv_row_bytes(KF, hd) / 2 + (lane >> 5); x < KS * kBlkK / 2; x += 2)
+                *reinterpret_cast<uint16_t *>(lds.kq.b + (lane & 31) * lds.kq.kRow + 2 * x) = 0;
+    }
+    if constexpr (VQ) v_on_way.start(kv_row_bytes(VF, hd), lane);
     auto load_k = [&](int place) {
         if constexpr (KQ) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint8_t *row = k_rows.row(__shfl(place, 16 * h + i, 64));
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const uint8_t *b = row + (s * 32 < hd ? s * kblk : 0);
-                    kd[h][s] = *reinterpret_cast<const uint16_t *>(b);
-                    kq[h][s] = *reinterpret_cast<const Bytes8 *>(b + 2 + (a.k_fmt == 1 ? 8 * g : 8 * (g & 1)));
-                }
-            }
+            k_on_way.load(k_rows, place);
         } else {
             const int ln = here(lane), piece = chunk_piece(ln) * 16;
 #pragma unroll
@@ -643,9 +721,11 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
         }
     };
     uint4 v[VQ ? 1 : NG][8];
-    Bytes8 vq[VQ ? NG : 1][8];
-    _Float16 vd[VQ ? NG : 1][8];
     auto load_v = [&](int place) {
+        if constexpr (VQ) {
+            v_on_way.load(v_rows, place);
+            return;
+        } else {
         lds.place[lane & 31] = place;
         __builtin_amdgcn_wave_barrier();
         const int4 pa = *reinterpret_cast<const int4 *>(lds.place + 4 * g);
@@ -657,16 +737,10 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
             const int d0 = n * 128 + 8 * (here(lane) & 15), dim = d0 < hd ? d0 : 0;  // past the head: never stored
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const uint8_t *row = v_rows.row(pl[j]);
-                if constexpr (VQ) {
-                    const uint8_t *b = row + (dim >> 5) * vblk;
-                    vd[n][j] = *reinterpret_cast<const _Float16 *>(b);
-                    vq[n][j] = *reinterpret_cast<const Bytes8 *>(b + 2 + (a.v_fmt == 1 ? 8 * (i & 3) : 8 * (i & 1)));
-                } else {
-                    const uint4 *src = reinterpret_cast<const uint4 *>(row + dim * 2);
-                    v[n][j] = ONCE ? load_stream16(src) : *src;
-                }
+                const uint4 *src = reinterpret_cast<const uint4 *>(v_rows.row(pl[j]) + dim * 2);
+                v[n][j] = ONCE ? load_stream16(src) : *src;
             }
+        }
         }
     };
     int id_next = page_ids(pc.p0 + kUnitA);
@@ -680,19 +754,28 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
         id_next = page_ids(t0 + 2 * kUnitA);
         float x[8];
         if constexpr (KQ) {
+            k_on_way.store(lds.kq, kv_row_bytes(KF, hd));
+            __builtin_amdgcn_wave_barrier();
+            if (t0 + kUnitA < pc.p1) load_k(place_next);
             float4v acc[2] = {};
+            const uint8_t *rows = lds.kq.b + i * lds.kq.kRow;
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    uint32_t w0 = kq[h][s].a, w1 = kq[h][s].b;
-                    if (a.k_fmt == 2) {  // dims 8 g .. of the block: low nibbles, then high ones
+                    const uint8_t *b = rows + 16 * h * lds.kq.kRow + s * kBlkK;
+                    const uint8_t *quants = b + (KF == 1 ? 8 * g : 8 * (g & 1));
+                    const Bytes8 w = s & 1 ? Bytes8{reinterpret_cast<const uint32_t *>(quants + 2)[0],
+                                                    reinterpret_cast<const uint32_t *>(quants + 2)[1]}
+                                           : pick8(quants, 2);
+                    uint32_t w0 = w.a, w1 = w.b;
+                    if (KF == 2) {  // dims 8 g .. of the block: low nibbles, then high ones
                         w0 = (w0 >> (4 * (g >> 1))) & 0x0f0f0f0fu;
                         w1 = (w1 >> (4 * (g >> 1))) & 0x0f0f0f0fu;
                     }
                     const long kk = (long)((uint64_t)w0 | ((uint64_t)w1 << 32));
                     const int4v is = __builtin_amdgcn_mfma_i32_16x16x32_i8(qq.q[s], kk, qq.sum8[s], 0, 0, 0);
-                    const float dk = f16_bits_to_f32(kd[h][s]);
+                    const float dk = f16_bits_to_f32(*reinterpret_cast<const uint16_t *>(b));
 #pragma unroll
                     for (int r = 0; r < 4; ++r) acc[h][r] = fmaf((float)is[r], dk * qq.d[s][r], acc[h][r]);
                 }
@@ -741,9 +824,12 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x[4 * h + r] = acc[h][0][r] + acc[h][1][r];
         }
-        pin();  // K's tile has been read, and no later load passes the next one's
-        if (t0 + kUnitA < pc.p1) load_k(place_next);
-        pin();
+        if constexpr (!KQ) {
+            pin();  // K's tile has been read, and no later load passes the next one's
+            if (t0 + kUnitA < pc.p1) load_k(place_next);
+            pin();
+        }
+        uint32_t v_there = 0xff;  // bit j: this lane's position j of V
         const bool edge = t0 < full_lo || t0 + kUnitA > full_hi || there != 0xffffffffu;
         if (edge) {
 #pragma unroll
@@ -751,18 +837,14 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
                 const int p = 16 * (e >> 2) + 4 * g + (e & 3), pos = t0 + p;
                 if (pos < vlo || pos >= vhi || !((there >> p) & 1)) x[e] = -INFINITY;
             }
+            // nothing is there: whatever was read must not meet a weight of 0
+            v_there = (there >> (4 * g) & 15) | (there >> (16 + 4 * g) & 15) << 4;
+            if constexpr (!VQ)
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (!((there >> (16 * (j >> 2) + 4 * g + (j & 3))) & 1)) {
-                    // nothing is there: whatever was read must not meet a weight of 0
+                for (int j = 0; j < 8; ++j)
+                    if (!(v_there >> j & 1))
 #pragma unroll
-                    for (int n = 0; n < NG; ++n) {
-                        if constexpr (VQ)
-                            vd[n][j] = (_Float16)0.0f;
-                        else
-                            v[n][j] = make_uint4(0, 0, 0, 0);
-                    }
-                }
+                        for (int n = 0; n < NG; ++n) v[n][j] = make_uint4(0, 0, 0, 0);
         }
         float f;
         if (softmax_step<8>(x, c, m, l, f)) {
@@ -775,11 +857,28 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
 #pragma unroll
         for (int e = 0; e < 4; ++e) split_p(x[2 * e], x[2 * e + 1], ph[e], pw[e]);
         const half8 p_hi = as_half8(ph[0], ph[1], ph[2], ph[3]), p_lo = as_half8(pw[0], pw[1], pw[2], pw[3]);
+        if constexpr (VQ) {
+            v_on_way.store(lds.vq, kv_row_bytes(VF, hd));
+            __builtin_amdgcn_wave_barrier();
+            if (t0 + kUnitA < pc.p1) load_v(place_next);
+        }
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
             if constexpr (VQ) {
+                const int d0 = n * 128 + 8 * i, dim = d0 < hd ? d0 : 0;  // past the head: never stored
+                const uint8_t *rows = lds.vq.b + 4 * g * lds.vq.kRow;
+                const int scale = (dim >> 5) * kBlkV, quants = scale + 2 + (VF == 1 ? 8 * (i & 3) : 8 * (i & 1));
+                Bytes8 vq[8];
+                _Float16 vd[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint8_t *b = rows + (16 * (j >> 2) + (j & 3)) * lds.vq.kRow;
+                    const _Float16 d = *reinterpret_cast<const _Float16 *>(b + scale);
+                    vd[j] = v_there >> j & 1 ? d : (_Float16)0.0f;
+                    vq[j] = pick8(b, quants);
+                }
                 // quants as unsigned bytes u, read as the f16 number 1024 + u, less 1024 and the bytes' offset
-                const bool q8 = a.v_fmt == 1;
+                constexpr bool q8 = VF == 1;
                 const int sh = 4 * ((i & 3) >> 1);
                 const half2v off = q8 ? half2v{(_Float16)-1152.0f, (_Float16)-1152.0f}
                                       : half2v{(_Float16)-1032.0f, (_Float16)-1032.0f};
@@ -787,11 +886,11 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
                 half2v d2[4];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    w[j][0] = q8 ? vq[n][j].a ^ 0x80808080u : (vq[n][j].a >> sh) & 0x0f0f0f0fu;
-                    w[j][1] = q8 ? vq[n][j].b ^ 0x80808080u : (vq[n][j].b >> sh) & 0x0f0f0f0fu;
+                    w[j][0] = q8 ? vq[j].a ^ 0x80808080u : (vq[j].a >> sh) & 0x0f0f0f0fu;
+                    w[j][1] = q8 ? vq[j].b ^ 0x80808080u : (vq[j].b >> sh) & 0x0f0f0f0fu;
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) d2[e] = half2v{vd[n][2 * e], vd[n][2 * e + 1]};
+                for (int e = 0; e < 4; ++e) d2[e] = half2v{vd[2 * e], vd[2 * e + 1]};
 #pragma unroll
                 for (int d = 0; d < 8; ++d) {
                     const uint32_t sel = 0x0c040c00u + 0x00010001u * (d & 3);
@@ -827,7 +926,9 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
                 }
             }
         }
-        if (t0 + kUnitA < pc.p1) load_v(place_next);
+        if constexpr (!VQ)
+            if (t0 + kUnitA < pc.p1) load_v(place_next);
+        __builtin_amdgcn_wave_barrier();
         place = place_next;
     }
     l = row_sum(l);
@@ -870,10 +971,10 @@ struct BlockLds {
 };
 
 template <int DP>
-__device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * waves_of(DP, false)> &sc, bool need_at, const Piece &pc,
+__device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * waves_of(DP, 0, 0)> &sc, bool need_at, const Piece &pc,
                                            BlockLds<DP> &lds, const Dest &to)
 {
-    constexpr int NW = waves_of(DP, false), R = tiles_of(DP), KS = DP / 32, NF = DP / 16, T = unit_b(DP);
+    constexpr int NW = waves_of(DP, 0, 0), R = tiles_of(DP), KS = DP / 32, NF = DP / 16, T = unit_b(DP);
     constexpr int SP = T < 64 || DP == 128 ? 32 : 64, NH = SP / 16, kAhead = 3;
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, g = lane >> 4, hd = a.head_dim;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1095,6 +1196,7 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
         store_v(tile + 1);
         set_places(tile + 2, id2);
     }
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): nothing is on its way to LDS any more
 #pragma unroll
     for (int u = 0; u < R; ++u) {
         const int mi = pc.row0 + (wave * R + u) * 16 + i;
@@ -1213,18 +1315,18 @@ __device__ __forceinline__ int find_piece(const PagedAttn &a, const Parts &parts
     return take;
 }
 
-template <int DP, bool KQ, bool BLOCKS>
+template <int DP, int KF, int VF>
 struct KernelLds {
-    Scan<64 * waves_of(DP, !BLOCKS)> scan;
+    Scan<64 * waves_of(DP, KF, VF)> scan;
+    WaveLds<DP, KF, VF> wave[waves_of(DP, KF, VF)];
+};
+template <int DP>
+struct KernelLds<DP, 0, 0> {
+    Scan<64 * waves_of(DP, 0, 0)> scan;
     union {
-        WaveLds<DP, KQ> wave[waves_of(DP, !BLOCKS)];
+        WaveLds<DP, 0, 0> wave[waves_of(DP, 0, 0)];
         BlockLds<DP> block;
     };
-};
-template <int DP, bool KQ>
-struct KernelLds<DP, KQ, false> {
-    Scan<64 * waves_of(DP, true)> scan;
-    WaveLds<DP, KQ> wave[waves_of(DP, true)];
 };
 
 // Quantised caches have stream items alone.  ONCE: K and V of stream items are
@@ -1232,13 +1334,13 @@ struct KernelLds<DP, KQ, false> {
 // (256 x 1000 positions of 4 heads of 256 dims: 212 us against 223; 4 x 32000 of 8 heads of 128: 107
 // against 116) and not beside a prefix's blocks (256 requests of 300 positions behind 8192: 225 us against 218).
 // At most two row tiles read the same rows of an f16 cache so; of a quantised one all do.
-template <int DP, bool KQ, bool VQ, bool ONCE>
-__global__ __launch_bounds__(64 * waves_of(DP, KQ || VQ)) void paged_attn_kernel(PagedAttn a, Parts parts)
+template <int DP, int KF, int VF, bool ONCE>
+__global__ __launch_bounds__(64 * waves_of(DP, KF, VF)) void paged_attn_kernel(PagedAttn a, Parts parts)
 {
-    constexpr bool kBlocks = !KQ && !VQ;
-    constexpr int kWaves = waves_of(DP, KQ || VQ), T = 64 * kWaves;
+    constexpr bool kBlocks = !KF && !VF;
+    constexpr int kWaves = waves_of(DP, KF, VF), T = 64 * kWaves;
     constexpr int kUnitB = unit_b(DP), kRowsB = kBlocks ? rows_b(DP) : 0;
-    __shared__ KernelLds<DP, KQ, kBlocks> lds;
+    __shared__ KernelLds<DP, KF, VF> lds;
     const Scan<T> &s = lds.scan;
     const int wg = blockIdx.x, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Totals totals = scan_requests<T, kRowsB, kUnitB>(a, lds.scan);
@@ -1298,7 +1400,7 @@ __global__ __launch_bounds__(64 * waves_of(DP, KQ || VQ)) void paged_attn_kernel
                               : Dest{parts.o_a + row * a.head_dim, parts.ml_a + row, false};
         if ((tid & 63) == 0 && first) parts.first[item] = worker;
         if ((tid & 63) == 0 && last) parts.last[item] = worker;
-        stream_item<DP, KQ, VQ, ONCE>(a, s, totals.need_at, pc, lds.wave[wave], to);
+        stream_item<DP, KF, VF, ONCE>(a, s, totals.need_at, pc, lds.wave[wave], to);
     }
 }
 
@@ -1511,7 +1613,7 @@ Parts layout(const PagedAttn &a, uint8_t *base, size_t &bytes)
     const bool quant = a.k_fmt != 0 || a.v_fmt != 0;
     const int dp = padded_dim(a.head_dim);
     p.wgs = 256;  // one a CU: they hold most of its registers or LDS
-    p.waves = waves_of(dp, quant);
+    p.waves = waves_of(dp, a.k_fmt, a.v_fmt);
     p.rows_b = quant ? 0 : rows_b(dp);
     const size_t heads = (size_t)a.max_rows * a.n_heads, hd = a.head_dim;
     const size_t group_rows = (size_t)a.max_rows * a.group;
@@ -1542,17 +1644,26 @@ template <int DP>
 void launch_dp(mrml_hip_ctx *ctx, const PagedAttn &a, const Parts &p)
 {
     const dim3 grid(p.wgs), block(64 * p.waves);
-    const bool kq = a.k_fmt != 0, vq = a.v_fmt != 0;
-    if (!kq && !vq && a.prefix_len == 0)
-        hipLaunchKernelGGL((paged_attn_kernel<DP, false, false, true>), grid, block, 0, ctx->stream, a, p);
-    else if (!kq && !vq)
-        hipLaunchKernelGGL((paged_attn_kernel<DP, false, false, false>), grid, block, 0, ctx->stream, a, p);
-    else if (!kq)
-        hipLaunchKernelGGL((paged_attn_kernel<DP, false, true, false>), grid, block, 0, ctx->stream, a, p);
-    else if (!vq)
-        hipLaunchKernelGGL((paged_attn_kernel<DP, true, false, false>), grid, block, 0, ctx->stream, a, p);
-    else
-        hipLaunchKernelGGL((paged_attn_kernel<DP, true, true, false>), grid, block, 0, ctx->stream, a, p);
+#define MRML_PAGED_CASE(KF, VF)                                                                                       \
+    case 3 * KF + VF:                                                                                                 \
+        hipLaunchKernelGGL((paged_attn_kernel<DP, KF, VF, false>), grid, block, 0, ctx->stream, a, p);               \
+        break;
+    switch (3 * a.k_fmt + a.v_fmt) {
+        MRML_PAGED_CASE(0, 1)
+        MRML_PAGED_CASE(0, 2)
+        MRML_PAGED_CASE(1, 0)
+        MRML_PAGED_CASE(1, 1)
+        MRML_PAGED_CASE(1, 2)
+        MRML_PAGED_CASE(2, 0)
+        MRML_PAGED_CASE(2, 1)
+        MRML_PAGED_CASE(2, 2)
+    default:
+        if (a.prefix_len == 0)
+            hipLaunchKernelGGL((paged_attn_kernel<DP, 0, 0, true>), grid, block, 0, ctx->stream, a, p);
+        else
+            hipLaunchKernelGGL((paged_attn_kernel<DP, 0, 0, false>), grid, block, 0, ctx->stream, a, p);
+    }
+#undef MRML_PAGED_CASE
 }
 
 }  // namespace
