@@ -539,7 +539,7 @@ struct QuantTile {
     static constexpr int kRow = ((DP / 32 * block_bytes(FMT) + 31) / 32 | 1) * 32;
     static constexpr int kPieces = (DP / 32 * block_bytes(FMT) + 15) / 16;  // of a row, at most
     static constexpr int kLoads = (32 * kPieces + 63) / 64;
-    alignas(16) uint8_t b[32 * kRow];
+    alignas(16) uint8_t b[32 * kRow + 16];  // words around a block's quants may end behind the last row
 };
 
 struct __attribute__((packed, aligned(2))) Bytes16 {
@@ -1587,7 +1587,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void paged_merge_kernel(Page
         for (int w = 1; w < W; ++w) most = fmaxf(most, s_m[w]);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            f[w] = s_l[w] == 0.0f ? 0.0f : exp2_hw(s_m[w] - most);
+            f[w] = s_l[w] == 0.0f ? 0.0f : s_l[w] != s_l[w] ? s_l[w] : exp2_hw(s_m[w] - most);  // NaN stays
             sum += f[w] == 0.0f ? 0.0f : s_l[w] * f[w];
         }
         for (int d = tid; d < hd; d += 64 * W) {

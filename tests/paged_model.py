@@ -109,9 +109,10 @@ def q8_values(q: np.ndarray) -> np.ndarray:
     return (d * np.clip(np.sign(t) * np.floor(np.abs(t) + 0.5), -128, 127)).reshape(q.shape)
 
 
-def attention(q, k, v, k_fmt, prefix, prefix_len, table, lens, row_start, page_size, group, scale, window, max_rows):
+def attention(q, k, v, k_fmt, prefix, prefix_len, table, lens, row_start, page_size, group, scale, window, max_rows, total=None):
     """(out, weight of |v|, largest score error unit) in 64 bits: rows [max_rows][heads][head_dim], NaN where a row
-    belongs to no request; the second is sum_t p_t |v_t|, the third max_t scale * sum_d |q_d k_td| a row and head."""
+    belongs to no request; the second is sum_t p_t |v_t|, the third max_t |scale| * sum_d |q_d k_td| a row and head.
+    total, if given, gets sum_t |v_t|."""
     heads, hd = q.shape[1:]
     out = np.full((max_rows, heads, hd), np.nan)
     mag, unit = np.zeros((max_rows, heads, hd)), np.zeros((max_rows, heads))
@@ -137,5 +138,7 @@ def attention(q, k, v, k_fmt, prefix, prefix_len, table, lens, row_start, page_s
                 p /= p.sum()
                 out[row, h] = p @ vv
                 mag[row, h] = p @ np.abs(vv)
-                unit[row, h] = scale * (np.abs(kk) @ np.abs(qv[row, h])).max()
+                if total is not None:
+                    total[row, h] = np.abs(vv).sum(0)
+                unit[row, h] = abs(scale) * (np.abs(kk) @ np.abs(qv[row, h])).max()
     return out, mag, unit

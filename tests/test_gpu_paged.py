@@ -264,23 +264,27 @@ class Batch:
                                  self.heads, self.kv_heads, self.hd, self.scale, self.window or None, self.k_format,
                                  self.v_format, self.q_stride)
 
-    def reference(self):
+    def reference(self, total=None):
         q = self.q[:, :self.heads * self.hd].reshape(self.max_rows, self.heads, self.hd)
         k, v = (pm.values(c, f, self.kv_heads, self.hd) for c, f in ((self.k, self.k_format), (self.v, self.v_format)))
         return pm.attention(q, k, v, self.k_format, self.prefix, self.prefix_len, self.table, self.lens, self.row_start,
-                            self.ps, self.heads // self.kv_heads, self.scale, self.window, self.max_rows)
+                            self.ps, self.heads // self.kv_heads, self.scale, self.window, self.max_rows, total)
 
     def check(self, what=""):
         """Within 1e-5 of the largest value (the documented bound), and within what 32-bit arithmetic can do
         elementwise: a score is off by at most (hd + 8) half-steps of its terms' sizes (a half-step for each of hd
         products' sums and the splits of q), which shifts each weight by that much twice over (its own and the sum's),
-        and the weights, their products and n sums by 64 half-steps more."""
+        and the weights, their products and n sums by 64 half-steps more.  A weight is held as two f16 terms of its
+        2^14-fold, relative to the largest one, rounded towards zero: in steps of 2^-24, so off by up to 2^-38 of the
+        largest weight however small it is, which counts where the largest weight meets a v of 0 (quantised caches
+        have many) and adds 2^-38 * sum_t |v_t|."""
         got = self.d["out"].numpy().reshape(self.max_rows, self.heads, self.hd).astype(np.float64)
-        ref, mag, unit = self.reference()
+        total = np.zeros((self.max_rows, self.heads, self.hd))
+        ref, mag, unit = self.reference(total)
         assert (got[self.rows:] == 5.0).all(), f"{what}: rows behind the last request changed"
         got, ref, mag, unit = got[:self.rows], ref[:self.rows], mag[:self.rows], unit[:self.rows]
         assert np.isfinite(got).all(), what
-        tol = mag * (2 * (self.hd + 8) * unit[..., None] + 64) * 2.0 ** -24
+        tol = mag * (2 * (self.hd + 8) * unit[..., None] + 64) * 2.0 ** -24 + total[:self.rows] * 2.0 ** -38
         off = np.abs(got - ref)
         worst = float((off / np.maximum(tol, 1e-300)).max())
         assert (off <= tol).all(), f"{what}: {worst:.3g} of the elementwise bound"
@@ -508,6 +512,168 @@ def test_attention_two_graphs_and_eager(backend, dev):
                     x.close()
     finally:
         one.close()
+
+
+@pytest.mark.parametrize("n,heads,kv_heads,head_dim,k_format,v_format", [
+    (700, 4, 2, 64, 0, 0), (513, 8, 1, 128, 0, 0), (600, 2, 1, 256, 1, 2), (300, 2, 1, 512, 0, 1), (4096, 2, 1, 32, 0, 0)])
+def test_attention_many_requests(backend, dev, n, heads, kv_heads, head_dim, k_format, v_format):
+    """More requests than a workgroup has threads: threads stand for several, some without rows, some with many."""
+    rng = np.random.default_rng(n)
+    before = rng.integers(0, 12, n)
+    new = np.where(rng.random(n) < 0.2, 0, 1)
+    new[[0, n // 2, n - 1]] = (3, 70, 0)
+    before[[1, n // 2 + 1]] = (900, 333)
+    for window in (0, 20):
+        Batch(backend, dev, 30, list(before), list(new), 37, 16, heads, kv_heads, head_dim, k_format, v_format,
+              window=window).run(f"window {window}")
+
+
+@pytest.mark.parametrize("head_dim,k_format", [(64, 0), (256, 0), (128, 1)])
+@pytest.mark.parametrize("window", [0, 7, 90])
+def test_attention_rows_before_the_first_position(backend, dev, head_dim, k_format, window):
+    """Rows of a request shorter than its rows stand inside the prefix, or before everything and see nothing (0)."""
+    for prefix_len in (0, 5, 160):
+        Batch(backend, dev, 31, [-3, 5, -150, -20], [5, 2, 160, 20], prefix_len, 16, 4, 2, head_dim, k_format, k_format,
+              window=window).run(f"prefix {prefix_len}")
+
+
+@pytest.mark.parametrize("k_format", [0, 1, 2])
+def test_attention_scale_of_any_sign(backend, dev, k_format):
+    for scale in (-0.2, 0.0, -3.0):
+        Batch(backend, dev, 32, [20, 300, 0], [1, 3, 40], 90, 16, 4, 2, 128, k_format, k_format, scale=scale).run(f"{scale}")
+
+
+@pytest.mark.parametrize("heads,kv_heads,head_dim", [(8, 4, 256), (4, 1, 128), (3, 3, 64), (2, 1, 512)])
+@pytest.mark.parametrize("window", [1, 33, 400])
+def test_attention_windows_over_many_rows(backend, dev, heads, kv_heads, head_dim, window):
+    """Prompts' chunks whose windows begin in the prefix, in the chunk, and in a tile's middle."""
+    Batch(backend, dev, 33, [0, 500, 77], [150, 300, 131], 290, 24, heads, kv_heads, head_dim, window=window).run()
+
+
+@pytest.mark.parametrize("k_format,v_format", [(0, 0), (1, 1), (2, 2)])
+@pytest.mark.parametrize("heads,kv_heads,rows", [(2, 1, 1), (32, 4, 140)])
+def test_attention_not_finite_in_quantised_and_wide_calls(backend, dev, k_format, v_format, heads, kv_heads, rows):
+    """A NaN in V's row or K's reaches every dim, or the block's dims, of the rows that see it and of its kv head."""
+    at = 20
+    for which in ("v", "k"):
+        b = Batch(backend, dev, 34, [60, 0], [1, rows], 0, 16, heads, kv_heads, 64, k_format, v_format, pad=1)
+        slot = int(b.table[0, at // 16]) * 16 + at % 16 if rows == 1 else int(b.table[1, at // 16]) * 16 + at % 16
+        fmt = k_format if which == "k" else v_format
+        cache = b.k if which == "k" else b.v
+        cache[slot, :2] = (0x00, 0x7E)  # f16: dim 0 of kv head 0; else the scale of its first block
+        b.upload()
+        b.call()
+        dev.sync()
+        got = b.d["out"].numpy().reshape(b.max_rows, heads, 64)[:b.rows]
+        bad = np.zeros(got.shape, bool)
+        seen = slice(0, 1) if rows == 1 else slice(1 + at, None)
+        bad[seen, :heads // kv_heads, slice(None) if which == "k" else slice(0, 1 if fmt == 0 else 32)] = True
+        assert np.isnan(got[bad]).all() and np.isfinite(got[~bad]).all(), which
+        if rows > 1:
+            assert heads * b.max_rows > 4096
+
+
+def test_attention_not_finite_k_alone_among_many(backend, dev):
+    """One NaN and one -inf among the scores of 64 positions: NaN, and no weight."""
+    for value in (np.nan, np.inf, -np.inf):
+        b = Batch(backend, dev, 35, [63], [1], 0, 16, 2, 1, 128, pad=0)
+        b.q[:] = np.abs(b.q)
+        slot = int(b.table[0, 1]) * 16 + 5
+        b.k.view(np.float16)[slot, 7] = value
+        b.upload()
+        b.call()
+        dev.sync()
+        got = b.d["out"].numpy().reshape(2, 128)
+        if value == -np.inf:
+            with np.errstate(invalid="ignore"):
+                ref = b.reference()[0][0]
+            assert np.abs(got - ref).max() <= 1e-5 * np.abs(ref).max()
+        else:
+            assert np.isnan(got).all(), value
+
+
+def test_attention_not_finite_q(backend, dev):
+    """A row of q that is not finite gives NaN in its own head and row alone."""
+    for k_format in (0, 1):
+        for value in (np.nan, np.inf):
+            b = Batch(backend, dev, 36, [70, 9], [1, 2], 40, 16, 4, 2, 64, k_format, k_format, pad=0)
+            b.q[1, 64 + 3] = value
+            b.upload()
+            b.call()
+            dev.sync()
+            got = b.d["out"].numpy().reshape(3, 4, 64)
+            ok = np.ones(got.shape, bool)
+            ok[1, 1] = False
+            assert np.isfinite(got[ok]).all(), (k_format, value)
+            if k_format == 0:
+                assert np.isnan(got[~ok]).all(), value
+
+
+@pytest.mark.parametrize("k_format,v_format", [(0, 0), (1, 2)])
+def test_places_past_four_gib(backend, dev, k_format, v_format):
+    """Append and attention at places whose bytes lie past 32 bits give what they give at the first places."""
+    heads, kv, hd, ps, m = 8, 8, 256, 16, 90
+    rb = min(pm.ROW_BYTES[f](kv * hd) for f in (k_format, v_format))
+    n_pages = (1 << 32) // (rb * ps) + 100
+    rng = np.random.default_rng(37)
+    width = (heads + 2 * kv) * hd
+    x = up(backend, dev, rng.standard_normal((m, width)).astype(np.float32))
+    k, v = (backend.HipBuffer.alloc(dev, n_pages * ps * pm.ROW_BYTES[f](kv * hd), np.uint8) for f in (k_format, v_format))
+    i32 = lambda a: up(backend, dev, np.array(a, np.int32))  # noqa: E731
+    pos, lens, starts = i32(np.arange(m)), i32([m - 40]), i32([0, 5])
+    outs = []
+    for pages in (rng.permutation(6), n_pages - 1 - rng.permutation(6)):
+        t = np.arange(m)
+        slots = i32(pages[t // ps] * ps + t % ps)
+        q, out = backend.HipBuffer.alloc(dev, m * heads * hd), up(backend, dev, np.zeros((5, heads * hd), np.float32))
+        dev.qkv_postprocess_paged(x, q, k, v, slots, pos, m, n_pages, ps, heads, kv, hd, 10000.0, k_format, v_format)
+        prefix, own = i32(pages[:2]), i32(pages[2:])  # the first 32 positions as the prefix, the others the request's
+        dev.attention_paged(q, k, v, out, n_pages, ps, prefix, 32, own, 4, lens, starts, 1, 5, heads,
+                            kv, hd, hd ** -0.5, None, k_format, v_format)
+        dev.sync()
+        outs.append(out.numpy())
+    assert np.isfinite(outs[0]).all() and np.array_equal(outs[0], outs[1])
+    for y in (k, v):
+        y.close()
+
+
+def test_attention_uncountable_work_is_refused(backend, dev):
+    """4096 requests over table rows of 2^21 positions could have more units of work than 32 bits count."""
+    b = Batch(backend, dev, 38, [3], [1], 4, 16, 8, 8, 64).upload()
+    d = b.d
+    with pytest.raises(backend.HipError, match="too many"):
+        dev.attention_paged(d["q"], d["k"], d["v"], d["out"], b.n_pages, 16, d["prefix"], 4, d["table"], 1 << 17,
+                            d["lens"], d["row_start"], 4096, 4096, 8, 8, 64, 0.1)
+
+
+def test_append_captured(backend, dev):
+    """A captured append replayed with other rows, slots and positions in between other work."""
+    heads, kv, hd, ps, n_pages, n = 4, 2, 64, 4, 6, 5
+    rng = np.random.default_rng(39)
+    width = (heads + 2 * kv) * hd
+    k, v = (up(backend, dev, np.zeros((n_pages * ps, kv * hd), np.float16)) for _ in range(2))
+    x, q = backend.HipBuffer.alloc(dev, n * width), backend.HipBuffer.alloc(dev, n * heads * hd)
+    slots, pos = up(backend, dev, np.zeros(n, np.int32)), up(backend, dev, np.zeros(n, np.int32))
+    call = lambda: dev.qkv_postprocess_paged(x, q, k, v, slots, pos, n, n_pages, ps, heads, kv, hd, 10000.0)  # noqa: E731
+    x.copy_from_host(np.zeros(n * width, np.float32))
+    call()
+    dev.sync()
+    graph = dev.capture(call)
+    for turn in range(4):
+        rows, at, place = rng.standard_normal(n * width).astype(np.float32), rng.integers(0, 500, n), rng.permutation(n_pages * ps)[:n]
+        got = []
+        for run in (graph.launch, call):
+            for c in (k, v):
+                c.copy_from_host(np.zeros((n_pages * ps, kv * hd), np.float16))
+            x.copy_from_host(rows)
+            pos.copy_from_host(at.astype(np.int32))
+            slots.copy_from_host(place.astype(np.int32))
+            run()
+            dev.sync()
+            got.append([y.numpy().copy() for y in (q, k, v)])
+        assert all(np.array_equal(a.view(np.uint8), b.view(np.uint8)) for a, b in zip(*got)), f"turn {turn}"
+        assert np.count_nonzero(got[0][1].reshape(n_pages * ps, -1).any(1)) == n
+    graph.close()
 
 
 # ------------------------------------------------------------ the three together
