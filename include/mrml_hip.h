@@ -584,7 +584,11 @@ int mrml_hip_rope_kv_append_paged(mrml_hip_ctx *ctx, const float *d_qkv, float *
  * Q8_0 or Q4_0 multiplied with q as Q8_0 blocks; softmax and sums in f32), added
  * in another order: within 1e-5 relative to the output's largest magnitude, like
  * mrml_hip_attention_causal_split.  Values of quantised V rows must be within
- * f16's range.  Limits as mrml_hip_rope_kv_append_paged. */
+ * f16's range.  Limits as mrml_hip_rope_kv_append_paged; besides, the work is
+ * counted in tiles of 16 query rows a kv head and 32 positions by what the
+ * arguments allow (n_seqs requests of table_stride * page_size positions, max_rows
+ * rows), and a call that could have 2^30 of them or rows times heads is refused.
+ * scale is finite and of any sign. */
 int mrml_hip_attention_paged(mrml_hip_ctx *ctx, const float *d_q, int32_t q_stride, const uint16_t *d_k_pages,
                              const uint16_t *d_v_pages, float *d_out, int32_t n_pages, int32_t page_size,
                              const int32_t *d_prefix, int32_t prefix_len, const int32_t *d_table,

@@ -1669,16 +1669,17 @@ void launch_dp(mrml_hip_ctx *ctx, const PagedAttn &a, const Parts &p)
 }  // namespace
 
 // Stream units: at most two row tiles a request where there are block items, else tiles of 16 of all rows, over
-// the longest table row; and the prefix's.  Block units are fewer than their rows in tiles of 16 would give.
+// the longest table row; and the prefix's.  Block units are fewer than half of what their rows would give in tiles
+// of 16 (64 rows of 32 positions, at least).  Rows times heads have to fit an int too.
 bool paged_attn_countable(const PagedAttn &a)
 {
     const double kv = a.n_kv_heads, rows = (double)a.max_rows * a.group, seqs = std::min(a.n_seqs, a.max_rows);
     const bool quant = a.k_fmt != 0 || a.v_fmt != 0;
     const double tiles = rows / kRowsA + seqs, own = a.longest / kUnitA + 1 + kItemCost, pre = a.prefix_len / kUnitA + 1 + kItemCost;
-    const double block = quant ? 1.0 : 1.0 / 8;  // a block tile is 64 rows at least and 32 positions
-    const double a_units = quant ? tiles * own : 2 * seqs * own;
-    return kv * (a_units + block * tiles * (own + pre) + 2 * pre) < (double)(1 << 30) &&
-           kv * (2 * tiles + 2.0 * a.n_seqs + 8) < (double)(1 << 30);
+    const double a_units = quant ? tiles * (own + pre) : 2 * seqs * own + 2 * pre;
+    const double b_units = quant ? 0 : tiles / 2 * (own + pre);
+    const double most = 1 << 30;
+    return kv * (a_units + b_units) < most && kv * (2 * tiles + 2.0 * a.n_seqs + 8) < most && (double)a.max_rows * a.n_heads < most;
 }
 
 size_t paged_attn_scratch_bytes(const PagedAttn &a)

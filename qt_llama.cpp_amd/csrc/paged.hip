@@ -7,6 +7,7 @@
 // requests that hold pages of one cache and share a prefix.
 
 #include <algorithm>
+#include <cmath>
 
 #include "paged.h"
 #include "rope.h"
@@ -472,6 +473,7 @@ int mrml_hip_attention_paged(mrml_hip_ctx *ctx, const float *q, int32_t q_stride
             "%s: q_stride=%d (a multiple of 4, at least n_heads * head_dim = %d)", name, q_stride, n_heads * head_dim);
     REQUIRE(ctx, ((((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)out) & 15) == 0),
             "%s: pointers must be 16-byte aligned", name);
+    REQUIRE(ctx, std::isfinite(scale), "%s: scale=%g", name, (double)scale);
     PagedAttn a{};
     a.q = q;
     a.k = reinterpret_cast<const uint8_t *>(k_pages);
@@ -494,7 +496,7 @@ int mrml_hip_attention_paged(mrml_hip_ctx *ctx, const float *q, int32_t q_stride
     a.group = n_heads / n_kv_heads;
     a.group_magic = a.group > 1 ? (uint32_t)((1ull << 32) / a.group) + 1u : 0u;
     a.longest = table_stride * page_size;
-    a.window = sliding_window > 0 ? sliding_window : 0;
+    a.window = sliding_window > 0 ? std::min(sliding_window, 2 * kMaxTablePositions) : 0;  // no row sees more
     a.k_fmt = k_format;
     a.v_fmt = v_format;
     a.scale = scale;

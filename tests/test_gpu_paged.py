@@ -646,6 +646,22 @@ def test_attention_uncountable_work_is_refused(backend, dev):
                             d["lens"], d["row_start"], 4096, 4096, 8, 8, 64, 0.1)
 
 
+def test_attention_largest_window_and_scales_refused(backend, dev):
+    """A window past every position is none, also for rows before the first position; a scale that is no number is
+    refused."""
+    for before, new in ([40, 0], [1, 9]), ([-3, -150], [5, 160]):
+        b = Batch(backend, dev, 40, before, new, 70, 16, 4, 2, 64, window=2 ** 31 - 1)
+        b.run()
+        wide = b.d["out"].numpy()
+        b.window = 0
+        b.run()
+        assert np.array_equal(wide[:b.rows], b.d["out"].numpy()[:b.rows])
+    for scale in (np.nan, np.inf, -np.inf):
+        b.scale = scale
+        with pytest.raises(backend.HipError, match="scale"):
+            b.call()
+
+
 def test_append_captured(backend, dev):
     """A captured append replayed with other rows, slots and positions in between other work."""
     heads, kv, hd, ps, n_pages, n = 4, 2, 64, 4, 6, 5
