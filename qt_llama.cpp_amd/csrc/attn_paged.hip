@@ -42,13 +42,21 @@ constexpr float kShift = 14.0f;   // p is kept as p * 2^14 (below 2^16, f16's en
 constexpr float kSlack = 1.5f;    // the maximum may grow by this much before o and l are rescaled
 constexpr float kBroken = -1.0f;  // in place of l: the part is not finite
 constexpr int kRowsA = 16, kUnitA = 32;  // rows and positions of a stream item's tile (one wave)
-constexpr int kFewRows = 32;             // groups of at most so many rows are stream items
-// Costs, for the split of the work, in stream units of one wave (about 7 us each where few workgroups stream): what
-// a stream item costs beside its units (q, the first K and V, the part's store: a
-// chain of round trips), and a block unit per 32 rows of it and wave.
+// Groups of at most so many rows are stream items (two waves' K and V come from memory or L2 twice; a block's rows
+// past the group's idle).  Lines of 16 | 32 | 64: 16 requests of 24 rows behind nothing, 2000 positions of 8 heads of
+// 128 dims 79 | 67 | 67 us, of 32 rows of 64 dims 60 | 46 | 46; 32 requests (64 rows) behind 4001 positions - | 34 | 42.
+constexpr int kFewRows = 32;
+// Costs for the split of the work.  A stream item's own cost (q, the first K and V, the part's store: a chain of
+// round trips) in its units; a block unit in stream units of one wave, per 32 rows of it and wave; a block item's own
+// cost is a time too (q and the first tiles in, o out: as many bytes at every head size), in units that take as long
+// as they have rows.  Measured on both sides, us:
+//   stream item 1 | 2 | 4: 32 requests behind 4001 positions 36.0 | 34.0 | 34.7, 20 of up to 30000 82.5 | 82.3 | 81.4
+//   block unit 0.1 | 0.15 | 0.22: 256 requests behind 32768 positions 234 | 223 | 238, 32 behind 4001 33.0 | 34.0 | 35.9
+//   block item of 128 rows 2 | 3 | 4 | 6: 11 chunks behind 3000 positions 183 | 172 | 160 | 166, 100 of 1..100 rows
+//   behind 3000 171 | 164 | 152 | 162; of 256 rows 2 | 3 | 4 | 6: 4 chunks of 500 behind 2000 249 | 251 | 259 | 268
 constexpr int kItemCost = 2;
-constexpr int kBlockItemCost = 2;  // the same of a block item, in its units
 constexpr float kBlockCost = 0.15f;
+constexpr int block_item_cost(int rows) { return rows ? 512 / rows : 0; }
 
 // Waves of a workgroup, rows of a block item and positions of its tile by padded head size: two waves a SIMD
 // while a wave's q and o fit 256 registers.
@@ -249,7 +257,7 @@ __device__ __forceinline__ void request_units(const PagedAttn &a, const Request 
     } else if constexpr (ROWS != 0) {
         for (int b = 0; b * ROWS < m; ++b) {
             tile_range<ROWS>(a, q, b, lo, hi);
-            ub += units_of<UNIT>(lo, hi) + kBlockItemCost;
+            ub += units_of<UNIT>(lo, hi) + block_item_cost(ROWS);
         }
         ub *= a.n_kv_heads;
     }
@@ -534,9 +542,9 @@ constexpr int block_bytes(int fmt) { return fmt == 1 ? 34 : 18; }
 // fetch their 8 bytes of a block each make an access to the cache each (1578 a tile of 32
 // positions of 128 dims, 94% of the time the caches could take them in).  A row's last piece
 // ends with the row.  Rows are an odd number of 32 bytes apart: 8 of them fill the 64 banks.
-template <int DP, int FMT>
+template <int DP, int FMT, int ALIGN>
 struct QuantTile {
-    static constexpr int kRow = ((DP / 32 * block_bytes(FMT) + 31) / 32 | 1) * 32;
+    static constexpr int kRow = ((DP / 32 * block_bytes(FMT) + ALIGN - 1) / ALIGN | 1) * ALIGN;
     static constexpr int kPieces = (DP / 32 * block_bytes(FMT) + 15) / 16;  // of a row, at most
     static constexpr int kLoads = (32 * kPieces + 63) / 64;
     alignas(16) uint8_t b[32 * kRow + 16];  // words around a block's quants may end behind the last row
@@ -547,9 +555,9 @@ struct __attribute__((packed, aligned(2))) Bytes16 {
 };
 
 // A wave's pieces of such a tile: where they lie and, on their way, what they hold.
-template <int DP, int FMT>
+template <class TILE>
 struct QuantPieces {
-    using Tile = QuantTile<DP, FMT>;
+    using Tile = TILE;
     uint32_t at[Tile::kLoads];  // row << 16 | byte in it
     uint4 x[Tile::kLoads];
     __device__ __forceinline__ void start(int row_bytes, int lane)
@@ -610,8 +618,8 @@ struct WaveLds {
     int place[VF ? 1 : 32];
     alignas(16) uint8_t k[KF ? 16 : DP / 16 * kChunk];  // 32 positions: chunks of 32 dims, of 16 positions
     float scores[KF ? 16 * kTrRow : 1];
-    std::conditional_t<KF != 0, QuantTile<DP, KF ? KF : 1>, None> kq;
-    std::conditional_t<VF != 0, QuantTile<DP, VF ? VF : 1>, None> vq;
+    std::conditional_t<KF != 0, QuantTile<DP, KF ? KF : 1, 16>, None> kq;
+    std::conditional_t<VF != 0, QuantTile<DP, VF ? VF : 1, 32>, None> vq;
 };
 
 // Query rows for a quantised K: operand bytes, and scale and sum of each block
@@ -697,8 +705,8 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
         if (place < 0 && pos < pc.p1 && lane < 32) page_fault(a.faults);
         return place;
     };
-    std::conditional_t<KQ, QuantPieces<DP, KF ? KF : 1>, None> k_on_way;
-    std::conditional_t<VQ, QuantPieces<DP, VF ? VF : 1>, None> v_on_way;
+    std::conditional_t<KQ, QuantPieces<QuantTile<DP, KF ? KF : 1, 16>>, None> k_on_way;
+    std::conditional_t<VQ, QuantPieces<QuantTile<DP, VF ? VF : 1, 32>>, None> v_on_way;
     if constexpr (KQ) {
         k_on_way.start(kv_row_bytes(KF, hd), lane);
         if (hd < DP)  // blocks past the head: scales and quants of 0
@@ -1238,7 +1246,7 @@ __device__ __forceinline__ Shared shared_work(const PagedAttn &a, const Scan<T> 
     p.hi = a.prefix_len;
     p.lo = a.window && t.low < INT32_MAX ? min(max(a.prefix_len + t.low - a.window + 1, 0), p.hi) : 0;
     p.items = (p.few ? (p.rows + kRowsA - 1) / kRowsA : (p.rows + ROWS - 1) / (ROWS ? ROWS : 1)) * a.n_kv_heads;
-    p.units = p.few ? units_of<kUnitA>(p.lo, p.hi) + kItemCost : units_of<UNIT>(p.lo, p.hi) + kBlockItemCost;
+    p.units = p.few ? units_of<kUnitA>(p.lo, p.hi) + kItemCost : units_of<UNIT>(p.lo, p.hi) + block_item_cost(ROWS);
     if (a.prefix_len == 0) p.items = 0;
     return p;
 }
@@ -1288,7 +1296,7 @@ __device__ __forceinline__ int find_piece(const PagedAttn &a, const Parts &parts
         } else {
             for (blk = 0;; ++blk) {
                 tile_range<ROWS>(a, q, blk, lo, hi);
-                units = units_of<UNIT>(lo, hi) + kBlockItemCost;
+                units = units_of<UNIT>(lo, hi) + block_item_cost(ROWS);
                 if (u < units * a.n_kv_heads) break;
                 u -= units * a.n_kv_heads;
             }
@@ -1301,7 +1309,7 @@ __device__ __forceinline__ int find_piece(const PagedAttn &a, const Parts &parts
     }
     units = uni(units);
     within = uni(within);
-    const int take = min(units - within, left), cost = BLOCK ? kBlockItemCost : kItemCost;
+    const int take = min(units - within, left), cost = BLOCK ? block_item_cost(ROWS) : kItemCost;
     const int from = max(within - cost, 0), to = max(within + take - cost, 0);
     item = uni(item);
     pc.table = pc.pre ? a.prefix : a.table + (size_t)uni(r) * a.table_stride;
@@ -1677,7 +1685,7 @@ bool paged_attn_countable(const PagedAttn &a)
     const bool quant = a.k_fmt != 0 || a.v_fmt != 0;
     const double tiles = rows / kRowsA + seqs, own = a.longest / kUnitA + 1 + kItemCost, pre = a.prefix_len / kUnitA + 1 + kItemCost;
     const double a_units = quant ? tiles * (own + pre) : 2 * seqs * own + 2 * pre;
-    const double b_units = quant ? 0 : tiles / 2 * (own + pre);
+    const double b_units = quant ? 0 : tiles / 2 * (own + pre + 16);  // 16: two block items' own costs at most
     const double most = 1 << 30;
     return kv * (a_units + b_units) < most && kv * (2 * tiles + 2.0 * a.n_seqs + 8) < most && (double)a.max_rows * a.n_heads < most;
 }

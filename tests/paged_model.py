@@ -125,7 +125,7 @@ def attention(q, k, v, k_fmt, prefix, prefix_len, table, lens, row_start, page_s
         mine = np.asarray(table[r], np.int64)[u // page_size] * page_size + u % page_size
         slots = np.concatenate([shared, mine]).astype(np.int64)
         for row in rows:
-            at = prefix_len + int(lens[r]) - (row_start[r + 1] - row)
+            at = prefix_len + int(lens[r]) - (int(row_start[r + 1]) - row)
             lo = max(0, at - window + 1) if window else 0
             see = slots[lo:at + 1]
             if at < 0 or not len(see):
