@@ -9,9 +9,10 @@
 // The softmax is taken apart over positions: any range of them gives (m, l, o)
 // = (max, sum of 2^(x - m), sum of 2^(x - m) v) with x = log2(e) * scale * q.k,
 // and ranges join exactly as sum 2^(m_i - M) (l_i, o_i).  So the work is a list
-// of items -- (16 or 128 query rows that share their K and V) x (a kv head) x
-// (a range of positions of the prefix or of one request) -- cut into units of
-// positions and dealt out evenly; paged_merge_kernel joins the parts.
+// of items -- (a tile of query rows that share their K and V: 16 of a stream item, 64 to
+// 256 of a block item) x (a kv head) x (the positions of the prefix or of one request) -- cut
+// into units of positions and dealt out evenly to 256 workgroups; paged_merge_kernel joins the
+// parts.  The prefix's K and V are read once for a tile of all requests' rows, not once a request.
 //
 // Query rows of one kv head (every head of its group, every row of a request,
 // and for the prefix every row of the batch) are the columns of the matrix
@@ -72,7 +73,7 @@ constexpr int unit_b(int dp) { return 16384 / dp; }
 struct Parts {
     float *o[2];         // first part of each row's prefix and own item: [row][head][head_dim]
     float2 *ml[2];       // (m, l) of those
-    float *o_a, *o_b;    // later parts, by worker: [worker][16][head_dim], [workgroup][128][head_dim]
+    float *o_a, *o_b;    // later parts, by worker: [worker][16][head_dim], [workgroup][rows_b][head_dim]
     float2 *ml_a, *ml_b;
     int32_t *first, *last;  // workers that hold an item's first and last unit
     int4 *row_item;         // of a row: {request, its first row, its rows}
@@ -495,7 +496,11 @@ __device__ __forceinline__ bool softmax_step(float *x, float c, float &m, float 
 // 8 apart over the operand's rows, which only the store of o has to know.  K of
 // an f16 cache goes through a tile of LDS of the wave's own (global_load_lds), so
 // that the next tile's K is on its way without registers; the next V is loaded as
-// soon as this one is used up.  A wave keeps up to 32 KB in flight (head_dim 256).
+// soon as this one is used up.  A wave keeps a tile of K and of V on its way, eight waves of 256
+// dims 256 KB a CU.  f16 caches are bound by their bytes: 256 requests of 1000 positions of 4 heads of 256 dims
+// (1.05 GB) take 212 us, 4.95 TB/s of the 5.14 that a copy reaches; 4 of 32000 of 8 heads of 128 106 us.
+// Quantised ones are bound by the instructions that take them apart and by the wait for LDS between
+// them (VALU busy 46% of the time, LDS 40%): the latter as Q8_0 98 us (2.85 TB/s), as Q4_0 77.
 //
 // Quantised K is multiplied as the ring attention does it: q as Q8_0 blocks,
 // each block's integer sum on the int8 MFMA (16x16x32: one block a
@@ -969,6 +974,12 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
 // item); V is transposed on its way by the thread that has loaded 8 positions of some
 // dims, and written as 16-byte runs of 8 positions.  A wave holds 16 * R rows; each
 // chunk read from LDS feeds 2 * R products.
+//
+// Bound by issue: 512 rows a kv head (256 requests, groups of 2) of 4 heads of 256 dims behind 32768 positions take 186 us,
+// 370 TFLOP/s of the formula and 740 with both terms of q and p, 64% of what an 8192^3 f16 matrix product of the vendor's
+// library reaches here.  MFMA is busy 40% of the time, other vector instructions take 24%, a wave
+// waits 34%.  Two tiles that fill LDS (128 KB) against smaller ones: a barrier a tile, and the next tile has the whole
+// tile's products to arrive in.
 
 template <int DP>
 struct BlockLds {
@@ -1461,7 +1472,8 @@ __device__ __forceinline__ void slow_row(const PagedAttn &a, int row, int r, int
 
 // Joins the parts of each row and head.  W waves share a row and head, lane groups
 // take a part each, a lane four dims of it, with a running maximum of their own; lane groups and waves
-// join as parts do.  Two round trips: where the parts are, then the parts.
+// join as parts do.  Two round trips after the row's request: where the parts are, then the parts.  Bound by them
+// (5.5 us for 8 pairs, 7 for 256 in some ten parts) or by the parts' bytes (17 us for 2134 rows of 8 heads of 256 dims: 54 MB).
 template <int W>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void paged_merge_kernel(PagedAttn a, Parts parts)
 {
@@ -1708,8 +1720,11 @@ int launch_paged_attn(mrml_hip_ctx *ctx, const PagedAttn &a, void *scratch)
     default: launch_dp<512>(ctx, a, p); break;
     }
     if (int rc = check_launch(ctx, "paged_attn_kernel")) return rc;
+    // Waves a row and head by how many there are, measured on both sides of the lines (us): 32 pairs in 500 parts
+    // each 86 with 4 and 60 with 16 (the whole call), 256 pairs 7.1 and 6.8, 408 pairs 7.2 and 9.0, 732 pairs 5.3 and 10.8;
+    // 408 pairs 16.2 with one and 7.4 with 4, 732 8.4 and 5.6, 2048 11.9 and 13.7, 4096 5.2 and 12.0.
     const int pairs = a.max_rows * a.n_heads;
-    if (pairs > 4096)
+    if (pairs > 1024)
         hipLaunchKernelGGL(paged_merge_kernel<1>, dim3((pairs + 3) / 4), dim3(256), 0, ctx->stream, a, p);
     else if (pairs > 256)
         hipLaunchKernelGGL(paged_merge_kernel<4>, dim3(pairs), dim3(256), 0, ctx->stream, a, p);
