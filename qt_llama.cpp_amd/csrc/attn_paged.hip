@@ -975,10 +975,10 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
 // dims, and written as 16-byte runs of 8 positions.  A wave holds 16 * R rows; each
 // chunk read from LDS feeds 2 * R products.
 //
-// Bound by issue: 512 rows a kv head (256 requests, groups of 2) of 4 heads of 256 dims behind 32768 positions take 186 us,
+// Bound by issue and power: 512 rows a kv head (256 requests, groups of 2) of 4 heads of 256 dims behind 32768 positions take 186 us,
 // 370 TFLOP/s of the formula and 740 with both terms of q and p, 64% of what an 8192^3 f16 matrix product of the vendor's
 // library reaches here.  MFMA is busy 40% of the time, other vector instructions take 24%, a wave
-// waits 34%.  Two tiles that fill LDS (128 KB) against smaller ones: a barrier a tile, and the next tile has the whole
+// waits 34%, and the clock falls to 1.9 GHz (2.4 in stream items).  Two tiles that fill LDS (128 KB) against smaller ones: a barrier a tile, and the next tile has the whole
 // tile's products to arrive in.
 
 template <int DP>

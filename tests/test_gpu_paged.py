@@ -662,6 +662,26 @@ def test_attention_largest_window_and_scales_refused(backend, dev):
             b.call()
 
 
+def test_attention_two_contexts_at_once(backend, dev):
+    """Calls of two contexts in flight together, each with its own stream and scratch."""
+    one = backend.HipDevice.new(0)
+    try:
+        a = Batch(backend, dev, 41, [900, 30, 7], [1, 1, 1], 1500, 16, 8, 4, 256).upload()
+        b = Batch(backend, one, 42, [3, 800], [60, 1], 700, 32, 16, 2, 128, 1, 2).upload()
+        for _ in range(20):
+            a.call()
+            b.call()
+        dev.sync()
+        one.sync()
+        a.check("first")
+        b.check("second")
+        for x in b.d.values():
+            if x is not None:
+                x.close()
+    finally:
+        one.close()
+
+
 def test_append_captured(backend, dev):
     """A captured append replayed with other rows, slots and positions in between other work."""
     heads, kv, hd, ps, n_pages, n = 4, 2, 64, 4, 6, 5
