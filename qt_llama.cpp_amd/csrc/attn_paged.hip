@@ -127,11 +127,6 @@ __device__ __forceinline__ float row_sum(float v) { return over_row(v, [](float 
 
 // A value that every lane of the wave holds, as a scalar.
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ float uni(float v) { return as_f((uint32_t)__builtin_amdgcn_readfirstlane((int)as_u(v))); }
-__device__ __forceinline__ size_t uni(size_t v)
-{
-    return (size_t)(uint32_t)uni((int)(v & 0xffffffffu)) | (size_t)(uint32_t)uni((int)(v >> 32)) << 32;
-}
 
 // No memory access is moved past this by the compiler (waits that count loads rely on their order).
 __device__ __forceinline__ void pin()
