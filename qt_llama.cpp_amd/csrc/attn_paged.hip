@@ -586,22 +586,28 @@ struct QuantPieces {
     // with its row is written in what both share.
     __device__ __forceinline__ void store(Tile &tile, int row_bytes) const
     {
+        typedef volatile __attribute__((address_space(3))) uint32_t *Words;
+        typedef volatile __attribute__((address_space(3))) uint16_t *Halves;
+        if ((row_bytes & 15) == 0) {
 #pragma unroll
-        for (int e = 0; e < Tile::kLoads; ++e) {
-            uint8_t *dst = tile.b + (at[e] >> 16) * Tile::kRow + (at[e] & 0xffff);
-            const uint32_t w[4] = {x[e].x, x[e].y, x[e].z, x[e].w};
-            if ((row_bytes & 15) == 0) {
-                *reinterpret_cast<uint4 *>(dst) = x[e];
-            } else if ((row_bytes & 3) == 0) {
+            for (int e = 0; e < Tile::kLoads; ++e) *reinterpret_cast<uint4 *>(tile.b + place(e)) = x[e];
+        } else if ((row_bytes & 3) == 0) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) ((volatile __attribute__((address_space(3))) uint32_t *)dst)[j] = w[j];
-            } else {
+            for (int e = 0; e < Tile::kLoads; ++e) {
+                const uint32_t w[4] = {x[e].x, x[e].y, x[e].z, x[e].w};
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    ((volatile __attribute__((address_space(3))) uint16_t *)dst)[j] = (uint16_t)(w[j / 2] >> 16 * (j & 1));
+                for (int j = 0; j < 4; ++j) ((Words)(tile.b + place(e)))[j] = w[j];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < Tile::kLoads; ++e) {
+                const uint32_t w[4] = {x[e].x, x[e].y, x[e].z, x[e].w};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ((Halves)(tile.b + place(e)))[j] = (uint16_t)(w[j / 2] >> 16 * (j & 1));
             }
         }
     }
+    __device__ __forceinline__ int place(int e) const { return (at[e] >> 16) * Tile::kRow + (at[e] & 0xffff); }
 };
 // 8 bytes at p + at, at even: of the words around them.
 __device__ __forceinline__ Bytes8 pick8(const uint8_t *p, int at)
@@ -613,26 +619,34 @@ __device__ __forceinline__ Bytes8 pick8(const uint8_t *p, int at)
 
 struct None {};
 
+// Scales and sums of q's blocks: in registers, but for heads of more than 256 dims in LDS, where with them a wave's
+// registers spill more (30 requests behind 4000 positions of 2 heads of 512 dims, Q4_0: 108 us so and 70 from LDS; 64
+// of 2000 positions, Q8_0: 394 and 364).
+constexpr bool q_scales_in_lds(int dp) { return dp > 256; }
+
 template <int DP, int KF, int VF>
 struct WaveLds {
     int place[VF ? 1 : 32];
     alignas(16) uint8_t k[KF ? 16 : DP / 16 * kChunk];  // 32 positions: chunks of 32 dims, of 16 positions
     float scores[KF ? 16 * kTrRow : 1];
+    alignas(16) float q_d[KF && q_scales_in_lds(DP) ? DP / 2 : 4];  // [block][row]
+    alignas(16) int q_sum8[KF == 2 && q_scales_in_lds(DP) ? DP / 2 : 4];
     std::conditional_t<KF != 0, QuantTile<DP, KF ? KF : 1, 16>, None> kq;
     std::conditional_t<VF != 0, QuantTile<DP, VF ? VF : 1, 32>, None> vq;
 };
 
 // Query rows for a quantised K: operand bytes, and scale and sum of each block
 // for the four rows that this lane's results belong to.
-template <int KS>
+template <int KS, bool IN_LDS>
 struct QuantQ {
     long q[KS];
-    float4v d[KS];
-    int4v sum8[KS];  // -8 * sum of the block's quants: what Q4_0's offset takes away
+    float4v d[IN_LDS ? 1 : KS];
+    int4v sum8[IN_LDS ? 1 : KS];  // -8 * sum of the block's quants: what Q4_0's offset takes away
 };
 
-template <int KS, int KF>
-__device__ __forceinline__ void load_quant_q(const PagedAttn &a, const float *row, bool live, int g, QuantQ<KS> &out)
+template <int KS, int KF, bool IN_LDS>
+__device__ __forceinline__ void load_quant_q(const PagedAttn &a, const float *row, bool live, int g, QuantQ<KS, IN_LDS> &out,
+                                             float *q_d, int *q_sum8)
 {
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
@@ -657,12 +671,22 @@ __device__ __forceinline__ void load_quant_q(const PagedAttn &a, const float *ro
         sum += __shfl_xor(sum, 16, 64);
         sum += __shfl_xor(sum, 32, 64);
         out.q[s] = (long)((uint64_t)w[0] | ((uint64_t)w[1] << 32));
+        const float sd = a.scale < 0.0f ? -d : d;
+        if constexpr (IN_LDS) {
+            const int i = threadIdx.x & 15;
+            if (g == 0) {
+                q_d[16 * s + i] = sd;
+                if (KF == 2) q_sum8[16 * s + i] = -8 * sum;
+            }
+        } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            out.d[s][r] = __shfl(a.scale < 0.0f ? -d : d, 4 * g + r, 64);
-            out.sum8[s][r] = KF == 2 ? -8 * __shfl(sum, 4 * g + r, 64) : 0;
+            for (int r = 0; r < 4; ++r) {
+                out.d[s][r] = __shfl(sd, 4 * g + r, 64);
+                out.sum8[s][r] = KF == 2 ? -8 * __shfl(sum, 4 * g + r, 64) : 0;
+            }
         }
     }
+    __builtin_amdgcn_wave_barrier();
 }
 
 template <int DP, int KF, int VF, bool ONCE>
@@ -677,10 +701,11 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
     const int i_row = div_group(a, mi), tok = pc.tok0 + i_row, head = pc.kvh * a.group + mi - i_row * a.group;
     const float *q_row = a.q + (size_t)tok * a.q_stride + (size_t)head * hd;
     half8 qh[KQ ? 1 : KS], ql[KQ ? 1 : KS];
-    QuantQ<KQ ? KS : 1> qq;
+    constexpr bool kFar = KQ && q_scales_in_lds(DP);
+    QuantQ<KQ ? KS : 1, kFar> qq;
     float c = score_factor(a);
     if constexpr (KQ)
-        load_quant_q<KS, KF>(a, q_row, live, g, qq);
+        load_quant_q<KS, KF, kFar>(a, q_row, live, g, qq, lds.q_d, lds.q_sum8);
     else
         c = fmaxf(c * load_q<KS>(a, q_row, live, g, qh, ql), 0x1p-126f);
     int vlo, vhi;
@@ -769,6 +794,12 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
             const uint8_t *rows = lds.kq.b + i * lds.kq.kRow;
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
+                float4v qd = qq.d[kFar ? 0 : s];
+                int4v sum8 = qq.sum8[kFar ? 0 : s];
+                if constexpr (kFar) {
+                    qd = *reinterpret_cast<const float4v *>(lds.q_d + 16 * s + 4 * g);
+                    sum8 = KF == 2 ? *reinterpret_cast<const int4v *>(lds.q_sum8 + 16 * s + 4 * g) : int4v{0, 0, 0, 0};
+                }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint8_t *b = rows + 16 * h * lds.kq.kRow + s * kBlkK;
@@ -782,10 +813,10 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
                         w1 = (w1 >> (4 * (g >> 1))) & 0x0f0f0f0fu;
                     }
                     const long kk = (long)((uint64_t)w0 | ((uint64_t)w1 << 32));
-                    const int4v is = __builtin_amdgcn_mfma_i32_16x16x32_i8(qq.q[s], kk, qq.sum8[s], 0, 0, 0);
+                    const int4v is = __builtin_amdgcn_mfma_i32_16x16x32_i8(qq.q[s], kk, sum8, 0, 0, 0);
                     const float dk = f16_bits_to_f32(*reinterpret_cast<const uint16_t *>(b));
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[h][r] = fmaf((float)is[r], dk * qq.d[s][r], acc[h][r]);
+                    for (int r = 0; r < 4; ++r) acc[h][r] = fmaf((float)is[r], dk * qd[r], acc[h][r]);
                 }
             }
 #pragma unroll
