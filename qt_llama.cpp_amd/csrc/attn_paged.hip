@@ -41,7 +41,11 @@ typedef int int4v __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kShift = 14.0f;   // p is kept as p * 2^14 (below 2^16, f16's end, with the slack below)
 constexpr float kSlack = 1.5f;    // the maximum may grow by this much before o and l are rescaled
-constexpr float kBroken = -1.0f;  // in place of l: the part is not finite
+constexpr float kBroken = -1.0f;  // in place of l: the part is no good (see usable)
+// Largest maximum (log2 domain, either sign) that a part may have.  p = 2^(fma(x, c, 14 - m)) is off by what the
+// roundings of m and of 14 - m leave in the exponent, half a step of m each: 2^-4 in all here, so p stays below
+// f16's end with the slack, and l and o share the error.  Beyond 2^24 a weight of 1 comes out as 2^6 or as nothing.
+constexpr float kFarScore = 0x1p20f;
 constexpr int kRowsA = 16, kUnitA = 32;  // rows and positions of a stream item's tile (one wave)
 // Groups of at most so many rows are stream items (two waves' K and V come from memory or L2 twice; a block's rows
 // past the group's idle).  Lines of 16 | 32 | 64: 16 requests of 24 rows behind nothing, 2000 positions of 8 heads of
@@ -480,6 +484,13 @@ __device__ __forceinline__ bool softmax_step(float *x, float c, float &m, float 
     }
     l += sum;
     return any;
+}
+
+// Whether a part's sums can be joined with others: they are finite (check: their sum) and its scores were near
+// enough to 0 for the weights to be right.
+__device__ __forceinline__ bool usable(float check, float m)
+{
+    return check - check == 0.0f && (m == -INFINITY || fabsf(m) < kFarScore);
 }
 
 // ---- stream items: a wave, 16 query rows, K and V straight from memory ------------
@@ -989,7 +1000,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
                 *reinterpret_cast<float4 *>(dst + dim) = make_float4(o[n][0][r], o[n][1][r], o[n][2][r], o[n][3][r]);
                 *reinterpret_cast<float4 *>(dst + dim + 4) = make_float4(o[n][4][r], o[n][5][r], o[n][6][r], o[n][7][r]);
             }
-        if (g == 0) to.ml[at] = make_float2(m - kShift, check - check == 0.0f ? l : kBroken);
+        if (g == 0) to.ml[at] = make_float2(m - kShift, usable(check, m) ? l : kBroken);
     }
 }
 
@@ -1259,7 +1270,7 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
                 if (f * 16 < hd)
                     *reinterpret_cast<float4 *>(dst + 16 * f + 4 * g) =
                         make_float4(o[u][f][0], o[u][f][1], o[u][f][2], o[u][f][3]);
-            if (g == 0) to.ml[at] = make_float2(m[u] - kShift, check - check == 0.0f ? lu : kBroken);
+            if (g == 0) to.ml[at] = make_float2(m[u] - kShift, usable(check, m[u]) ? lu : kBroken);
         }
     }
 }
@@ -1452,9 +1463,10 @@ __global__ __launch_bounds__(64 * waves_of(DP, KF, VF)) void paged_attn_kernel(P
 // ---- joining the parts ---------------------------------------------------------------
 
 // The f16 terms of p and q turn an infinite value into NaN, and a weight of 0
-// times an infinity that its row does not see is one too.  So a row with a part
-// that is not finite is formed again here, one position after the other in f32
-// (`waves` waves taking turns, q and o in LDS); a program whose values are finite never gets here.
+// times an infinity that its row does not see is one too; and scores beyond
+// kFarScore leave p's range.  So a row with a part that is not usable is formed again here, one position after the
+// other in f32 (`waves` waves taking turns, q and o in LDS); a program whose values are finite and whose scores
+// are below 7e5 never gets here.
 __device__ __forceinline__ void slow_row(const PagedAttn &a, int row, int r, int h, int wave, int waves, float *s_q,
                                          float *s_o, float &m, float &l)
 {
