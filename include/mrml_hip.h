@@ -578,7 +578,8 @@ int mrml_hip_rope_kv_append_paged(mrml_hip_ctx *ctx, const float *d_qkv, float *
  * sliding_window of them -- and gives row i of d_out ([max_rows][n_heads *
  * head_dim]).  The shared prefix is read once for the rows of all requests.  Query
  * rows are q_stride floats apart (a multiple of 4).  Rows of no request are left
- * as they are; a row that sees nothing gives zeros.
+ * as they are; a row that sees nothing gives zeros, one whose every score is -inf
+ * NaN.
  *
  * The values are those of mrml_hip_attention_causal over the same rows (K in
  * Q8_0 or Q4_0 multiplied with q as Q8_0 blocks; softmax and sums in f32), added

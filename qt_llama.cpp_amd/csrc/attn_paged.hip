@@ -487,10 +487,11 @@ __device__ __forceinline__ bool softmax_step(float *x, float c, float &m, float 
 }
 
 // Whether a part's sums can be joined with others: they are finite (check: their sum) and its scores were near
-// enough to 0 for the weights to be right.
-__device__ __forceinline__ bool usable(float check, float m)
+// enough to 0 for the weights to be right.  sees: its row sees one of its positions; then no maximum means that
+// every score there was -inf, which is not the same as nothing seen.
+__device__ __forceinline__ bool usable(float check, float m, bool sees)
 {
-    return check - check == 0.0f && (m == -INFINITY || fabsf(m) < kFarScore);
+    return check - check == 0.0f && (m == -INFINITY ? !sees : fabsf(m) < kFarScore);
 }
 
 // ---- stream items: a wave, 16 query rows, K and V straight from memory ------------
@@ -1000,7 +1001,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
                 *reinterpret_cast<float4 *>(dst + dim) = make_float4(o[n][0][r], o[n][1][r], o[n][2][r], o[n][3][r]);
                 *reinterpret_cast<float4 *>(dst + dim + 4) = make_float4(o[n][4][r], o[n][5][r], o[n][6][r], o[n][7][r]);
             }
-        if (g == 0) to.ml[at] = make_float2(m - kShift, usable(check, m) ? l : kBroken);
+        if (g == 0) to.ml[at] = make_float2(m - kShift, usable(check, m, max(vlo, pc.p0) < min(vhi, pc.p1)) ? l : kBroken);
     }
 }
 
@@ -1270,7 +1271,8 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
                 if (f * 16 < hd)
                     *reinterpret_cast<float4 *>(dst + 16 * f + 4 * g) =
                         make_float4(o[u][f][0], o[u][f][1], o[u][f][2], o[u][f][3]);
-            if (g == 0) to.ml[at] = make_float2(m[u] - kShift, usable(check, m[u]) ? lu : kBroken);
+            const bool sees = max(vlo[u], pc.p0) < min(vhi[u], pc.p1);
+            if (g == 0) to.ml[at] = make_float2(m[u] - kShift, usable(check, m[u], sees) ? lu : kBroken);
         }
     }
 }
@@ -1466,8 +1468,9 @@ __global__ __launch_bounds__(64 * waves_of(DP, KF, VF)) void paged_attn_kernel(P
 // times an infinity that its row does not see is one too; and scores beyond
 // kFarScore leave p's range.  So a row with a part that is not usable is formed again here, one position after the
 // other in f32 (`waves` waves taking turns, q and o in LDS); a program whose values are finite and whose scores
-// are below 7e5 never gets here.
-__device__ __forceinline__ void slow_row(const PagedAttn &a, int row, int r, int h, int wave, int waves, float *s_q,
+// are below 7e5 never gets here.  True if a place was there for one of the positions that the row sees: with l 0 all
+// scores were -inf.
+__device__ __forceinline__ bool slow_row(const PagedAttn &a, int row, int r, int h, int wave, int waves, float *s_q,
                                          float *s_o, float &m, float &l)
 {
     const int lane = threadIdx.x & 63, hd = a.head_dim, kvh = div_group(a, h);
@@ -1488,11 +1491,13 @@ __device__ __forceinline__ void slow_row(const PagedAttn &a, int row, int r, int
     }
     m = -INFINITY;
     l = 0.0f;
+    bool seen = false;
 #pragma unroll 1
     for (int t = first + wave; t <= at; t += waves) {
         const bool pre = t < a.prefix_len;
         const int place = pre ? place_at(a, a.prefix, t) : place_at(a, a.table + (size_t)r * a.table_stride, t - a.prefix_len);
         if (place < 0) continue;
+        seen = true;
         const uint8_t *kr = k_rows.row(place), *vr = v_rows.row(place);
         float s = 0.0f;
 #pragma unroll 1
@@ -1506,6 +1511,7 @@ __device__ __forceinline__ void slow_row(const PagedAttn &a, int row, int r, int
         for (int d = lane; d < hd; d += 64) s_o[d] = s_o[d] * f + w * kv_value(vr, a.v_fmt, d);
         m = m2;
     }
+    return seen;
 }
 
 // Joins the parts of each row and head.  W waves share a row and head, lane groups
@@ -1612,8 +1618,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void paged_merge_kernel(Page
     }
     if constexpr (W == 1) {
         if (broken) {
-            slow_row(a, row, ri.x, h, 0, 1, s_q[wave], s_o[wave], m, l);
-            for (int d = lane; d < hd; d += 64) a.out[base * hd + d] = l == 0.0f ? 0.0f : s_o[wave][d] / l;
+            const bool seen = slow_row(a, row, ri.x, h, 0, 1, s_q[wave], s_o[wave], m, l);
+            for (int d = lane; d < hd; d += 64)  // 0 / 0 where all scores are -inf
+                a.out[base * hd + d] = l == 0.0f && !seen ? 0.0f : s_o[wave][d] / l;
             return;
         }
 #pragma unroll
@@ -1632,13 +1639,14 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void paged_merge_kernel(Page
             s_m[wave] = m;
             s_l[wave] = l;
         }
+        bool seen = false;
         if (__syncthreads_or(broken)) {
-            slow_row(a, row, ri.x, h, wave, W, s_q[wave], s_o[wave], m, l);
+            seen = slow_row(a, row, ri.x, h, wave, W, s_q[wave], s_o[wave], m, l);
             if (lane == 0) {
                 s_m[wave] = m;
                 s_l[wave] = l;
             }
-            __syncthreads();
+            seen = __syncthreads_or(seen);
         }
         float most = s_m[0], sum = 0.0f, f[W];
 #pragma unroll
@@ -1652,7 +1660,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void paged_merge_kernel(Page
             float x = 0.0f;
 #pragma unroll
             for (int w = 0; w < W; ++w) x += f[w] == 0.0f ? 0.0f : s_o[w][d] * f[w];
-            a.out[base * hd + d] = sum == 0.0f ? 0.0f : x / sum;
+            a.out[base * hd + d] = sum == 0.0f && !seen ? 0.0f : x / sum;  // 0 / 0 where all scores are -inf
         }
     }
 }

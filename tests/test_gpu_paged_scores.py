@@ -1,4 +1,5 @@
-"""Attention over a paged cache where its scores are very large, against the formula in 64 bits."""
+"""Attention over a paged cache where its scores are very large or all minus infinity, against the formula in 64
+bits."""
 
 from __future__ import annotations
 
@@ -65,3 +66,61 @@ def test_large_scores_leave_one_position(backend, dev, heads, kv_heads, head_dim
                     assert (np.abs(got[row, h] - want) <= np.abs(want) * 2.0 ** -20 + others).all(), \
                         (seed, row, h, s[h, top], got[row, h][:4], want[:4])
         assert led == all_rows if before == [0] else spread == 1e3 or led > all_rows // 2
+
+
+@pytest.mark.parametrize("k_format,v_format", [(0, 0), (0, 1)])
+@pytest.mark.parametrize("n", [1, 40, 900])
+def test_scores_of_minus_infinity_only(backend, dev, k_format, v_format, n):
+    """0 / 0 where every score that a row sees is minus infinity: NaN, as mrml_hip_attention_causal gives; a finite one
+    among them takes the whole weight."""
+    heads, kv, hd = 2, 1, 64
+    for finite in (False, True):
+        b = Batch(backend, dev, 60 + n, [n - 1, 3], [1, 1], 0, 16, heads, kv, hd, k_format, v_format, pad=0)
+        b.q[:] = np.abs(b.q) + np.float32(0.5)
+        u = np.arange(n)
+        slots = b.table[0, u // 16].astype(np.int64) * 16 + u % 16
+        b.k.view(np.float16)[slots, 9] = -np.inf
+        if finite:
+            b.k.view(np.float16)[slots[n // 2], 9] = 1.0
+        b.upload()
+        b.call()
+        dev.sync()
+        got = b.d["out"].numpy().reshape(2, heads, hd)
+        if finite:
+            v = pm.values(b.v, v_format, kv, hd)[slots[n // 2], 0]
+            assert (np.abs(got[0] - v) <= np.abs(v) * 2.0 ** -20).all()
+        else:
+            assert np.isnan(got[0]).all()
+        assert np.isfinite(got[1]).all()
+        ring = backend.HipBuffer.alloc(dev, heads * hd)
+        if not finite and (k_format, v_format) == (0, 0):
+            d = {x: backend.HipBuffer.from_host(dev, np.ascontiguousarray(getattr(b, x)[slots])) for x in ("k", "v")}
+            dev.attention_causal_ref(backend.HipBuffer.from_host(dev, b.q[0]), d["k"], d["v"], ring, n - 1, heads, kv, hd,
+                                     b.scale, None, n, 0, 0)
+            dev.sync()
+            assert np.isnan(ring.numpy()).all()
+
+
+def test_products_past_f32_give_what_the_formula_in_f32_gives(backend, dev):
+    """q and K so large that the scores themselves leave f32: +inf or -inf only; 0 / 0 either way."""
+    for sign in (1.0, -1.0):
+        b = Batch(backend, dev, 70, [40], [1], 20, 16, 2, 1, 64, pad=0)
+        b.k.view(np.float16)[np.isfinite(b.k.view(np.float16))] = 6e4
+        b.q[:] = np.float32(sign * 3e38)
+        b.scale = 1.0
+        b.upload()
+        b.call()
+        dev.sync()
+        assert np.isnan(b.d["out"].numpy()).all(), sign
+
+
+def test_rows_that_see_nothing_stay_zero(backend, dev):
+    """Beside rows whose scores are all minus infinity, rows before the first position still give 0."""
+    b = Batch(backend, dev, 71, [-3, 20], [5, 2], 0, 16, 2, 1, 64)
+    b.q[:] = np.abs(b.q) + np.float32(0.5)
+    b.k.view(np.float16)[:, 9] = -np.inf
+    b.upload()
+    b.call()
+    dev.sync()
+    got = b.d["out"].numpy().reshape(b.max_rows, -1)
+    assert (got[:3] == 0.0).all() and np.isnan(got[3:7]).all() and (got[7:] == 5.0).all()
