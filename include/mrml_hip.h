@@ -538,7 +538,9 @@ int mrml_hip_attention_prefill(mrml_hip_ctx *ctx, const float *d_q, int32_t q_st
  * idle, -1 has finished.  In the requests' order:
  *  - a finished request's pages (of the tokens it holds) return to the free list
  *    (d_free, a stack of page ids with room for n_pages, *d_n_free of them
- *    free), its length becomes 0;
+ *    free), its length becomes 0; if that makes more than n_pages, some page is
+ *    there twice, those past the list's room are dropped and the next
+ *    mrml_hip_sync fails, as after a *d_n_free outside 0..n_pages;
  *  - then every request that adds tokens takes the pages it lacks from the top
  *    of the list into its row of d_table ([n_seqs][table_stride]), and gets rows
  *    d_row_start[r] .. d_row_start[r + 1] of the step (n_seqs + 1 entries).

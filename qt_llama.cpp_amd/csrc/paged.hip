@@ -98,7 +98,7 @@ __global__ __launch_bounds__(kTablesT) void block_tables_kernel(BlockTablesArgs 
     const int n = a.n_seqs, T = blockDim.x, tid = threadIdx.x, ps = a.map.page_size;
     int32_t *s_len = s_mem, *s_new0 = s_mem + n, *s_row = s_mem + 2 * n, *s_back = s_mem + 3 * n;
     const int per = (n + T - 1) / T, r0 = tid * per;
-    const int F0 = min(max(*a.n_free, 0), a.map.n_pages);
+    const int free0 = *a.n_free, F0 = min(max(free0, 0), a.map.n_pages);
     const int longest = a.table_stride * ps;
 
     int len[kTablesPer], add[kTablesPer], need[kTablesPer], code[kTablesPer];
@@ -121,7 +121,10 @@ __global__ __launch_bounds__(kTablesT) void block_tables_kernel(BlockTablesArgs 
         sum[2] += need[e];
     }
     block_exclusive<3>(sum, total, s_sum);
-    const int F1 = (int)min(add_sat(F0, total[0]), (uint32_t)a.map.n_pages);  // free pages once the finished requests' are back
+    const uint32_t F = add_sat(F0, total[0]);
+    const int F1 = (int)min(F, (uint32_t)a.map.n_pages);  // free pages once the finished requests' are back
+    // more pages than there are: somebody's are counted twice, and those past the list's room are lost
+    if (tid == 0 && (F0 != free0 || F > (uint32_t)a.map.n_pages)) page_fault(a.faults);
     // served: the rows and the pages of every request so far are there
     uint32_t got[2] = {0, 0}, all[2];
     {

@@ -233,8 +233,8 @@ int mrml_hip_sync(mrml_hip_ctx *ctx)
     if (int rc = launch_zero(ctx, ctx->page_faults, sizeof faults)) return rc;
     if ((e = hipStreamSynchronize(ctx->stream)) != hipSuccess) return hip_fail(ctx, e, "hipStreamSynchronize");
     return fail(ctx, MRML_HIP_E_INVALID,
-                "paged ops since the last sync met page ids, slots or lengths outside the cache (%u seen): those places "
-                "were left out", faults);
+                "paged ops since the last sync met page ids, slots, lengths or counts of pages outside the cache (%u seen): "
+                "those were left out", faults);
 }
 
 int mrml_hip_set_wait_limit(mrml_hip_ctx *ctx, int32_t polls)
