@@ -82,7 +82,9 @@ const char *mrml_hip_last_error(const mrml_hip_ctx *ctx);
 const char *mrml_hip_status_string(int status);
 /* Waits for the context's stream.  Also fails with MRML_HIP_E_HIP when a
  * kernel's bounded wait for other waves of its workgroup gave up since the
- * last sync on the device (its results are then wrong). */
+ * last sync on the device (its results are then wrong), and with
+ * MRML_HIP_E_INVALID when a paged op since the context's last sync met places
+ * outside its cache (they are left out). */
 int         mrml_hip_sync(mrml_hip_ctx *ctx);
 /* Poll limit of those bounded waits on the context's device (every context
  * on it): polls < 0 restores the default (2^20), 0 makes every wait give up

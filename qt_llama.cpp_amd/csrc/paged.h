@@ -5,7 +5,7 @@
 // format), so that a ring cache read in page_size steps is a paged one.  A
 // place is page * page_size + offset.  Page tables, lengths and slots come from
 // device memory: whatever they hold, a kernel touches no place outside the
-// cache; it leaves such a place out and counts it in the context's
+// cache; it leaves such a place out and says so in the context's
 // page_faults, which mrml_hip_sync turns into an error.
 #pragma once
 
@@ -17,7 +17,7 @@ namespace mrml {
 
 __device__ __forceinline__ void page_fault(uint32_t *faults)
 {
-    __hip_atomic_fetch_add(faults, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(faults, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 
 // Bytes of one head's row in a cache format (0 f16, 1 Q8_0, 2 Q4_0).

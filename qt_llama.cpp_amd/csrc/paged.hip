@@ -357,7 +357,7 @@ int launch_append_paged(mrml_hip_ctx *ctx, const float *qkv, float *q, void *k, 
 #define APPEND(KF, VF)                                                                                            \
     hipLaunchKernelGGL((append_paged_kernel<KF, VF>), grid, dim3(256), 0, ctx->stream, src, dst, kp, vp,          \
                        slots + first, pos + first, n_slots, n_heads, n_kv_heads, head_dim, item_wgs, rope,        \
-                       ctx->page_faults)
+                       ctx->d_page_faults)
         switch (k_fmt * 3 + v_fmt) {
         case 0: APPEND(0, 0); break;
         case 1: APPEND(0, 1); break;
@@ -428,9 +428,8 @@ int mrml_hip_block_tables(mrml_hip_ctx *ctx, const int32_t *lens, const int32_t 
     if (int rc = pages_ok(ctx, "block_tables", n_pages, page_size)) return rc;
     if (int rc = table_ok(ctx, "block_tables", n_seqs, table_stride, page_size, max_rows)) return rc;
     REQUIRE(ctx, pos0 >= 0 && pos0 <= kMaxTablePositions, "block_tables: pos0=%d (0..%d)", pos0, kMaxTablePositions);
-    ctx->paged_used = true;
     const BlockTablesArgs a{lens, want, table, free_pages, n_free, lens_out, n_free_out, row_start, slots, pos, status,
-                            n_seqs, table_stride, max_rows, pos0, page_map(n_pages, page_size), ctx->page_faults};
+                            n_seqs, table_stride, max_rows, pos0, page_map(n_pages, page_size), ctx->d_page_faults};
     // one thread a request or row, whichever are more, up to the workgroup
     const int threads = std::min(kTablesT, (std::max(n_seqs, max_rows) + 63) / 64 * 64);
     const int t = std::max(threads, (n_seqs + kTablesPer * 64 - 1) / (kTablesPer * 64) * 64);
@@ -454,7 +453,6 @@ int mrml_hip_rope_kv_append_paged(mrml_hip_ctx *ctx, const float *qkv, float *q,
     REQUIRE(ctx, ((((uintptr_t)qkv | (uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0),
             "%s: pointers must be 16-byte aligned", name);
     REQUIRE(ctx, ((uintptr_t)d_table & 7) == 0 && n_table >= 0, "%s: table", name);
-    ctx->paged_used = true;
     return launch_append_paged(ctx, qkv, q, k_pages, v_pages, slots, pos, n_rows, n_pages * page_size, n_heads,
                                n_kv_heads, head_dim, k_format, v_format,
                                rope_args(d_table, n_table, freq_base, freq_scale, nullptr));
@@ -490,7 +488,7 @@ int mrml_hip_attention_paged(mrml_hip_ctx *ctx, const float *q, int32_t q_stride
     a.table = table;
     a.lens = lens;
     a.row_start = row_start;
-    a.faults = ctx->page_faults;
+    a.faults = ctx->d_page_faults;
     a.map = page_map(n_pages, page_size);
     a.q_stride = q_stride;
     a.prefix_len = prefix_len;
@@ -512,7 +510,6 @@ int mrml_hip_attention_paged(mrml_hip_ctx *ctx, const float *q, int32_t q_stride
             max_rows, a.longest, prefix_len);
     void *scratch = workspace(ctx, std::max<size_t>(paged_attn_scratch_bytes(a), 16));
     if (!scratch) return MRML_HIP_E_ALLOC;
-    ctx->paged_used = true;
     return launch_paged_attn(ctx, a, scratch);
 }
 

@@ -182,13 +182,17 @@ int mrml_hip_create(int32_t device, mrml_hip_ctx **out)
         delete ctx;
         return MRML_HIP_E_HIP;
     }
-    if (hipMalloc(&ctx->page_faults, sizeof(uint32_t)) != hipSuccess ||
-        launch_zero(ctx, ctx->page_faults, sizeof(uint32_t)) != MRML_HIP_OK) {
-        (void)hipFree(ctx->page_faults);
+    void *faults = nullptr, *d_faults = nullptr;
+    if (hipHostMalloc(&faults, sizeof(uint32_t), hipHostMallocMapped | hipHostMallocCoherent) != hipSuccess ||
+        hipHostGetDevicePointer(&d_faults, faults, 0) != hipSuccess) {
+        if (faults) (void)hipHostFree(faults);
         (void)hipStreamDestroy(ctx->stream);
         delete ctx;
         return MRML_HIP_E_ALLOC;
     }
+    ctx->page_faults = (volatile uint32_t *)faults;
+    ctx->d_page_faults = (uint32_t *)d_faults;
+    *ctx->page_faults = 0;
     *out = ctx;
     return MRML_HIP_OK;
 }
@@ -200,7 +204,7 @@ int mrml_hip_destroy(mrml_hip_ctx *ctx)
     if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
     if (ctx->ws) (void)hipFree(ctx->ws);
     for (void *p : ctx->retired) (void)hipFree(p);
-    if (ctx->page_faults) (void)hipFree(ctx->page_faults);
+    if (ctx->page_faults) (void)hipHostFree((void *)ctx->page_faults);
     if (ctx->stream) (void)hipStreamDestroy(ctx->stream);
     delete ctx;
     return MRML_HIP_OK;
@@ -224,17 +228,12 @@ int mrml_hip_sync(mrml_hip_ctx *ctx)
         return fail(ctx, MRML_HIP_E_HIP,
                     "%u bounded LDS-counter waits gave up (%u matvec, %u decode): the results since the last sync "
                     "are wrong", t_gemv + t_decode, t_gemv, t_decode);
-    if (!ctx->paged_used) return MRML_HIP_OK;
     // Paged ops leave out places that their page tables, lengths or slots put outside the cache.
-    uint32_t faults = 0;
-    if ((e = hipMemcpy(&faults, ctx->page_faults, sizeof faults, hipMemcpyDeviceToHost)) != hipSuccess)
-        return hip_fail(ctx, e, "page faults");
-    if (!faults) return MRML_HIP_OK;
-    if (int rc = launch_zero(ctx, ctx->page_faults, sizeof faults)) return rc;
-    if ((e = hipStreamSynchronize(ctx->stream)) != hipSuccess) return hip_fail(ctx, e, "hipStreamSynchronize");
+    if (!*ctx->page_faults) return MRML_HIP_OK;
+    *ctx->page_faults = 0;
     return fail(ctx, MRML_HIP_E_INVALID,
-                "paged ops since the last sync met page ids, slots, lengths or counts of pages outside the cache (%u seen): "
-                "those were left out", faults);
+                "paged ops since the last sync met page ids, slots, lengths or counts of pages outside the cache: those "
+                "were left out");
 }
 
 int mrml_hip_set_wait_limit(mrml_hip_ctx *ctx, int32_t polls)

@@ -40,3 +40,31 @@ def test_block_tables_every_page_free_again_is_no_fault(backend, dev):
     t.call()
     dev.sync()
     t.check(ref, table, free)
+
+
+def test_faults_of_replays_and_of_each_context_are_reported_once(backend, dev):
+    """Every replay of a graph that holds a bad call is reported by the sync after it, and by that one alone; a graph
+    captured without a fault reports one that its inputs bring later; another context's syncs stay clean."""
+    one = backend.HipDevice.new(0)
+    heads, kv, hd = 2, 1, 64
+    try:
+        k, v = (up(backend, one, np.zeros((8, kv * hd), np.float16)) for _ in range(2))
+        x, q = up(backend, one, np.ones((2, (heads + 2 * kv) * hd), np.float32)), backend.HipBuffer.alloc(one, 2 * heads * hd)
+        slots, pos = up(backend, one, np.array([3, 5], np.int32)), up(backend, one, np.zeros(2, np.int32))
+        call = lambda: one.qkv_postprocess_paged(x, q, k, v, slots, pos, 2, 2, 4, heads, kv, hd, 10000.0)  # noqa: E731
+        call()
+        one.sync()
+        graph = one.capture(call)
+        for bad in (False, True, False, True, True):
+            slots.copy_from_host(np.array([3, 8 if bad else 5], np.int32))
+            graph.launch()
+            dev.sync()
+            if bad:
+                with pytest.raises(backend.HipError, match="outside the cache"):
+                    one.sync()
+            one.sync()
+        graph.close()
+        for b in (k, v, x, q, slots, pos):
+            b.close()
+    finally:
+        one.close()
