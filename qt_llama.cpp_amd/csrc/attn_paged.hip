@@ -27,6 +27,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "any_bytes.h"
 #include "paged.h"
 
 namespace mrml {
@@ -137,6 +138,15 @@ __device__ __forceinline__ void pin()
 {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
+}
+
+// What lanes of this wave wrote to LDS before is there for its other lanes after (a wave's LDS accesses keep their
+// order; the barrier alone tells the compiler nothing about memory).
+__device__ __forceinline__ void wave_handover()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
 }
 
 // v, as a value that the compiler forms anew where it is used: what follows from it is
@@ -598,11 +608,11 @@ struct QuantPieces {
     // with its row is written in what both share.
     __device__ __forceinline__ void store(Tile &tile, int row_bytes) const
     {
-        typedef volatile __attribute__((address_space(3))) uint32_t *Words;
-        typedef volatile __attribute__((address_space(3))) uint16_t *Halves;
+        typedef volatile __attribute__((address_space(3))) Any32 *Words;
+        typedef volatile __attribute__((address_space(3))) Any16 *Halves;
         if ((row_bytes & 15) == 0) {
 #pragma unroll
-            for (int e = 0; e < Tile::kLoads; ++e) *reinterpret_cast<uint4 *>(tile.b + place(e)) = x[e];
+            for (int e = 0; e < Tile::kLoads; ++e) *reinterpret_cast<Any128 *>(tile.b + place(e)) = Any128{x[e].x, x[e].y, x[e].z, x[e].w};
         } else if ((row_bytes & 3) == 0) {
 #pragma unroll
             for (int e = 0; e < Tile::kLoads; ++e) {
@@ -624,8 +634,8 @@ struct QuantPieces {
 // 8 bytes at p + at, at even: of the words around them.
 __device__ __forceinline__ Bytes8 pick8(const uint8_t *p, int at)
 {
-    const uint32_t *w = reinterpret_cast<const uint32_t *>(p + (at & ~2));
-    const uint32_t w0 = w[0], w1 = w[1], w2 = w[2];
+    const uint8_t *w = p + (at & ~2);
+    const uint32_t w0 = get32(w), w1 = get32(w + 4), w2 = get32(w + 8);
     return Bytes8{__builtin_amdgcn_alignbyte(w1, w0, at & 2), __builtin_amdgcn_alignbyte(w2, w1, at & 2)};
 }
 
@@ -698,7 +708,7 @@ __device__ __forceinline__ void load_quant_q(const PagedAttn &a, const float *ro
             }
         }
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_handover();
 }
 
 template <int DP, int KF, int VF, bool ONCE>
@@ -748,7 +758,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
         k_on_way.start(kv_row_bytes(KF, hd), lane);
         if (hd < DP)  // blocks past the head: scales and quants of 0
             for (int x = kv_row_bytes(KF, hd) / 2 + (lane >> 5); x < KS * kBlkK / 2; x += 2)
-                *reinterpret_cast<uint16_t *>(lds.kq.b + (lane & 31) * lds.kq.kRow + 2 * x) = 0;
+                put16(lds.kq.b + (lane & 31) * lds.kq.kRow + 2 * x, 0);
     }
     if constexpr (VQ) v_on_way.start(kv_row_bytes(VF, hd), lane);
     auto load_k = [&](int place) {
@@ -772,10 +782,10 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
             return;
         } else {
         lds.place[lane & 31] = place;
-        __builtin_amdgcn_wave_barrier();
+        wave_handover();
         const int4 pa = *reinterpret_cast<const int4 *>(lds.place + 4 * g);
         const int4 pb = *reinterpret_cast<const int4 *>(lds.place + 16 + 4 * g);
-        __builtin_amdgcn_wave_barrier();
+        wave_handover();
         const int pl[8] = {pa.x, pa.y, pa.z, pa.w, pb.x, pb.y, pb.z, pb.w};
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
@@ -800,7 +810,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
         float x[8];
         if constexpr (KQ) {
             k_on_way.store(lds.kq, kv_row_bytes(KF, hd));
-            __builtin_amdgcn_wave_barrier();
+            wave_handover();
             if (t0 + kUnitA < pc.p1) load_k(place_next);
             float4v acc[2] = {};
             const uint8_t *rows = lds.kq.b + i * lds.kq.kRow;
@@ -816,9 +826,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
                 for (int h = 0; h < 2; ++h) {
                     const uint8_t *b = rows + 16 * h * lds.kq.kRow + s * kBlkK;
                     const uint8_t *quants = b + (KF == 1 ? 8 * g : 8 * (g & 1));
-                    const Bytes8 w = s & 1 ? Bytes8{reinterpret_cast<const uint32_t *>(quants + 2)[0],
-                                                    reinterpret_cast<const uint32_t *>(quants + 2)[1]}
-                                           : pick8(quants, 2);
+                    const Bytes8 w = s & 1 ? Bytes8{get32(quants + 2), get32(quants + 6)} : pick8(quants, 2);
                     uint32_t w0 = w.a, w1 = w.b;
                     if (KF == 2) {  // dims 8 g .. of the block: low nibbles, then high ones
                         w0 = (w0 >> (4 * (g >> 1))) & 0x0f0f0f0fu;
@@ -826,7 +834,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
                     }
                     const long kk = (long)((uint64_t)w0 | ((uint64_t)w1 << 32));
                     const int4v is = __builtin_amdgcn_mfma_i32_16x16x32_i8(qq.q[s], kk, sum8, 0, 0, 0);
-                    const float dk = f16_bits_to_f32(*reinterpret_cast<const uint16_t *>(b));
+                    const float dk = f16_bits_to_f32(get16(b));
 #pragma unroll
                     for (int r = 0; r < 4; ++r) acc[h][r] = fmaf((float)is[r], dk * qd[r], acc[h][r]);
                 }
@@ -835,13 +843,13 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) lds.scores[(4 * g + r) * kTrRow + 16 * h + i] = acc[h][r];
-            __builtin_amdgcn_wave_barrier();
+            wave_handover();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const float4 y = *reinterpret_cast<const float4 *>(lds.scores + i * kTrRow + 16 * h + 4 * g);
                 x[4 * h] = y.x, x[4 * h + 1] = y.y, x[4 * h + 2] = y.z, x[4 * h + 3] = y.w;
             }
-            __builtin_amdgcn_wave_barrier();
+            wave_handover();
         } else {
             // K is in LDS once no more than this tile's V (loaded after it) is on its way
             constexpr int kLeft = VQ ? 0 : NG * 8;
@@ -910,7 +918,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
         const half8 p_hi = as_half8(ph[0], ph[1], ph[2], ph[3]), p_lo = as_half8(pw[0], pw[1], pw[2], pw[3]);
         if constexpr (VQ) {
             v_on_way.store(lds.vq, kv_row_bytes(VF, hd));
-            __builtin_amdgcn_wave_barrier();
+            wave_handover();
             if (t0 + kUnitA < pc.p1) load_v(place_next);
         }
 #pragma unroll
@@ -924,7 +932,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const uint8_t *b = rows + (16 * (j >> 2) + (j & 3)) * lds.vq.kRow;
-                    const _Float16 d = *reinterpret_cast<const _Float16 *>(b + scale);
+                    const _Float16 d = __builtin_bit_cast(_Float16, get16(b + scale));
                     vd[j] = v_there >> j & 1 ? d : (_Float16)0.0f;
                     vq[j] = pick8(b, quants);
                 }
@@ -979,7 +987,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
         }
         if constexpr (!VQ)
             if (t0 + kUnitA < pc.p1) load_v(place_next);
-        __builtin_amdgcn_wave_barrier();
+        wave_handover();
         place = place_next;
     }
     l = row_sum(l);
