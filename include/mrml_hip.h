@@ -106,7 +106,10 @@ int         mrml_hip_workspace_bytes(mrml_hip_ctx *ctx, size_t *bytes);
  *      (cuda.rs:1841-1858, 1957-2003).  Ops issued on the context between
  *      begin and end are recorded, not run; launch replays them on the
  *      stream.  Ops that would grow the workspace fail during capture, so call
- *      mrml_hip_reserve_workspace (or run the ops once) first. --------------- */
+ *      mrml_hip_reserve_workspace (or run the ops once) first.  A graph keeps the
+ *      workspace it was captured with: while one lives, a workspace that grows
+ *      at least doubles, and outgrown ones (together smaller than it) are kept
+ *      until it grows after the last graph was destroyed. -------------------- */
 int mrml_hip_graph_begin(mrml_hip_ctx *ctx);
 int mrml_hip_graph_end(mrml_hip_ctx *ctx, void **graph_exec_out);
 int mrml_hip_graph_launch(mrml_hip_ctx *ctx, void *graph_exec);

@@ -18,8 +18,8 @@ struct mrml_hip_ctx {
     size_t ws_bytes = 0;
     void *noalloc_scratch = nullptr;  // the device's copy of the allocation-free GEMM's scratch
     bool rows_loaded = false;         // attn_rows.hip's code is on the device (load_attn_rows)
-    bool captured = false;            // a graph was captured on this context: it may hold the scratch's address
-    std::vector<void *> retired;      // outgrown scratch that such a graph may still use, freed with the context
+    std::vector<void *> graphs;       // captured on this context and not destroyed: they may hold the scratch's address
+    std::vector<void *> retired;      // outgrown scratch that such graphs may still use
     // Not 0 once a kernel met and left out a place outside a paged cache.  Host memory that kernels write to, so that
     // sync looks without a copy (which cost every later sync of the context 11 us on 24).
     volatile uint32_t *page_faults = nullptr;

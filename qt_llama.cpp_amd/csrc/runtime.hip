@@ -6,6 +6,7 @@
 // and a per-device stream; here, libamdhip64 linked directly, gfx950 code
 // objects linked into this library, and one stream per context.
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -49,7 +50,7 @@ int check_launch(mrml_hip_ctx *ctx, const char *kernel)
     return e == hipSuccess ? 0 : hip_fail(ctx, e, kernel);
 }
 
-// Keeps outgrown scratch that a captured graph may still use until the context ends.
+// Keeps outgrown scratch that a captured graph may still use.
 static void retire(mrml_hip_ctx *ctx, void *p)
 {
     try {
@@ -58,23 +59,34 @@ static void retire(mrml_hip_ctx *ctx, void *p)
     }
 }
 
+// While a captured graph lives, outgrown scratch is kept, and the new one is at least twice the old one, so that all
+// that is kept together is smaller than the scratch in use.  It is freed when the scratch grows after the last graph
+// was destroyed (not at once: freeing waits for the device, and destroying a graph never did), or with the context.
 void *workspace(mrml_hip_ctx *ctx, size_t bytes)
 {
     if (bytes <= ctx->ws_bytes) return ctx->ws;
-    size_t want = align_up(bytes, (size_t)1 << 20);
+    size_t want = align_up(bytes, (size_t)1 << 20), least = want;
     if (ctx->ws) {
         // The old scratch may still be read by queued work.
         hipError_t e = hipStreamSynchronize(ctx->stream);
         if (e != hipSuccess) { hip_fail(ctx, e, "hipStreamSynchronize (workspace)"); return nullptr; }
-        if (!ctx->captured)
+        if (ctx->graphs.empty()) {
             (void)hipFree(ctx->ws);
-        else
+            for (void *p : ctx->retired) (void)hipFree(p);
+            ctx->retired.clear();
+        } else {
             retire(ctx, ctx->ws);
+            want = want > 2 * ctx->ws_bytes ? want : 2 * ctx->ws_bytes;
+        }
         ctx->ws = nullptr;
         ctx->ws_bytes = 0;
     }
     void *p = nullptr;
     hipError_t e = hipMalloc(&p, want);
+    if (e != hipSuccess && want > least) {
+        (void)hipGetLastError();
+        e = hipMalloc(&p, want = least);
+    }
     if (e != hipSuccess) {
         fail(ctx, MRML_HIP_E_ALLOC, "workspace hipMalloc(%zu): %s", want, hipGetErrorString(e));
         return nullptr;
@@ -295,7 +307,6 @@ int mrml_hip_graph_begin(mrml_hip_ctx *ctx)
 {
     CTX_GUARD(ctx);
     hipError_t e = hipStreamBeginCapture(ctx->stream, hipStreamCaptureModeThreadLocal);
-    if (e == hipSuccess) ctx->captured = true;
     return e == hipSuccess ? 0 : hip_fail(ctx, e, "hipStreamBeginCapture");
 }
 
@@ -311,6 +322,12 @@ int mrml_hip_graph_end(mrml_hip_ctx *ctx, void **graph_exec_out)
     e = hipGraphInstantiate(&exec, graph, nullptr, nullptr, 0);
     (void)hipGraphDestroy(graph);
     if (e != hipSuccess) return hip_fail(ctx, e, "hipGraphInstantiate");
+    try {
+        ctx->graphs.push_back((void *)exec);
+    } catch (...) {
+        (void)hipGraphExecDestroy(exec);
+        return fail(ctx, MRML_HIP_E_ALLOC, "graph_end: out of memory");
+    }
     *graph_exec_out = (void *)exec;
     return MRML_HIP_OK;
 }
@@ -328,6 +345,8 @@ int mrml_hip_graph_destroy(mrml_hip_ctx *ctx, void *graph_exec)
     CTX_GUARD(ctx);
     if (!graph_exec) return MRML_HIP_OK;
     hipError_t e = hipGraphExecDestroy((hipGraphExec_t)graph_exec);
+    const auto at = std::find(ctx->graphs.begin(), ctx->graphs.end(), graph_exec);
+    if (e == hipSuccess && at != ctx->graphs.end()) ctx->graphs.erase(at);
     return e == hipSuccess ? 0 : hip_fail(ctx, e, "hipGraphExecDestroy");
 }
 
