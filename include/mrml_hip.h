@@ -555,9 +555,14 @@ int mrml_hip_attention_prefill(mrml_hip_ctx *ctx, const float *d_q, int32_t q_st
  * lengths and the free pages afterwards (they may be d_lens and d_n_free).
  * d_status[r]: 0, or why the request was left as it is, without rows: 1 no page
  * left for it, 2 its table row is too short, 3 no row left for it, 4 a negative
- * or too large length or d_new below -1.  Rows and pages are counted over all
- * requests before it that want some, so after one that had to wait for them
- * (status 3, 1) no later one overtakes it. */
+ * or too large length or d_new below -1.  Pages are counted over all requests
+ * before it that lack some, rows over all before it that want some and do not
+ * lack pages (3 is said where both are missing).  So no request takes a page
+ * ahead of one that waits for pages, or a row ahead of one that waits for rows;
+ * one that still has room in its pages goes on beside one that waits for pages.
+ * What the caller has to see to: a request that wants more than max_rows holds
+ * back every later one, and when all wait for pages one must end (-1), or the
+ * first of them want less. */
 int mrml_hip_block_tables(mrml_hip_ctx *ctx, const int32_t *d_lens, const int32_t *d_new, int32_t n_seqs,
                           int32_t *d_table, int32_t table_stride, int32_t page_size, int32_t *d_free,
                           const int32_t *d_n_free, int32_t n_pages, int32_t *d_lens_out, int32_t *d_n_free_out,

@@ -94,7 +94,7 @@ __device__ __forceinline__ void upper(const int32_t *ends, int n, const int *x, 
 __global__ __launch_bounds__(kTablesT) void block_tables_kernel(BlockTablesArgs a)
 {
     extern __shared__ int32_t s_mem[];
-    __shared__ uint32_t s_sum[3 * 16], s_got[2 * 16];
+    __shared__ uint32_t s_sum[3 * 16], s_rows[16], s_got[2 * 16];
     const int n = a.n_seqs, T = blockDim.x, tid = threadIdx.x, ps = a.map.page_size;
     int32_t *s_len = s_mem, *s_new0 = s_mem + n, *s_row = s_mem + 2 * n, *s_back = s_mem + 3 * n;
     const int per = (n + T - 1) / T, r0 = tid * per;
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(kTablesT) void block_tables_kernel(BlockTablesArgs 
     const int longest = a.table_stride * ps;
 
     int len[kTablesPer], add[kTablesPer], need[kTablesPer], code[kTablesPer];
-    uint32_t sum[3] = {0, 0, 0}, total[3];  // a request's share is below 2^22
+    uint32_t sum[3] = {0, 0, 0}, total[3];  // returned pages, rows, lacking pages; a request's share is below 2^22
 #pragma unroll
     for (int e = 0; e < kTablesPer; ++e) {
         if (e >= per) break;
@@ -125,7 +125,21 @@ __global__ __launch_bounds__(kTablesT) void block_tables_kernel(BlockTablesArgs 
     const int F1 = (int)min(F, (uint32_t)a.map.n_pages);  // free pages once the finished requests' are back
     // more pages than there are: somebody's are counted twice, and those past the list's room are lost
     if (tid == 0 && (F0 != free0 || F > (uint32_t)a.map.n_pages)) page_fault(a.faults);
-    // served: the rows and the pages of every request so far are there
+    // Served: the pages of every request so far are there, and the rows of every one so far that has its pages.  So none
+    // takes a page or a row ahead of one that waits for the same, and one that waits for pages keeps no row from the others.
+    bool waits[kTablesPer] = {};
+    if (total[2] > (uint32_t)F1) {  // somebody waits for pages: the rows without theirs
+        uint32_t asked[1] = {0}, all[1], pages = sum[2];
+#pragma unroll
+        for (int e = 0; e < kTablesPer; ++e) {
+            if (e >= per) break;
+            pages = add_sat(pages, need[e]);
+            waits[e] = need[e] > 0 && pages > (uint32_t)F1;
+            asked[0] += waits[e] ? 0 : add[e];
+        }
+        block_exclusive<1>(asked, all, s_rows);
+        sum[1] = asked[0];
+    }
     uint32_t got[2] = {0, 0}, all[2];
     {
         uint32_t back = sum[0], rows = sum[1], pages = sum[2];
@@ -139,13 +153,11 @@ __global__ __launch_bounds__(kTablesT) void block_tables_kernel(BlockTablesArgs 
                 s_new0[r] = (int32_t)min(pages, (uint32_t)INT32_MAX);
                 s_len[r] = len[e];
             }
-            rows = add_sat(rows, add[e]);
             pages = add_sat(pages, need[e]);
             if (code[e] == 0 && add[e] > 0) {
-                if (rows > (uint32_t)a.max_rows)
-                    code[e] = 3;
-                else if (need[e] > 0 && pages > (uint32_t)F1)
-                    code[e] = 1;
+                const uint32_t with = add_sat(rows, add[e]);
+                code[e] = with > (uint32_t)a.max_rows ? 3 : waits[e] ? 1 : 0;
+                if (!waits[e]) rows = with;
             }
             if (code[e] > 0) add[e] = need[e] = 0;
             got[0] += add[e];
