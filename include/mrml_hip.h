@@ -573,7 +573,7 @@ int mrml_hip_block_tables(mrml_hip_ctx *ctx, const int32_t *d_lens, const int32_
  * rotated at position d_pos[i], its q to row i of d_q ([n_rows][n_heads *
  * head_dim]), its k and v to place d_slots[i] of the paged caches in their
  * formats -- each the bits that entry point gives.  Rows with a negative slot
- * are left out, their row of d_q too.  Angles as there: d_table (nullable) for
+ * are left out, their row of d_q too.  d_q shares no memory with d_qkv.  Angles as there: d_table (nullable) for
  * positions below n_table, else evaluated on the device.  No two rows of a call
  * may have the same slot.  head_dim a multiple of 32 up to 512, groups up to
  * 16. */
@@ -589,7 +589,8 @@ int mrml_hip_rope_kv_append_paged(mrml_hip_ctx *ctx, const float *d_qkv, float *
  * request's own positions up to itself -- with sliding_window > 0 the last
  * sliding_window of them -- and gives row i of d_out ([max_rows][n_heads *
  * head_dim]).  The shared prefix is read once for the rows of all requests.  Query
- * rows are q_stride floats apart (a multiple of 4).  Rows of no request are left
+ * rows are q_stride floats apart (a multiple of 4).  d_out may be d_q where
+ * q_stride is n_heads * head_dim, and shares no memory with it else.  Rows of no request are left
  * as they are; a row that sees nothing gives zeros, one whose every score is -inf
  * NaN.
  *

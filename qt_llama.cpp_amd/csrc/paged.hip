@@ -421,6 +421,12 @@ int formats_ok(mrml_hip_ctx *ctx, const char *name, int32_t n_heads, int32_t n_k
     return MRML_HIP_OK;
 }
 
+// Whether n floats at x and m floats at y share memory.
+bool overlap(const float *x, size_t n, const float *y, size_t m)
+{
+    return (uintptr_t)x < (uintptr_t)(y + m) && (uintptr_t)y < (uintptr_t)(x + n);
+}
+
 }  // namespace
 
 }  // namespace mrml
@@ -458,10 +464,12 @@ int mrml_hip_rope_kv_append_paged(mrml_hip_ctx *ctx, const float *qkv, float *q,
     CTX_GUARD(ctx);
     const char *name = "rope_kv_append_paged";
     REQUIRE(ctx, qkv && q && k_pages && v_pages && slots && pos, "%s: null pointer", name);
-    REQUIRE(ctx, q != qkv, "%s: q must not be the stacked rows", name);
     if (int rc = formats_ok(ctx, name, n_heads, n_kv_heads, head_dim, k_format, v_format)) return rc;
     if (int rc = pages_ok(ctx, name, n_pages, page_size)) return rc;
     REQUIRE(ctx, n_rows >= 1 && n_rows <= (1 << 20), "%s: n_rows=%d (1..2^20)", name, n_rows);
+    const size_t q_dim = (size_t)n_heads * head_dim, width = (size_t)(n_heads + 2 * n_kv_heads) * head_dim;
+    REQUIRE(ctx, !overlap(q, n_rows * q_dim, qkv, n_rows * width), "%s: q must not share memory with the stacked rows",
+            name);
     REQUIRE(ctx, ((((uintptr_t)qkv | (uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0),
             "%s: pointers must be 16-byte aligned", name);
     REQUIRE(ctx, ((uintptr_t)d_table & 7) == 0 && n_table >= 0, "%s: table", name);
@@ -520,6 +528,10 @@ int mrml_hip_attention_paged(mrml_hip_ctx *ctx, const float *q, int32_t q_stride
     REQUIRE(ctx, paged_attn_countable(a),
             "%s: n_seqs=%d, max_rows=%d and positions (%d of a table row, prefix %d) are too many for one call", name, n_seqs,
             max_rows, a.longest, prefix_len);
+    // The joining launch may read a row and head of q again before it writes the same of out, in any order of them.
+    const size_t q_dim = (size_t)n_heads * head_dim, q_span = (size_t)(max_rows - 1) * q_stride + q_dim;
+    REQUIRE(ctx, !overlap(out, max_rows * q_dim, q, q_span) || (out == q && (size_t)q_stride == q_dim),
+            "%s: out shares memory with q (it may be q itself where the rows of q are not apart)", name);
     void *scratch = workspace(ctx, std::max<size_t>(paged_attn_scratch_bytes(a), 16));
     if (!scratch) return MRML_HIP_E_ALLOC;
     return launch_paged_attn(ctx, a, scratch);
