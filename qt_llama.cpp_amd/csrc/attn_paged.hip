@@ -497,11 +497,10 @@ __device__ __forceinline__ bool softmax_step(float *x, float c, float &m, float 
 }
 
 // Whether a part's sums can be joined with others: they are finite (check: their sum) and its scores were near
-// enough to 0 for the weights to be right.  sees: its row sees one of its positions; then no maximum means that
-// every score there was -inf, which is not the same as nothing seen.
-__device__ __forceinline__ bool usable(float check, float m, bool sees)
+// enough to 0 for the weights to be right.
+__device__ __forceinline__ bool usable(float check, float m)
 {
-    return check - check == 0.0f && (m == -INFINITY ? !sees : fabsf(m) < kFarScore);
+    return check - check == 0.0f && (m == -INFINITY || fabsf(m) < kFarScore);
 }
 
 // ---- stream items: a wave, 16 query rows, K and V straight from memory ------------
@@ -1009,7 +1008,7 @@ __device__ __forceinline__ void stream_item(const PagedAttn &a, const Scan<64 * 
                 *reinterpret_cast<float4 *>(dst + dim) = make_float4(o[n][0][r], o[n][1][r], o[n][2][r], o[n][3][r]);
                 *reinterpret_cast<float4 *>(dst + dim + 4) = make_float4(o[n][4][r], o[n][5][r], o[n][6][r], o[n][7][r]);
             }
-        if (g == 0) to.ml[at] = make_float2(m - kShift, usable(check, m, max(vlo, pc.p0) < min(vhi, pc.p1)) ? l : kBroken);
+        if (g == 0) to.ml[at] = make_float2(m - kShift, usable(check, m) ? l : kBroken);
     }
 }
 
@@ -1279,8 +1278,7 @@ __device__ __forceinline__ void block_item(const PagedAttn &a, const Scan<64 * w
                 if (f * 16 < hd)
                     *reinterpret_cast<float4 *>(dst + 16 * f + 4 * g) =
                         make_float4(o[u][f][0], o[u][f][1], o[u][f][2], o[u][f][3]);
-            const bool sees = max(vlo[u], pc.p0) < min(vhi[u], pc.p1);
-            if (g == 0) to.ml[at] = make_float2(m[u] - kShift, usable(check, m[u], sees) ? lu : kBroken);
+            if (g == 0) to.ml[at] = make_float2(m[u] - kShift, usable(check, m[u]) ? lu : kBroken);
         }
     }
 }
@@ -1476,9 +1474,8 @@ __global__ __launch_bounds__(64 * waves_of(DP, KF, VF)) void paged_attn_kernel(P
 // times an infinity that its row does not see is one too; and scores beyond
 // kFarScore leave p's range.  So a row with a part that is not usable is formed again here, one position after the
 // other in f32 (`waves` waves taking turns, q and o in LDS); a program whose values are finite and whose scores
-// are below 7e5 never gets here.  True if a place was there for one of the positions that the row sees: with l 0 all
-// scores were -inf.
-__device__ __forceinline__ bool slow_row(const PagedAttn &a, int row, int r, int h, int wave, int waves, float *s_q,
+// are below 7e5 never gets here.
+__device__ __forceinline__ void slow_row(const PagedAttn &a, int row, int r, int h, int wave, int waves, float *s_q,
                                          float *s_o, float &m, float &l)
 {
     const int lane = threadIdx.x & 63, hd = a.head_dim, kvh = div_group(a, h);
@@ -1499,13 +1496,11 @@ __device__ __forceinline__ bool slow_row(const PagedAttn &a, int row, int r, int
     }
     m = -INFINITY;
     l = 0.0f;
-    bool seen = false;
 #pragma unroll 1
     for (int t = first + wave; t <= at; t += waves) {
         const bool pre = t < a.prefix_len;
         const int place = pre ? place_at(a, a.prefix, t) : place_at(a, a.table + (size_t)r * a.table_stride, t - a.prefix_len);
         if (place < 0) continue;
-        seen = true;
         const uint8_t *kr = k_rows.row(place), *vr = v_rows.row(place);
         float s = 0.0f;
 #pragma unroll 1
@@ -1519,7 +1514,19 @@ __device__ __forceinline__ bool slow_row(const PagedAttn &a, int row, int r, int
         for (int d = lane; d < hd; d += 64) s_o[d] = s_o[d] * f + w * kv_value(vr, a.v_fmt, d);
         m = m2;
     }
-    return seen;
+}
+
+// What a row without any weight gives: 0 if no position that it sees has a place, else 0 / 0, since all its scores
+// were -inf.
+__device__ __forceinline__ float without_weight(const PagedAttn &a, int row, int r)
+{
+    const int len = clamp_len(a, a.lens[r]), at = a.prefix_len + len - (a.row_start[r + 1] - row);
+#pragma unroll 1
+    for (int t = a.window ? max(0, at - a.window + 1) : 0; t <= at; ++t)
+        if ((t < a.prefix_len ? place_at(a, a.prefix, t)
+                              : place_at(a, a.table + (size_t)r * a.table_stride, t - a.prefix_len)) >= 0)
+            return NAN;
+    return 0.0f;
 }
 
 // Joins the parts of each row and head.  W waves share a row and head, lane groups
@@ -1625,10 +1632,10 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void paged_merge_kernel(Page
         }
     }
     if constexpr (W == 1) {
+        if (broken) slow_row(a, row, ri.x, h, 0, 1, s_q[wave], s_o[wave], m, l);
+        const float none = l == 0.0f ? without_weight(a, row, ri.x) : 0.0f;
         if (broken) {
-            const bool seen = slow_row(a, row, ri.x, h, 0, 1, s_q[wave], s_o[wave], m, l);
-            for (int d = lane; d < hd; d += 64)  // 0 / 0 where all scores are -inf
-                a.out[base * hd + d] = l == 0.0f && !seen ? 0.0f : s_o[wave][d] / l;
+            for (int d = lane; d < hd; d += 64) a.out[base * hd + d] = l == 0.0f ? none : s_o[wave][d] / l;
             return;
         }
 #pragma unroll
@@ -1636,7 +1643,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void paged_merge_kernel(Page
             const int d = d0 + 256 * y;
             if (lane < lanes && d < hd)
                 *reinterpret_cast<float4 *>(a.out + base * hd + d) =
-                    l == 0.0f ? make_float4(0, 0, 0, 0) : make_float4(o[y].x / l, o[y].y / l, o[y].z / l, o[y].w / l);
+                    l == 0.0f ? make_float4(none, none, none, none) : make_float4(o[y].x / l, o[y].y / l, o[y].z / l, o[y].w / l);
         }
     } else {
         if (lane < lanes) {
@@ -1647,14 +1654,13 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void paged_merge_kernel(Page
             s_m[wave] = m;
             s_l[wave] = l;
         }
-        bool seen = false;
         if (__syncthreads_or(broken)) {
-            seen = slow_row(a, row, ri.x, h, wave, W, s_q[wave], s_o[wave], m, l);
+            slow_row(a, row, ri.x, h, wave, W, s_q[wave], s_o[wave], m, l);
             if (lane == 0) {
                 s_m[wave] = m;
                 s_l[wave] = l;
             }
-            seen = __syncthreads_or(seen);
+            __syncthreads();
         }
         float most = s_m[0], sum = 0.0f, f[W];
 #pragma unroll
@@ -1664,11 +1670,12 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void paged_merge_kernel(Page
             f[w] = s_l[w] == 0.0f ? 0.0f : s_l[w] != s_l[w] ? s_l[w] : exp2_hw(s_m[w] - most);  // NaN stays
             sum += f[w] == 0.0f ? 0.0f : s_l[w] * f[w];
         }
+        const float none = sum == 0.0f ? without_weight(a, row, ri.x) : 0.0f;
         for (int d = tid; d < hd; d += 64 * W) {
             float x = 0.0f;
 #pragma unroll
             for (int w = 0; w < W; ++w) x += f[w] == 0.0f ? 0.0f : s_o[w][d] * f[w];
-            a.out[base * hd + d] = sum == 0.0f && !seen ? 0.0f : x / sum;  // 0 / 0 where all scores are -inf
+            a.out[base * hd + d] = sum == 0.0f ? none : x / sum;
         }
     }
 }

@@ -68,3 +68,23 @@ def test_faults_of_replays_and_of_each_context_are_reported_once(backend, dev):
             b.close()
     finally:
         one.close()
+
+
+@pytest.mark.parametrize("requests", [1, 40, 300])  # each of the join's forms
+@pytest.mark.parametrize("k_format", [0, 1])
+def test_rows_whose_every_page_is_outside_give_zeros(backend, dev, requests, k_format):
+    """All positions of request 0 are left out: zeros, as a row that sees nothing gives; the others as they are."""
+    b = Batch(backend, dev, 140, [45] * requests, [1] * requests, 0, 16, 8, 2, 64, k_format, k_format)
+    want = b.reference()[0]
+    b.upload()
+    table = b.table.copy()
+    table[0] = [-1, b.n_pages, 2 ** 31 - 1, -2 ** 31][:b.stride]
+    b.d["table"].copy_from_host(table)
+    b.call()
+    with pytest.raises(backend.HipError, match="outside the cache"):
+        dev.sync()
+    dev.sync()
+    got = b.d["out"].numpy().reshape(b.max_rows, 8, 64)
+    assert (got[0] == 0.0).all() and (got[b.rows:] == 5.0).all()
+    if requests > 1:
+        assert np.abs(got[1:b.rows] - want[1:b.rows]).max() <= 1e-5 * np.abs(want[1:b.rows]).max()
