@@ -1781,9 +1781,11 @@ int launch_paged_attn(mrml_hip_ctx *ctx, const PagedAttn &a, void *scratch)
     default: launch_dp<512>(ctx, a, p); break;
     }
     if (int rc = check_launch(ctx, "paged_attn_kernel")) return rc;
-    // Waves a row and head by how many there are, measured on both sides of the lines (us): 32 pairs in 500 parts
-    // each 86 with 4 and 60 with 16 (the whole call), 256 pairs 7.1 and 6.8, 408 pairs 7.2 and 9.0, 732 pairs 5.3 and 10.8;
-    // 408 pairs 16.2 with one and 7.4 with 4, 732 8.4 and 5.6, 2048 11.9 and 13.7, 4096 5.2 and 12.0.
+    // Waves a row and head by how many there can be; how many there are is on the device (32 requests of 8 heads with
+    // max_rows 256 or more get one wave a pair: 39 us a call, 30 with max_rows 32).  Measured on both sides of the
+    // lines (us): 32 pairs in 500 parts each 86 with 4 and 60 with 16 (the whole call), 256 pairs 7.1 and 6.8, 408 pairs
+    // 7.2 and 9.0, 732 pairs 5.3 and 10.8; 408 pairs 16.2 with one and 7.4 with 4, 732 8.4 and 5.6, 2048 11.9 and
+    // 13.7, 4096 5.2 and 12.0.
     const int pairs = a.max_rows * a.n_heads;
     if (pairs > 1024)
         hipLaunchKernelGGL(paged_merge_kernel<1>, dim3((pairs + 3) / 4), dim3(256), 0, ctx->stream, a, p);

@@ -88,7 +88,7 @@ __device__ __forceinline__ void upper(const int32_t *ends, int n, const int *x, 
 // bound by the latency of a few dependent round trips (lengths, free list or
 // table, stores), not by its bytes, so everything runs in one launch and
 // every list (rows, returned pages) is walked flat over all threads.  6 requests
-// take 2.9 us; 700 with 4816 rows and 948 returned pages 9.8 us, most of it the rows'
+// take 2.9 us; 700 with 4816 rows and 948 returned pages 9.9 us, most of it the rows'
 // bisections (LDS reads).  Four rows of a thread side by side save 0.8 us of those; eight save 0.2
 // more and cost 0.4 where rows are few.
 __global__ __launch_bounds__(kTablesT) void block_tables_kernel(BlockTablesArgs a)
@@ -243,12 +243,14 @@ __global__ __launch_bounds__(kTablesT) void block_tables_kernel(BlockTablesArgs 
 // four rotation pairs (values d and d + head_dim/2) of a q or k head, or
 // eight values of a v head, with 16-byte loads; heads of quantised caches are
 // left to the block part of the grid.  Rows without a place (slot < 0) are
-// left out whole.  Bound by its bytes: 1717 rows of 8 + 2 * 4 heads of 256 dims (47 MB) take 9.9 us,
-// 4.7 TB/s; few rows by the launch (24 rows 2.5 us).
+// left out whole.  Bound by its bytes: 1717 rows of 8 + 2 * 4 heads of 256 dims (47 MB) take 10.1 us,
+// 4.7 TB/s; few rows by the launch (24 rows 2.6 us).  Without an angle table by the angles (a pow in 64 bits, a
+// sine and a cosine a pair and row: 63 us for 1710 rows).
 //
 // The block part: one wave a pair of 32-value blocks (each half wave one), the
 // value rotated by its own lane, then the reference's block quantisers
-// (kv_append_any_kernel's rule).
+// (kv_append_any_kernel's rule).  Bound by issue: both quantisers for each value and stores of single bytes; 1710 rows
+// into Q8_0 take 27 us, 1.8 TB/s, into Q4_0 26.
 template <int KF, int VF>
 __global__ __launch_bounds__(256) void append_paged_kernel(const float *__restrict__ qkv, float *__restrict__ q_out,
                                                            uint8_t *__restrict__ k_pages, uint8_t *__restrict__ v_pages,
