@@ -1517,15 +1517,16 @@ __device__ __forceinline__ void slow_row(const PagedAttn &a, int row, int r, int
 }
 
 // What a row without any weight gives: 0 if no position that it sees has a place, else 0 / 0, since all its scores
-// were -inf.
+// were -inf.  64 positions a step, since a table that leads nowhere has them all looked at.
 __device__ __forceinline__ float without_weight(const PagedAttn &a, int row, int r)
 {
     const int len = clamp_len(a, a.lens[r]), at = a.prefix_len + len - (a.row_start[r + 1] - row);
 #pragma unroll 1
-    for (int t = a.window ? max(0, at - a.window + 1) : 0; t <= at; ++t)
-        if ((t < a.prefix_len ? place_at(a, a.prefix, t)
-                              : place_at(a, a.table + (size_t)r * a.table_stride, t - a.prefix_len)) >= 0)
-            return NAN;
+    for (int t0 = a.window ? max(0, at - a.window + 1) : 0; t0 <= at; t0 += 64) {
+        const int t = t0 + (threadIdx.x & 63);
+        const int32_t *table = t < a.prefix_len ? a.prefix : a.table + (size_t)r * a.table_stride;
+        if (__any(t <= at && place_at(a, table, t < a.prefix_len ? t : t - a.prefix_len) >= 0)) return NAN;
+    }
     return 0.0f;
 }
 
