@@ -108,8 +108,9 @@ int         mrml_hip_workspace_bytes(mrml_hip_ctx *ctx, size_t *bytes);
  *      stream.  Ops that would grow the workspace fail during capture, so call
  *      mrml_hip_reserve_workspace (or run the ops once) first.  A graph keeps the
  *      workspace it was captured with: while one lives, a workspace that grows
- *      at least doubles, and outgrown ones (together smaller than it) are kept
- *      until it grows after the last graph was destroyed. -------------------- */
+ *      at least doubles (where memory allows), and outgrown ones (together
+ *      smaller than it) are kept until it grows after the last graph was
+ *      destroyed. ------------------------------------------------------------- */
 int mrml_hip_graph_begin(mrml_hip_ctx *ctx);
 int mrml_hip_graph_end(mrml_hip_ctx *ctx, void **graph_exec_out);
 int mrml_hip_graph_launch(mrml_hip_ctx *ctx, void *graph_exec);
@@ -573,10 +574,10 @@ int mrml_hip_block_tables(mrml_hip_ctx *ctx, const int32_t *d_lens, const int32_
  * rotated at position d_pos[i], its q to row i of d_q ([n_rows][n_heads *
  * head_dim]), its k and v to place d_slots[i] of the paged caches in their
  * formats -- each the bits that entry point gives.  Rows with a negative slot
- * are left out, their row of d_q too.  d_q shares no memory with d_qkv.  Angles as there: d_table (nullable) for
- * positions below n_table, else evaluated on the device.  No two rows of a call
- * may have the same slot.  head_dim a multiple of 32 up to 512, groups up to
- * 16. */
+ * are left out, their row of d_q too.  d_q shares no memory with d_qkv.  Angles as
+ * there: d_table (nullable) for positions below n_table, else evaluated on the
+ * device.  No two rows of a call may have the same slot.  head_dim a multiple of
+ * 32 up to 512, groups up to 16. */
 int mrml_hip_rope_kv_append_paged(mrml_hip_ctx *ctx, const float *d_qkv, float *d_q, uint16_t *d_k_pages,
                                   uint16_t *d_v_pages, const int32_t *d_slots, const int32_t *d_pos, int32_t n_rows,
                                   int32_t n_pages, int32_t page_size, int32_t n_heads, int32_t n_kv_heads,
@@ -590,9 +591,9 @@ int mrml_hip_rope_kv_append_paged(mrml_hip_ctx *ctx, const float *d_qkv, float *
  * sliding_window of them -- and gives row i of d_out ([max_rows][n_heads *
  * head_dim]).  The shared prefix is read once for the rows of all requests.  Query
  * rows are q_stride floats apart (a multiple of 4).  d_out may be d_q where
- * q_stride is n_heads * head_dim, and shares no memory with it else.  Rows of no request are left
- * as they are; a row that sees nothing gives zeros, one whose every score is -inf
- * NaN.
+ * q_stride is n_heads * head_dim, and shares no memory with it else.  Rows of no
+ * request are left as they are; a row that sees nothing gives zeros, one whose
+ * every score is -inf NaN.
  *
  * The values are those of mrml_hip_attention_causal over the same rows (K in
  * Q8_0 or Q4_0 multiplied with q as Q8_0 blocks; softmax and sums in f32), added
