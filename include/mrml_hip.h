@@ -84,7 +84,8 @@ const char *mrml_hip_status_string(int status);
  * kernel's bounded wait for other waves of its workgroup gave up since the
  * last sync on the device (its results are then wrong), and with
  * MRML_HIP_E_INVALID when a paged op since the context's last sync met places
- * outside its cache (they are left out). */
+ * outside its cache (they are left out), or an expert op ids, starts and order
+ * that do not agree. */
 int         mrml_hip_sync(mrml_hip_ctx *ctx);
 /* Poll limit of those bounded waits on the context's device (every context
  * on it): polls < 0 restores the default (2^20), 0 makes every wait give up
@@ -610,6 +611,99 @@ int mrml_hip_attention_paged(mrml_hip_ctx *ctx, const float *d_q, int32_t q_stri
                              int32_t table_stride, const int32_t *d_lens, const int32_t *d_row_start, int32_t n_seqs,
                              int32_t max_rows, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, float scale,
                              int32_t sliding_window, int32_t k_format, int32_t v_format);
+
+/* ---- a mixture-of-experts layer for a batch of tokens --------------------------
+ * The reference's own model has one in every layer (cuda_ptx/kernels.rs:887-984
+ * the router, kernels.rs:1563-1821 the experts' products).  A token goes through
+ * k of n_experts experts, each a gated FFN with Q4_0 weights of its own.  A step
+ * of the layer is: the residual's addition and norm; the router's logits; the
+ * route; the experts' gate and up products with the gated activation; their down
+ * product, summed over a token's experts by its weights.
+ *
+ * Assignment t * k + s is slot s of token t.  The weights of all experts are one
+ * backend-layout matrix of n_experts * rows rows (mrml_hip_repack_q4_0 of the
+ * GGUF tensor as it stands: expert e's rows begin at row e * rows).  Nothing goes
+ * through the host, so the calls can be captured and replayed (run them once
+ * before, or reserve the workspace).  Ids, starts and orders are read from device
+ * memory; where they do not agree with each other or lead outside the experts or
+ * the batch, that is left out, and the next mrml_hip_sync fails with
+ * MRML_HIP_E_INVALID.  Limits: at most 512 experts,
+ * 32 experts a token, batch * k at most 2^20, cols a multiple of 32 up to 32768.
+ * Outputs share no memory with other arguments unless it says so. */
+
+/* mrml_hip_residual_rms_norm for `batch` rows of dim values (model.rs:1185-2260):
+ *   h_out = h + t                              (norm_t == 0)
+ *   h_out = h + rms_norm(t, w_post)            (norm_t != 0; w_post nullable: no weight)
+ *   xn    = rms_norm(h_out, w_next)            -> d_xn, d_pack (w_next nullable)
+ * d_xn (f32 rows) and d_pack (the activation pack of batch * dim values, which
+ * mrml_hip_gemm_q4_0_q8 and mrml_hip_moe_gate_up_q4_0_q8 take) are nullable, both
+ * too.  The sums of squares are held in 64 bits and rounded once, so a row's bits
+ * do not depend on the batch; they are within 1e-6 of the sequential f32 sums of
+ * mrml_hip_residual_rms_norm.  Each later step rounds to f32 in the order of the
+ * CPU path.  d_h_out may be d_h, and d_xn may be d_t.  dim as mrml_hip_rms_norm;
+ * batch at most 2^20. */
+int mrml_hip_residual_rms_norm_batch(mrml_hip_ctx *ctx, const float *d_t, const float *d_w_post, const float *d_h,
+                                     float *d_h_out, const float *d_w_next, float *d_xn, void *d_pack, int32_t dim,
+                                     int32_t batch, float eps, int32_t norm_t);
+/* The router's product (kernels.rs:887-926): d_logits[t][e] = sum_c d_x[t][c] *
+ * d_w[e][c], all f32 (GGUF keeps this matrix in f32); within 1e-5 relative to the
+ * largest logit of the sequential sum.  d_x [batch][cols], d_w [n_experts][cols]. */
+int mrml_hip_moe_logits(mrml_hip_ctx *ctx, const float *d_x, const float *d_w, float *d_logits, int32_t n_experts,
+                        int32_t cols, int32_t batch);
+/* The experts of every token (kernels.rs:928-984 has top 8 of a softmax), their
+ * weights, and the assignments sorted by expert.
+ *  - score = softmax of the token's logits, or 1 / (1 + exp(-logit)).  A logit of
+ *    -inf or NaN is an expert that is switched off; logits of +inf share the
+ *    softmax between them.
+ *  - An expert is chosen by its value: its score plus d_bias[e] (nullable; a bias
+ *    that balances the experts' load); without a bias (and with group_best == 1)
+ *    its logit, whose order is the same.  Values are compared in 64 bits; equal
+ *    ones go to the lower id, NaN and -inf are never chosen.
+ *  - With n_groups > 1 the experts are n_groups runs of equal length; only those
+ *    of the top_groups best groups can be chosen, a group's rank being the sum of
+ *    its group_best (1 or 2) best values, equal ranks going to the lower group.
+ *  - d_ids[t][0..k) are the k best, best first; -1 with weight 0 where no expert is
+ *    left.  d_weights[t][s] is the score (without the bias), divided by the sum of
+ *    the token's chosen scores if renormalise != 0 (0 where that is 0), times scale.
+ *  - d_starts (n_experts + 1 entries) and d_order (batch * k), both nullable:
+ *    d_order[d_starts[e] .. d_starts[e+1]) are the assignments of expert e in
+ *    ascending order; entries behind the last are -1. */
+enum { MRML_HIP_MOE_SOFTMAX = 0, MRML_HIP_MOE_SIGMOID = 1 };
+int mrml_hip_moe_route(mrml_hip_ctx *ctx, const float *d_logits, const float *d_bias, int32_t *d_ids, float *d_weights,
+                       int32_t *d_starts, int32_t *d_order, int32_t n_experts, int32_t batch, int32_t k,
+                       int32_t scoring, int32_t n_groups, int32_t top_groups, int32_t group_best, int32_t renormalise,
+                       float scale);
+/* The experts' gate and up products (kernels.rs:1563-1710) and the gated
+ * activation, for every assignment a = t * k + s with expert e = d_ids[t][s]:
+ *   d_act[a][r] = f(sum_c Wg[e][r][c] q[t][c]) * sum_c Wu[e][r][c] q[t][c]
+ * where q is Q8_0(d_x[t]) as in every Q4_0 product here, and f is gelu_tanh
+ * (MRML_HIP_MOE_GEGLU) or silu (MRML_HIP_MOE_SWIGLU).  Each block of 32 is summed
+ * exactly, the blocks' sums in f32 in an order that depends on the batch: within
+ * 1e-5 of mrml_hip_gemm_q4_0 and mrml_hip_geglu relative to the largest output.
+ * d_x [batch][cols], d_act [batch * k][rows].  d_ids, d_starts and d_order as
+ * mrml_hip_moe_route gives them; rows of assignments without an expert are left
+ * as they were.  A row of d_x with a block whose scale passes f16 (magnitudes
+ * above 127 * 65504, infinities) gives values that are not finite. */
+enum { MRML_HIP_MOE_GEGLU = 0, MRML_HIP_MOE_SWIGLU = 1 };
+int mrml_hip_moe_gate_up_q4_0(mrml_hip_ctx *ctx, const void *d_w_gate, const void *d_w_up, const float *d_x,
+                              const int32_t *d_ids, const int32_t *d_starts, const int32_t *d_order, float *d_act,
+                              int32_t n_experts, int32_t rows, int32_t cols, int32_t batch, int32_t k,
+                              int32_t activation);
+/* As mrml_hip_moe_gate_up_q4_0 with the batch already quantised: d_xpack is the
+ * activation pack of batch * cols values. */
+int mrml_hip_moe_gate_up_q4_0_q8(mrml_hip_ctx *ctx, const void *d_w_gate, const void *d_w_up, const void *d_xpack,
+                                 const int32_t *d_ids, const int32_t *d_starts, const int32_t *d_order, float *d_act,
+                                 int32_t n_experts, int32_t rows, int32_t cols, int32_t batch, int32_t k,
+                                 int32_t activation);
+/* The experts' down product (kernels.rs:1711-1821) summed over a token's experts
+ * in the order of its slots:
+ *   d_y[t][r] = sum_s d_weights[t][s] * sum_c Wd[e][r][c] Q8_0(d_act[t * k + s])[c]
+ * with the arithmetic of the products above.  Slots without an expert add
+ * nothing; a token without any gives zeros.  d_act [batch * k][cols], d_y
+ * [batch][rows].  Uses the workspace. */
+int mrml_hip_moe_down_q4_0(mrml_hip_ctx *ctx, const void *d_w_down, const float *d_act, const int32_t *d_ids,
+                           const float *d_weights, const int32_t *d_starts, const int32_t *d_order, float *d_y,
+                           int32_t n_experts, int32_t rows, int32_t cols, int32_t batch, int32_t k);
 
 /* ---- Gemma-2-shape token step (model.rs forward_token, model.rs:1185-2260,
  * and greedy selection, model.rs:2833-2907) ----------------------------------- */

@@ -104,6 +104,9 @@ class Gemma2Layer(ctypes.Structure):
 
 SCORE_CPU, SCORE_DEVICE = 0, 1
 
+MOE_SOFTMAX, MOE_SIGMOID = 0, 1
+MOE_GEGLU, MOE_SWIGLU = 0, 1
+
 
 class Sampler(ctypes.Structure):
     """mrml_hip_sampler: the pick of the token step (model.rs:2842-2907)."""
@@ -193,6 +196,12 @@ _SIGNATURES = {
     "mrml_hip_rope_kv_append_paged": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _F, _I, _I, _P, _I],
     "mrml_hip_attention_paged": [_P, _P, _I, _P, _P, _P, _I, _I, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _F, _I, _I,
                                  _I],
+    "mrml_hip_residual_rms_norm_batch": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _F, _I],
+    "mrml_hip_moe_logits": [_P, _P, _P, _P, _I, _I, _I],
+    "mrml_hip_moe_route": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _F],
+    "mrml_hip_moe_gate_up_q4_0": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I],
+    "mrml_hip_moe_gate_up_q4_0_q8": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I],
+    "mrml_hip_moe_down_q4_0": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I],
     "mrml_hip_gemma2_create": [_P, _P, _P, _P, _P, ctypes.POINTER(_P)],
     "mrml_hip_gemma2_destroy": [_P, _P],
     "mrml_hip_gemma2_step": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _I],
@@ -659,6 +668,48 @@ class HipDevice:
             _ptr(out), n_pages, page_size, _ptr(prefix), prefix_len, _ptr(table), table_stride, _ptr(lens),
             _ptr(row_start), n_seqs, max_rows, n_heads, n_kv_heads, head_dim, scale,
             -1 if sliding_window is None else int(sliding_window), k_format, v_format))
+
+    # ---- a mixture-of-experts layer for a batch of tokens ----------------------------
+    def residual_rms_norm_batch(self, t, w_post, h, h_out, w_next, xn, dim: int, batch: int, eps: float, pack=None,
+                                norm_t: bool = True) -> None:
+        """The residual's addition and the next norm of `batch` rows, in f32 and as Q8_0
+        (mrml_hip_residual_rms_norm_batch)."""
+        self._check(self.lib.mrml_hip_residual_rms_norm_batch(
+            self.ctx, _ptr(t), _ptr(w_post), _ptr(h), _ptr(h_out), _ptr(w_next), _ptr(xn), _ptr(pack), dim, batch, eps,
+            int(norm_t)))
+
+    def moe_logits(self, x, w, logits, n_experts: int, cols: int, batch: int) -> None:
+        """The router's f32 product (mrml_hip_moe_logits)."""
+        self._check(self.lib.mrml_hip_moe_logits(self.ctx, _ptr(x), _ptr(w), _ptr(logits), n_experts, cols, batch))
+
+    def moe_route(self, logits, bias, ids, weights, starts, order, n_experts: int, batch: int, k: int,
+                  scoring: int = 0, n_groups: int = 1, top_groups: int = 1, group_best: int = 1,
+                  renormalise: bool = True, scale: float = 1.0) -> None:
+        """Every token's k experts and weights, and the assignments sorted by expert (mrml_hip_moe_route)."""
+        self._check(self.lib.mrml_hip_moe_route(
+            self.ctx, _ptr(logits), _ptr(bias), _ptr(ids), _ptr(weights), _ptr(starts), _ptr(order), n_experts, batch, k,
+            scoring, n_groups, top_groups, group_best, int(renormalise), scale))
+
+    def moe_gate_up_q4_0(self, w_gate, w_up, x, ids, starts, order, act, n_experts: int, rows: int, cols: int,
+                         batch: int, k: int, activation: int = 0) -> None:
+        """The experts' gate and up products and the gated activation (mrml_hip_moe_gate_up_q4_0)."""
+        self._check(self.lib.mrml_hip_moe_gate_up_q4_0(
+            self.ctx, _ptr(w_gate), _ptr(w_up), _ptr(x), _ptr(ids), _ptr(starts), _ptr(order), _ptr(act), n_experts, rows,
+            cols, batch, k, activation))
+
+    def moe_gate_up_q4_0_q8(self, w_gate, w_up, xpack, ids, starts, order, act, n_experts: int, rows: int, cols: int,
+                            batch: int, k: int, activation: int = 0) -> None:
+        """moe_gate_up_q4_0 over an activation pack of the batch (mrml_hip_moe_gate_up_q4_0_q8)."""
+        self._check(self.lib.mrml_hip_moe_gate_up_q4_0_q8(
+            self.ctx, _ptr(w_gate), _ptr(w_up), _ptr(xpack), _ptr(ids), _ptr(starts), _ptr(order), _ptr(act), n_experts,
+            rows, cols, batch, k, activation))
+
+    def moe_down_q4_0(self, w_down, act, ids, weights, starts, order, y, n_experts: int, rows: int, cols: int,
+                      batch: int, k: int) -> None:
+        """The experts' down product, summed over a token's experts by its weights (mrml_hip_moe_down_q4_0)."""
+        self._check(self.lib.mrml_hip_moe_down_q4_0(
+            self.ctx, _ptr(w_down), _ptr(act), _ptr(ids), _ptr(weights), _ptr(starts), _ptr(order), _ptr(y), n_experts,
+            rows, cols, batch, k))
 
 
 class Gemma2Model:

@@ -24,6 +24,9 @@ struct mrml_hip_ctx {
     // sync looks without a copy (which cost every later sync of the context 11 us on 24).
     volatile uint32_t *page_faults = nullptr;
     uint32_t *d_page_faults = nullptr;  // its device address
+    // The same for an expert op's ids and orders: the word after it.
+    volatile uint32_t *moe_faults = nullptr;
+    uint32_t *d_moe_faults = nullptr;
     std::string err;
 };
 

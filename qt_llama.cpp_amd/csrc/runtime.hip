@@ -195,7 +195,7 @@ int mrml_hip_create(int32_t device, mrml_hip_ctx **out)
         return MRML_HIP_E_HIP;
     }
     void *faults = nullptr, *d_faults = nullptr;
-    if (hipHostMalloc(&faults, sizeof(uint32_t), hipHostMallocMapped | hipHostMallocCoherent) != hipSuccess ||
+    if (hipHostMalloc(&faults, 2 * sizeof(uint32_t), hipHostMallocMapped | hipHostMallocCoherent) != hipSuccess ||
         hipHostGetDevicePointer(&d_faults, faults, 0) != hipSuccess) {
         if (faults) (void)hipHostFree(faults);
         (void)hipStreamDestroy(ctx->stream);
@@ -205,6 +205,9 @@ int mrml_hip_create(int32_t device, mrml_hip_ctx **out)
     ctx->page_faults = (volatile uint32_t *)faults;
     ctx->d_page_faults = (uint32_t *)d_faults;
     *ctx->page_faults = 0;
+    ctx->moe_faults = ctx->page_faults + 1;
+    ctx->d_moe_faults = ctx->d_page_faults + 1;
+    *ctx->moe_faults = 0;
     *out = ctx;
     return MRML_HIP_OK;
 }
@@ -240,9 +243,16 @@ int mrml_hip_sync(mrml_hip_ctx *ctx)
         return fail(ctx, MRML_HIP_E_HIP,
                     "%u bounded LDS-counter waits gave up (%u matvec, %u decode): the results since the last sync "
                     "are wrong", t_gemv + t_decode, t_gemv, t_decode);
-    // Paged ops leave out places that their page tables, lengths or slots put outside the cache.
-    if (!*ctx->page_faults) return MRML_HIP_OK;
+    // Paged ops leave out places that their page tables, lengths or slots put outside the cache, expert ops what
+    // ids, starts and orders that do not agree put outside the experts or the batch.
+    const uint32_t paged = *ctx->page_faults, moe = *ctx->moe_faults;
+    if (!paged && !moe) return MRML_HIP_OK;
     *ctx->page_faults = 0;
+    *ctx->moe_faults = 0;
+    if (moe)
+        return fail(ctx, MRML_HIP_E_INVALID,
+                    "expert ops since the last sync met ids, starts and orders that do not agree or lead outside the "
+                    "batch%s: those were left out", paged ? ", and paged ops places outside the cache" : "");
     return fail(ctx, MRML_HIP_E_INVALID,
                 "paged ops since the last sync met page ids, slots, lengths or counts of pages outside the cache: those "
                 "were left out");

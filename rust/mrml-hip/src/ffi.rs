@@ -208,6 +208,12 @@ api! {
     attention_paged: fn(Ctx, *const f32, i32, *const u16, *const u16, *mut f32, i32, i32, *const i32, i32, *const i32, i32, *const i32, *const i32, i32, i32, i32, i32, i32, f32, i32, i32, i32) -> c_int = "mrml_hip_attention_paged";
     attention_causal: fn(Ctx, *const f32, *const u16, *const u16, *mut f32, i32, i32, i32, i32, f32, i32, i32, i32, i32) -> c_int = "mrml_hip_attention_causal";
     attention_causal_split: fn(Ctx, *const f32, *const u16, *const u16, *mut f32, i32, i32, i32, i32, f32, i32, i32, i32, i32) -> c_int = "mrml_hip_attention_causal_split";
+    residual_rms_norm_batch: fn(Ctx, *const f32, *const f32, *const f32, *mut f32, *const f32, *mut f32, *mut c_void, i32, i32, f32, i32) -> c_int = "mrml_hip_residual_rms_norm_batch";
+    moe_logits: fn(Ctx, *const f32, *const f32, *mut f32, i32, i32, i32) -> c_int = "mrml_hip_moe_logits";
+    moe_route: fn(Ctx, *const f32, *const f32, *mut i32, *mut f32, *mut i32, *mut i32, i32, i32, i32, i32, i32, i32, i32, i32, f32) -> c_int = "mrml_hip_moe_route";
+    moe_gate_up_q4_0: fn(Ctx, *const c_void, *const c_void, *const f32, *const i32, *const i32, *const i32, *mut f32, i32, i32, i32, i32, i32, i32) -> c_int = "mrml_hip_moe_gate_up_q4_0";
+    moe_gate_up_q4_0_q8: fn(Ctx, *const c_void, *const c_void, *const c_void, *const i32, *const i32, *const i32, *mut f32, i32, i32, i32, i32, i32, i32) -> c_int = "mrml_hip_moe_gate_up_q4_0_q8";
+    moe_down_q4_0: fn(Ctx, *const c_void, *const f32, *const i32, *const f32, *const i32, *const i32, *mut f32, i32, i32, i32, i32, i32) -> c_int = "mrml_hip_moe_down_q4_0";
     gemma2_create: fn(Ctx, *const MrmlHipGemma2Config, *const c_void, *const f32, *const MrmlHipGemma2Layer, *mut Model) -> c_int = "mrml_hip_gemma2_create";
     gemma2_destroy: fn(Ctx, Model) -> c_int = "mrml_hip_gemma2_destroy";
     gemma2_step: fn(Ctx, Model, *mut i32, *mut u16, *mut u16, *mut f32, *mut i32, *mut i32, i32, *const i32, i32) -> c_int = "mrml_hip_gemma2_step";
