@@ -1,4 +1,13 @@
 // moe_ffn.hip -- the experts' products of a mixture-of-experts layer.
+//
+// y[row] = sum over blocks b of dw_b * (sum over the block's 32 of (q - 8) * x),
+// with x = da_b * a the Q8_0 values of an activation row.  x has 18 significant
+// bits and is split into two halves, hi + lo, exactly (after a power of two per
+// row that keeps both in range), q - 8 is a half as it stands, so a block's sum is
+// two f16 MFMAs whose f32 result only has to be multiplied by dw and added: one
+// FMA an output and block.  (The int8 product gives a whole number that takes a
+// conversion, two products and an addition: a wave spends 48 cycles of VALU on 16
+// x 16 outputs of a block against 32 of MFMA and 16 of VALU side by side here.)
 
 #include <algorithm>
 
@@ -9,95 +18,421 @@ namespace mrml {
 
 namespace {
 
-// Row `row` of a Q4_0 matrix with `nblk` blocks in all times block-quantised values (blocks b0.. of an activation pack
-// with `total` blocks), over the wave's lanes.
-__device__ __forceinline__ float row_dot(const uint8_t *w, size_t nblk, size_t row, int nb, const uint8_t *pack,
-                                         size_t total, size_t b0, int lane)
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half4v __attribute__((ext_vector_type(4)));
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+
+// ---- activation rows for the MFMA -----------------------------------------------
+
+// A row of nb blocks is nb * 128 bytes: of each block the hi halves (64 bytes), then the lo halves, in the order in
+// which a Q4_0 word's nibbles come apart: group g = 0..3 (16 bytes, one lane's operand) has the values 4g, 4g + 2,
+// 4g + 1, 4g + 3 and the same + 16.
+constexpr int kXBlock = 128;
+
+struct Tile {
+    int expert, first, count, pad;  // places first .. first + count of the order
+};
+
+constexpr int kTileRows = 16;
+
+// Tiles of at most NT groups of 16 that a call can have.
+int max_tiles(const ExpertArgs &a, int nt)
 {
-    float s = 0.0f;
-    for (int b = lane; b < nb; b += 64) {
-        const uint4 q = reinterpret_cast<const uint4 *>(w)[row * nb + b];
-        const float dw = f16_bits_to_f32(reinterpret_cast<const uint16_t *>(w + nblk * 16)[row * nb + b]);
-        const uint4 lo = reinterpret_cast<const uint4 *>(pack)[2 * (b0 + b)];
-        const uint4 hi = reinterpret_cast<const uint4 *>(pack)[2 * (b0 + b) + 1];
-        const float da = reinterpret_cast<const float *>(pack + total * 32)[b0 + b];
-        int n = -8 * reinterpret_cast<const int32_t *>(pack + total * 36)[b0 + b];
-        n = sdot4(q.x & kLoNib, lo.x, n);
-        n = sdot4(q.y & kLoNib, lo.y, n);
-        n = sdot4(q.z & kLoNib, lo.z, n);
-        n = sdot4(q.w & kLoNib, lo.w, n);
-        n = sdot4((q.x >> 4) & kLoNib, hi.x, n);
-        n = sdot4((q.y >> 4) & kLoNib, hi.y, n);
-        n = sdot4((q.z >> 4) & kLoNib, hi.z, n);
-        n = sdot4((q.w >> 4) & kLoNib, hi.w, n);
-        s += (float)n * (dw * da);
+    const int n = a.batch * a.k;
+    return std::min(n, n / (kTileRows * nt) + std::min(a.n_experts, n));
+}
+
+// One wave a row (rows_wgs workgroups of four), then one thread an assignment that checks the plan, then one workgroup
+// that lists the tiles: tiles[0].expert of them behind tiles[0].
+template <bool PACKED>
+__global__ __launch_bounds__(256) void moe_pack_kernel(ExpertArgs a, int rows, int rows_wgs, uint8_t *__restrict__ xp,
+                                                       float *__restrict__ xscale, Tile *__restrict__ tiles, int nt,
+                                                       int most)
+{
+    const int lane = threadIdx.x & 63, nb = a.cols / 32, n = a.batch * a.k;
+    if ((int)blockIdx.x == (int)gridDim.x - 1) {
+        __shared__ int ends[kMaxExperts];
+        const int tid = threadIdx.x;
+        int groups[2], mine[2], first[2], count[2];
+        for (int v = 0; v < 2; ++v) {
+            const int e = tid * 2 + v;
+            int s0 = 0, s1 = 0;
+            if (e < a.n_experts) {
+                s0 = min(max(a.starts[e], 0), n);
+                s1 = min(max(a.starts[e + 1], s0), n);
+            }
+            first[v] = s0;
+            count[v] = s1 - s0;
+            groups[v] = (count[v] + kTileRows - 1) / kTileRows;
+            mine[v] = (groups[v] + nt - 1) / nt;
+        }
+        ends[tid] = mine[0] + mine[1];
+        __syncthreads();
+        for (int d = 1; d < 256; d *= 2) {
+            const int before = tid >= d ? ends[tid - d] : 0;
+            __syncthreads();
+            ends[tid] += before;
+            __syncthreads();
+        }
+        int at = ends[tid] - mine[0] - mine[1];
+        for (int v = 0; v < 2; ++v) {
+            int from = first[v], left = count[v];
+            for (int i = 0; i < mine[v]; ++i, ++at) {
+                const int c = min(left, kTileRows * (groups[v] / mine[v] + (i < groups[v] % mine[v])));
+                if (at < most) tiles[1 + at] = {tid * 2 + v, from, c, 0};  // runs that overlap could ask for more
+                from += c;
+                left -= c;
+            }
+        }
+        if (tid == 255) tiles[0] = {min(ends[255], most), 0, 0, 0};
+        return;
     }
-    return mrml_xsum::wave_sum_f32(s);
-}
-
-__device__ __forceinline__ float silu(float x) { return x / (1.0f + expf(-x)); }
-
-// One wave an assignment and row.
-__global__ __launch_bounds__(256) void moe_gate_up_kernel(ExpertArgs a, const uint8_t *pack)
-{
-    const int as = blockIdx.x, row = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, nb = a.cols / 32;
-    if (row >= a.rows) return;
-    if (row == 0 && !plan_ok(a, as)) moe_fault(a.faults);
-    const int e = a.ids[as];
-    if (e < 0 || e >= a.n_experts) return;
-    const size_t nblk = (size_t)a.n_experts * a.rows * nb, r = (size_t)e * a.rows + row, total = (size_t)a.batch * nb;
-    const size_t b0 = (size_t)(as / a.k) * nb;
-    const float g = row_dot(a.w[0], nblk, r, nb, pack, total, b0, lane);
-    const float u = row_dot(a.w[1], nblk, r, nb, pack, total, b0, lane);
-    if (lane == 0) a.out[(size_t)as * a.rows + row] = (a.activation == MRML_HIP_MOE_GEGLU ? gelu_tanh(g) : silu(g)) * u;
-}
-
-// One wave a token and row.
-__global__ __launch_bounds__(256) void moe_down_kernel(ExpertArgs a, const uint8_t *pack)
-{
-    const int t = blockIdx.x, row = blockIdx.y * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, nb = a.cols / 32;
-    if (row >= a.rows) return;
-    const size_t nblk = (size_t)a.n_experts * a.rows * nb, total = (size_t)a.batch * a.k * nb;
-    float y = 0.0f;
-    for (int s = 0; s < a.k; ++s) {
-        const int as = t * a.k + s, e = a.ids[as];
-        if (row == 0 && !plan_ok(a, as)) moe_fault(a.faults);
-        if (e < 0 || e >= a.n_experts) continue;
-        y += a.weights[as] * row_dot(a.w[0], nblk, (size_t)e * a.rows + row, nb, pack, total, (size_t)as * nb, lane);
+    if ((int)blockIdx.x >= rows_wgs) {
+        const int j = (blockIdx.x - rows_wgs) * 256 + threadIdx.x;
+        if (j < n && !plan_ok(a, j)) moe_fault(a.faults);
+        return;
     }
-    if (lane == 0) a.out[(size_t)t * a.rows + row] = y;
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const int n4 = a.cols / 4;
+    const float4 *x = reinterpret_cast<const float4 *>(a.x + (size_t)row * a.cols);
+    const size_t total = (size_t)rows * nb, b0 = (size_t)row * nb;
+    const uint32_t *pq = reinterpret_cast<const uint32_t *>(a.xpack);
+    const float *pd = reinterpret_cast<const float *>(a.xpack + total * 32);
+    float top = 0.0f;
+    if (PACKED) {
+        for (int b = lane; b < nb; b += 64) top = fmaxf(top, pd[b0 + b]);
+    } else {
+        for (int c = lane; c < n4; c += 64) {
+            const float4 v = x[c];
+            top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+        }
+    }
+    for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+    if (!PACKED) top = f16_bits_to_f32(f32_to_f16_trunc(top / 127.0f));
+    // the largest scale becomes 2^7 .. 2^8, so that values stay below 2^15; infinity counts as the largest half
+    const int exp = top > 0.0f ? (int)(__builtin_bit_cast(uint32_t, fminf(top, 65504.0f)) >> 23) - 127 - 7 : 0;
+    const float down = __builtin_bit_cast(float, (uint32_t)(127 - exp) << 23);
+    if (lane == 0) xscale[row] = __builtin_bit_cast(float, (uint32_t)(127 + exp) << 23);
+    uint8_t *dst = xp + b0 * kXBlock;
+    for (int c0 = 0; c0 < n4; c0 += 64) {
+        const int c = c0 + lane, cc = c < n4 ? c : 0, l = c & 7;
+        uint32_t q;
+        float d;
+        if (PACKED) {
+            q = pq[b0 * 8 + cc];
+            d = pd[b0 + (cc >> 3)];
+        } else {
+            uint32_t dbits;
+            int sum;
+            q = q8_0_block8x4(x[cc], dbits, sum);
+            d = f16_bits_to_f32(dbits);
+        }
+        if (c >= n4) continue;
+        d *= down;
+        const float v0 = d * (float)(int8_t)q, v1 = d * (float)(int8_t)(q >> 16), v2 = d * (float)(int8_t)(q >> 8),
+                    v3 = d * (float)(int8_t)(q >> 24);
+        const half4v hi = {(_Float16)v0, (_Float16)v1, (_Float16)v2, (_Float16)v3};
+        const half4v lo = {(_Float16)(v0 - (float)hi.x), (_Float16)(v1 - (float)hi.y), (_Float16)(v2 - (float)hi.z),
+                           (_Float16)(v3 - (float)hi.w)};
+        uint8_t *p = dst + (size_t)(c >> 3) * kXBlock + (l & 3) * 16 + (l >> 2) * 8;
+        *reinterpret_cast<half4v *>(p) = hi;
+        *reinterpret_cast<half4v *>(p + 64) = lo;
+    }
 }
 
-// The activation pack of n values in the workspace.
-int pack_rows(mrml_hip_ctx *ctx, const ExpertArgs &a, size_t n, const uint8_t **pack)
+// ---- the products -----------------------------------------------------------------
+
+// The eight halves q - 8 of a Q4_0 word, in the order of an activation group.  A nibble put under the exponent of 1024
+// is 1024 + q (the high one 1024 + 16 q).
+__device__ __forceinline__ half8v nibbles(uint32_t w)
 {
-    *pack = a.xpack;
-    if (a.xpack) return MRML_HIP_OK;
-    REQUIRE(ctx, n <= INT32_MAX, "moe: too many activations for one call");
-    uint8_t *ws = (uint8_t *)workspace(ctx, act_pack_bytes(n / 32));
+    constexpr uint32_t k1024 = 0x64006400u;
+    const half2v low = {(_Float16)1032.0f, (_Float16)1032.0f}, by = {(_Float16)0.0625f, (_Float16)0.0625f},
+                 high = {(_Float16)-72.0f, (_Float16)-72.0f};
+    auto as_half = [](uint32_t x) { return __builtin_bit_cast(half2v, x); };
+    const uint32_t v = w >> 8;
+    const half2v a = as_half((w & 0x000F000Fu) | k1024) - low, b = as_half((v & 0x000F000Fu) | k1024) - low;
+    const half2v c = __builtin_elementwise_fma(as_half((w & 0x00F000F0u) | k1024), by, high);
+    const half2v d = __builtin_elementwise_fma(as_half((v & 0x00F000F0u) | k1024), by, high);
+    return {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// Words w[i] of lane row g (16 lanes) become words w[g] of lane row i: every lane gets its own part of one block after
+// the other where it had loaded one block whole.
+__device__ __forceinline__ void turn(uint32_t &w0, uint32_t &w1, uint32_t &w2, uint32_t &w3)
+{
+    auto swap32 = [](uint32_t &a, uint32_t &b) {
+        const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+        a = r[0];
+        b = r[1];
+    };
+    auto swap16 = [](uint32_t &a, uint32_t &b) {
+        const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+        a = r[0];
+        b = r[1];
+    };
+    swap32(w0, w2);
+    swap32(w1, w3);
+    swap16(w0, w1);
+    swap16(w2, w3);
+}
+
+// The value of every lane row, in all rows.
+__device__ __forceinline__ void spread(uint32_t v, uint32_t (&out)[4])
+{
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    const auto even = __builtin_amdgcn_permlane32_swap(r[0], r[0], false, false);
+    const auto odd = __builtin_amdgcn_permlane32_swap(r[1], r[1], false, false);
+    out[0] = even[0];
+    out[1] = odd[0];
+    out[2] = even[1];
+    out[3] = odd[1];
+}
+
+// z / (1 + e^-s(z)) with the hardware's exponential and reciprocal (one step each); gelu_tanh is z * sigmoid(2 u).
+__device__ __forceinline__ float gated(float g, float u, int activation)
+{
+    const float s = activation == MRML_HIP_MOE_GEGLU ? 1.5957691216f * __builtin_fmaf(0.044715f * g * g, g, g) : g;
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950409f * s)) * u;
+}
+
+constexpr int kWaves = 4;
+constexpr int kGroups = 4;  // weight groups of 16 rows a wave
+constexpr int kChunk = 4;   // blocks staged at once
+
+// Weight rows of a wave: two groups of gate and the same of up, or four.
+template <bool DOWN>
+constexpr int wave_rows()
+{
+    return DOWN ? 64 : 32;
+}
+
+// 16 NT tokens of one expert times the rows of a workgroup.  Lane (g, i): row i of each weight group, and of the
+// activations row i of each token group.
+template <bool DOWN, int NT, int NTM>
+__device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &tile, int chunk_rows, const uint8_t *xp,
+                                             uint4 *lds, const int *s_as, const float *s_scale)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15, nb = a.cols / 32;
+    const int r0 = chunk_rows + wave * wave_rows<DOWN>();
+    const size_t all = (size_t)a.n_experts * a.rows * nb * 16, base = (size_t)tile.expert * a.rows;
+    const uint8_t *wq[kGroups], *ws[kGroups];
+#pragma unroll
+    for (int q = 0; q < kGroups; ++q) {
+        const int r = min(r0 + (DOWN ? q : q & 1) * 16 + i, a.rows - 1);
+        const uint8_t *w = a.w[DOWN ? 0 : q >> 1];
+        wq[q] = w + (base + r) * nb * 16;
+        ws[q] = w + all + (base + r) * nb * 2;
+    }
+    const uint8_t *xrow[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int as = max(s_as[t * 16 + i], 0);
+        xrow[t] = xp + (size_t)(DOWN ? as : as / a.k) * nb * kXBlock + g * 16;
+    }
+    const int chunks = (nb + kChunk - 1) / kChunk;
+    auto load_x = [&](int c, int buf) {
+        const int b = min(c * kChunk + wave, nb - 1);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                __builtin_amdgcn_global_load_lds(
+                    (const __attribute__((address_space(1))) void *)(xrow[t] + (size_t)b * kXBlock + h * 64),
+                    (__attribute__((address_space(3))) void *)(lds + (((buf * kChunk + wave) * NTM + t) * 2 + h) * 64), 16, 0, 0);
+    };
+    uint4 wv[kGroups];
+    uint32_t sv[kGroups];
+    auto load_w = [&](int c) {
+        const int b = min(c * kChunk + g, nb - 1);
+#pragma unroll
+        for (int q = 0; q < kGroups; ++q) {
+            wv[q] = *reinterpret_cast<const uint4 *>(wq[q] + (size_t)b * 16);
+            sv[q] = *reinterpret_cast<const uint16_t *>(ws[q] + (size_t)b * 2);
+        }
+    };
+    float4v acc[kGroups][NT];
+#pragma unroll
+    for (int q = 0; q < kGroups; ++q)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[q][t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+    load_x(0, 0);
+    load_w(0);
+    for (int c = 0; c < chunks; ++c) {
+        uint32_t w[kGroups][4], s[kGroups][4];
+#pragma unroll
+        for (int q = 0; q < kGroups; ++q) {
+            w[q][0] = wv[q].x;
+            w[q][1] = wv[q].y;
+            w[q][2] = wv[q].z;
+            w[q][3] = wv[q].w;
+            turn(w[q][0], w[q][1], w[q][2], w[q][3]);
+            spread(sv[q], s[q]);
+        }
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): what went to LDS past the registers
+        __syncthreads();  // chunk c is whole, and everyone is through with chunk c - 1
+        if (c + 1 < chunks) {
+            load_x(c + 1, (c + 1) & 1);
+            load_w(c + 1);
+        }
+        const uint4 *x = lds + (size_t)(c & 1) * kChunk * NTM * 2 * 64 + lane;
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+            if (c * kChunk + j >= nb) break;
+            half8v wh[kGroups];
+            float d[kGroups];
+#pragma unroll
+            for (int q = 0; q < kGroups; ++q) {
+                wh[q] = nibbles(w[q][j]);
+                d[q] = f16_bits_to_f32(s[q][j]);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const half8v hi = __builtin_bit_cast(half8v, x[((j * NTM + t) * 2) * 64]);
+                const half8v lo = __builtin_bit_cast(half8v, x[((j * NTM + t) * 2 + 1) * 64]);
+                float4v p[kGroups];
+#pragma unroll
+                for (int q = 0; q < kGroups; ++q)
+                    p[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wh[q], float4v{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+                for (int q = 0; q < kGroups; ++q) p[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wh[q], p[q], 0, 0, 0);
+#pragma unroll
+                for (int q = 0; q < kGroups; ++q)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) acc[q][t][v] = __builtin_fmaf(p[q][v], d[q], acc[q][t][v]);
+            }
+        }
+    }
+    // outputs: token row 4g + v of each group, weight row i
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const int as = s_as[t * 16 + 4 * g + v];
+            if (as < 0) continue;
+            const float scale = s_scale[t * 16 + 4 * g + v];
+            float *out = a.out + (size_t)as * a.rows;
+            if (DOWN) {
+#pragma unroll
+                for (int q = 0; q < kGroups; ++q)
+                    if (r0 + q * 16 + i < a.rows) out[r0 + q * 16 + i] = acc[q][t][v] * scale;
+            } else {
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    if (r0 + q * 16 + i < a.rows)
+                        out[r0 + q * 16 + i] = gated(acc[q][t][v] * scale, acc[q + 2][t][v] * scale, a.activation);
+            }
+        }
+}
+
+template <bool DOWN, int NTM>
+__global__ __launch_bounds__(64 * kWaves, 2) void moe_tile_kernel(ExpertArgs a, const Tile *__restrict__ tiles,
+                                                                  const uint8_t *__restrict__ xp,
+                                                                  const float *__restrict__ xscale, int row_wgs)
+{
+    __shared__ __align__(16) uint4 lds[2 * kChunk * NTM * 2 * 64];
+    __shared__ int s_as[NTM * 16];
+    __shared__ float s_scale[NTM * 16];
+    // workgroups go to the eight XCDs in turn; each XCD gets a run of the list, so that an expert's weights and a tile's
+    // activations meet in one L2
+    const int total = tiles[0].expert * row_wgs, per = (total + 7) / 8;
+    const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
+    const int at = id / row_wgs;
+    const Tile tile = tiles[1 + at];
+    const int n = a.batch * a.k;
+    if (threadIdx.x < NTM * 16) {
+        const int j = tile.first + (int)threadIdx.x;
+        const int o = (int)threadIdx.x < tile.count ? a.order[j] : -1;
+        const bool ok = o >= 0 && o < n;
+        s_as[threadIdx.x] = ok ? o : -1;
+        s_scale[threadIdx.x] = ok ? xscale[DOWN ? o : o / a.k] * (DOWN ? a.weights[o] : 1.0f) : 0.0f;
+    }
+    __syncthreads();
+    const int groups = (tile.count + 15) / 16, chunk_rows = (id - at * row_wgs) * kWaves * wave_rows<DOWN>();
+    if (NTM >= 4 && groups == 4) tile_product<DOWN, NTM >= 4 ? 4 : 1, NTM>(a, tile, chunk_rows, xp, lds, s_as, s_scale);
+    else if (NTM >= 4 && groups == 3) tile_product<DOWN, NTM >= 4 ? 3 : 1, NTM>(a, tile, chunk_rows, xp, lds, s_as, s_scale);
+    else if (NTM >= 2 && groups == 2) tile_product<DOWN, NTM >= 2 ? 2 : 1, NTM>(a, tile, chunk_rows, xp, lds, s_as, s_scale);
+    else tile_product<DOWN, 1, NTM>(a, tile, chunk_rows, xp, lds, s_as, s_scale);
+}
+
+// y = the sum of a token's weighted products in the order of its slots; VEC values a thread.
+template <int VEC>
+__global__ __launch_bounds__(256) void moe_combine_kernel(ExpertArgs a, const float *__restrict__ part, float *__restrict__ y)
+{
+    const int t = blockIdx.x, r = (blockIdx.y * 256 + threadIdx.x) * VEC;
+    if (r >= a.rows) return;
+    typedef float vec __attribute__((ext_vector_type(VEC)));
+    vec s = 0.0f;
+    for (int i = 0; i < a.k; ++i) {
+        const int as = t * a.k + i, e = a.ids[as];
+        if (e >= 0 && e < a.n_experts) s += *reinterpret_cast<const vec *>(part + (size_t)as * a.rows + r);
+    }
+    *reinterpret_cast<vec *>(y + (size_t)t * a.rows + r) = s;
+}
+
+template <bool DOWN>
+int launch_tiles(mrml_hip_ctx *ctx, const ExpertArgs &a, int nt, const Tile *tiles, const uint8_t *xp, const float *xscale)
+{
+    const int row_wgs = (a.rows + kWaves * wave_rows<DOWN>() - 1) / (kWaves * wave_rows<DOWN>());
+    const int64_t grid = ((int64_t)max_tiles(a, nt) * row_wgs + 7) / 8 * 8;
+    REQUIRE(ctx, grid <= INT32_MAX, "moe: batch * k = %d assignments of %d rows are too many for one call", a.batch * a.k,
+            a.rows);
+#define MOE_TILES(NTM)                                                                                              \
+    hipLaunchKernelGGL((moe_tile_kernel<DOWN, NTM>), dim3((uint32_t)grid), dim3(64 * kWaves), 0, ctx->stream, a, tiles, \
+                       xp, xscale, row_wgs)
+    if (nt == 1) MOE_TILES(1);
+    else if (nt == 2) MOE_TILES(2);
+    else MOE_TILES(4);
+#undef MOE_TILES
+    return check_launch(ctx, "moe_tile_kernel");
+}
+
+// Token groups of 16 a tile at most, by the tokens that an expert has on average.
+int tile_groups(const ExpertArgs &a)
+{
+    const int mean = a.batch * a.k / a.n_experts;
+    return mean <= 12 ? 1 : mean <= 24 ? 2 : 4;
+}
+
+// The product itself: activations in MFMA order and the list of tiles in the workspace, then the tiles.
+template <bool DOWN>
+int launch_product(mrml_hip_ctx *ctx, const ExpertArgs &a)
+{
+    const int nt = tile_groups(a), most = max_tiles(a, nt), nb = a.cols / 32, n = a.batch * a.k, rows = DOWN ? n : a.batch;
+    const size_t list = align_up((size_t)(1 + most) * sizeof(Tile), 256), scales = align_up((size_t)rows * 4, 256);
+    const size_t packed = (size_t)rows * nb * kXBlock, part = DOWN ? (size_t)n * a.rows * 4 : 0;
+    uint8_t *ws = (uint8_t *)workspace(ctx, list + scales + packed + part);
     if (!ws) return MRML_HIP_E_ALLOC;
-    *pack = ws;
-    return launch_quantize_q8_0(ctx, a.x, nullptr, ws, (int32_t)n);
+    Tile *tiles = (Tile *)ws;
+    float *xscale = (float *)(ws + list);
+    uint8_t *xp = ws + list + scales;
+    const int rows_wgs = (rows + 3) / 4, grid = rows_wgs + (n + 255) / 256 + 1;
+    if (a.xpack)
+        hipLaunchKernelGGL(moe_pack_kernel<true>, dim3(grid), dim3(256), 0, ctx->stream, a, rows, rows_wgs, xp, xscale,
+                           tiles, nt, most);
+    else
+        hipLaunchKernelGGL(moe_pack_kernel<false>, dim3(grid), dim3(256), 0, ctx->stream, a, rows, rows_wgs, xp, xscale,
+                           tiles, nt, most);
+    if (int rc = check_launch(ctx, "moe_pack_kernel")) return rc;
+    ExpertArgs p = a;
+    if (DOWN) p.out = (float *)(xp + packed);
+    if (int rc = launch_tiles<DOWN>(ctx, p, nt, tiles, xp, xscale)) return rc;
+    if (!DOWN) return MRML_HIP_OK;
+    if (a.rows % 4 == 0)
+        hipLaunchKernelGGL(moe_combine_kernel<4>, dim3(a.batch, (a.rows / 4 + 255) / 256), dim3(256), 0, ctx->stream, a,
+                           p.out, a.out);
+    else
+        hipLaunchKernelGGL(moe_combine_kernel<1>, dim3(a.batch, (a.rows + 255) / 256), dim3(256), 0, ctx->stream, a, p.out,
+                           a.out);
+    return check_launch(ctx, "moe_combine_kernel");
 }
 
 }  // namespace
 
-int launch_moe_gate_up(mrml_hip_ctx *ctx, const ExpertArgs &a)
-{
-    const uint8_t *pack;
-    if (int rc = pack_rows(ctx, a, (size_t)a.batch * a.cols, &pack)) return rc;
-    REQUIRE(ctx, a.rows <= 65535 * 4, "moe: rows=%d", a.rows);
-    hipLaunchKernelGGL(moe_gate_up_kernel, dim3(a.batch * a.k, (a.rows + 3) / 4), dim3(256), 0, ctx->stream, a, pack);
-    return check_launch(ctx, "moe_gate_up_kernel");
-}
-
-int launch_moe_down(mrml_hip_ctx *ctx, const ExpertArgs &a)
-{
-    const uint8_t *pack;
-    if (int rc = pack_rows(ctx, a, (size_t)a.batch * a.k * a.cols, &pack)) return rc;
-    REQUIRE(ctx, a.rows <= 65535 * 4, "moe: rows=%d", a.rows);
-    hipLaunchKernelGGL(moe_down_kernel, dim3(a.batch, (a.rows + 3) / 4), dim3(256), 0, ctx->stream, a, pack);
-    return check_launch(ctx, "moe_down_kernel");
-}
+int launch_moe_gate_up(mrml_hip_ctx *ctx, const ExpertArgs &a) { return launch_product<false>(ctx, a); }
+int launch_moe_down(mrml_hip_ctx *ctx, const ExpertArgs &a) { return launch_product<true>(ctx, a); }
 
 }  // namespace mrml
