@@ -628,7 +628,8 @@ int mrml_hip_attention_paged(mrml_hip_ctx *ctx, const float *d_q, int32_t q_stri
  * memory; where they do not agree with each other or lead outside the experts or
  * the batch, that is left out, and the next mrml_hip_sync fails with
  * MRML_HIP_E_INVALID.  Limits: at most 512 experts,
- * 32 experts a token, batch * k at most 2^20, cols a multiple of 32 up to 32768.
+ * 32 experts a token, batch * k at most 2^20, cols a multiple of 32 up to 32768,
+ * an expert's matrix below 4 GiB of quants.
  * Outputs share no memory with other arguments unless it says so. */
 
 /* mrml_hip_residual_rms_norm for `batch` rows of dim values (model.rs:1185-2260):

@@ -354,6 +354,8 @@ int product_ok(mrml_hip_ctx *ctx, const char *name, const ExpertArgs &a, bool do
             name, a.cols, kMaxExpertCols);
     REQUIRE(ctx, a.rows >= 1 && a.rows <= (1 << 20) && (int64_t)a.rows * a.n_experts <= INT32_MAX,
             "%s: rows=%d of %d experts (at least one, at most 2^20, below 2^31 in all)", name, a.rows, a.n_experts);
+    REQUIRE(ctx, (int64_t)a.rows * (a.cols / 32) < (1 << 28), "%s: a matrix of %d x %d values has 2^28 blocks or more", name,
+            a.rows, a.cols);
     const uintptr_t bits = (uintptr_t)a.w[0] | (uintptr_t)a.w[1] | (uintptr_t)x | (uintptr_t)a.xpack | (uintptr_t)a.out;
     REQUIRE(ctx, aligned(bits, 16), "%s: pointers must be 16-byte aligned", name);
     REQUIRE(ctx, aligned((uintptr_t)a.ids | (uintptr_t)a.starts | (uintptr_t)a.order | (uintptr_t)a.weights, 4),

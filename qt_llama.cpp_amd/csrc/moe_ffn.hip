@@ -358,6 +358,271 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_tile_kernel(ExpertArgs a, 
     else tile_product<DOWN, 1, NTM>(a, tile, chunk_rows, xp, lds, s_as, s_scale);
 }
 
+// ---- few tokens an expert -------------------------------------------------------------
+
+// Bound by the stream of weights: one launch, one workgroup for a run of rows and up to 16 tokens of one expert.  The
+// activations are quantised into LDS by every workgroup; a wave has kUnits runs of 16 rows one after the other, whose
+// weights go from memory to registers kAhead steps ahead and without a barrier, 128 bytes of a row at once (a stream of 64
+// bytes a row reaches 4.9 TB/s here, of 128 bytes 6.1), and through 2 KB of LDS of the wave's own to the lanes that need
+// them.  The block sums are int8 MFMA: 16 (q - 8) is a byte after one xor, a shift and two ands, half of what a half of it
+// takes, and an int8 activation is a quarter of hi and lo.  Token t is row 4 (t & 3) + t / 4 of the MFMA, so that a lane's
+// V results are its tokens' and up to 4 V tokens fold V values a lane and not four.
+constexpr int kStreamBlocks = 128;  // of a row at most: they are all in LDS
+constexpr int kStreamTokens = 16;   // a workgroup at most
+constexpr int kStep = 8;            // blocks of a row at once
+constexpr int kAhead = 4;           // steps; their scales are read kAhead steps at once
+constexpr int kStageAhead = 4;      // loads of activations a thread has under way
+
+// Runs of 16 rows of a wave: gate and up of the same rows, or four of down.
+template <bool DOWN>
+constexpr int stream_units()
+{
+    return DOWN ? 4 : 2;
+}
+
+// Bytes of a block of 4 V tokens in LDS: [group of 8 values][token][8], then 16 to spread the banks.  Scales follow all
+// blocks: [run of 4 blocks][token / 4][token & 3][block of the run].  Before them the waves' own parts.
+constexpr int stream_block(int v) { return 4 * v * 32 + 16; }
+__host__ __device__ constexpr int stream_blocks(int nb) { return (nb + kStep - 1) / kStep * kStep; }
+constexpr int kBounce = 16 * kStep * 16;
+size_t stream_lds(int nb, int tokens)
+{
+    return kWaves * kBounce + (size_t)stream_blocks(nb) * (stream_block(tokens / 4) + tokens * 4);
+}
+
+// `count` rows into LDS as Q8_0; scales of 0 behind the last block, up to a whole step.  loaded() is called once the
+// first loads are under way.
+template <bool PACKED, int V, class F>
+__device__ __forceinline__ void stream_stage(const ExpertArgs &a, const int *s_row, int count, int in_rows, uint8_t *lds,
+                                             float *scales, F loaded)
+{
+    const int nb = a.cols / 32, n4 = nb * 8, all = count * n4;
+    auto scale_at = [&](int t, int b) -> float & {
+        return scales[(((b / kChunk) * V + (t >> 2)) * 4 + (t & 3)) * kChunk + b % kChunk];
+    };
+    int t = 0, c = (int)threadIdx.x;
+    for (int k0 = 0; k0 < all; k0 += 64 * kWaves * kStageAhead) {
+        float4 x[kStageAhead];
+        uint32_t q[kStageAhead];
+        float d[kStageAhead];
+        int tt[kStageAhead], cc[kStageAhead];
+#pragma unroll
+        for (int k = 0; k < kStageAhead; ++k) {
+            for (; c >= n4 && t < count; ++t) c -= n4;
+            tt[k] = t;
+            cc[k] = t < count ? c : 0;
+            const size_t at = (size_t)s_row[t < count ? t : 0] * n4 + cc[k];
+            if (PACKED) {
+                q[k] = reinterpret_cast<const uint32_t *>(a.xpack)[at];
+                d[k] = reinterpret_cast<const float *>(a.xpack + (size_t)in_rows * nb * 32)[at >> 3];
+            } else {
+                x[k] = reinterpret_cast<const float4 *>(a.x)[at];
+            }
+            c += 64 * kWaves;
+        }
+        if (k0 == 0) loaded();
+#pragma unroll
+        for (int k = 0; k < kStageAhead; ++k) {
+            if (!PACKED) {
+                uint32_t dbits;
+                int sum;
+                q[k] = q8_0_block8x4(x[k], dbits, sum);
+                d[k] = f16_bits_to_f32(dbits);
+            }
+            const int l = cc[k] & 7, b = cc[k] >> 3;
+            if (tt[k] >= count) continue;
+            *reinterpret_cast<uint32_t *>(lds + b * stream_block(V) + ((l & 3) * 4 * V + tt[k]) * 8 + (l >> 2) * 4) = q[k];
+            if (l == 0) scale_at(tt[k], b) = d[k] * 0.0625f;  // the weights' factor of 16
+        }
+    }
+    if ((int)threadIdx.x < 4 * V)
+        for (int b = nb; b % kStep; ++b) scale_at(threadIdx.x, b) = 0.0f;
+}
+
+typedef int int4v __attribute__((ext_vector_type(4)));
+
+// Eight scales of a row from block b on, read eight, four, two or one at a time as the blocks in a row align them; behind
+// the row's last block any.
+template <int AT_ONCE>
+__device__ __forceinline__ uint4 load_scales(const uint8_t *ws, uint32_t row_at, int b, int nb)
+{
+    auto at = [&](int i) { return ws + (row_at + min(i, nb - AT_ONCE)) * 2ull; };
+    auto one = [&](int i) { return *reinterpret_cast<const uint32_t *>(at(i)); };
+    auto two = [&](int i) { return *reinterpret_cast<const uint2 *>(at(i)); };
+    auto half = [&](int i) {
+        return (uint32_t)*reinterpret_cast<const uint16_t *>(at(i)) | (uint32_t)*reinterpret_cast<const uint16_t *>(at(i + 1)) << 16;
+    };
+    if (AT_ONCE == 8) return *reinterpret_cast<const uint4 *>(at(b));
+    if (AT_ONCE == 4) return make_uint4(two(b).x, two(b).y, two(b + 4).x, two(b + 4).y);
+    if (AT_ONCE == 2) return make_uint4(one(b), one(b + 2), one(b + 4), one(b + 6));
+    return make_uint4(half(b), half(b + 2), half(b + 4), half(b + 6));
+}
+
+// Up to 4 V tokens of one expert.
+template <bool DOWN, bool PACKED, int AT_ONCE, int V>
+__device__ __forceinline__ void stream_pass(const ExpertArgs &a, int expert, int count, uint8_t *lds, const int *s_as,
+                                            const int *s_row, const float *s_weight)
+{
+    constexpr int kUnits = stream_units<DOWN>(), kRows = DOWN ? 16 * kUnits : 16;  // rows of a wave
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
+    const int nb = a.cols / 32, steps = (nb + kStep - 1) / kStep;
+    const int r0 = (blockIdx.x * kWaves + wave) * kRows;
+    const int units = r0 >= a.rows ? 0 : DOWN ? min(kUnits, (a.rows - r0 + 15) / 16) : kUnits;
+    // the expert's matrices, 32-bit offsets within one
+    const size_t first_block = (size_t)expert * a.rows * nb, blocks = (size_t)a.n_experts * a.rows * nb;
+    uint8_t *bounce = lds + wave * kBounce;
+    lds += kWaves * kBounce;
+    float *scales = reinterpret_cast<float *>(lds + stream_blocks(nb) * stream_block(V));
+    // row i of the activations is token 4 (i & 3) + i / 4; rows of no token repeat another
+    const uint8_t *xa = lds + (g * 4 * V + ((i & 3) < V ? (i & 3) * 4 : 0) + (i >> 2)) * 8;
+    const float *sa = scales + g * 4;
+    // A step's loads: lane l has block l & 7 of rows l / 8 and 8 + l / 8.  In LDS block b of row r is at b ^ r ^ (r / 8) of
+    // the row's eight: both the writes and the reads (word g of one block of row i) go to all banks.
+    const int lr = lane >> 3, lb = lane & 7;
+    uint4 *put[2];
+    const uint32_t *get[kStep];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) put[h] = reinterpret_cast<uint4 *>(bounce) + (h * 8 + lr) * 8 + (lb ^ lr ^ h);
+#pragma unroll
+    for (int j = 0; j < kStep; ++j)
+        get[j] = reinterpret_cast<const uint32_t *>(bounce) + (i * 8 + (j ^ (i & 7) ^ (i >> 3))) * 4 + g;
+    uint4 wv[kAhead][2], sv;
+    // unit u's rows of this lane: of the quants (two), and of the scales
+    auto matrix = [&](int u) { return a.w[DOWN ? 0 : u]; };
+    auto row_at = [&](int u, int r) { return (uint32_t)min(r0 + (DOWN ? u * 16 : 0) + r, a.rows - 1) * nb; };
+    auto load = [&](int k, int u, int c) {
+        const uint8_t *w = matrix(u) + first_block * 16;
+        const int b = min(c * kStep + lb, nb - 1);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            wv[k][h] = load_stream16(reinterpret_cast<const uint4 *>(w + (row_at(u, h * 8 + lr) + b) * 16ull));
+    };
+    auto load_scale = [&](int u, int c) {  // lane (g, i): of row i, the blocks of step c + g
+        sv = load_scales<AT_ONCE>(matrix(u) + blocks * 16 + first_block * 2, row_at(u, i), (c + g) * kStep, nb);
+    };
+    stream_stage<PACKED, V>(a, s_row, count, DOWN ? a.batch * a.k : a.batch, lds, scales, [&]() {
+        if (units == 0) return;
+        load_scale(0, 0);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+            if (k < steps) load(k, 0, k);
+    });
+    mrml_xsum::lds_barrier();
+    float acc[V] = {}, gate[V] = {};
+    for (int unit = 0; unit < units; ++unit) {
+        for (int c0 = 0; c0 < steps; c0 += kAhead) {
+            uint32_t d[4][4];  // scales 2 n and 2 n + 1 of step c0 + k
+            {
+                uint32_t t[4];
+                const uint32_t v[4] = {sv.x, sv.y, sv.z, sv.w};
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    spread(v[n], t);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) d[k][n] = t[k];
+                }
+            }
+            if (c0 + kAhead < steps) load_scale(unit, c0 + kAhead);
+            else if (unit + 1 < units) load_scale(unit + 1, 0);
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int c = c0 + k;
+                if (c >= steps) break;
+                *put[0] = wv[k][0];
+                *put[1] = wv[k][1];
+                if (c + kAhead < steps) load(k, unit, c + kAhead);
+                else if (unit + 1 < units) load(k, unit + 1, k);
+                const uint8_t *x = xa + c * kStep * stream_block(V);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float4v s[V];
+#pragma unroll
+                    for (int v = 0; v < V; ++v) s[v] = *reinterpret_cast<const float4v *>(sa + ((c * 2 + h) * V + v) * 16);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t y = *get[4 * h + j] ^ 0x88888888u;
+                        const uint64_t both = (uint64_t)(y & 0xF0F0F0F0u) << 32 | ((y << 4) & 0xF0F0F0F0u);
+                        const int4v p = __builtin_amdgcn_mfma_i32_16x16x32_i8(
+                            *reinterpret_cast<const long *>(x + (4 * h + j) * stream_block(V)), (long)both,
+                            int4v{0, 0, 0, 0}, 0, 0, 0);
+                        const float dw = f16_bits_to_f32(d[k][2 * h + (j >> 1)] >> (j & 1) * 16 & 0xffffu);
+#pragma unroll
+                        for (int v = 0; v < V; ++v) acc[v] = __builtin_fmaf((float)p[v], dw * s[v][j], acc[v]);
+                    }
+                }
+            }
+        }
+        // the unit's sums are whole
+        const int row = r0 + (DOWN ? unit * 16 : 0) + i;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int t = 4 * v + g;
+            if ((DOWN || unit == 1) && t < count && s_as[t] >= 0 && row < a.rows)
+                a.out[(size_t)s_as[t] * a.rows + row] = DOWN ? acc[v] * s_weight[t] : gated(gate[v], acc[v], a.activation);
+            gate[v] = acc[v];
+            acc[v] = 0.0f;
+        }
+    }
+}
+
+// Workgroup (x, y): rows of chunk x, and tile y of all experts' tiles of `tokens` tokens.
+template <bool DOWN, bool PACKED, int AT_ONCE>
+__global__ __launch_bounds__(64 * kWaves, 4) void moe_stream_kernel(ExpertArgs a, int tokens)
+{
+    extern __shared__ __align__(16) uint8_t lds[];
+    __shared__ int s_as[kStreamTokens], s_row[kStreamTokens], s_tile[3], s_ends[kWaves];
+    __shared__ float s_weight[kStreamTokens];
+    const int n = a.batch * a.k, tid = threadIdx.x;
+    const int j = (blockIdx.y * gridDim.x + blockIdx.x) * 64 * kWaves + tid;
+    if (tid == 0) s_tile[2] = 0;
+    // tiles of the experts of each thread, and before them
+    static_assert(kMaxExperts == 2 * 64 * kWaves, "two experts a thread");
+    int first[2], count[2], mine = 0;
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        const int e = 2 * tid + v;
+        const int s0 = e < a.n_experts ? min(max(a.starts[e], 0), n) : 0;
+        const int s1 = e < a.n_experts ? min(max(a.starts[e + 1], s0), n) : 0;
+        first[v] = s0;
+        count[v] = s1 - s0;
+        mine += (count[v] + tokens - 1) / tokens;
+    }
+    int ends = mine;
+    for (int m = 1; m < 64; m *= 2) {
+        const int before = __shfl_up(ends, m, 64);
+        if ((tid & 63) >= m) ends += before;
+    }
+    if ((tid & 63) == 63) s_ends[tid >> 6] = ends;
+    mrml_xsum::lds_barrier();
+    int at = ends - mine;
+    for (int w = 0; w < (tid >> 6); ++w) at += s_ends[w];
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+        const int tiles = (count[v] + tokens - 1) / tokens, t = (int)blockIdx.y - at;
+        if (t >= 0 && t < tiles) {
+            s_tile[0] = 2 * tid + v;
+            s_tile[1] = first[v] + t * tokens;
+            s_tile[2] = min(tokens, count[v] - t * tokens);
+        }
+        at += tiles;
+    }
+    mrml_xsum::lds_barrier();
+    if (j < n && !plan_ok(a, j)) moe_fault(a.faults);
+    const int e = s_tile[0], from = s_tile[1], tokens_here = s_tile[2];
+    if (tokens_here == 0) return;
+    if (tid < kStreamTokens) {
+        const int o = tid < tokens_here ? a.order[from + tid] : -1;
+        const bool ok = o >= 0 && o < n;
+        s_as[tid] = ok ? o : -1;
+        s_row[tid] = ok ? (DOWN ? o : o / a.k) : 0;
+        s_weight[tid] = DOWN && ok ? a.weights[o] : 0.0f;
+    }
+    mrml_xsum::lds_barrier();
+    if (tokens_here <= 4) stream_pass<DOWN, PACKED, AT_ONCE, 1>(a, e, tokens_here, lds, s_as, s_row, s_weight);
+    else if (tokens_here <= 8) stream_pass<DOWN, PACKED, AT_ONCE, 2>(a, e, tokens_here, lds, s_as, s_row, s_weight);
+    else stream_pass<DOWN, PACKED, AT_ONCE, 4>(a, e, tokens_here, lds, s_as, s_row, s_weight);
+}
+
 // y = the sum of a token's weighted products in the order of its slots; VEC values a thread.
 template <int VEC>
 __global__ __launch_bounds__(256) void moe_combine_kernel(ExpertArgs a, const float *__restrict__ part, float *__restrict__ y)
@@ -383,8 +648,7 @@ int launch_tiles(mrml_hip_ctx *ctx, const ExpertArgs &a, int nt, const Tile *til
 #define MOE_TILES(NTM)                                                                                              \
     hipLaunchKernelGGL((moe_tile_kernel<DOWN, NTM>), dim3((uint32_t)grid), dim3(64 * kWaves), 0, ctx->stream, a, tiles, \
                        xp, xscale, row_wgs)
-    if (nt == 1) MOE_TILES(1);
-    else if (nt == 2) MOE_TILES(2);
+    if (nt == 2) MOE_TILES(2);
     else MOE_TILES(4);
 #undef MOE_TILES
     return check_launch(ctx, "moe_tile_kernel");
@@ -394,7 +658,45 @@ int launch_tiles(mrml_hip_ctx *ctx, const ExpertArgs &a, int nt, const Tile *til
 int tile_groups(const ExpertArgs &a)
 {
     const int mean = a.batch * a.k / a.n_experts;
-    return mean <= 12 ? 1 : mean <= 24 ? 2 : 4;
+    return mean <= 24 ? 2 : 4;
+}
+
+// Few tokens an expert on average.
+bool streams(const ExpertArgs &a) { return a.batch * a.k <= 12 * a.n_experts && a.cols / 32 <= kStreamBlocks; }
+
+template <bool DOWN>
+int launch_stream(mrml_hip_ctx *ctx, const ExpertArgs &a)
+{
+    const int n = a.batch * a.k, nb = a.cols / 32, rows = 16 * kWaves * (DOWN ? stream_units<DOWN>() : 1);
+    // the tokens of a tile: room for more costs workgroups on a CU
+    const int tokens = n <= 4 * a.n_experts ? 8 : kStreamTokens;
+    const dim3 grid((a.rows + rows - 1) / rows, std::min(n, n / tokens + a.n_experts));
+#define MOE_STREAM(PACKED, AT_ONCE)                                                                                \
+    hipLaunchKernelGGL((moe_stream_kernel<DOWN, PACKED, AT_ONCE>), grid, dim3(64 * kWaves), stream_lds(nb, tokens), \
+                       ctx->stream, a, tokens)
+#define MOE_STREAM_AT(PACKED)                        \
+    do {                                             \
+        if (nb % 8 == 0) MOE_STREAM(PACKED, 8);      \
+        else if (nb % 4 == 0) MOE_STREAM(PACKED, 4); \
+        else if (nb % 2 == 0) MOE_STREAM(PACKED, 2); \
+        else MOE_STREAM(PACKED, 1);                  \
+    } while (0)
+    if (!DOWN && a.xpack) MOE_STREAM_AT(!DOWN);
+    else MOE_STREAM_AT(false);
+#undef MOE_STREAM_AT
+#undef MOE_STREAM
+    return check_launch(ctx, "moe_stream_kernel");
+}
+
+int launch_combine(mrml_hip_ctx *ctx, const ExpertArgs &a, const float *part)
+{
+    if (a.rows % 4 == 0)
+        hipLaunchKernelGGL(moe_combine_kernel<4>, dim3(a.batch, (a.rows / 4 + 255) / 256), dim3(256), 0, ctx->stream, a,
+                           part, a.out);
+    else
+        hipLaunchKernelGGL(moe_combine_kernel<1>, dim3(a.batch, (a.rows + 255) / 256), dim3(256), 0, ctx->stream, a, part,
+                           a.out);
+    return check_launch(ctx, "moe_combine_kernel");
 }
 
 // The product itself: activations in MFMA order and the list of tiles in the workspace, then the tiles.
@@ -420,19 +722,24 @@ int launch_product(mrml_hip_ctx *ctx, const ExpertArgs &a)
     ExpertArgs p = a;
     if (DOWN) p.out = (float *)(xp + packed);
     if (int rc = launch_tiles<DOWN>(ctx, p, nt, tiles, xp, xscale)) return rc;
-    if (!DOWN) return MRML_HIP_OK;
-    if (a.rows % 4 == 0)
-        hipLaunchKernelGGL(moe_combine_kernel<4>, dim3(a.batch, (a.rows / 4 + 255) / 256), dim3(256), 0, ctx->stream, a,
-                           p.out, a.out);
-    else
-        hipLaunchKernelGGL(moe_combine_kernel<1>, dim3(a.batch, (a.rows + 255) / 256), dim3(256), 0, ctx->stream, a, p.out,
-                           a.out);
-    return check_launch(ctx, "moe_combine_kernel");
+    return DOWN ? launch_combine(ctx, a, p.out) : MRML_HIP_OK;
 }
 
 }  // namespace
 
-int launch_moe_gate_up(mrml_hip_ctx *ctx, const ExpertArgs &a) { return launch_product<false>(ctx, a); }
-int launch_moe_down(mrml_hip_ctx *ctx, const ExpertArgs &a) { return launch_product<true>(ctx, a); }
+int launch_moe_gate_up(mrml_hip_ctx *ctx, const ExpertArgs &a)
+{
+    return streams(a) ? launch_stream<false>(ctx, a) : launch_product<false>(ctx, a);
+}
+
+int launch_moe_down(mrml_hip_ctx *ctx, const ExpertArgs &a)
+{
+    if (!streams(a)) return launch_product<true>(ctx, a);
+    ExpertArgs p = a;
+    p.out = (float *)workspace(ctx, (size_t)a.batch * a.k * a.rows * 4);
+    if (!p.out) return MRML_HIP_E_ALLOC;
+    if (int rc = launch_stream<true>(ctx, p)) return rc;
+    return launch_combine(ctx, a, p.out);
+}
 
 }  // namespace mrml
