@@ -10,6 +10,7 @@
 // x 16 outputs of a block against 32 of MFMA and 16 of VALU side by side here.)
 
 #include <algorithm>
+#include <type_traits>
 
 #include "moe.h"
 #include "exact_sum.h"
@@ -360,8 +361,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_tile_kernel(ExpertArgs a, 
 
 // ---- few tokens an expert -------------------------------------------------------------
 
-// Bound by the stream of weights: one launch, one workgroup for a run of rows and up to 16 tokens of one expert.  The
-// activations are quantised into LDS by every workgroup; a wave has kUnits runs of 16 rows one after the other, whose
+// Bound by the stream of weights: one workgroup for a run of rows and up to 16 tokens of one expert.  The
+// activations come quantised (a launch before; every workgroup quantising its own took 10 us of 57 for 40 tokens) and are
+// put in LDS by every workgroup; a wave has kUnits runs of 16 rows one after the other, whose
 // weights go from memory to registers kAhead steps ahead and without a barrier, 128 bytes of a row at once (a stream of 64
 // bytes a row reaches 4.9 TB/s here, of 128 bytes 6.1), and through 2 KB of LDS of the wave's own to the lanes that need
 // them.  The block sums are int8 MFMA: 16 (q - 8) is a byte after one xor, a shift and two ands, half of what a half of it
@@ -390,49 +392,43 @@ size_t stream_lds(int nb, int tokens)
     return kWaves * kBounce + (size_t)stream_blocks(nb) * (stream_block(tokens / 4) + tokens * 4);
 }
 
-// `count` rows into LDS as Q8_0; scales of 0 behind the last block, up to a whole step.  loaded() is called once the
-// first loads are under way.
-template <bool PACKED, int V, class F>
-__device__ __forceinline__ void stream_stage(const ExpertArgs &a, const int *s_row, int count, int in_rows, uint8_t *lds,
-                                             float *scales, F loaded)
+// `count` rows of an activation pack of `total` blocks into LDS; scales of 0 behind the last block, up to a whole step.
+// loaded() is called once the first loads are under way.
+template <int V, class F>
+__device__ __forceinline__ void stream_stage(const uint8_t *pack, size_t total, int nb, const int *s_row, int count,
+                                             uint8_t *lds, float *scales, F loaded)
 {
-    const int nb = a.cols / 32, n4 = nb * 8, all = count * n4;
+    const float *pd = reinterpret_cast<const float *>(pack + total * 32);
     auto scale_at = [&](int t, int b) -> float & {
-        return scales[(((b / kChunk) * V + (t >> 2)) * 4 + (t & 3)) * kChunk + b % kChunk];
+        return scales[(((b / 4) * V + (t >> 2)) * 4 + (t & 3)) * 4 + b % 4];
     };
+    const int n2 = nb * 2, all = count * n2;  // halves of blocks
     int t = 0, c = (int)threadIdx.x;
     for (int k0 = 0; k0 < all; k0 += 64 * kWaves * kStageAhead) {
-        float4 x[kStageAhead];
-        uint32_t q[kStageAhead];
+        uint4 q[kStageAhead];
         float d[kStageAhead];
         int tt[kStageAhead], cc[kStageAhead];
 #pragma unroll
         for (int k = 0; k < kStageAhead; ++k) {
-            for (; c >= n4 && t < count; ++t) c -= n4;
+            for (; c >= n2 && t < count; ++t) c -= n2;
             tt[k] = t;
             cc[k] = t < count ? c : 0;
-            const size_t at = (size_t)s_row[t < count ? t : 0] * n4 + cc[k];
-            if (PACKED) {
-                q[k] = reinterpret_cast<const uint32_t *>(a.xpack)[at];
-                d[k] = reinterpret_cast<const float *>(a.xpack + (size_t)in_rows * nb * 32)[at >> 3];
-            } else {
-                x[k] = reinterpret_cast<const float4 *>(a.x)[at];
-            }
+            const size_t at = (size_t)s_row[t < count ? t : 0] * n2 + cc[k];
+            q[k] = reinterpret_cast<const uint4 *>(pack)[at];
+            d[k] = pd[at >> 1];
             c += 64 * kWaves;
         }
         if (k0 == 0) loaded();
 #pragma unroll
         for (int k = 0; k < kStageAhead; ++k) {
-            if (!PACKED) {
-                uint32_t dbits;
-                int sum;
-                q[k] = q8_0_block8x4(x[k], dbits, sum);
-                d[k] = f16_bits_to_f32(dbits);
-            }
-            const int l = cc[k] & 7, b = cc[k] >> 3;
             if (tt[k] >= count) continue;
-            *reinterpret_cast<uint32_t *>(lds + b * stream_block(V) + ((l & 3) * 4 * V + tt[k]) * 8 + (l >> 2) * 4) = q[k];
-            if (l == 0) scale_at(tt[k], b) = d[k] * 0.0625f;  // the weights' factor of 16
+            const int b = cc[k] >> 1, h = cc[k] & 1;
+            uint32_t *dst = reinterpret_cast<uint32_t *>(lds + b * stream_block(V) + tt[k] * 8 + h * 4);
+            dst[0] = q[k].x;
+            dst[4 * V * 2] = q[k].y;
+            dst[8 * V * 2] = q[k].z;
+            dst[12 * V * 2] = q[k].w;
+            if (h == 0) scale_at(tt[k], b) = d[k] * 0.0625f;  // the weights' factor of 16
         }
     }
     if ((int)threadIdx.x < 4 * V)
@@ -459,7 +455,7 @@ __device__ __forceinline__ uint4 load_scales(const uint8_t *ws, uint32_t row_at,
 }
 
 // Up to 4 V tokens of one expert.
-template <bool DOWN, bool PACKED, int AT_ONCE, int V>
+template <bool DOWN, int AT_ONCE, int V>
 __device__ __forceinline__ void stream_pass(const ExpertArgs &a, int expert, int count, uint8_t *lds, const int *s_as,
                                             const int *s_row, const float *s_weight)
 {
@@ -500,7 +496,8 @@ __device__ __forceinline__ void stream_pass(const ExpertArgs &a, int expert, int
     auto load_scale = [&](int u, int c) {  // lane (g, i): of row i, the blocks of step c + g
         sv = load_scales<AT_ONCE>(matrix(u) + blocks * 16 + first_block * 2, row_at(u, i), (c + g) * kStep, nb);
     };
-    stream_stage<PACKED, V>(a, s_row, count, DOWN ? a.batch * a.k : a.batch, lds, scales, [&]() {
+    const size_t total = (size_t)(DOWN ? a.batch * a.k : a.batch) * nb;
+    stream_stage<V>(a.xpack, total, nb, s_row, count, lds, scales, [&]() {
         if (units == 0) return;
         load_scale(0, 0);
 #pragma unroll
@@ -566,7 +563,7 @@ __device__ __forceinline__ void stream_pass(const ExpertArgs &a, int expert, int
 }
 
 // Workgroup (x, y): rows of chunk x, and tile y of all experts' tiles of `tokens` tokens.
-template <bool DOWN, bool PACKED, int AT_ONCE>
+template <bool DOWN, int AT_ONCE>
 __global__ __launch_bounds__(64 * kWaves, 4) void moe_stream_kernel(ExpertArgs a, int tokens)
 {
     extern __shared__ __align__(16) uint8_t lds[];
@@ -618,12 +615,249 @@ __global__ __launch_bounds__(64 * kWaves, 4) void moe_stream_kernel(ExpertArgs a
         s_weight[tid] = DOWN && ok ? a.weights[o] : 0.0f;
     }
     mrml_xsum::lds_barrier();
-    if (tokens_here <= 4) stream_pass<DOWN, PACKED, AT_ONCE, 1>(a, e, tokens_here, lds, s_as, s_row, s_weight);
-    else if (tokens_here <= 8) stream_pass<DOWN, PACKED, AT_ONCE, 2>(a, e, tokens_here, lds, s_as, s_row, s_weight);
-    else stream_pass<DOWN, PACKED, AT_ONCE, 4>(a, e, tokens_here, lds, s_as, s_row, s_weight);
+    if (tokens_here <= 4) stream_pass<DOWN, AT_ONCE, 1>(a, e, tokens_here, lds, s_as, s_row, s_weight);
+    else if (tokens_here <= 8) stream_pass<DOWN, AT_ONCE, 2>(a, e, tokens_here, lds, s_as, s_row, s_weight);
+    else stream_pass<DOWN, AT_ONCE, 4>(a, e, tokens_here, lds, s_as, s_row, s_weight);
 }
 
-// y = the sum of a token's weighted products in the order of its slots; VEC values a thread.
+// ---- a handful of assignments ------------------------------------------------------------
+
+// Each assignment by itself, in one launch, from the activations as they come (a launch to quantise and one for the lists
+// would take as long as the products).  The block sums are the matvecs' (v_dot8 on raw weight words and split-nibble
+// activations): lane (r, b) = (lane / 8, lane % 8) has block 8 c + b of row r of 8 in step c, a load of 128 bytes a row.
+//  A unit's scales are read as one run of memory into LDS of the wave's own (read where they are needed they
+// are as many requests as the weights).  What it comes to is a few microseconds of latencies one after the other and the
+// rate at which a CU takes loads, so:
+//  - units are small, since the CU with the most of them sets the time (eight assignments of 704 rows and 2816 columns:
+//    352 workgroups of 16 rows, two on some CUs and one on others, 9.4 us; 704 of 8 rows, three or two, see below);
+//  - waves of their own quantise: a CU takes 1.5 to 4 us to accept the loads of its weights, and a wave that issues those
+//    first cannot quantise meanwhile.
+constexpr int kGateRows = 8, kDownRows = 16;  // of a workgroup
+
+__host__ __device__ constexpr size_t dot_scales_bytes(int nb, int rows) { return (size_t)nb * rows * 2; }  // of a wave
+__host__ __device__ constexpr size_t dot_token_bytes(int nb) { return ((size_t)nb * 40 + 15) / 16 * 16; }
+
+// A token's blocks in LDS: lo and hi (device.h), then behind all blocks {d, c}.
+struct DotToken {
+    uint4 *x;
+    float2 *dc;
+    __device__ DotToken(uint8_t *lds, int nb) : x(reinterpret_cast<uint4 *>(lds)), dc(reinterpret_cast<float2 *>(lds + nb * 32)) {}
+};
+
+// Block b from its 32 quants.
+__device__ __forceinline__ void dot_put(const DotToken &t, int b, uint4 x, uint4 y, float d)
+{
+    t.x[2 * b] = make_uint4(split_lo(x.x, y.x), split_lo(x.y, y.y), split_lo(x.z, y.z), split_lo(x.w, y.w));
+    t.x[2 * b + 1] = make_uint4(split_hi(x.x, y.x), split_hi(x.y, y.y), split_hi(x.z, y.z), split_hi(x.w, y.w));
+    const int c = -8 * (lo_nib_sum(x.x) + lo_nib_sum(x.y) + lo_nib_sum(x.z) + lo_nib_sum(x.w) + lo_nib_sum(y.x) +
+                        lo_nib_sum(y.y) + lo_nib_sum(y.z) + lo_nib_sum(y.w));
+    t.dc[b] = make_float2(d, __builtin_bit_cast(float, c));
+}
+
+// A row of f32 quantised by `threads` threads (whole waves), this one `tid`; ahead() once the first loads are under way.
+template <class F>
+__device__ __forceinline__ void dot_quantize(const float *x, int nb, int tid, int threads, const DotToken &t, F ahead)
+{
+    constexpr int kBatch = 4;
+    const int n4 = nb * 8;
+    for (int c0 = 0; c0 < n4; c0 += kBatch * threads) {
+        float4 v[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) v[k] = reinterpret_cast<const float4 *>(x)[min(c0 + k * threads + tid, n4 - 1)];
+        if (c0 == 0) ahead();
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            if (c0 + k * threads >= n4) break;
+            const int c = c0 + k * threads + tid, l = c & 7;
+            uint32_t dbits;
+            int sum;
+            const uint32_t q = q8_0_block8x4(v[k], dbits, sum);
+            const uint32_t w = q8_split8(q, l, sum);
+            if (c < n4) {
+                reinterpret_cast<uint32_t *>(t.x)[c] = w;
+                if (l == 0) t.dc[c >> 3] = make_float2(f16_bits_to_f32(dbits), __builtin_bit_cast(float, sum));
+            }
+        }
+    }
+}
+
+// A unit's 8 H rows of an expert's matrix, and what a wave has of them.
+template <int H>
+struct DotUnit {
+    static constexpr int kScales = kStreamBlocks * H / 64;  // pieces of 16 bytes a lane
+    const uint8_t *w, *ws;  // the expert's quants and scales
+    uint32_t row, rows;     // first row; rows of the matrix
+    uint4 sv[kScales];
+    uint4 st[kAhead][H];
+    bool wide;
+
+    __device__ __forceinline__ DotUnit(const ExpertArgs &a, int matrix, int expert, int r, int nb) : row(r), rows(a.rows)
+    {
+        const size_t first = (size_t)expert * a.rows * nb, all = (size_t)a.n_experts * a.rows * nb;
+        w = a.w[matrix] + first * 16;
+        ws = a.w[matrix] + all * 16 + first * 2;
+    }
+
+    __device__ __forceinline__ int halves(int nb) const { return min(8 * H, (int)(rows - row)) * nb; }
+
+    // Scales from memory to registers, 16 bytes a lane, where they lie so; on to LDS.  Rows past the matrix's last get
+    // some scales of it.
+    __device__ __forceinline__ void load_scales(int nb, int lane)
+    {
+        const uint8_t *src = ws + (size_t)row * nb * 2;
+        wide = (((uintptr_t)src | (uintptr_t)(halves(nb) * 2)) & 15) == 0;
+        if (!wide) return;
+#pragma unroll
+        for (int k = 0; k < kScales; ++k)
+            if (k * 64 < nb * H) sv[k] = reinterpret_cast<const uint4 *>(src)[min(k * 64 + lane, halves(nb) / 8 - 1)];
+    }
+    __device__ __forceinline__ void store_scales(int nb, int lane, uint16_t *lds) const
+    {
+        if (wide) {
+#pragma unroll
+            for (int k = 0; k < kScales; ++k)
+                if (k * 64 + lane < nb * H) reinterpret_cast<uint4 *>(lds)[k * 64 + lane] = sv[k];
+        } else {
+            const uint16_t *src = reinterpret_cast<const uint16_t *>(ws) + (size_t)row * nb;
+            for (int k = lane; k < 8 * H * nb; k += 64) lds[k] = src[min(k, halves(nb) - 1)];
+        }
+    }
+
+    __device__ __forceinline__ void load(int k, int nb, int c, int lane)
+    {
+        const int b = min(c * kStep + (lane & 7), nb - 1);
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+            st[k][h] = load_stream16(
+                reinterpret_cast<const uint4 *>(w + (min(row + h * 8 + (lane >> 3), rows - 1) * nb + b) * 16ull));
+    }
+
+    // Steps c0 .. c1, whose first kAhead are on the way: the sums of rows lane / 8 + 8 h, in all lanes of a row.
+    __device__ __forceinline__ void sum(int nb, int c0, int c1, int lane, const uint16_t *scales, const DotToken &x,
+                                        float (&acc)[H])
+    {
+#pragma unroll
+        for (int h = 0; h < H; ++h) acc[h] = 0.0f;
+        for (int s0 = c0; s0 < c1; s0 += kAhead)
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int c = s0 + k, bt = c * kStep + (lane & 7), b = min(bt, nb - 1);
+                if (c >= c1) break;
+                uint4 q[H];
+#pragma unroll
+                for (int h = 0; h < H; ++h) q[h] = st[k][h];
+                if (c + kAhead < c1) load(k, nb, c + kAhead, lane);
+                const uint4 lo = x.x[2 * b], hi = x.x[2 * b + 1];
+                const float2 dc = x.dc[b];
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    const float dw = f16_bits_to_f32(scales[(h * 8 + (lane >> 3)) * nb + b]);
+                    const int n = q4_0_isum_split(q[h].x, q[h].y, q[h].z, q[h].w, lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z,
+                                                  hi.w, __builtin_bit_cast(int, dc.y));
+                    acc[h] = __builtin_fmaf((float)n, (bt < nb ? dw : 0.0f) * dc.x, acc[h]);
+                }
+            }
+        auto from = [](float v, auto ctrl) {
+            return __builtin_bit_cast(float, dpp_mov<decltype(ctrl)::value>(__builtin_bit_cast(int, v)));
+        };
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            acc[h] += from(acc[h], std::integral_constant<int, 0xB1>{});
+            acc[h] += from(acc[h], std::integral_constant<int, 0x4E>{});
+            acc[h] += from(acc[h], std::integral_constant<int, 0x141>{});
+        }
+    }
+};
+
+// One assignment (blockIdx.y) and 8 rows of gate and of up, each by two waves that have half of the blocks; four waves more
+// quantise the token.
+constexpr int kPutWaves = 4, kGetWaves = 4;
+__global__ __launch_bounds__(64 * (kPutWaves + kGetWaves)) void moe_gate_up_one_kernel(ExpertArgs a)
+{
+    extern __shared__ __align__(16) uint8_t lds[];
+    __shared__ float part[kGetWaves][kGateRows];
+    const int n = a.batch * a.k, tid = threadIdx.x, lane = tid & 63, nb = a.cols / 32, as = blockIdx.y;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), row0 = blockIdx.x * kGateRows;
+    const DotToken token(lds, nb);
+    if (wave < kPutWaves) {
+        const size_t t = as / a.k;
+        if (a.xpack) {
+            const uint4 *q = reinterpret_cast<const uint4 *>(a.xpack + t * nb * 32);
+            const float *d = reinterpret_cast<const float *>(a.xpack + (size_t)a.batch * nb * 32) + t * nb;
+            for (int b = tid; b < nb; b += 64 * kPutWaves) dot_put(token, b, q[2 * b], q[2 * b + 1], d[b]);
+        } else {
+            dot_quantize(a.x + t * a.cols, nb, tid, 64 * kPutWaves, token, []() {});
+        }
+        mrml_xsum::lds_barrier();
+        mrml_xsum::lds_barrier();
+        const int j = (blockIdx.y * gridDim.x + blockIdx.x) * 64 * kPutWaves + tid;
+        if (j < n && !plan_ok(a, j)) moe_fault(a.faults);
+        return;
+    }
+    const int e = a.ids[as], w = wave - kPutWaves;
+    const bool there = e >= 0 && e < a.n_experts;
+    const int steps = there ? (nb + kStep - 1) / kStep : 0, half = (steps + 1) / 2;
+    const int c0 = (w & 1) * half, c1 = min(c0 + half, steps);
+    uint16_t *scales = reinterpret_cast<uint16_t *>(lds + dot_token_bytes(nb) + w * dot_scales_bytes(nb, kGateRows));
+    DotUnit<1> unit(a, w >> 1, there ? e : 0, row0, nb);
+    if (c0 < c1) unit.load_scales(nb, lane);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+        if (c0 + k < c1) unit.load(k, nb, c0 + k, lane);
+    if (c0 < c1) unit.store_scales(nb, lane, scales);
+    mrml_xsum::lds_barrier();
+    float v[1];
+    unit.sum(nb, c0, c1, lane, scales, token, v);
+    if ((lane & 7) == 0) part[w][lane >> 3] = v[0];
+    mrml_xsum::lds_barrier();
+    const int r = tid - 64 * kPutWaves;
+    if (r < kGateRows && row0 + r < a.rows && there)
+        a.out[(size_t)as * a.rows + row0 + r] = gated(part[0][r] + part[1][r], part[2][r] + part[3][r], a.activation);
+}
+
+// One token (blockIdx.y) and 16 rows of down, eight of its assignments at a time, a wave each, which quantises it; y itself.
+constexpr int kDownWaves = 8;
+__global__ __launch_bounds__(64 * kDownWaves) void moe_down_one_kernel(ExpertArgs a)
+{
+    extern __shared__ __align__(16) uint8_t lds[];
+    __shared__ float part[kMaxTopK][kDownRows];
+    const int n = a.batch * a.k, tid = threadIdx.x, lane = tid & 63, nb = a.cols / 32, t = blockIdx.y;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int row0 = blockIdx.x * kDownRows, steps = (nb + kStep - 1) / kStep;
+    uint8_t *mine = lds + wave * (dot_token_bytes(nb) + dot_scales_bytes(nb, kDownRows));
+    const DotToken token(mine, nb);
+    uint16_t *scales = reinterpret_cast<uint16_t *>(mine + dot_token_bytes(nb));
+    for (int s = wave; s < a.k; s += kDownWaves) {
+        const int as = t * a.k + s, e = a.ids[as];
+        const bool there = e >= 0 && e < a.n_experts;
+        const float weight = there ? a.weights[as] : 0.0f;
+        float v[2] = {0.0f, 0.0f};
+        if (there) {
+            DotUnit<2> unit(a, 0, e, row0, nb);
+            dot_quantize(a.x + (size_t)as * a.cols, nb, lane, 64, token, [&]() {
+                unit.load_scales(nb, lane);
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k)
+                    if (k < steps) unit.load(k, nb, k, lane);
+            });
+            unit.store_scales(nb, lane, scales);
+            unit.sum(nb, 0, steps, lane, scales, token, v);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if ((lane & 7) == 0) part[s][h * 8 + (lane >> 3)] = there ? v[h] * weight : 0.0f;
+    }
+    mrml_xsum::lds_barrier();
+    if (tid < kDownRows && row0 + tid < a.rows) {
+        float y = 0.0f;
+        for (int s = 0; s < a.k; ++s) y += part[s][tid];
+        a.out[(size_t)t * a.rows + row0 + tid] = y;
+    }
+    const int j = (blockIdx.y * gridDim.x + blockIdx.x) * 64 * kDownWaves + tid;
+    if (j < n && !plan_ok(a, j)) moe_fault(a.faults);
+}
+
+// y = the sum of a token's weighted products in the order of its slots; VEC values a thread, eight slots' loads at once.
 template <int VEC>
 __global__ __launch_bounds__(256) void moe_combine_kernel(ExpertArgs a, const float *__restrict__ part, float *__restrict__ y)
 {
@@ -631,9 +865,17 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(ExpertArgs a, const fl
     if (r >= a.rows) return;
     typedef float vec __attribute__((ext_vector_type(VEC)));
     vec s = 0.0f;
-    for (int i = 0; i < a.k; ++i) {
-        const int as = t * a.k + i, e = a.ids[as];
-        if (e >= 0 && e < a.n_experts) s += *reinterpret_cast<const vec *>(part + (size_t)as * a.rows + r);
+    for (int i0 = 0; i0 < a.k; i0 += 8) {
+        vec v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int as = t * a.k + min(i0 + i, a.k - 1), e = a.ids[as];
+            const bool there = i0 + i < a.k && e >= 0 && e < a.n_experts;
+            v[i] = 0.0f;
+            if (there) v[i] = *reinterpret_cast<const vec *>(part + (size_t)as * a.rows + r);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += v[i];
     }
     *reinterpret_cast<vec *>(y + (size_t)t * a.rows + r) = s;
 }
@@ -661,8 +903,29 @@ int tile_groups(const ExpertArgs &a)
     return mean <= 24 ? 2 : 4;
 }
 
+// A handful of assignments: each by itself, from the activations as they come.
+bool one_by_one(const ExpertArgs &a) { return a.batch * a.k <= 16 && a.cols / 32 <= kStreamBlocks; }
+
+int launch_gate_up_one(mrml_hip_ctx *ctx, const ExpertArgs &a)
+{
+    const int nb = a.cols / 32;
+    const size_t lds = dot_token_bytes(nb) + kGetWaves * dot_scales_bytes(nb, kGateRows);
+    hipLaunchKernelGGL(moe_gate_up_one_kernel, dim3((a.rows + kGateRows - 1) / kGateRows, a.batch * a.k),
+                       dim3(64 * (kPutWaves + kGetWaves)), lds, ctx->stream, a);
+    return check_launch(ctx, "moe_gate_up_one_kernel");
+}
+
+int launch_down_one(mrml_hip_ctx *ctx, const ExpertArgs &a)
+{
+    const int nb = a.cols / 32;
+    const size_t lds = kDownWaves * (dot_token_bytes(nb) + dot_scales_bytes(nb, kDownRows));
+    hipLaunchKernelGGL(moe_down_one_kernel, dim3((a.rows + kDownRows - 1) / kDownRows, a.batch), dim3(64 * kDownWaves), lds,
+                       ctx->stream, a);
+    return check_launch(ctx, "moe_down_one_kernel");
+}
+
 // Few tokens an expert on average.
-bool streams(const ExpertArgs &a) { return a.batch * a.k <= 12 * a.n_experts && a.cols / 32 <= kStreamBlocks; }
+bool streams(const ExpertArgs &a) { return a.batch * a.k <= 12 * a.n_experts && a.cols / 32 <= kStreamBlocks; }  // n * cols < 2^25
 
 template <bool DOWN>
 int launch_stream(mrml_hip_ctx *ctx, const ExpertArgs &a)
@@ -671,19 +934,13 @@ int launch_stream(mrml_hip_ctx *ctx, const ExpertArgs &a)
     // the tokens of a tile: room for more costs workgroups on a CU
     const int tokens = n <= 4 * a.n_experts ? 8 : kStreamTokens;
     const dim3 grid((a.rows + rows - 1) / rows, std::min(n, n / tokens + a.n_experts));
-#define MOE_STREAM(PACKED, AT_ONCE)                                                                                \
-    hipLaunchKernelGGL((moe_stream_kernel<DOWN, PACKED, AT_ONCE>), grid, dim3(64 * kWaves), stream_lds(nb, tokens), \
-                       ctx->stream, a, tokens)
-#define MOE_STREAM_AT(PACKED)                        \
-    do {                                             \
-        if (nb % 8 == 0) MOE_STREAM(PACKED, 8);      \
-        else if (nb % 4 == 0) MOE_STREAM(PACKED, 4); \
-        else if (nb % 2 == 0) MOE_STREAM(PACKED, 2); \
-        else MOE_STREAM(PACKED, 1);                  \
-    } while (0)
-    if (!DOWN && a.xpack) MOE_STREAM_AT(!DOWN);
-    else MOE_STREAM_AT(false);
-#undef MOE_STREAM_AT
+#define MOE_STREAM(AT_ONCE)                                                                                              \
+    hipLaunchKernelGGL((moe_stream_kernel<DOWN, AT_ONCE>), grid, dim3(64 * kWaves), stream_lds(nb, tokens), ctx->stream, a, \
+                       tokens)
+    if (nb % 8 == 0) MOE_STREAM(8);
+    else if (nb % 4 == 0) MOE_STREAM(4);
+    else if (nb % 2 == 0) MOE_STREAM(2);
+    else MOE_STREAM(1);
 #undef MOE_STREAM
     return check_launch(ctx, "moe_stream_kernel");
 }
@@ -729,15 +986,30 @@ int launch_product(mrml_hip_ctx *ctx, const ExpertArgs &a)
 
 int launch_moe_gate_up(mrml_hip_ctx *ctx, const ExpertArgs &a)
 {
-    return streams(a) ? launch_stream<false>(ctx, a) : launch_product<false>(ctx, a);
+    if (one_by_one(a)) return launch_gate_up_one(ctx, a);
+    if (!streams(a)) return launch_product<false>(ctx, a);
+    ExpertArgs p = a;
+    if (!p.xpack) {
+        uint8_t *pack = (uint8_t *)workspace(ctx, act_pack_bytes((size_t)a.batch * (a.cols / 32)));
+        if (!pack) return MRML_HIP_E_ALLOC;
+        if (int rc = launch_quantize_q8_0(ctx, a.x, nullptr, pack, a.batch * a.cols)) return rc;
+        p.xpack = pack;
+    }
+    return launch_stream<false>(ctx, p);
 }
 
 int launch_moe_down(mrml_hip_ctx *ctx, const ExpertArgs &a)
 {
+    if (one_by_one(a)) return launch_down_one(ctx, a);
     if (!streams(a)) return launch_product<true>(ctx, a);
+    const int n = a.batch * a.k;
+    const size_t part = align_up((size_t)n * a.rows * 4, 16);
+    uint8_t *ws = (uint8_t *)workspace(ctx, part + act_pack_bytes(n * (a.cols / 32)));
+    if (!ws) return MRML_HIP_E_ALLOC;
+    if (int rc = launch_quantize_q8_0(ctx, a.x, nullptr, ws + part, n * a.cols)) return rc;
     ExpertArgs p = a;
-    p.out = (float *)workspace(ctx, (size_t)a.batch * a.k * a.rows * 4);
-    if (!p.out) return MRML_HIP_E_ALLOC;
+    p.xpack = ws + part;
+    p.out = (float *)ws;
     if (int rc = launch_stream<true>(ctx, p)) return rc;
     return launch_combine(ctx, a, p.out);
 }
