@@ -146,10 +146,10 @@ __global__ __launch_bounds__(256) void moe_pack_kernel(ExpertArgs a, int rows, i
 // ---- the products -----------------------------------------------------------------
 
 // The eight halves q - 8 of a Q4_0 word, in the order of an activation group.  A nibble put under the exponent of 1024
-// is 1024 + q (the high one 1024 + 16 q).
-__device__ __forceinline__ half8v nibbles(uint32_t w)
+// is 1024 + q (the high one 1024 + 16 q).  k1024: 0x64006400 in a register of the caller's (a second literal would keep the
+// and from being one instruction with the or).
+__device__ __forceinline__ half8v nibbles(uint32_t w, uint32_t k1024)
 {
-    constexpr uint32_t k1024 = 0x64006400u;
     const half2v low = {(_Float16)1032.0f, (_Float16)1032.0f}, by = {(_Float16)0.0625f, (_Float16)0.0625f},
                  high = {(_Float16)-72.0f, (_Float16)-72.0f};
     auto as_half = [](uint32_t x) { return __builtin_bit_cast(half2v, x); };
@@ -210,14 +210,34 @@ constexpr int wave_rows()
     return DOWN ? 64 : 32;
 }
 
-// 16 NT tokens of one expert times the rows of a workgroup.  Lane (g, i): row i of each weight group, and of the
-// activations row i of each token group.
-template <bool DOWN, int NT, int NTM>
-__device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &tile, int chunk_rows, const uint8_t *xp,
-                                             uint4 *lds, const int *s_as, const float *s_scale)
+// 16 bytes a lane from memory to LDS at `to` + 16 * lane, without registers.  In asm, since the compiler would wait for it
+// before any later read of LDS; the reader's loads_barrier waits for it.
+__device__ __forceinline__ void load_to_lds(const uint8_t *from, uint32_t to)
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15, nb = a.cols / 32;
-    const int r0 = chunk_rows + wave * wave_rows<DOWN>();
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "{m0}"(to) : "memory");
+}
+
+// A barrier of the workgroup behind this wave's LDS accesses and all its loads but the last LEFT issued.
+template <int LEFT>
+__device__ __forceinline__ void loads_barrier()
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+}
+
+constexpr int kTileGroups = 6;                 // token groups of 16 a tile at most
+constexpr int kHalf = kChunk / 2;              // blocks of activations in each of two buffers
+constexpr int kTilePart = kHalf * kTileGroups * 2048;  // bytes of a buffer: [block][token group][row / 8] 1 KB each
+
+// 16 NT tokens of one expert times the rows of a workgroup.  Lane (g, i): row i of each weight group, and of the
+// activations row i of each token group.  A block of a row of activations is one line of 128 bytes; 1 KB has eight rows,
+// whose pieces p lie at p ^ row, so that the 16-byte reads of 16 rows meet all banks.  Two blocks of all groups go to one
+// buffer while the two in the other are multiplied; a step's weights are on their way for two of those.
+template <bool DOWN, int NT>
+__device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &tile, int chunk_rows, const uint8_t *xp,
+                                             uint8_t *lds, const int *s_as, const float *s_scale)
+{
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
+    const int nb = a.cols / 32, r0 = chunk_rows + wave * wave_rows<DOWN>();
     const size_t all = (size_t)a.n_experts * a.rows * nb * 16, base = (size_t)tile.expert * a.rows;
     const uint8_t *wq[kGroups], *ws[kGroups];
 #pragma unroll
@@ -227,22 +247,19 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
         wq[q] = w + (base + r) * nb * 16;
         ws[q] = w + all + (base + r) * nb * 2;
     }
+    // this wave's share of a buffer: block wave & 1, rows 8 (wave / 2) .. + 8 of every group
     const uint8_t *xrow[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int as = max(s_as[t * 16 + i], 0);
-        xrow[t] = xp + (size_t)(DOWN ? as : as / a.k) * nb * kXBlock + g * 16;
+        const int as = max(s_as[t * 16 + (wave >> 1) * 8 + (lane >> 3)], 0);
+        xrow[t] = xp + (size_t)(DOWN ? as : as / a.k) * nb * kXBlock + ((lane & 7) ^ (lane >> 3)) * 16;
     }
-    const int chunks = (nb + kChunk - 1) / kChunk;
-    auto load_x = [&](int c, int buf) {
-        const int b = min(c * kChunk + wave, nb - 1);
+    const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
+    const uint32_t put = lds_at + ((wave & 1) * kTileGroups * 2 + (wave >> 1)) * 1024;
+    auto load_x = [&](int c, int half) {
+        const size_t b = (size_t)min(c * kChunk + half * kHalf + (wave & 1), nb - 1) * kXBlock;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                __builtin_amdgcn_global_load_lds(
-                    (const __attribute__((address_space(1))) void *)(xrow[t] + (size_t)b * kXBlock + h * 64),
-                    (__attribute__((address_space(3))) void *)(lds + (((buf * kChunk + wave) * NTM + t) * 2 + h) * 64), 16, 0, 0);
+        for (int t = 0; t < NT; ++t) load_to_lds(xrow[t] + b, __builtin_amdgcn_readfirstlane(put + half * kTilePart + t * 2048));
     };
     uint4 wv[kGroups];
     uint32_t sv[kGroups];
@@ -259,8 +276,13 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
     for (int q = 0; q < kGroups; ++q)
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[q][t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
-    load_x(0, 0);
+    uint32_t k1024 = 0x64006400u;
+    asm volatile("" : "+v"(k1024));
+    const uint8_t *hi_at = lds + (i >> 3) * 1024 + (i & 7) * 128 + ((g ^ (i & 7)) * 16);
+    const uint8_t *lo_at = lds + (i >> 3) * 1024 + (i & 7) * 128 + (((g ^ (i & 7)) ^ 4) * 16);
+    const int chunks = (nb + kChunk - 1) / kChunk;
     load_w(0);
+    load_x(0, 0);
     for (int c = 0; c < chunks; ++c) {
         uint32_t w[kGroups][4], s[kGroups][4];
 #pragma unroll
@@ -271,38 +293,47 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
             w[q][3] = wv[q].w;
             turn(w[q][0], w[q][1], w[q][2], w[q][3]);
             spread(sv[q], s[q]);
-        }
-        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): what went to LDS past the registers
-        __syncthreads();  // chunk c is whole, and everyone is through with chunk c - 1
-        if (c + 1 < chunks) {
-            load_x(c + 1, (c + 1) & 1);
-            load_w(c + 1);
-        }
-        const uint4 *x = lds + (size_t)(c & 1) * kChunk * NTM * 2 * 64 + lane;
+            // done before the barrier: a wait for these weights behind it would be one for the loads issued there too
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-            if (c * kChunk + j >= nb) break;
-            half8v wh[kGroups];
-            float d[kGroups];
+            for (int j = 0; j < kChunk; ++j) asm volatile("" : "+v"(w[q][j]), "+v"(s[q][j]));
+        }
 #pragma unroll
-            for (int q = 0; q < kGroups; ++q) {
-                wh[q] = nibbles(w[q][j]);
-                d[q] = f16_bits_to_f32(s[q][j]);
+        for (int half = 0; half < 2; ++half) {
+            // the buffer's loads: before the first half nothing was issued after them, before the second the weights
+            if (half == 0) loads_barrier<0>();
+            else loads_barrier<2 * kGroups>();  // it is whole, and everyone is through with the other one
+            if (half == 0) {
+                load_x(c, 1);
+                load_w(min(c + 1, chunks - 1));  // always, for the count above
+            } else if (c + 1 < chunks) {
+                load_x(c + 1, 0);
             }
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const half8v hi = __builtin_bit_cast(half8v, x[((j * NTM + t) * 2) * 64]);
-                const half8v lo = __builtin_bit_cast(half8v, x[((j * NTM + t) * 2 + 1) * 64]);
-                float4v p[kGroups];
+            for (int jj = 0; jj < kHalf; ++jj) {
+                const int j = half * kHalf + jj;
+                if (c * kChunk + j >= nb) break;
+                half8v wh[kGroups];
+                float d[kGroups];
 #pragma unroll
-                for (int q = 0; q < kGroups; ++q)
-                    p[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wh[q], float4v{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+                for (int q = 0; q < kGroups; ++q) {
+                    wh[q] = nibbles(w[q][j], k1024);
+                    d[q] = f16_bits_to_f32(s[q][j]);
+                }
 #pragma unroll
-                for (int q = 0; q < kGroups; ++q) p[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wh[q], p[q], 0, 0, 0);
+                for (int t = 0; t < NT; ++t) {
+                    const int at = half * kTilePart + (jj * kTileGroups + t) * 2048;
+                    const half8v hi = *reinterpret_cast<const half8v *>(hi_at + at), lo = *reinterpret_cast<const half8v *>(lo_at + at);
+                    float4v p[kGroups];
 #pragma unroll
-                for (int q = 0; q < kGroups; ++q)
+                    for (int q = 0; q < kGroups; ++q)
+                        p[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wh[q], float4v{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) acc[q][t][v] = __builtin_fmaf(p[q][v], d[q], acc[q][t][v]);
+                    for (int q = 0; q < kGroups; ++q) p[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wh[q], p[q], 0, 0, 0);
+#pragma unroll
+                    for (int q = 0; q < kGroups; ++q)
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) acc[q][t][v] = __builtin_fmaf(p[q][v], d[q], acc[q][t][v]);
+                }
             }
         }
     }
@@ -328,14 +359,14 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
         }
 }
 
-template <bool DOWN, int NTM>
+template <bool DOWN>
 __global__ __launch_bounds__(64 * kWaves, 2) void moe_tile_kernel(ExpertArgs a, const Tile *__restrict__ tiles,
                                                                   const uint8_t *__restrict__ xp,
                                                                   const float *__restrict__ xscale, int row_wgs)
 {
-    __shared__ __align__(16) uint4 lds[2 * kChunk * NTM * 2 * 64];
-    __shared__ int s_as[NTM * 16];
-    __shared__ float s_scale[NTM * 16];
+    __shared__ __align__(16) uint8_t lds[2 * kTilePart];
+    __shared__ int s_as[kTileGroups * 16];
+    __shared__ float s_scale[kTileGroups * 16];
     // workgroups go to the eight XCDs in turn; each XCD gets a run of the list, so that an expert's weights and a tile's
     // activations meet in one L2
     const int total = tiles[0].expert * row_wgs, per = (total + 7) / 8;
@@ -344,7 +375,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_tile_kernel(ExpertArgs a, 
     const int at = id / row_wgs;
     const Tile tile = tiles[1 + at];
     const int n = a.batch * a.k;
-    if (threadIdx.x < NTM * 16) {
+    if (threadIdx.x < kTileGroups * 16) {
         const int j = tile.first + (int)threadIdx.x;
         const int o = (int)threadIdx.x < tile.count ? a.order[j] : -1;
         const bool ok = o >= 0 && o < n;
@@ -352,11 +383,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_tile_kernel(ExpertArgs a, 
         s_scale[threadIdx.x] = ok ? xscale[DOWN ? o : o / a.k] * (DOWN ? a.weights[o] : 1.0f) : 0.0f;
     }
     __syncthreads();
-    const int groups = (tile.count + 15) / 16, chunk_rows = (id - at * row_wgs) * kWaves * wave_rows<DOWN>();
-    if (NTM >= 4 && groups == 4) tile_product<DOWN, NTM >= 4 ? 4 : 1, NTM>(a, tile, chunk_rows, xp, lds, s_as, s_scale);
-    else if (NTM >= 4 && groups == 3) tile_product<DOWN, NTM >= 4 ? 3 : 1, NTM>(a, tile, chunk_rows, xp, lds, s_as, s_scale);
-    else if (NTM >= 2 && groups == 2) tile_product<DOWN, NTM >= 2 ? 2 : 1, NTM>(a, tile, chunk_rows, xp, lds, s_as, s_scale);
-    else tile_product<DOWN, 1, NTM>(a, tile, chunk_rows, xp, lds, s_as, s_scale);
+    const int chunk_rows = (id - at * row_wgs) * kWaves * wave_rows<DOWN>();
+    switch ((tile.count + 15) / 16) {
+    case 1: tile_product<DOWN, 1>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
+    case 2: tile_product<DOWN, 2>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
+    case 3: tile_product<DOWN, 3>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
+    case 4: tile_product<DOWN, 4>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
+    case 5: tile_product<DOWN, 5>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
+    default: tile_product<DOWN, 6>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
+    }
 }
 
 // ---- few tokens an expert -------------------------------------------------------------
@@ -881,26 +916,15 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(ExpertArgs a, const fl
 }
 
 template <bool DOWN>
-int launch_tiles(mrml_hip_ctx *ctx, const ExpertArgs &a, int nt, const Tile *tiles, const uint8_t *xp, const float *xscale)
+int launch_tiles(mrml_hip_ctx *ctx, const ExpertArgs &a, int most, const Tile *tiles, const uint8_t *xp, const float *xscale)
 {
     const int row_wgs = (a.rows + kWaves * wave_rows<DOWN>() - 1) / (kWaves * wave_rows<DOWN>());
-    const int64_t grid = ((int64_t)max_tiles(a, nt) * row_wgs + 7) / 8 * 8;
+    const int64_t grid = ((int64_t)most * row_wgs + 7) / 8 * 8;
     REQUIRE(ctx, grid <= INT32_MAX, "moe: batch * k = %d assignments of %d rows are too many for one call", a.batch * a.k,
             a.rows);
-#define MOE_TILES(NTM)                                                                                              \
-    hipLaunchKernelGGL((moe_tile_kernel<DOWN, NTM>), dim3((uint32_t)grid), dim3(64 * kWaves), 0, ctx->stream, a, tiles, \
-                       xp, xscale, row_wgs)
-    if (nt == 2) MOE_TILES(2);
-    else MOE_TILES(4);
-#undef MOE_TILES
+    hipLaunchKernelGGL((moe_tile_kernel<DOWN>), dim3((uint32_t)grid), dim3(64 * kWaves), 0, ctx->stream, a, tiles, xp, xscale,
+                       row_wgs);
     return check_launch(ctx, "moe_tile_kernel");
-}
-
-// Token groups of 16 a tile at most, by the tokens that an expert has on average.
-int tile_groups(const ExpertArgs &a)
-{
-    const int mean = a.batch * a.k / a.n_experts;
-    return mean <= 24 ? 2 : 4;
 }
 
 // A handful of assignments: each by itself, from the activations as they come.
@@ -960,7 +984,7 @@ int launch_combine(mrml_hip_ctx *ctx, const ExpertArgs &a, const float *part)
 template <bool DOWN>
 int launch_product(mrml_hip_ctx *ctx, const ExpertArgs &a)
 {
-    const int nt = tile_groups(a), most = max_tiles(a, nt), nb = a.cols / 32, n = a.batch * a.k, rows = DOWN ? n : a.batch;
+    const int nt = kTileGroups, most = max_tiles(a, nt), nb = a.cols / 32, n = a.batch * a.k, rows = DOWN ? n : a.batch;
     const size_t list = align_up((size_t)(1 + most) * sizeof(Tile), 256), scales = align_up((size_t)rows * 4, 256);
     const size_t packed = (size_t)rows * nb * kXBlock, part = DOWN ? (size_t)n * a.rows * 4 : 0;
     uint8_t *ws = (uint8_t *)workspace(ctx, list + scales + packed + part);
@@ -978,7 +1002,7 @@ int launch_product(mrml_hip_ctx *ctx, const ExpertArgs &a)
     if (int rc = check_launch(ctx, "moe_pack_kernel")) return rc;
     ExpertArgs p = a;
     if (DOWN) p.out = (float *)(xp + packed);
-    if (int rc = launch_tiles<DOWN>(ctx, p, nt, tiles, xp, xscale)) return rc;
+    if (int rc = launch_tiles<DOWN>(ctx, p, most, tiles, xp, xscale)) return rc;
     return DOWN ? launch_combine(ctx, a, p.out) : MRML_HIP_OK;
 }
 
