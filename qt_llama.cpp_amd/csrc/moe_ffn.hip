@@ -23,6 +23,7 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half4v __attribute__((ext_vector_type(4)));
 typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef float float4v __attribute__((ext_vector_type(4)));
+typedef uint32_t uint4v __attribute__((ext_vector_type(4)));
 
 // ---- activation rows for the MFMA -----------------------------------------------
 
@@ -35,25 +36,24 @@ struct Tile {
     int expert, first, count, pad;  // places first .. first + count of the order
 };
 
-constexpr int kTileRows = 16;
+constexpr int kTileRows = 16, kTileGroups = 4;  // rows of a group, groups of a tile at most
 
-// Tiles of at most NT groups of 16 that a call can have.
-int max_tiles(const ExpertArgs &a, int nt)
+// Tiles that a call can have.
+int max_tiles(const ExpertArgs &a)
 {
     const int n = a.batch * a.k;
-    return std::min(n, n / (kTileRows * nt) + std::min(a.n_experts, n));
+    return std::min(n, n / (kTileRows * kTileGroups) + std::min(a.n_experts, n));
 }
 
 // One wave a row (rows_wgs workgroups of four), then one thread an assignment that checks the plan, then one workgroup
 // that lists the tiles: tiles[0].expert of them behind tiles[0].
 template <bool PACKED>
 __global__ __launch_bounds__(256) void moe_pack_kernel(ExpertArgs a, int rows, int rows_wgs, uint8_t *__restrict__ xp,
-                                                       float *__restrict__ xscale, Tile *__restrict__ tiles, int nt,
-                                                       int most)
+                                                       float *__restrict__ xscale, Tile *__restrict__ tiles, int most)
 {
     const int lane = threadIdx.x & 63, nb = a.cols / 32, n = a.batch * a.k;
     if ((int)blockIdx.x == (int)gridDim.x - 1) {
-        __shared__ int ends[kMaxExperts];
+        __shared__ int sizes[kTileGroups];
         const int tid = threadIdx.x;
         int groups[2], mine[2], first[2], count[2];
         for (int v = 0; v < 2; ++v) {
@@ -66,27 +66,39 @@ __global__ __launch_bounds__(256) void moe_pack_kernel(ExpertArgs a, int rows, i
             first[v] = s0;
             count[v] = s1 - s0;
             groups[v] = (count[v] + kTileRows - 1) / kTileRows;
-            mine[v] = (groups[v] + nt - 1) / nt;
+            mine[v] = (groups[v] + kTileGroups - 1) / kTileGroups;
         }
-        ends[tid] = mine[0] + mine[1];
+        // tiles of each size (in groups, less one), then where they begin: the largest first
+        if (tid < kTileGroups) sizes[tid] = 0;
         __syncthreads();
-        for (int d = 1; d < 256; d *= 2) {
-            const int before = tid >= d ? ends[tid - d] : 0;
-            __syncthreads();
-            ends[tid] += before;
-            __syncthreads();
-        }
-        int at = ends[tid] - mine[0] - mine[1];
-        for (int v = 0; v < 2; ++v) {
-            int from = first[v], left = count[v];
-            for (int i = 0; i < mine[v]; ++i, ++at) {
-                const int c = min(left, kTileRows * (groups[v] / mine[v] + (i < groups[v] % mine[v])));
-                if (at < most) tiles[1 + at] = {tid * 2 + v, from, c, 0};  // runs that overlap could ask for more
-                from += c;
-                left -= c;
+        auto each = [&](auto f) {
+            for (int v = 0; v < 2; ++v) {
+                int from = first[v], left = count[v];
+                for (int i = 0; i < mine[v]; ++i) {
+                    const int c = min(left, kTileRows * (groups[v] / mine[v] + (i < groups[v] % mine[v])));
+                    f(Tile{tid * 2 + v, from, c, 0}, (c - 1) / kTileRows);
+                    from += c;
+                    left -= c;
+                }
             }
+        };
+        each([&](const Tile &, int size) { atomicAdd(&sizes[size], 1); });
+        __syncthreads();
+        if (tid == 0) {
+            int at = 0;
+            for (int k = kTileGroups - 1; k >= 0; --k) {
+                const int c = sizes[k];
+                sizes[k] = at;
+                at += c;
+            }
+            tiles[0] = {min(at, most), 0, 0, 0};
         }
-        if (tid == 255) tiles[0] = {min(ends[255], most), 0, 0, 0};
+        __syncthreads();
+        // (equal sizes in any order: no tile's result depends on its place; runs that overlap could ask for more than `most`)
+        each([&](const Tile &t, int size) {
+            const int at = atomicAdd(&sizes[size], 1);
+            if (at < most) tiles[1 + at] = t;
+        });
         return;
     }
     if ((int)blockIdx.x >= rows_wgs) {
@@ -145,19 +157,18 @@ __global__ __launch_bounds__(256) void moe_pack_kernel(ExpertArgs a, int rows, i
 
 // ---- the products -----------------------------------------------------------------
 
-// The eight halves q - 8 of a Q4_0 word, in the order of an activation group.  A nibble put under the exponent of 1024
-// is 1024 + q (the high one 1024 + 16 q).  k1024: 0x64006400 in a register of the caller's (a second literal would keep the
-// and from being one instruction with the or).
-__device__ __forceinline__ half8v nibbles(uint32_t w, uint32_t k1024)
+// Halves 2 PART and 2 PART + 1 of the eight q - 8 of a Q4_0 word, in the order of an activation group.  A nibble put under
+// the exponent of 1024 is 1024 + q (the high one 1024 + 16 q).  k1024: 0x64006400 in a register of the caller's (a second
+// literal would keep the and from being one instruction with the or).
+template <int PART>
+__device__ __forceinline__ uint32_t nibble_pair(uint32_t w, uint32_t k1024)
 {
     const half2v low = {(_Float16)1032.0f, (_Float16)1032.0f}, by = {(_Float16)0.0625f, (_Float16)0.0625f},
                  high = {(_Float16)-72.0f, (_Float16)-72.0f};
-    auto as_half = [](uint32_t x) { return __builtin_bit_cast(half2v, x); };
-    const uint32_t v = w >> 8;
-    const half2v a = as_half((w & 0x000F000Fu) | k1024) - low, b = as_half((v & 0x000F000Fu) | k1024) - low;
-    const half2v c = __builtin_elementwise_fma(as_half((w & 0x00F000F0u) | k1024), by, high);
-    const half2v d = __builtin_elementwise_fma(as_half((v & 0x00F000F0u) | k1024), by, high);
-    return {a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+    const uint32_t v = PART & 1 ? w >> 8 : w;
+    const half2v h = PART < 2 ? __builtin_bit_cast(half2v, (v & 0x000F000Fu) | k1024) - low
+                              : __builtin_elementwise_fma(__builtin_bit_cast(half2v, (v & 0x00F000F0u) | k1024), by, high);
+    return __builtin_bit_cast(uint32_t, h);
 }
 
 // Words w[i] of lane row g (16 lanes) become words w[g] of lane row i: every lane gets its own part of one block after
@@ -224,7 +235,6 @@ __device__ __forceinline__ void loads_barrier()
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
 
-constexpr int kTileGroups = 6;                 // token groups of 16 a tile at most
 constexpr int kHalf = kChunk / 2;              // blocks of activations in each of two buffers
 constexpr int kTilePart = kHalf * kTileGroups * 2048;  // bytes of a buffer: [block][token group][row / 8] 1 KB each
 
@@ -232,21 +242,27 @@ constexpr int kTilePart = kHalf * kTileGroups * 2048;  // bytes of a buffer: [bl
 // activations row i of each token group.  A block of a row of activations is one line of 128 bytes; 1 KB has eight rows,
 // whose pieces p lie at p ^ row, so that the 16-byte reads of 16 rows meet all banks.  Two blocks of all groups go to one
 // buffer while the two in the other are multiplied; a step's weights are on their way for two of those.
-template <bool DOWN, int NT>
+//
+// An MFMA keeps its unit for 16 cycles, of which the wave can fill 12 with VALU instructions: the order is written out, a
+// product of one token group beside the additions of the last one and a part of the next block's halves.  (Left to the
+// compiler the two were one after the other for the most part, 281 us for 1501 tokens.)  ODD: the blocks in a row are odd
+// in number, and its scales are read one by one.
+// (pin: a value is formed in its place, which sched_barrier alone does not see to.)
+template <class T>
+__device__ __forceinline__ void pin(T &x)
+{
+    asm volatile("" : "+v"(x));
+}
+
+template <bool DOWN, bool ODD, int NT>
 __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &tile, int chunk_rows, const uint8_t *xp,
                                              uint8_t *lds, const int *s_as, const float *s_scale)
 {
+    constexpr int kLoadsW = kGroups * (1 + (ODD ? 4 : 2));
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
     const int nb = a.cols / 32, r0 = chunk_rows + wave * wave_rows<DOWN>();
-    const size_t all = (size_t)a.n_experts * a.rows * nb * 16, base = (size_t)tile.expert * a.rows;
-    const uint8_t *wq[kGroups], *ws[kGroups];
-#pragma unroll
-    for (int q = 0; q < kGroups; ++q) {
-        const int r = min(r0 + (DOWN ? q : q & 1) * 16 + i, a.rows - 1);
-        const uint8_t *w = a.w[DOWN ? 0 : q >> 1];
-        wq[q] = w + (base + r) * nb * 16;
-        ws[q] = w + all + (base + r) * nb * 2;
-    }
+    // the expert's matrices, 32-bit offsets within one
+    const size_t first_block = (size_t)tile.expert * a.rows * nb, blocks = (size_t)a.n_experts * a.rows * nb;
     // this wave's share of a buffer: block wave & 1, rows 8 (wave / 2) .. + 8 of every group
     const uint8_t *xrow[NT];
 #pragma unroll
@@ -261,14 +277,26 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
 #pragma unroll
         for (int t = 0; t < NT; ++t) load_to_lds(xrow[t] + b, __builtin_amdgcn_readfirstlane(put + half * kTilePart + t * 2048));
     };
+    uint32_t row_at[kGroups];
+#pragma unroll
+    for (int q = 0; q < kGroups; ++q) row_at[q] = (uint32_t)min(r0 + (DOWN ? q : q & 1) * 16 + i, a.rows - 1) * nb;
     uint4 wv[kGroups];
-    uint32_t sv[kGroups];
-    auto load_w = [&](int c) {
-        const int b = min(c * kChunk + g, nb - 1);
+    uint2 sv[kGroups];
+    auto load_w = [&](int c) {  // kLoadsW loads
+        const uint32_t b = min(c * kChunk + g, nb - 1);
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) {
-            wv[q] = *reinterpret_cast<const uint4 *>(wq[q] + (size_t)b * 16);
-            sv[q] = *reinterpret_cast<const uint16_t *>(ws[q] + (size_t)b * 2);
+            const uint8_t *w = a.w[DOWN ? 0 : q >> 1] + first_block * 16, *ws = a.w[DOWN ? 0 : q >> 1] + blocks * 16 + first_block * 2;
+            uint32_t at_row = row_at[q];
+            asm volatile("" : "+v"(at_row));  // addresses are formed here: kept over the loop they cost 16 registers
+            wv[q] = *reinterpret_cast<const uint4 *>(w + (at_row + b) * 16ull);
+            auto two = [&](int at) {
+                if (!ODD) return *reinterpret_cast<const uint32_t *>(ws + (at_row + min(at, nb - 2)) * 2ull);
+                const uint32_t lo = *reinterpret_cast<const uint16_t *>(ws + (at_row + min(at, nb - 1)) * 2ull);
+                const uint32_t hi = *reinterpret_cast<const uint16_t *>(ws + (at_row + min(at + 1, nb - 1)) * 2ull);
+                return lo | (at + 1 < nb ? hi << 16 : 0u);  // the block behind the last counts nothing
+            };
+            sv[q] = make_uint2(two(c * kChunk), two(c * kChunk + 2));
         }
     };
     float4v acc[kGroups][NT];
@@ -284,7 +312,8 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
     load_w(0);
     load_x(0, 0);
     for (int c = 0; c < chunks; ++c) {
-        uint32_t w[kGroups][4], s[kGroups][4];
+        uint32_t w[kGroups][4];
+        half4v d[kGroups];
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) {
             w[q][0] = wv[q].x;
@@ -292,49 +321,84 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
             w[q][2] = wv[q].z;
             w[q][3] = wv[q].w;
             turn(w[q][0], w[q][1], w[q][2], w[q][3]);
-            spread(sv[q], s[q]);
+            d[q] = __builtin_bit_cast(half4v, sv[q]);
             // done before the barrier: a wait for these weights behind it would be one for the loads issued there too
-#pragma unroll
-            for (int j = 0; j < kChunk; ++j) asm volatile("" : "+v"(w[q][j]), "+v"(s[q][j]));
+            asm volatile("" : "+v"(w[q][0]), "+v"(w[q][1]), "+v"(w[q][2]), "+v"(w[q][3]), "+v"(d[q]));
         }
+        uint4v wh[kGroups];
+        uint32_t part[kGroups][4];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             // the buffer's loads: before the first half nothing was issued after them, before the second the weights
             if (half == 0) loads_barrier<0>();
-            else loads_barrier<2 * kGroups>();  // it is whole, and everyone is through with the other one
+            else loads_barrier<kLoadsW>();  // it is whole, and everyone is through with the other one
             if (half == 0) {
                 load_x(c, 1);
                 load_w(min(c + 1, chunks - 1));  // always, for the count above
             } else if (c + 1 < chunks) {
                 load_x(c + 1, 0);
             }
+            if (c * kChunk + half * kHalf >= nb) break;
+            half8v x[2][2];
+            float4v p[2][kGroups];
+            auto read = [&](int to, int step) {
+                const int at = half * kTilePart + (step / NT * kTileGroups + step % NT) * 2048;
+                x[to][0] = *reinterpret_cast<const half8v *>(hi_at + at);
+                x[to][1] = *reinterpret_cast<const half8v *>(lo_at + at);
+            };
+            auto add = [&](int from, int q, int step) {
+                const float dw = (float)d[q][half * kHalf + step / NT];
 #pragma unroll
-            for (int jj = 0; jj < kHalf; ++jj) {
-                const int j = half * kHalf + jj;
-                if (c * kChunk + j >= nb) break;
-                half8v wh[kGroups];
-                float d[kGroups];
+                for (int v = 0; v < 4; ++v)
+                    acc[q][step % NT][v] = __builtin_fmaf(p[from][q][v], dw, acc[q][step % NT][v]);
+            };
+            read(0, 0);
+            if (half == 0)
 #pragma unroll
                 for (int q = 0; q < kGroups; ++q) {
-                    wh[q] = nibbles(w[q][j], k1024);
-                    d[q] = f16_bits_to_f32(s[q][j]);
+                    wh[q].x = nibble_pair<0>(w[q][0], k1024);
+                    wh[q].y = nibble_pair<1>(w[q][0], k1024);
+                    wh[q].z = nibble_pair<2>(w[q][0], k1024);
+                    wh[q].w = nibble_pair<3>(w[q][0], k1024);
                 }
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const int at = half * kTilePart + (jj * kTileGroups + t) * 2048;
-                    const half8v hi = *reinterpret_cast<const half8v *>(hi_at + at), lo = *reinterpret_cast<const half8v *>(lo_at + at);
-                    float4v p[kGroups];
+            for (int step = 0; step < kHalf * NT; ++step) {  // block step / NT, token group step % NT
+                const int now = step & 1, t = step % NT, j = half * kHalf + step / NT;
+                if (step + 1 < kHalf * NT) read(now ^ 1, step + 1);
+                auto weights = [&](int q) { return __builtin_bit_cast(half8v, wh[q]); };
 #pragma unroll
-                    for (int q = 0; q < kGroups; ++q)
-                        p[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, wh[q], float4v{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-#pragma unroll
-                    for (int q = 0; q < kGroups; ++q) p[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, wh[q], p[q], 0, 0, 0);
-#pragma unroll
-                    for (int q = 0; q < kGroups; ++q)
-#pragma unroll
-                        for (int v = 0; v < 4; ++v) acc[q][t][v] = __builtin_fmaf(p[q][v], d[q], acc[q][t][v]);
+                for (int q = 0; q < kGroups; ++q) {
+                    p[now][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[now][0], weights(q), float4v{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+                    if (step > 0) {
+                        add(now ^ 1, q, step - 1);
+                        pin(acc[q][(step - 1) % NT]);
+                    }
+                    pin(p[now][q]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+#pragma unroll
+                for (int q = 0; q < kGroups; ++q) {
+                    p[now][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[now][1], weights(q), p[now][q], 0, 0, 0);
+                    if (j + 1 < kChunk)
+#pragma unroll
+                        for (int n = t * kGroups / NT; n < (t + 1) * kGroups / NT; ++n) {
+                            if (q == 0) part[n][0] = nibble_pair<0>(w[n][j + 1], k1024);
+                            if (q == 1) part[n][1] = nibble_pair<1>(w[n][j + 1], k1024);
+                            if (q == 2) part[n][2] = nibble_pair<2>(w[n][j + 1], k1024);
+                            if (q == 3) part[n][3] = nibble_pair<3>(w[n][j + 1], k1024);
+                        }
+                    if (j + 1 < kChunk)
+#pragma unroll
+                        for (int n = t * kGroups / NT; n < (t + 1) * kGroups / NT; ++n) pin(part[n][q]);
+                    pin(p[now][q]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (t == NT - 1 && j + 1 < kChunk)
+#pragma unroll
+                    for (int q = 0; q < kGroups; ++q) wh[q] = uint4v{part[q][0], part[q][1], part[q][2], part[q][3]};
             }
+#pragma unroll
+            for (int q = 0; q < kGroups; ++q) add((kHalf * NT - 1) & 1, q, kHalf * NT - 1);
         }
     }
     // outputs: token row 4g + v of each group, weight row i
@@ -359,7 +423,7 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
         }
 }
 
-template <bool DOWN>
+template <bool DOWN, bool ODD>
 __global__ __launch_bounds__(64 * kWaves, 2) void moe_tile_kernel(ExpertArgs a, const Tile *__restrict__ tiles,
                                                                   const uint8_t *__restrict__ xp,
                                                                   const float *__restrict__ xscale, int row_wgs)
@@ -367,12 +431,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_tile_kernel(ExpertArgs a, 
     __shared__ __align__(16) uint8_t lds[2 * kTilePart];
     __shared__ int s_as[kTileGroups * 16];
     __shared__ float s_scale[kTileGroups * 16];
-    // workgroups go to the eight XCDs in turn; each XCD gets a run of the list, so that an expert's weights and a tile's
-    // activations meet in one L2
-    const int total = tiles[0].expert * row_wgs, per = (total + 7) / 8;
-    const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
-    const int at = id / row_wgs;
+    // Workgroups go to the eight XCDs in turn.  All of a tile go to one, whose L2 then has its activations; the list is by
+    // size, the largest first, and dealt back and forth.
+    const int xcd = blockIdx.x & 7, turn = (blockIdx.x >> 3) / row_wgs, at = turn * 8 + (turn & 1 ? 7 - xcd : xcd);
+    if (at >= tiles[0].expert) return;
     const Tile tile = tiles[1 + at];
     const int n = a.batch * a.k;
     if (threadIdx.x < kTileGroups * 16) {
@@ -383,14 +445,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_tile_kernel(ExpertArgs a, 
         s_scale[threadIdx.x] = ok ? xscale[DOWN ? o : o / a.k] * (DOWN ? a.weights[o] : 1.0f) : 0.0f;
     }
     __syncthreads();
-    const int chunk_rows = (id - at * row_wgs) * kWaves * wave_rows<DOWN>();
+    const int chunk_rows = ((blockIdx.x >> 3) - turn * row_wgs) * kWaves * wave_rows<DOWN>();
     switch ((tile.count + 15) / 16) {
-    case 1: tile_product<DOWN, 1>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
-    case 2: tile_product<DOWN, 2>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
-    case 3: tile_product<DOWN, 3>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
-    case 4: tile_product<DOWN, 4>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
-    case 5: tile_product<DOWN, 5>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
-    default: tile_product<DOWN, 6>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
+    case 1: tile_product<DOWN, ODD, 1>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
+    case 2: tile_product<DOWN, ODD, 2>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
+    case 3: tile_product<DOWN, ODD, 3>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
+    default: tile_product<DOWN, ODD, 4>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
     }
 }
 
@@ -919,11 +979,15 @@ template <bool DOWN>
 int launch_tiles(mrml_hip_ctx *ctx, const ExpertArgs &a, int most, const Tile *tiles, const uint8_t *xp, const float *xscale)
 {
     const int row_wgs = (a.rows + kWaves * wave_rows<DOWN>() - 1) / (kWaves * wave_rows<DOWN>());
-    const int64_t grid = ((int64_t)most * row_wgs + 7) / 8 * 8;
+    const int64_t grid = (int64_t)(most + 7) / 8 * 8 * row_wgs;
     REQUIRE(ctx, grid <= INT32_MAX, "moe: batch * k = %d assignments of %d rows are too many for one call", a.batch * a.k,
             a.rows);
-    hipLaunchKernelGGL((moe_tile_kernel<DOWN>), dim3((uint32_t)grid), dim3(64 * kWaves), 0, ctx->stream, a, tiles, xp, xscale,
-                       row_wgs);
+    if (a.cols / 32 % 2)
+        hipLaunchKernelGGL((moe_tile_kernel<DOWN, true>), dim3((uint32_t)grid), dim3(64 * kWaves), 0, ctx->stream, a, tiles, xp,
+                           xscale, row_wgs);
+    else
+        hipLaunchKernelGGL((moe_tile_kernel<DOWN, false>), dim3((uint32_t)grid), dim3(64 * kWaves), 0, ctx->stream, a, tiles, xp,
+                           xscale, row_wgs);
     return check_launch(ctx, "moe_tile_kernel");
 }
 
@@ -984,7 +1048,7 @@ int launch_combine(mrml_hip_ctx *ctx, const ExpertArgs &a, const float *part)
 template <bool DOWN>
 int launch_product(mrml_hip_ctx *ctx, const ExpertArgs &a)
 {
-    const int nt = kTileGroups, most = max_tiles(a, nt), nb = a.cols / 32, n = a.batch * a.k, rows = DOWN ? n : a.batch;
+    const int most = max_tiles(a), nb = a.cols / 32, n = a.batch * a.k, rows = DOWN ? n : a.batch;
     const size_t list = align_up((size_t)(1 + most) * sizeof(Tile), 256), scales = align_up((size_t)rows * 4, 256);
     const size_t packed = (size_t)rows * nb * kXBlock, part = DOWN ? (size_t)n * a.rows * 4 : 0;
     uint8_t *ws = (uint8_t *)workspace(ctx, list + scales + packed + part);
@@ -995,10 +1059,10 @@ int launch_product(mrml_hip_ctx *ctx, const ExpertArgs &a)
     const int rows_wgs = (rows + 3) / 4, grid = rows_wgs + (n + 255) / 256 + 1;
     if (a.xpack)
         hipLaunchKernelGGL(moe_pack_kernel<true>, dim3(grid), dim3(256), 0, ctx->stream, a, rows, rows_wgs, xp, xscale,
-                           tiles, nt, most);
+                           tiles, most);
     else
         hipLaunchKernelGGL(moe_pack_kernel<false>, dim3(grid), dim3(256), 0, ctx->stream, a, rows, rows_wgs, xp, xscale,
-                           tiles, nt, most);
+                           tiles, most);
     if (int rc = check_launch(ctx, "moe_pack_kernel")) return rc;
     ExpertArgs p = a;
     if (DOWN) p.out = (float *)(xp + packed);
