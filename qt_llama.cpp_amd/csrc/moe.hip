@@ -12,13 +12,40 @@ namespace mrml {
 
 namespace {
 
+using f32x4 = float __attribute__((ext_vector_type(4)));
+
+constexpr int kOneRoute = 16;  // tokens that one workgroup routes and plans
+
 // ---- residual and norm -----------------------------------------------------------
 
+// v of the lane that a DPP control names, as two words; 0 where it names none or ROWS leaves the row out.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double dpp_f64(double v)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+__device__ __forceinline__ double lane_f64(double v, int lane)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, lane);
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// Sum over the wave, in a fixed order: within rows of 16 lanes, then rows 0 and 1, 2 and 3, then both halves.
 __device__ __forceinline__ double wave_sum_f64(double v)
 {
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
+    v += dpp_f64<0xB1>(v);        // quad_perm 1,0,3,2
+    v += dpp_f64<0x4E>(v);        // quad_perm 2,3,0,1
+    v += dpp_f64<0x124>(v);       // row_ror:4
+    v += dpp_f64<0x128>(v);       // row_ror:8
+    v += dpp_f64<0x142, 0xa>(v);  // row_bcast:15
+    v += dpp_f64<0x143, 0xc>(v);  // row_bcast:31
+    return lane_f64(v, 63);
 }
 
 // Sum over the workgroup; red: a double a wave, free again after the next barrier.
@@ -38,14 +65,14 @@ __device__ __forceinline__ double sq_f64(float4 a)
 }
 
 // One workgroup a row, CH float4 a thread.
-template <int CH>
-__global__ __launch_bounds__(256) void residual_norm_rows_kernel(const float *t, const float *__restrict__ w_post,
+template <int CH, int THREADS>
+__global__ __launch_bounds__(THREADS) void residual_norm_rows_kernel(const float *t, const float *__restrict__ w_post,
                                                                  const float *h, float *h_out,
                                                                  const float *__restrict__ w_next, float *xn,
                                                                  uint8_t *__restrict__ pack, int dim, float eps,
                                                                  int norm_t)
 {
-    __shared__ double red[2][4];
+    __shared__ double red[2][THREADS / 64];
     const int n4 = dim >> 2, nb = dim >> 5;
     const size_t row = blockIdx.x, at = row * n4;
     const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -103,7 +130,7 @@ __global__ __launch_bounds__(256) void residual_norm_rows_kernel(const float *t,
 
 // ---- the router's product ----------------------------------------------------------
 
-// One wave a token and expert.
+// For a few tokens: one wave a token and expert.
 __global__ __launch_bounds__(256) void moe_logits_kernel(const float *__restrict__ x, const float *__restrict__ w,
                                                          float *__restrict__ logits, int n_experts, int cols, int batch)
 {
@@ -120,150 +147,343 @@ __global__ __launch_bounds__(256) void moe_logits_kernel(const float *__restrict
     if (lane == 0) logits[(size_t)blockIdx.x * n_experts + e] = s;
 }
 
-// ---- the route -----------------------------------------------------------------------
-
-// Whether (a, i) comes before (b, j): larger first, equal ones by index.
-__device__ __forceinline__ bool before(double a, int i, double b, int j) { return a > b || (a == b && i < j); }
-
-// One wave a token; lane l holds the experts l, l + 64, ...
-template <int V>
-__global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a)
+// For more: a workgroup makes T * 16 tokens by T * 16 experts on f32 MFMA, its eight waves every eighth block of 32
+// columns each, and adds the eight partial products.  The lanes of an operand's row are 16 or 32 apart, so that next lanes
+// hold other rows, and a load of that form fetches 16 bytes a clock (51 us for the case below).  Whole lines of 8 rows an
+// instruction therefore go through LDS, each wave through a part of its own (no barrier), 16-byte column c of row r at
+// c ^ r % 8 so that the rows of a read lie in different banks.  A lane reads 16 bytes: component j of a row's lanes are
+// the columns that MFMA j takes, of x and w alike.
+// 1999 tokens, 128 experts of 2816 columns: 17.6 us (one wave a token and expert: 173), against 9.2 that f32 MFMA takes
+// for them and 4.7 for the bytes; the loads' way through L1 and LDS, about as long again, hides behind the MFMA only in part.
+// T = 2 reads half as much a product; T = 1 fills the chip with fewer tokens.  128 experts, T = 1 / 2: 64 tokens 6.5 / 16.7
+// us, 512 7.9 / 17.5, 1024 12.5 / 18.0, 1999 22.4 / 19.5.
+template <int T>
+__global__ __launch_bounds__(512) void moe_logits_tile_kernel(const float *__restrict__ x, const float *__restrict__ w,
+                                                              float *__restrict__ logits, int n_experts, int cols,
+                                                              int batch)
 {
-    __shared__ double values[4][V * 64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t = blockIdx.x * 4 + wave;
-    if (t >= a.batch) return;  // no barrier below: the values are a wave's own
-    const double off = -INFINITY;
-    const float *x = a.logits + (size_t)t * a.n_experts;
-    double l[V], score[V], value[V];
-    bool on[V];
-    double top = off;
+    constexpr int S = T * 16, K = 64 / S, W = 8;  // rows, lanes a row, waves
+    using Acc = float __attribute__((ext_vector_type(S * S / 64)));
+    union Shared {
+        f32x4 lines[W][2 * S * 8];
+        float part[W][S][S + 1];
+    };
+    __shared__ Shared sh;
+    // the tiles of one group of tokens on one XCD (workgroups go to the eight in turn), whose L2 then reads them once
+    const int across = (n_experts + S - 1) / S, id = blockIdx.x / 8;
+    const int t0 = (id / across * 8 + blockIdx.x % 8) * S, e0 = id % across * S;
+    if (t0 >= batch) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int m = lane % S, g = lane / S, row = lane >> 3, chunks = cols / 32, n = (chunks - wave + W - 1) / W;
+    const float *p[4 * T];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const int e = v * 64 + lane;
-        l[v] = e < a.n_experts ? (double)x[e] : off;
-        on[v] = l[v] > off;
-        if (on[v]) top = fmax(top, l[v]);
+    for (int i = 0; i < 2 * T; ++i) {  // rows behind the last one read that one; their results are not stored
+        p[i] = x + (size_t)min(t0 + i * 8 + row, batch - 1) * cols + (lane & 7) * 4;
+        p[2 * T + i] = w + (size_t)min(e0 + i * 8 + row, n_experts - 1) * cols + (lane & 7) * 4;
     }
-    if (a.scoring == MRML_HIP_MOE_SOFTMAX) {
-        for (int m = 32; m >= 1; m >>= 1) top = fmax(top, __shfl_xor(top, m, 64));
-        double s = 0.0;
+    f32x4 *mine = sh.lines[wave];
+    f32x4 next[2][4 * T];
+    auto load = [&](f32x4 (&v)[4 * T], int i) {
+        const int at = min(wave + i * W, chunks - 1) * 32;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            score[v] = !on[v] ? 0.0 : l[v] == top ? 1.0 : exp(l[v] - top);
-            s += score[v];
-        }
-        s = wave_sum_f64(s);
+        for (int r = 0; r < 4 * T; ++r) v[r] = *reinterpret_cast<const f32x4 *>(p[r] + at);
+        __builtin_amdgcn_sched_barrier(0);  // loads stay in this order, so that a wait leaves the later ones out
+    };
+    Acc acc[2] = {};
+    auto product = [&](const f32x4 (&v)[4 * T]) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) score[v] /= s;
-    } else {
+        for (int r = 0; r < 4 * T; ++r) mine[r * 64 + row * 8 + ((lane ^ row) & 7)] = v[r];
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int v = 0; v < V; ++v) score[v] = on[v] ? 1.0 / (1.0 + exp(-l[v])) : 0.0;
-    }
-    const bool by_score = a.bias || (a.group_best == 2 && a.n_groups > 1);
+        for (int i = 0; i < 2 * T; ++i) {
+            const f32x4 a = mine[m * 8 + ((i * K + g) ^ (m & 7))], b = mine[(S + m) * 8 + ((i * K + g) ^ (m & 7))];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const int e = v * 64 + lane;
-        value[v] = by_score ? score[v] + (a.bias && e < a.n_experts ? (double)a.bias[e] : 0.0) : l[v];
-        if (!on[v] || !(value[v] > off)) value[v] = off;
-    }
-    if (a.n_groups > 1) {
-        const int size = a.n_experts / a.n_groups;
-        double *mine = values[wave];
-#pragma unroll
-        for (int v = 0; v < V; ++v) mine[v * 64 + lane] = value[v];
-        double b1 = off, b2 = off;
-        if (lane < a.n_groups)
-            for (int i = 0; i < size; ++i) {
-                const double y = mine[lane * size + i];
-                if (y > b1) {
-                    b2 = b1;
-                    b1 = y;
-                } else if (y > b2) {
-                    b2 = y;
-                }
-            }
-        const double rank = a.group_best == 2 && b2 > off ? b1 + b2 : b1;
-        int ahead = 0;
-        for (int g = 0; g < a.n_groups; ++g) ahead += before(__shfl(rank, g, 64), g, rank, lane);
-        const uint64_t kept = __ballot(lane < a.n_groups && ahead < a.top_groups);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int e = v * 64 + lane;
-            if (e < a.n_experts && !((kept >> (e / size)) & 1)) value[v] = off;
-        }
-    }
-    int id = -1;  // of slot `lane`
-    double got = 0.0;
-    for (int s = 0; s < a.k; ++s) {
-        double best = off, sc = 0.0;
-        int e = 1 << 30;
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-            if (value[v] > best) {
-                best = value[v];
-                e = v * 64 + lane;
-                sc = score[v];
-            }
-        for (int m = 32; m >= 1; m >>= 1) {
-            const double b = __shfl_xor(best, m, 64), o = __shfl_xor(sc, m, 64);
-            const int i = __shfl_xor(e, m, 64);
-            if (before(b, i, best, e)) {
-                best = b;
-                e = i;
-                sc = o;
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (T == 2) acc[j & 1] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], acc[j & 1], 0, 0, 0);
+                else acc[j & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], acc[j & 1], 0, 0, 0);
             }
         }
-        if (!(best > off)) break;
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-            if (v * 64 + lane == e) value[v] = off;
-        if (lane == s) {
-            id = e;
-            got = sc;
-        }
+        __builtin_amdgcn_wave_barrier();
+    };
+    load(next[0], 0);
+    for (int i = 0; i + 1 < n; i += 2) {
+        load(next[1], i + 1);
+        product(next[0]);
+        load(next[0], i + 2);
+        product(next[1]);
     }
-    const double total = wave_sum_f64(got);
-    if (lane < a.k) {
-        if (a.renormalise) got = total > 0.0 ? got / total : 0.0;
-        a.ids[(size_t)t * a.k + lane] = id;
-        a.weights[(size_t)t * a.k + lane] = (float)(got * (double)a.scale);
+    if (n & 1) product(next[0]);
+    acc[0] += acc[1];
+    __syncthreads();  // the parts lie where the lines did
+#pragma unroll
+    for (int r = 0; r < T * T * 4; ++r) sh.part[wave][r / 4 * 8 + g * 4 + r % 4][m] = acc[0][r];
+    __syncthreads();
+    for (int i = threadIdx.x; i < S * S; i += W * 64) {
+        const int t = i / S, e = i % S;
+        float s = sh.part[0][t][e];
+#pragma unroll
+        for (int v = 1; v < W; ++v) s += sh.part[v][t][e];
+        if (t0 + t < batch && e0 + e < n_experts) logits[(size_t)(t0 + t) * n_experts + e0 + e] = s;
     }
 }
 
-// The assignments of expert blockIdx.x in ascending order, behind those of the lower experts; the last workgroup writes
-// the end of the list.
-__global__ __launch_bounds__(256) void moe_plan_kernel(const int32_t *__restrict__ ids, int32_t *__restrict__ starts,
-                                                       int32_t *__restrict__ order, int n_experts, int n)
+// ---- the route -----------------------------------------------------------------------
+
+// A value as a number whose order is the values': 0 for one that cannot be chosen (switched off, not a number, the
+// lowest infinity), which no other value gives.  Both zeros give the same.
+__device__ __forceinline__ uint64_t sort_key(double v)
 {
-    __shared__ int red[2][4];
-    const int e = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    int lower = 0;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const int id = ids[i];
-        lower += id >= 0 && id < e;
+    if (!(v > -INFINITY)) return 0;
+    const uint64_t b = __builtin_bit_cast(uint64_t, v + 0.0);
+    return b >> 63 ? ~b : b | 1ull << 63;
+}
+
+__device__ __forceinline__ double key_value(uint64_t k)
+{
+    return k == 0 ? -INFINITY : __builtin_bit_cast(double, k >> 63 ? k & ~(1ull << 63) : ~k);
+}
+
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v)
+{
+    auto step = [](uint32_t a, int b) { return max(a, (uint32_t)b); };
+    v = step(v, dpp_mov<0xB1>((int)v));
+    v = step(v, dpp_mov<0x4E>((int)v));
+    v = step(v, dpp_mov<0x124>((int)v));
+    v = step(v, dpp_mov<0x128>((int)v));
+    v = step(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));
+    v = step(v, __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
+    return __builtin_amdgcn_readlane((int)v, 63);
+}
+
+// The lane that holds the largest key, of equal ones that with the lowest id; -1 if every key is 0.  Two keys seldom
+// agree in their upper halves, so one maximum over 32 bits mostly decides.
+__device__ __forceinline__ int wave_first(uint64_t key, int id)
+{
+    const uint32_t hi = wave_max_u32(key >> 32);
+    if (hi == 0) return -1;
+    uint64_t lanes = __ballot((uint32_t)(key >> 32) == hi);
+    if (lanes & (lanes - 1)) {
+        bool in = (uint32_t)(key >> 32) == hi;
+        const uint32_t lo = wave_max_u32(in ? (uint32_t)key : 0);
+        in = in && (uint32_t)key == lo;
+        const uint32_t first = wave_max_u32(in ? ~(uint32_t)id : 0);
+        lanes = __ballot(in && ~(uint32_t)id == first);
     }
-    for (int m = 32; m >= 1; m >>= 1) lower += __shfl_xor(lower, m, 64);
-    if (lane == 0) red[0][wave] = lower;
+    return __ffsll((unsigned long long)lanes) - 1;
+}
+
+// The plan of places [lo, hi) of n ids, by a workgroup of whole waves, at most 16: counts of every expert, before lo and
+// in all, give where its run goes on; then, blockDim.x ids at a time, a place is its run's end, the ids of the same
+// expert in lower waves and those in lower lanes.  Additions to the counters are whole numbers, so their order does not
+// matter.  The workgroup with lo = 0 writes the starts as well.
+struct PlanShared {
+    int count[2][kMaxExperts];          // of ids before lo, and from lo on; then count[0]: where the run goes on
+    int waves[16][kMaxExperts];         // of this wave in the present part
+    int sums[16];
+};
+
+__device__ __forceinline__ void plan_range(const int32_t *ids, int32_t *__restrict__ starts, int32_t *__restrict__ order,
+                                           int n_experts, int n, int lo, int hi, PlanShared &sh)
+{
+    const int threads = blockDim.x, wave = threadIdx.x >> 6, n_waves = threads >> 6, lane = threadIdx.x & 63;
+    for (int e = threadIdx.x; e < n_experts; e += threads) {
+        sh.count[0][e] = sh.count[1][e] = 0;
+        for (int w = 0; w < n_waves; ++w) sh.waves[w][e] = 0;
+    }
     __syncthreads();
-    int at = red[0][0] + red[0][1] + red[0][2] + red[0][3];
-    if (threadIdx.x == 0) starts[e] = at;
-    if (e == n_experts) {
-        for (int i = at + threadIdx.x; i < n; i += 256) order[i] = -1;
-        return;
+    for (int i0 = threadIdx.x; i0 < n; i0 += threads * 4) {
+        int id[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) id[u] = i0 + u * threads < n ? ids[i0 + u * threads] : -1;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (id[u] >= 0) atomicAdd(&sh.count[i0 + u * threads >= lo][id[u]], 1);
     }
-    for (int i0 = 0; i0 < n; i0 += 256) {
-        const int i = i0 + threadIdx.x;
-        const bool mine = i < n && ids[i] == e;
-        const uint64_t all = __ballot(mine);
-        __syncthreads();
-        if (lane == 0) red[1][wave] = __popcll(all);
-        __syncthreads();
-        int p = at;
-        for (int w = 0; w < 4; ++w) {
-            if (w < wave) p += red[1][w];
-            at += red[1][w];
+    __syncthreads();
+    int base = 0;  // the runs of a thread's experts, threads at a time
+    for (int e0 = 0; e0 < n_experts; e0 += threads) {
+        const int e = e0 + threadIdx.x, before = e < n_experts ? sh.count[0][e] : 0;
+        const int all = e < n_experts ? before + sh.count[1][e] : 0;
+        int upto = all;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int v = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += v;
         }
-        if (mine) order[p + __popcll(all & ((1ull << lane) - 1))] = i;
+        if (lane == 63) sh.sums[wave] = upto;
+        __syncthreads();
+        int start = base + upto - all;
+        for (int w = 0; w < n_waves; ++w) {
+            if (w < wave) start += sh.sums[w];
+            base += sh.sums[w];
+        }
+        if (e < n_experts) {
+            sh.count[0][e] = start + before;
+            if (lo == 0) starts[e] = start;
+        }
+        __syncthreads();
+    }
+    if (lo == 0 && threadIdx.x == 0) starts[n_experts] = base;
+    for (int i = max(lo, base) + threadIdx.x; i < hi; i += threads) order[i] = -1;
+    for (int i0 = lo; i0 < hi; i0 += threads) {
+        const int i = i0 + threadIdx.x, id = i < hi ? ids[i] : -1;
+        uint64_t same = __ballot(id >= 0);
+        for (int b = 0; (1 << b) < n_experts; ++b) {
+            const bool set = (id >> b) & 1;
+            const uint64_t with = __ballot(set);
+            same &= set ? with : ~with;
+        }
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        if (id >= 0 && rank == 0) sh.waves[wave][id] = __popcll(same);
+        __syncthreads();
+        for (int e = threadIdx.x; e < n_experts; e += threads) {
+            int at = sh.count[0][e];
+            for (int w = 0; w < n_waves; ++w) {
+                const int c = sh.waves[w][e];
+                sh.waves[w][e] = at;
+                at += c;
+            }
+            sh.count[0][e] = at;
+        }
+        __syncthreads();
+        if (id >= 0) order[sh.waves[wave][id] + rank] = i;
+        if (i0 + threads >= hi) break;
+        __syncthreads();
+        for (int e = threadIdx.x; e < n_experts; e += threads)
+            for (int w = 0; w < n_waves; ++w) sh.waves[w][e] = 0;
+        __syncthreads();
+    }
+}
+
+// A workgroup's ids from `per` of them on.
+__global__ __launch_bounds__(1024) void moe_plan_kernel(const int32_t *__restrict__ ids, int32_t *__restrict__ starts,
+                                                        int32_t *__restrict__ order, int n_experts, int n, int per)
+{
+    __shared__ PlanShared sh;
+    const int lo = blockIdx.x * per;
+    plan_range(ids, starts, order, n_experts, n, lo, min(lo + per, n), sh);
+}
+
+// One wave a token; lane l holds the experts l, l + 64, ...  Scores, values and their sums are f64, so that the choice
+// does not hang on how a score was rounded.  PLAN: the only workgroup, which goes on to the plan.
+template <int V, bool PLAN>
+__global__ __launch_bounds__(PLAN ? 1024 : 256) void moe_route_kernel(RouteArgs a)
+{
+    constexpr int kWaves = PLAN ? kOneRoute : 4;
+    struct Shared {
+        double values[kWaves][V * 64];
+        int32_t ids[PLAN ? kWaves * kMaxTopK : 1];
+    };
+    __shared__ Shared sh;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t = blockIdx.x * 4 + wave;
+    const double off = -INFINITY;
+    if (t < a.batch) {  // no barrier inside: the values are a wave's own
+        const float *x = a.logits + (size_t)t * a.n_experts;
+        double l[V], score[V];
+        float bias[V];
+        uint64_t key[V];
+        double top = off;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int e = v * 64 + lane;
+            l[v] = e < a.n_experts ? (double)x[e] : off;
+            bias[v] = a.bias && e < a.n_experts ? a.bias[e] : 0.0f;
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) top = l[v] > top ? l[v] : top;
+        if (a.scoring == MRML_HIP_MOE_SOFTMAX) {
+            // l are f32 values, so their maximum is one of 32 bits
+            const uint32_t b = __builtin_bit_cast(uint32_t, (float)top + 0.0f);
+            const uint32_t m = wave_max_u32(b >> 31 ? ~b : b | 1u << 31);
+            top = (double)__builtin_bit_cast(float, m >> 31 ? m & ~(1u << 31) : ~m);
+            double s = 0.0;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                score[v] = !(l[v] > off) ? 0.0 : l[v] == top ? 1.0 : exp(l[v] - top);
+                s += score[v];
+            }
+            s = wave_sum_f64(s);
+#pragma unroll
+            for (int v = 0; v < V; ++v) score[v] /= s;
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v) score[v] = l[v] > off ? 1.0 / (1.0 + exp(-l[v])) : 0.0;
+        }
+        const bool by_score = a.bias || (a.group_best == 2 && a.n_groups > 1);
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            key[v] = l[v] > off ? sort_key(by_score ? score[v] + (double)bias[v] : l[v]) : 0;
+        if (a.n_groups > 1) {
+            // as many lanes a group as there are, a power of two of them: each the two best of its share, then theirs
+            const int size = a.n_experts / a.n_groups, shift = 31 - __clz(64 / a.n_groups), g = lane >> shift;
+            double *mine = sh.values[wave];
+#pragma unroll
+            for (int v = 0; v < V; ++v) mine[v * 64 + lane] = key_value(key[v]);
+            __builtin_amdgcn_wave_barrier();
+            double b1 = off, b2 = off;
+            if (g < a.n_groups)
+                for (int i = lane & ((1 << shift) - 1); i < size; i += 1 << shift) {
+                    const double y = mine[g * size + i];
+                    b2 = y > b1 ? b1 : y > b2 ? y : b2;
+                    b1 = y > b1 ? y : b1;
+                }
+            for (int m = 1; m < 1 << shift; m *= 2) {
+                const double c1 = __shfl_xor(b1, m, 64), c2 = __shfl_xor(b2, m, 64);
+                const double low = c1 > b1 ? b1 : c1;
+                b1 = c1 > b1 ? c1 : b1;
+                b2 = c2 > b2 ? c2 : b2;
+                b2 = low > b2 ? low : b2;
+            }
+            const double rank = a.group_best == 2 && b2 > off ? b1 + b2 : b1;
+            int ahead = 0;  // groups before this one: larger first, equal ones by number
+            for (int o = 0; o < a.n_groups; ++o) {
+                const double r = lane_f64(rank, o << shift);
+                ahead += r > rank || (r == rank && o < g);
+            }
+            const uint64_t kept = __ballot(ahead < a.top_groups);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const int e = v * 64 + lane;
+                if (e < a.n_experts && !((kept >> ((e / size) << shift)) & 1)) key[v] = 0;
+            }
+        }
+        int id = -1;  // of slot `lane`
+        double got = 0.0;
+        for (int s = 0; s < a.k; ++s) {
+            uint64_t best = 0;
+            double sc = 0.0;
+            int e = 1 << 30;
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (key[v] > best) {
+                    best = key[v];
+                    e = v * 64 + lane;
+                    sc = score[v];
+                }
+            const int first = wave_first(best, e);
+            if (first < 0) break;
+            const int chosen = __builtin_amdgcn_readlane(e, first);
+            sc = lane_f64(sc, first);
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (v * 64 + lane == chosen) key[v] = 0;
+            if (lane == s) {
+                id = chosen;
+                got = sc;
+            }
+        }
+        const double total = wave_sum_f64(got);
+        if (lane < a.k) {
+            if (a.renormalise) got = total > 0.0 ? got / total : 0.0;
+            a.ids[(size_t)t * a.k + lane] = id;
+            a.weights[(size_t)t * a.k + lane] = (float)(got * (double)a.scale);
+            if constexpr (PLAN) sh.ids[t * a.k + lane] = id;
+        }
+    }
+    if constexpr (PLAN) {
+        __shared__ PlanShared plan;
+        __syncthreads();
+        plan_range(sh.ids, a.starts, a.order, a.n_experts, a.batch * a.k, 0, a.batch * a.k, plan);
     }
 }
 
@@ -272,16 +492,27 @@ __global__ __launch_bounds__(256) void moe_plan_kernel(const int32_t *__restrict
 int launch_residual_norm_rows(mrml_hip_ctx *ctx, const float *t, const float *w_post, const float *h, float *h_out,
                               const float *w_next, float *xn, void *pack, int dim, int batch, float eps, bool norm_t)
 {
-    const int chunks = (dim / 4 + 255) / 256;
-#define NORM_ROWS(CH)                                                                                               \
-    hipLaunchKernelGGL((residual_norm_rows_kernel<CH>), dim3(batch), dim3(256), 0, ctx->stream, t, w_post, h, h_out, \
-                       w_next, xn, (uint8_t *)pack, dim, eps, (int)norm_t)
-    if (chunks <= 1) NORM_ROWS(1);
-    else if (chunks <= 2) NORM_ROWS(2);
-    else if (chunks <= 3) NORM_ROWS(3);
-    else if (chunks <= 4) NORM_ROWS(4);
-    else if (chunks <= 8) NORM_ROWS(8);
-    else NORM_ROWS(12);
+#define NORM_ROWS(CH, THREADS)                                                                                    \
+    hipLaunchKernelGGL((residual_norm_rows_kernel<CH, THREADS>), dim3(batch), dim3(threads), 0, ctx->stream, t, w_post, \
+                       h, h_out, w_next, xn, (uint8_t *)pack, dim, eps, (int)norm_t)
+    const int n4 = dim / 4;
+    // a row a CU or fewer: as many threads as there are, which shortens the chain of a thread; more rows: 256, so that
+    // several rows overlap.  2816 values, up to 1024 / 256 threads: 1 row 4.6 / 5.4 us, 256 6.9 / 7.7, 512 10.1 / 10.6,
+    // 1024 15.3 / 14.4
+    if (batch <= 256) {
+        const int chunks = (n4 + 1023) / 1024, threads = ((n4 + chunks - 1) / chunks + 63) / 64 * 64;
+        if (chunks <= 1) NORM_ROWS(1, 1024);
+        else if (chunks <= 2) NORM_ROWS(2, 1024);
+        else NORM_ROWS(3, 1024);
+    } else {
+        const int chunks = (n4 + 255) / 256, threads = 256;
+        if (chunks <= 1) NORM_ROWS(1, 256);
+        else if (chunks <= 2) NORM_ROWS(2, 256);
+        else if (chunks <= 3) NORM_ROWS(3, 256);
+        else if (chunks <= 4) NORM_ROWS(4, 256);
+        else if (chunks <= 8) NORM_ROWS(8, 256);
+        else NORM_ROWS(12, 256);
+    }
 #undef NORM_ROWS
     return check_launch(ctx, "residual_norm_rows_kernel");
 }
@@ -289,22 +520,45 @@ int launch_residual_norm_rows(mrml_hip_ctx *ctx, const float *t, const float *w_
 int launch_moe_logits(mrml_hip_ctx *ctx, const float *x, const float *w, float *logits, int n_experts, int cols,
                       int batch)
 {
-    hipLaunchKernelGGL(moe_logits_kernel, dim3(batch, (n_experts + 3) / 4), dim3(256), 0, ctx->stream, x, w, logits,
-                       n_experts, cols, batch);
-    return check_launch(ctx, "moe_logits_kernel");
+    // 128 experts, one wave each / tiles: 16 tokens 5.7 / 6.2 us, 40 6.0 / 6.3, 64 8.8 / 6.5
+    if (batch <= 40) {
+        hipLaunchKernelGGL(moe_logits_kernel, dim3(batch, (n_experts + 3) / 4), dim3(256), 0, ctx->stream, x, w, logits,
+                           n_experts, cols, batch);
+        return check_launch(ctx, "moe_logits_kernel");
+    }
+    // a multiple of eight groups of tokens; the rest have none
+    auto tiles = [&](int s) { return ((batch + s - 1) / s + 7) / 8 * 8 * ((n_experts + s - 1) / s); };
+    const dim3 block(512);
+    if (tiles(16) <= 768)
+        hipLaunchKernelGGL(moe_logits_tile_kernel<1>, dim3(tiles(16)), block, 0, ctx->stream, x, w, logits, n_experts, cols,
+                           batch);
+    else
+        hipLaunchKernelGGL(moe_logits_tile_kernel<2>, dim3(tiles(32)), block, 0, ctx->stream, x, w, logits, n_experts, cols,
+                           batch);
+    return check_launch(ctx, "moe_logits_tile_kernel");
+}
+
+template <bool PLAN>
+static void launch_route(mrml_hip_ctx *ctx, const RouteArgs &a, dim3 grid, dim3 block)
+{
+    if (a.n_experts <= 64) hipLaunchKernelGGL((moe_route_kernel<1, PLAN>), grid, block, 0, ctx->stream, a);
+    else if (a.n_experts <= 128) hipLaunchKernelGGL((moe_route_kernel<2, PLAN>), grid, block, 0, ctx->stream, a);
+    else if (a.n_experts <= 256) hipLaunchKernelGGL((moe_route_kernel<4, PLAN>), grid, block, 0, ctx->stream, a);
+    else hipLaunchKernelGGL((moe_route_kernel<8, PLAN>), grid, block, 0, ctx->stream, a);
 }
 
 int launch_moe_route(mrml_hip_ctx *ctx, const RouteArgs &a)
 {
-    const dim3 grid((a.batch + 3) / 4), block(256);
-    if (a.n_experts <= 64) hipLaunchKernelGGL(moe_route_kernel<1>, grid, block, 0, ctx->stream, a);
-    else if (a.n_experts <= 128) hipLaunchKernelGGL(moe_route_kernel<2>, grid, block, 0, ctx->stream, a);
-    else if (a.n_experts <= 256) hipLaunchKernelGGL(moe_route_kernel<4>, grid, block, 0, ctx->stream, a);
-    else hipLaunchKernelGGL(moe_route_kernel<8>, grid, block, 0, ctx->stream, a);
+    if (a.starts && a.batch <= kOneRoute) {
+        launch_route<true>(ctx, a, dim3(1), dim3(64 * std::max(a.batch, 4)));
+        return check_launch(ctx, "moe_route_kernel");
+    }
+    launch_route<false>(ctx, a, dim3((a.batch + 3) / 4), dim3(256));
     if (int rc = check_launch(ctx, "moe_route_kernel")) return rc;
     if (!a.starts) return MRML_HIP_OK;
-    hipLaunchKernelGGL(moe_plan_kernel, dim3(a.n_experts + 1), block, 0, ctx->stream, a.ids, a.starts, a.order, a.n_experts,
-                       a.batch * a.k);
+    const int n = a.batch * a.k, per = ((n + 255) / 256 + 1023) / 1024 * 1024;
+    hipLaunchKernelGGL(moe_plan_kernel, dim3((n + per - 1) / per), dim3(1024), 0, ctx->stream, a.ids, a.starts, a.order,
+                       a.n_experts, n, per);
     return check_launch(ctx, "moe_plan_kernel");
 }
 
