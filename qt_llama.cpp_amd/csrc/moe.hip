@@ -278,25 +278,24 @@ __device__ __forceinline__ int wave_first(uint64_t key, int id)
 // matter.  The workgroup with lo = 0 writes the starts as well.
 struct PlanShared {
     int count[2][kMaxExperts];          // of ids before lo, and from lo on; then count[0]: where the run goes on
-    int waves[16][kMaxExperts];         // of this wave in the present part
+    int waves[16 * kMaxExperts];        // of a wave's ids of one expert in the present part
     int sums[16];
 };
 
 __device__ __forceinline__ void plan_range(const int32_t *ids, int32_t *__restrict__ starts, int32_t *__restrict__ order,
                                            int n_experts, int n, int lo, int hi, PlanShared &sh)
 {
+    constexpr int kAhead = 8;  // loads in flight
     const int threads = blockDim.x, wave = threadIdx.x >> 6, n_waves = threads >> 6, lane = threadIdx.x & 63;
-    for (int e = threadIdx.x; e < n_experts; e += threads) {
-        sh.count[0][e] = sh.count[1][e] = 0;
-        for (int w = 0; w < n_waves; ++w) sh.waves[w][e] = 0;
-    }
+    for (int e = threadIdx.x; e < n_experts; e += threads) sh.count[0][e] = sh.count[1][e] = 0;
+    for (int i = threadIdx.x; i < n_waves * n_experts; i += threads) sh.waves[i] = 0;
     __syncthreads();
-    for (int i0 = threadIdx.x; i0 < n; i0 += threads * 4) {
-        int id[4];
+    for (int i0 = threadIdx.x; i0 < n; i0 += threads * kAhead) {
+        int id[kAhead];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) id[u] = i0 + u * threads < n ? ids[i0 + u * threads] : -1;
+        for (int u = 0; u < kAhead; ++u) id[u] = i0 + u * threads < n ? ids[i0 + u * threads] : -1;
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < kAhead; ++u)
             if (id[u] >= 0) atomicAdd(&sh.count[i0 + u * threads >= lo][id[u]], 1);
     }
     __syncthreads();
@@ -334,23 +333,24 @@ __device__ __forceinline__ void plan_range(const int32_t *ids, int32_t *__restri
             same &= set ? with : ~with;
         }
         const int rank = __popcll(same & ((1ull << lane) - 1));
-        if (id >= 0 && rank == 0) sh.waves[wave][id] = __popcll(same);
+        if (id >= 0 && rank == 0) sh.waves[wave * n_experts + id] = __popcll(same);
         __syncthreads();
         for (int e = threadIdx.x; e < n_experts; e += threads) {
-            int at = sh.count[0][e];
-            for (int w = 0; w < n_waves; ++w) {
-                const int c = sh.waves[w][e];
-                sh.waves[w][e] = at;
-                at += c;
+            int c[16], at = sh.count[0][e];
+#pragma unroll
+            for (int w = 0; w < 16; ++w) c[w] = w < n_waves ? sh.waves[w * n_experts + e] : 0;
+#pragma unroll
+            for (int w = 0; w < 16; ++w) {
+                if (w < n_waves) sh.waves[w * n_experts + e] = at;
+                at += c[w];
             }
             sh.count[0][e] = at;
         }
         __syncthreads();
-        if (id >= 0) order[sh.waves[wave][id] + rank] = i;
+        if (id >= 0) order[sh.waves[wave * n_experts + id] + rank] = i;
         if (i0 + threads >= hi) break;
         __syncthreads();
-        for (int e = threadIdx.x; e < n_experts; e += threads)
-            for (int w = 0; w < n_waves; ++w) sh.waves[w][e] = 0;
+        for (int i = threadIdx.x; i < n_waves * n_experts; i += threads) sh.waves[i] = 0;
         __syncthreads();
     }
 }

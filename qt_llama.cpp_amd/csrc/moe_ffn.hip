@@ -45,14 +45,15 @@ int max_tiles(const ExpertArgs &a)
     return std::min(n, n / (kTileRows * kTileGroups) + std::min(a.n_experts, n));
 }
 
-// One wave a row (rows_wgs workgroups of four), then one thread an assignment that checks the plan, then one workgroup
-// that lists the tiles: tiles[0].expert of them behind tiles[0].
-template <bool PACKED>
-__global__ __launch_bounds__(256) void moe_pack_kernel(ExpertArgs a, int rows, int rows_wgs, uint8_t *__restrict__ xp,
+// One workgroup that lists the tiles: tiles[0].expert of them behind tiles[0]; then one thread an assignment that checks
+// the plan (check_wgs workgroups), then WAVES waves a row.  A row of f32 of up to WAVES * CH * 256 values is read once and
+// stays in registers; CH = 0 reads it twice.
+template <bool PACKED, int WAVES, int CH>
+__global__ __launch_bounds__(256) void moe_pack_kernel(ExpertArgs a, int rows, int check_wgs, uint8_t *__restrict__ xp,
                                                        float *__restrict__ xscale, Tile *__restrict__ tiles, int most)
 {
-    const int lane = threadIdx.x & 63, nb = a.cols / 32, n = a.batch * a.k;
-    if ((int)blockIdx.x == (int)gridDim.x - 1) {
+    const int nb = a.cols / 32, n = a.batch * a.k;
+    if (blockIdx.x == 0) {
         __shared__ int sizes[kTileGroups];
         const int tid = threadIdx.x;
         int groups[2], mine[2], first[2], count[2];
@@ -101,48 +102,50 @@ __global__ __launch_bounds__(256) void moe_pack_kernel(ExpertArgs a, int rows, i
         });
         return;
     }
-    if ((int)blockIdx.x >= rows_wgs) {
-        const int j = (blockIdx.x - rows_wgs) * 256 + threadIdx.x;
+    if ((int)blockIdx.x <= check_wgs) {
+        const int j = (blockIdx.x - 1) * 256 + threadIdx.x;
         if (j < n && !plan_ok(a, j)) moe_fault(a.faults);
         return;
     }
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
+    constexpr int T = WAVES * 64;  // threads a row
+    const int row = (blockIdx.x - 1 - check_wgs) * (256 / T) + threadIdx.x / T, tid = threadIdx.x % T;
+    if (row >= rows) return;  // (WAVES = 4: of the whole workgroup)
     const int n4 = a.cols / 4;
     const float4 *x = reinterpret_cast<const float4 *>(a.x + (size_t)row * a.cols);
     const size_t total = (size_t)rows * nb, b0 = (size_t)row * nb;
     const uint32_t *pq = reinterpret_cast<const uint32_t *>(a.xpack);
     const float *pd = reinterpret_cast<const float *>(a.xpack + total * 32);
     float top = 0.0f;
+    auto largest = [&](float4 v) {
+        top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+    };
+    float4 held[CH ? CH : 1];
     if (PACKED) {
-        for (int b = lane; b < nb; b += 64) top = fmaxf(top, pd[b0 + b]);
+        for (int b = tid; b < nb; b += T) top = fmaxf(top, pd[b0 + b]);
+    } else if (CH) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) held[i] = x[min(i * T + tid, n4 - 1)];
+#pragma unroll
+        for (int i = 0; i < CH; ++i) largest(held[i]);
     } else {
-        for (int c = lane; c < n4; c += 64) {
-            const float4 v = x[c];
-            top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-        }
+        for (int c = tid; c < n4; c += T) largest(x[c]);
     }
     for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+    if (WAVES > 1) {
+        __shared__ float tops[4];
+        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    }
     if (!PACKED) top = f16_bits_to_f32(f32_to_f16_trunc(top / 127.0f));
     // the largest scale becomes 2^7 .. 2^8, so that values stay below 2^15; infinity counts as the largest half
     const int exp = top > 0.0f ? (int)(__builtin_bit_cast(uint32_t, fminf(top, 65504.0f)) >> 23) - 127 - 7 : 0;
     const float down = __builtin_bit_cast(float, (uint32_t)(127 - exp) << 23);
-    if (lane == 0) xscale[row] = __builtin_bit_cast(float, (uint32_t)(127 + exp) << 23);
+    if (tid == 0) xscale[row] = __builtin_bit_cast(float, (uint32_t)(127 + exp) << 23);
     uint8_t *dst = xp + b0 * kXBlock;
-    for (int c0 = 0; c0 < n4; c0 += 64) {
-        const int c = c0 + lane, cc = c < n4 ? c : 0, l = c & 7;
-        uint32_t q;
-        float d;
-        if (PACKED) {
-            q = pq[b0 * 8 + cc];
-            d = pd[b0 + (cc >> 3)];
-        } else {
-            uint32_t dbits;
-            int sum;
-            q = q8_0_block8x4(x[cc], dbits, sum);
-            d = f16_bits_to_f32(dbits);
-        }
-        if (c >= n4) continue;
+    auto emit = [&](int c, uint32_t q, float d) {
+        if (c >= n4) return;
+        const int l = c & 7;
         d *= down;
         const float v0 = d * (float)(int8_t)q, v1 = d * (float)(int8_t)(q >> 16), v2 = d * (float)(int8_t)(q >> 8),
                     v3 = d * (float)(int8_t)(q >> 24);
@@ -152,6 +155,23 @@ __global__ __launch_bounds__(256) void moe_pack_kernel(ExpertArgs a, int rows, i
         uint8_t *p = dst + (size_t)(c >> 3) * kXBlock + (l & 3) * 16 + (l >> 2) * 8;
         *reinterpret_cast<half4v *>(p) = hi;
         *reinterpret_cast<half4v *>(p + 64) = lo;
+    };
+    auto quantised = [&](int c, float4 v) {
+        uint32_t dbits;
+        int sum;
+        const uint32_t q = q8_0_block8x4(v, dbits, sum);
+        emit(c, q, f16_bits_to_f32(dbits));
+    };
+    if (CH) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+            if (i * T < n4) quantised(i * T + tid, held[i]);
+    } else {
+        for (int c0 = 0; c0 < n4; c0 += T) {
+            const int c = c0 + tid, cc = min(c, n4 - 1);
+            if (PACKED) emit(c, pq[b0 * 8 + cc], pd[b0 + (cc >> 3)]);
+            else quantised(c, x[cc]);
+        }
     }
 }
 
@@ -1056,13 +1076,19 @@ int launch_product(mrml_hip_ctx *ctx, const ExpertArgs &a)
     Tile *tiles = (Tile *)ws;
     float *xscale = (float *)(ws + list);
     uint8_t *xp = ws + list + scales;
-    const int rows_wgs = (rows + 3) / 4, grid = rows_wgs + (n + 255) / 256 + 1;
-    if (a.xpack)
-        hipLaunchKernelGGL(moe_pack_kernel<true>, dim3(grid), dim3(256), 0, ctx->stream, a, rows, rows_wgs, xp, xscale,
-                           tiles, most);
-    else
-        hipLaunchKernelGGL(moe_pack_kernel<false>, dim3(grid), dim3(256), 0, ctx->stream, a, rows, rows_wgs, xp, xscale,
-                           tiles, most);
+    // more than 1024 values: four waves a row, so that few long rows fill the chip as well (1501 rows of 2816: 12 us, one
+    // wave a row 16)
+    const int check_wgs = (n + 255) / 256, waves = a.cols <= 1024 ? 1 : 4;
+    const dim3 grid(1 + check_wgs + (rows * waves + 3) / 4), block(256);
+#define PACK(...)                                                                                             \
+    hipLaunchKernelGGL((moe_pack_kernel<__VA_ARGS__>), grid, block, 0, ctx->stream, a, rows, check_wgs, xp, xscale, tiles, \
+                       most)
+    if (a.xpack && waves == 1) PACK(true, 1, 0);
+    else if (a.xpack) PACK(true, 4, 0);
+    else if (waves == 1) PACK(false, 1, 4);
+    else if (a.cols <= 4096) PACK(false, 4, 4);
+    else PACK(false, 4, 0);
+#undef PACK
     if (int rc = check_launch(ctx, "moe_pack_kernel")) return rc;
     ExpertArgs p = a;
     if (DOWN) p.out = (float *)(xp + packed);
