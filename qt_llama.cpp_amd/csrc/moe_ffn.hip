@@ -1032,8 +1032,14 @@ int launch_down_one(mrml_hip_ctx *ctx, const ExpertArgs &a)
     return check_launch(ctx, "moe_down_one_kernel");
 }
 
-// Few tokens an expert on average.
-bool streams(const ExpertArgs &a) { return a.batch * a.k <= 12 * a.n_experts && a.cols / 32 <= kStreamBlocks; }  // n * cols < 2^25
+// Few tokens an expert on average.  Streamed / in tiles, 128 experts of 704 x 2816, eight a token: gate and up 64 tokens 59 /
+// 110 us, 192 100 / 132, 384 152 / 157 (eight experts, two a token: 96 tokens 28 / 55); down 64 54 / 57, 128 68 / 68, 192
+// 77 / 71.
+template <bool DOWN>
+bool streams(const ExpertArgs &a)
+{
+    return a.batch * a.k <= (DOWN ? 8 : 24) * a.n_experts && a.cols / 32 <= kStreamBlocks;  // n * cols < 2^26
+}
 
 template <bool DOWN>
 int launch_stream(mrml_hip_ctx *ctx, const ExpertArgs &a)
@@ -1101,7 +1107,7 @@ int launch_product(mrml_hip_ctx *ctx, const ExpertArgs &a)
 int launch_moe_gate_up(mrml_hip_ctx *ctx, const ExpertArgs &a)
 {
     if (one_by_one(a)) return launch_gate_up_one(ctx, a);
-    if (!streams(a)) return launch_product<false>(ctx, a);
+    if (!streams<false>(a)) return launch_product<false>(ctx, a);
     ExpertArgs p = a;
     if (!p.xpack) {
         uint8_t *pack = (uint8_t *)workspace(ctx, act_pack_bytes((size_t)a.batch * (a.cols / 32)));
@@ -1115,7 +1121,7 @@ int launch_moe_gate_up(mrml_hip_ctx *ctx, const ExpertArgs &a)
 int launch_moe_down(mrml_hip_ctx *ctx, const ExpertArgs &a)
 {
     if (one_by_one(a)) return launch_down_one(ctx, a);
-    if (!streams(a)) return launch_product<true>(ctx, a);
+    if (!streams<true>(a)) return launch_product<true>(ctx, a);
     const int n = a.batch * a.k;
     const size_t part = align_up((size_t)n * a.rows * 4, 16);
     uint8_t *ws = (uint8_t *)workspace(ctx, part + act_pack_bytes(n * (a.cols / 32)));

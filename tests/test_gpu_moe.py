@@ -97,6 +97,7 @@ def test_residual_norm_values_that_are_not_finite(backend, dev, synth):
 # ---- the router's product -----------------------------------------------------------
 
 @pytest.mark.parametrize("batch,experts,cols", [(1, 1, 32), (1, 128, 2816), (3, 5, 64), (5, 128, 2816), (17, 60, 2048),
+                                                (40, 8, 96), (41, 8, 96), (41, 1, 32), (90, 33, 288), (1537, 100, 64),
                                                 (33, 31, 160), (64, 64, 96), (65, 130, 352), (130, 128, 704),
                                                 (257, 512, 64), (300, 3, 4096), (1000, 128, 2816)])
 def test_logits(backend, dev, synth, batch, experts, cols):
@@ -160,7 +161,8 @@ def check_route(backend, dev, logits, bias, k, **how):
 @pytest.mark.parametrize("n,e,k,groups,top,best", [
     (1, 1, 1, 1, 1, 1), (1, 128, 8, 1, 1, 1), (3, 4, 4, 1, 1, 1), (5, 7, 3, 1, 1, 1), (9, 60, 4, 1, 1, 1),
     (65, 64, 1, 1, 1, 1), (130, 65, 6, 5, 2, 1), (33, 128, 8, 8, 4, 2), (200, 256, 8, 8, 4, 2), (17, 512, 32, 64, 9, 2),
-    (40, 12, 3, 6, 2, 2), (40, 12, 2, 12, 2, 2), (2, 96, 8, 3, 3, 1), (1030, 16, 2, 1, 1, 1)])
+    (16, 40, 5, 1, 1, 1), (17, 40, 5, 1, 1, 1), (16, 512, 32, 1, 1, 1), (15, 512, 32, 2, 1, 2), (7, 130, 32, 13, 5, 2),
+    (300, 192, 8, 64, 16, 2), (40, 12, 3, 6, 2, 2), (40, 12, 2, 12, 2, 2), (2, 96, 8, 3, 3, 1), (1030, 16, 2, 1, 1, 1)])
 def test_route(backend, dev, synth, n, e, k, groups, top, best, with_bias, scoring):
     rng = synth.rng_for(n + 13 * e + k + 2 * scoring + with_bias)
     logits = (rng.standard_normal((n, e)) * 2).astype(np.float32)
@@ -281,7 +283,10 @@ SHAPES = [(1, 1, 1, 1, 32, "even"), (4, 2, 1, 17, 64, "even"), (3, 3, 2, 5, 96, 
           (5, 2, 16, 31, 160, "one"), (5, 2, 17, 32, 160, "skew"), (6, 2, 40, 70, 416, "holes"),
           (3, 1, 65, 48, 128, "one"), (4, 2, 130, 16, 224, "skew"), (40, 6, 64, 129, 64, "even"),
           (2, 2, 200, 15, 32, "even"), (7, 3, 90, 257, 192, "holes"), (128, 8, 50, 12, 96, "even"),
-          (9, 1, 300, 80, 480, "skew"), (2, 1, 9, 4, 4128, "even")]
+          (9, 1, 300, 80, 480, "skew"), (2, 1, 9, 4, 4128, "even"), (2, 1, 70, 20, 4128, "skew"),
+          (40, 32, 3, 20, 64, "even"), (33, 32, 60, 18, 96, "even"), (8, 2, 110, 65, 1056, "holes"),
+          (4, 2, 14, 33, 4096, "even"), (3, 2, 130, 33, 4096, "even"), (512, 8, 40, 5, 64, "even"),
+          (4, 4, 4, 30, 4064, "holes"), (2, 1, 400, 9, 32, "even")]
 
 
 @pytest.mark.parametrize("activation", [0, 1])
@@ -375,8 +380,9 @@ def test_products_keep_rows_that_are_not_finite_apart(backend, dev, synth, n):
         assert np.array_equal(got[rest], a[rest])
 
 
-def test_bad_ids_and_orders_are_left_out_and_reported(backend, dev, synth):
-    e, k, n, rows, cols = 4, 2, 30, 24, 64
+@pytest.mark.parametrize("n", [8, 30, 130])
+def test_bad_ids_and_orders_are_left_out_and_reported(backend, dev, synth, n):
+    e, k, rows, cols = 4, 2, 24, 64
     rng = synth.rng_for(9)
     gu, dn = Experts(backend, dev, synth, 1, e, rows, cols, 2), Experts(backend, dev, synth, 2, e, cols, 32)
     x = up(backend, dev, rng.standard_normal((n, cols)).astype(np.float32))
