@@ -502,9 +502,9 @@ constexpr int stream_units()
 constexpr int stream_block(int v) { return 4 * v * 32 + 16; }
 __host__ __device__ constexpr int stream_blocks(int nb) { return (nb + kStep - 1) / kStep * kStep; }
 constexpr int kBounce = 16 * kStep * 16;
-size_t stream_lds(int nb, int tokens)
+size_t stream_lds(int nb, int tokens, int part)
 {
-    return kWaves * kBounce + (size_t)stream_blocks(nb) * (stream_block(tokens / 4) + tokens * 4);
+    return kWaves * part + (size_t)stream_blocks(nb) * (stream_block(tokens / 4) + tokens * 4);
 }
 
 // `count` rows of an activation pack of `total` blocks into LDS; scales of 0 behind the last block, up to a whole step.
@@ -677,7 +677,101 @@ __device__ __forceinline__ void stream_pass(const ExpertArgs &a, int expert, int
     }
 }
 
-// Workgroup (x, y): rows of chunk x, and tile y of all experts' tiles of `tokens` tokens.
+// For short rows: the quants of 16 rows lie behind one another in memory, and their scales, so that a wave reads a whole unit
+// as it lies and puts it into LDS of its own, one unit ahead.  (In runs of 128 bytes a row, rows of 22 blocks are read across
+// lines, and their scales four bytes at once.)
+constexpr int kWholeBlocks = 32;  // of a row at most
+constexpr int kWholeLoads = kWholeBlocks * 16 / 64;
+// LDS of a wave: rows of nb | 1 blocks, which spread over the banks, then the scales as they lie.
+__host__ __device__ constexpr int whole_quants(int nb) { return 16 * (nb | 1) * 16; }
+__host__ __device__ constexpr int whole_part(int nb) { return whole_quants(nb) + 16 * nb * 2; }
+
+template <bool DOWN, int V>
+__device__ __forceinline__ void stream_whole(const ExpertArgs &a, int expert, int count, uint8_t *lds, const int *s_as,
+                                             const int *s_row, const float *s_weight)
+{
+    typedef uint16_t Half __attribute__((may_alias));
+    typedef uint32_t Word __attribute__((may_alias));
+    constexpr int kUnits = stream_units<DOWN>(), kRows = DOWN ? 16 * kUnits : 16;  // rows of a wave
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
+    const int nb = a.cols / 32, r0 = (blockIdx.x * kWaves + wave) * kRows;
+    const int units = r0 >= a.rows ? 0 : DOWN ? min(kUnits, (a.rows - r0 + 15) / 16) : kUnits;
+    const size_t first_block = (size_t)expert * a.rows * nb, blocks = (size_t)a.n_experts * a.rows * nb;
+    uint8_t *mine = lds + wave * whole_part(nb), *halves = mine + whole_quants(nb);
+    lds += kWaves * whole_part(nb);
+    float *scales = reinterpret_cast<float *>(lds + stream_blocks(nb) * stream_block(V));
+    const uint8_t *xa = lds + (g * 4 * V + ((i & 3) < V ? (i & 3) * 4 : 0) + (i >> 2)) * 8;  // as in stream_pass
+    const float *sa = scales + g * 4;
+    const uint8_t *get = mine + i * (nb | 1) * 16 + g * 4, *half_at = halves + i * nb * 2;
+    uint32_t put[kWholeLoads];
+#pragma unroll
+    for (int k = 0; k < kWholeLoads; ++k) {
+        const uint32_t q = k * 64 + lane, r = q / (uint32_t)nb;
+        put[k] = r < 16 ? (r * (nb | 1) + q - r * nb) * 16 : 0;
+    }
+    uint4 wv[kWholeLoads], sv;
+    auto load = [&](int u) {
+        const uint8_t *w = a.w[DOWN ? 0 : u];
+        const uint32_t at = (r0 + (DOWN ? u * 16 : 0)) * nb, last = a.rows * nb - 1;  // blocks of the expert
+        const uint8_t *quants = w + first_block * 16, *ws = w + blocks * 16 + first_block * 2;
+        sv = load_stream16(reinterpret_cast<const uint4 *>(ws) + min(at / 8 + (uint32_t)lane, last / 8));
+#pragma unroll
+        for (int k = 0; k < kWholeLoads; ++k)
+            if (k * 64 < 16 * nb)
+                wv[k] = load_stream16(reinterpret_cast<const uint4 *>(quants) + min(at + k * 64 + lane, last));
+    };
+    const size_t total = (size_t)(DOWN ? a.batch * a.k : a.batch) * nb;
+    stream_stage<V>(a.xpack, total, nb, s_row, count, lds, scales, [&]() {
+        if (units) load(0);
+    });
+    mrml_xsum::lds_barrier();
+    float acc[V] = {}, gate[V] = {};
+    for (int unit = 0; unit < units; ++unit) {
+#pragma unroll
+        for (int k = 0; k < kWholeLoads; ++k)
+            if (k * 64 + lane < 16 * nb) *reinterpret_cast<uint4 *>(mine + put[k]) = wv[k];
+        if (lane < 2 * nb) reinterpret_cast<uint4 *>(halves)[lane] = sv;
+        __builtin_amdgcn_wave_barrier();
+        if (unit + 1 < units) load(unit + 1);
+        auto block = [&](int b, const float4v (&s)[V], int j) {
+            const uint32_t y = *reinterpret_cast<const Word *>(get + (b + j) * 16) ^ 0x88888888u;
+            const uint64_t both = (uint64_t)(y & 0xF0F0F0F0u) << 32 | ((y << 4) & 0xF0F0F0F0u);
+            const int4v p = __builtin_amdgcn_mfma_i32_16x16x32_i8(
+                *reinterpret_cast<const long *>(xa + (b + j) * stream_block(V)), (long)both, int4v{0, 0, 0, 0}, 0, 0, 0);
+            const float dw = f16_bits_to_f32(*reinterpret_cast<const Half *>(half_at + (b + j) * 2));
+#pragma unroll
+            for (int v = 0; v < V; ++v) acc[v] = __builtin_fmaf((float)p[v], dw * s[v][j], acc[v]);
+        };
+        int b = 0;
+        for (; b + 4 <= nb; b += 4) {
+            float4v s[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) s[v] = *reinterpret_cast<const float4v *>(sa + (b / 4 * V + v) * 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) block(b, s, j);
+        }
+        if (b < nb) {
+            float4v s[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) s[v] = *reinterpret_cast<const float4v *>(sa + (b / 4 * V + v) * 16);
+#pragma unroll
+            for (int j = 0; j < 3; ++j)
+                if (b + j < nb) block(b, s, j);
+        }
+        __builtin_amdgcn_wave_barrier();
+        const int row = r0 + (DOWN ? unit * 16 : 0) + i;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int t = 4 * v + g;
+            if ((DOWN || unit == 1) && t < count && s_as[t] >= 0 && row < a.rows)
+                a.out[(size_t)s_as[t] * a.rows + row] = DOWN ? acc[v] * s_weight[t] : gated(gate[v], acc[v], a.activation);
+            gate[v] = acc[v];
+            acc[v] = 0.0f;
+        }
+    }
+}
+
+// Workgroup (x, y): rows of chunk x, and tile y of all experts' tiles of `tokens` tokens.  AT_ONCE = 0: by whole units.
 template <bool DOWN, int AT_ONCE>
 __global__ __launch_bounds__(64 * kWaves, 4) void moe_stream_kernel(ExpertArgs a, int tokens)
 {
@@ -730,9 +824,13 @@ __global__ __launch_bounds__(64 * kWaves, 4) void moe_stream_kernel(ExpertArgs a
         s_weight[tid] = DOWN && ok ? a.weights[o] : 0.0f;
     }
     mrml_xsum::lds_barrier();
-    if (tokens_here <= 4) stream_pass<DOWN, AT_ONCE, 1>(a, e, tokens_here, lds, s_as, s_row, s_weight);
-    else if (tokens_here <= 8) stream_pass<DOWN, AT_ONCE, 2>(a, e, tokens_here, lds, s_as, s_row, s_weight);
-    else stream_pass<DOWN, AT_ONCE, 4>(a, e, tokens_here, lds, s_as, s_row, s_weight);
+#define PASS(V)                                                                                          \
+    if constexpr (AT_ONCE == 0) stream_whole<DOWN, V>(a, e, tokens_here, lds, s_as, s_row, s_weight);     \
+    else stream_pass<DOWN, AT_ONCE, V>(a, e, tokens_here, lds, s_as, s_row, s_weight)
+    if (tokens_here <= 4) PASS(1);
+    else if (tokens_here <= 8) PASS(2);
+    else PASS(4);
+#undef PASS
 }
 
 // ---- a handful of assignments ------------------------------------------------------------
@@ -1048,13 +1146,16 @@ int launch_stream(mrml_hip_ctx *ctx, const ExpertArgs &a)
     // the tokens of a tile: room for more costs workgroups on a CU
     const int tokens = n <= 4 * a.n_experts ? 8 : kStreamTokens;
     const dim3 grid((a.rows + rows - 1) / rows, std::min(n, n / tokens + a.n_experts));
-#define MOE_STREAM(AT_ONCE)                                                                                              \
-    hipLaunchKernelGGL((moe_stream_kernel<DOWN, AT_ONCE>), grid, dim3(64 * kWaves), stream_lds(nb, tokens), ctx->stream, a, \
-                       tokens)
-    if (nb % 8 == 0) MOE_STREAM(8);
-    else if (nb % 4 == 0) MOE_STREAM(4);
-    else if (nb % 2 == 0) MOE_STREAM(2);
-    else MOE_STREAM(1);
+#define MOE_STREAM(AT_ONCE, PART)                                                                            \
+    hipLaunchKernelGGL((moe_stream_kernel<DOWN, AT_ONCE>), grid, dim3(64 * kWaves), stream_lds(nb, tokens, PART), \
+                       ctx->stream, a, tokens)
+    // Whole units / runs of 128 bytes a row, 40 tokens, 128 experts, eight a token: down of 2816 rows of 22 blocks 40 / 45 us,
+    // of 30 54 / 58, of 24 (whole lines as it is) 42 / 41, of 32 48 / 48.  An expert's scales have to begin at 16 bytes.
+    if (nb <= kWholeBlocks && nb % 8 && (int64_t)a.rows * nb % 8 == 0) MOE_STREAM(0, whole_part(nb));
+    else if (nb % 8 == 0) MOE_STREAM(8, kBounce);
+    else if (nb % 4 == 0) MOE_STREAM(4, kBounce);
+    else if (nb % 2 == 0) MOE_STREAM(2, kBounce);
+    else MOE_STREAM(1, kBounce);
 #undef MOE_STREAM
     return check_launch(ctx, "moe_stream_kernel");
 }

@@ -286,7 +286,8 @@ SHAPES = [(1, 1, 1, 1, 32, "even"), (4, 2, 1, 17, 64, "even"), (3, 3, 2, 5, 96, 
           (9, 1, 300, 80, 480, "skew"), (2, 1, 9, 4, 4128, "even"), (2, 1, 70, 20, 4128, "skew"),
           (40, 32, 3, 20, 64, "even"), (33, 32, 60, 18, 96, "even"), (8, 2, 110, 65, 1056, "holes"),
           (4, 2, 14, 33, 4096, "even"), (3, 2, 130, 33, 4096, "even"), (512, 8, 40, 5, 64, "even"),
-          (4, 4, 4, 30, 4064, "holes"), (2, 1, 400, 9, 32, "even")]
+          (4, 4, 4, 30, 4064, "holes"), (2, 1, 400, 9, 32, "even"), (16, 2, 20, 40, 704, "even"),
+          (16, 2, 20, 88, 992, "holes"), (6, 3, 30, 8, 32, "skew"), (6, 3, 30, 24, 224, "even"), (20, 4, 9, 200, 160, "even")]
 
 
 @pytest.mark.parametrize("activation", [0, 1])
