@@ -572,6 +572,107 @@ impl HipDevice {
         self.inner.expect(st, "attention_paged");
     }
 
+    /// The residual's addition and the next norm for a batch of rows (`mrml_hip_residual_rms_norm_batch`): `h_out` is `h`
+    /// plus `t`, or plus `t`'s norm times `w_post`; its norm times `w_next` goes to `xn`, its Q8_0 blocks to `pack`.
+    #[allow(clippy::too_many_arguments)]
+    pub fn residual_rms_norm_batch(&self, t: &HipBuffer<f32>, w_post: Option<&HipBuffer<f32>>, h: &HipBuffer<f32>,
+                                   h_out: &mut HipBuffer<f32>, w_next: Option<&HipBuffer<f32>>, xn: &mut HipBuffer<f32>,
+                                   pack: Option<&mut HipBuffer<u8>>, dim: usize, eps: f32, norm_t: bool) {
+        let batch = t.len / dim;
+        assert!(t.len == batch * dim && h.len == t.len && h_out.len == t.len && xn.len == t.len);
+        assert!(pack.as_ref().map_or(true, |p| p.len >= t.len / 32 * 40));
+        let post = w_post.map_or(std::ptr::null(), |w| w.ptr as *const f32);
+        let next = w_next.map_or(std::ptr::null(), |w| w.ptr as *const f32);
+        let pack = pack.map_or(std::ptr::null_mut(), |p| p.ptr as *mut c_void);
+        let st = unsafe {
+            (self.inner.api.residual_rms_norm_batch)(self.inner.ctx, t.ptr, post, h.ptr, h_out.ptr, next, xn.ptr, pack,
+                                                     i32_of(dim, "dim"), i32_of(batch, "batch"), eps, norm_t as i32)
+        };
+        self.inner.expect(st, "residual_rms_norm_batch");
+    }
+
+    /// The router's product for a batch of tokens (`mrml_hip_moe_logits`).
+    pub fn moe_logits(&self, x: &HipBuffer<f32>, w: &HipBuffer<f32>, logits: &mut HipBuffer<f32>, n_experts: usize,
+                      cols: usize) {
+        let batch = logits.len / n_experts;
+        assert!(x.len == batch * cols && w.len == n_experts * cols && logits.len == batch * n_experts);
+        let st = unsafe {
+            (self.inner.api.moe_logits)(self.inner.ctx, x.ptr, w.ptr, logits.ptr, i32_of(n_experts, "n_experts"),
+                                        i32_of(cols, "cols"), i32_of(batch, "batch"))
+        };
+        self.inner.expect(st, "moe_logits");
+    }
+
+    /// The `k` experts of every token, their weights, and the assignments sorted by expert (`mrml_hip_moe_route`).
+    #[allow(clippy::too_many_arguments)]
+    pub fn moe_route(&self, logits: &HipBuffer<f32>, bias: Option<&HipBuffer<f32>>, ids: &mut HipBuffer<i32>,
+                     weights: &mut HipBuffer<f32>, starts: &mut HipBuffer<i32>, order: &mut HipBuffer<i32>,
+                     n_experts: usize, k: usize, scoring: i32, n_groups: usize, top_groups: usize, group_best: usize,
+                     renormalise: bool, scale: f32) {
+        let batch = logits.len / n_experts;
+        assert!(ids.len == batch * k && weights.len == ids.len && order.len == ids.len && starts.len == n_experts + 1);
+        assert!(bias.map_or(true, |b| b.len == n_experts));
+        let bias = bias.map_or(std::ptr::null(), |b| b.ptr as *const f32);
+        let st = unsafe {
+            (self.inner.api.moe_route)(self.inner.ctx, logits.ptr, bias, ids.ptr, weights.ptr, starts.ptr, order.ptr,
+                                       i32_of(n_experts, "n_experts"), i32_of(batch, "batch"), i32_of(k, "k"), scoring,
+                                       i32_of(n_groups, "n_groups"), i32_of(top_groups, "top_groups"),
+                                       i32_of(group_best, "group_best"), renormalise as i32, scale)
+        };
+        self.inner.expect(st, "moe_route");
+    }
+
+    /// The experts' first two products and the gated activation (`mrml_hip_moe_gate_up_q4_0`).
+    #[allow(clippy::too_many_arguments)]
+    pub fn moe_gate_up_q4_0(&self, w_gate: &HipBuffer<u8>, w_up: &HipBuffer<u8>, x: &HipBuffer<f32>, ids: &HipBuffer<i32>,
+                            starts: &HipBuffer<i32>, order: &HipBuffer<i32>, act: &mut HipBuffer<f32>, n_experts: usize,
+                            rows: usize, cols: usize, k: usize, activation: i32) {
+        let batch = x.len / cols;
+        assert!(ids.len == batch * k && order.len == ids.len && starts.len == n_experts + 1 && act.len == ids.len * rows);
+        let st = unsafe {
+            (self.inner.api.moe_gate_up_q4_0)(self.inner.ctx, w_gate.ptr as *const c_void, w_up.ptr as *const c_void, x.ptr,
+                                              ids.ptr, starts.ptr, order.ptr, act.ptr, i32_of(n_experts, "n_experts"),
+                                              i32_of(rows, "rows"), i32_of(cols, "cols"), i32_of(batch, "batch"),
+                                              i32_of(k, "k"), activation)
+        };
+        self.inner.expect(st, "moe_gate_up_q4_0");
+    }
+
+    /// `moe_gate_up_q4_0` of the pack that `residual_rms_norm_batch` wrote (`mrml_hip_moe_gate_up_q4_0_q8`).
+    #[allow(clippy::too_many_arguments)]
+    pub fn moe_gate_up_q4_0_q8(&self, w_gate: &HipBuffer<u8>, w_up: &HipBuffer<u8>, xpack: &HipBuffer<u8>,
+                               ids: &HipBuffer<i32>, starts: &HipBuffer<i32>, order: &HipBuffer<i32>,
+                               act: &mut HipBuffer<f32>, n_experts: usize, rows: usize, cols: usize, k: usize,
+                               activation: i32) {
+        let batch = ids.len / k;
+        assert!(xpack.len >= batch * cols / 32 * 40 && ids.len == batch * k && order.len == ids.len);
+        assert!(starts.len == n_experts + 1 && act.len == ids.len * rows);
+        let st = unsafe {
+            (self.inner.api.moe_gate_up_q4_0_q8)(self.inner.ctx, w_gate.ptr as *const c_void, w_up.ptr as *const c_void,
+                                                 xpack.ptr as *const c_void, ids.ptr, starts.ptr, order.ptr, act.ptr,
+                                                 i32_of(n_experts, "n_experts"), i32_of(rows, "rows"),
+                                                 i32_of(cols, "cols"), i32_of(batch, "batch"), i32_of(k, "k"), activation)
+        };
+        self.inner.expect(st, "moe_gate_up_q4_0_q8");
+    }
+
+    /// The experts' last product, summed over a token's experts by its weights (`mrml_hip_moe_down_q4_0`).
+    #[allow(clippy::too_many_arguments)]
+    pub fn moe_down_q4_0(&self, w_down: &HipBuffer<u8>, act: &HipBuffer<f32>, ids: &HipBuffer<i32>,
+                         weights: &HipBuffer<f32>, starts: &HipBuffer<i32>, order: &HipBuffer<i32>, y: &mut HipBuffer<f32>,
+                         n_experts: usize, rows: usize, cols: usize, k: usize) {
+        let batch = y.len / rows;
+        assert!(ids.len == batch * k && weights.len == ids.len && order.len == ids.len && y.len == batch * rows);
+        assert!(starts.len == n_experts + 1 && act.len == ids.len * cols);
+        let st = unsafe {
+            (self.inner.api.moe_down_q4_0)(self.inner.ctx, w_down.ptr as *const c_void, act.ptr, ids.ptr, weights.ptr,
+                                           starts.ptr, order.ptr, y.ptr, i32_of(n_experts, "n_experts"),
+                                           i32_of(rows, "rows"), i32_of(cols, "cols"), i32_of(batch, "batch"),
+                                           i32_of(k, "k"))
+        };
+        self.inner.expect(st, "moe_down_q4_0");
+    }
+
     /// `CudaDevice::rope_256k` (cuda.rs:2248-2285): RoPE of `n_heads` heads of
     /// `d_vec` in place at position `pos`.
     pub fn rope_256k(&self, d_vec: &mut HipBuffer<f32>, pos: usize, head_dim: usize, n_heads: usize, freq_base: f32,

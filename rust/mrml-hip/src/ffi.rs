@@ -24,6 +24,12 @@ pub const MRML_HIP_Q4_0: i32 = 2;
 pub const MRML_HIP_Q8_0: i32 = 8;
 pub const MRML_HIP_Q4_K: i32 = 12;
 
+/// Scoring of `moe_route`, activation of `moe_gate_up_q4_0`.
+pub const MRML_HIP_MOE_SOFTMAX: i32 = 0;
+pub const MRML_HIP_MOE_SIGMOID: i32 = 1;
+pub const MRML_HIP_MOE_GEGLU: i32 = 0;
+pub const MRML_HIP_MOE_SWIGLU: i32 = 1;
+
 pub const MRML_HIP_SCORE_CPU: i32 = 0;
 pub const MRML_HIP_SCORE_DEVICE: i32 = 1;
 pub const MRML_HIP_NUMERICS_EXACT: i32 = 0;
