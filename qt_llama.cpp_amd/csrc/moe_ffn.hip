@@ -6,8 +6,8 @@
 // row that keeps both in range), q - 8 is a half as it stands, so a block's sum is
 // two f16 MFMAs whose f32 result only has to be multiplied by dw and added: one
 // FMA an output and block.  (The int8 product gives a whole number that takes a
-// conversion, two products and an addition: a wave spends 48 cycles of VALU on 16
-// x 16 outputs of a block against 32 of MFMA and 16 of VALU side by side here.)
+// conversion, a product of the two scales and an FMA: three vector instructions
+// for one, and those are what bounds the tiles.)
 
 #include <algorithm>
 #include <type_traits>
@@ -263,10 +263,12 @@ constexpr int kTilePart = kHalf * kTileGroups * 2048;  // bytes of a buffer: [bl
 // whose pieces p lie at p ^ row, so that the 16-byte reads of 16 rows meet all banks.  Two blocks of all groups go to one
 // buffer while the two in the other are multiplied; a step's weights are on their way for two of those.
 //
-// An MFMA keeps its unit for 16 cycles, of which the wave can fill 12 with VALU instructions: the order is written out, a
-// product of one token group beside the additions of the last one and a part of the next block's halves.  (Left to the
-// compiler the two were one after the other for the most part, 281 us for 1501 tokens.)  ODD: the blocks in a row are odd
-// in number, and its scales are read one by one.
+// Bound by the issue of vector instructions: with two waves a SIMD an MFMA takes 20 cycles, with two FMAs beside it 22, with
+// four 31, and there are 4.5 here, two of them the blocks' FMAs.  So the order is written out, a product of one token group
+// beside the additions of the last one and a part of the next block's halves.  (Left to the compiler the two were one after
+// the other for the most part.)  1501 tokens, 128 experts of 704 x 2816, eight a token: gate and up 270 us, 350 TFLOP/s; down
+// about 145.  Tiles of up to 96 tokens, which take a block's halves apart less often, spill registers around the counted
+// waits.  ODD: the blocks in a row are odd in number, and its scales are read one by one.
 // (pin: a value is formed in its place, which sched_barrier alone does not see to.)
 template <class T>
 __device__ __forceinline__ void pin(T &x)
