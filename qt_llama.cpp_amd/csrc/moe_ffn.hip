@@ -268,7 +268,7 @@ constexpr int kTilePart = kHalf * kTileGroups * 2048;  // bytes of a buffer: [bl
 // beside the additions of the last one and a part of the next block's halves.  (Left to the compiler the two were one after
 // the other for the most part.)  1501 tokens, 128 experts of 704 x 2816, eight a token: gate and up 270 us, 350 TFLOP/s; down
 // about 145.  Tiles of up to 96 tokens, which take a block's halves apart less often, spill registers around the counted
-// waits.  ODD: the blocks in a row are odd in number, and its scales are read one by one.
+// waits.  AT_ONCE: scales of a row read together, as its blocks' number allows.
 // (pin: a value is formed in its place, which sched_barrier alone does not see to.)
 template <class T>
 __device__ __forceinline__ void pin(T &x)
@@ -276,13 +276,14 @@ __device__ __forceinline__ void pin(T &x)
     asm volatile("" : "+v"(x));
 }
 
-template <bool DOWN, bool ODD, int NT>
+template <bool DOWN, int AT_ONCE, int NT>
 __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &tile, int chunk_rows, const uint8_t *xp,
                                              uint8_t *lds, const int *s_as, const float *s_scale)
 {
-    constexpr int kLoadsW = kGroups * (1 + (ODD ? 4 : 2));
+    constexpr int kLoadsW = kGroups + 4 / AT_ONCE;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
     const int nb = a.cols / 32, r0 = chunk_rows + wave * wave_rows<DOWN>();
+    const bool idle = r0 >= a.rows;  // loads for the others, and leaves the SIMD to them
     // the expert's matrices, 32-bit offsets within one
     const size_t first_block = (size_t)tile.expert * a.rows * nb, blocks = (size_t)a.n_experts * a.rows * nb;
     // this wave's share of a buffer: block wave & 1, rows 8 (wave / 2) .. + 8 of every group
@@ -303,23 +304,31 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
 #pragma unroll
     for (int q = 0; q < kGroups; ++q) row_at[q] = (uint32_t)min(r0 + (DOWN ? q : q & 1) * 16 + i, a.rows - 1) * nb;
     uint4 wv[kGroups];
-    uint2 sv[kGroups];
+    struct __attribute__((packed, aligned(4))) Pair {  // eight bytes from a multiple of four
+        uint32_t x, y;
+    };
+    // quants: of a block of row i of every group; scales: lane row g has the group g's, which saves requests
+    Pair sv;
+    static_assert(kGroups == 4, "a lane row a group");
+    const uint8_t *ws = a.w[DOWN ? 0 : g >> 1] + blocks * 16 +
+                        (first_block + (uint32_t)min(r0 + (DOWN ? g : g & 1) * 16 + i, a.rows - 1) * nb) * 2;
     auto load_w = [&](int c) {  // kLoadsW loads
         const uint32_t b = min(c * kChunk + g, nb - 1);
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) {
-            const uint8_t *w = a.w[DOWN ? 0 : q >> 1] + first_block * 16, *ws = a.w[DOWN ? 0 : q >> 1] + blocks * 16 + first_block * 2;
+            const uint8_t *w = a.w[DOWN ? 0 : q >> 1] + first_block * 16;
             uint32_t at_row = row_at[q];
             asm volatile("" : "+v"(at_row));  // addresses are formed here: kept over the loop they cost 16 registers
-            wv[q] = *reinterpret_cast<const uint4 *>(w + (at_row + b) * 16ull);
-            auto two = [&](int at) {
-                if (!ODD) return *reinterpret_cast<const uint32_t *>(ws + (at_row + min(at, nb - 2)) * 2ull);
-                const uint32_t lo = *reinterpret_cast<const uint16_t *>(ws + (at_row + min(at, nb - 1)) * 2ull);
-                const uint32_t hi = *reinterpret_cast<const uint16_t *>(ws + (at_row + min(at + 1, nb - 1)) * 2ull);
-                return lo | (at + 1 < nb ? hi << 16 : 0u);  // the block behind the last counts nothing
-            };
-            sv[q] = make_uint2(two(c * kChunk), two(c * kChunk + 2));
+            // (an offset of less than 2^32 from an address that all lanes share)
+            wv[q] = *reinterpret_cast<const uint4 *>(w + (at_row + b) * 16u);
         }
+        auto one = [&](int at) { return (uint32_t)*reinterpret_cast<const uint16_t *>(ws + min(at, nb - 1) * 2); };
+        auto two = [&](int at) {
+            if (AT_ONCE == 2) return *reinterpret_cast<const uint32_t *>(ws + min(at, nb - 2) * 2);
+            return one(at) | (at + 1 < nb ? one(at + 1) << 16 : 0u);  // the block behind the last counts nothing
+        };
+        if (AT_ONCE == 4) sv = *reinterpret_cast<const Pair *>(ws + min(c * kChunk, nb - kChunk) * 2);
+        else sv = {two(c * kChunk), two(c * kChunk + 2)};
     };
     float4v acc[kGroups][NT];
 #pragma unroll
@@ -336,6 +345,9 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
     for (int c = 0; c < chunks; ++c) {
         uint32_t w[kGroups][4];
         half4v d[kGroups];
+        uint32_t scales[2][4];
+        spread(AT_ONCE == 4 && c * kChunk + 2 == nb ? sv.y : sv.x, scales[0]);  // a row's last two come with the two before
+        spread(sv.y, scales[1]);
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) {
             w[q][0] = wv[q].x;
@@ -343,12 +355,11 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
             w[q][2] = wv[q].z;
             w[q][3] = wv[q].w;
             turn(w[q][0], w[q][1], w[q][2], w[q][3]);
-            d[q] = __builtin_bit_cast(half4v, sv[q]);
+            d[q] = __builtin_bit_cast(half4v, (uint64_t)scales[1][q] << 32 | scales[0][q]);
             // done before the barrier: a wait for these weights behind it would be one for the loads issued there too
             asm volatile("" : "+v"(w[q][0]), "+v"(w[q][1]), "+v"(w[q][2]), "+v"(w[q][3]), "+v"(d[q]));
         }
-        uint4v wh[kGroups];
-        uint32_t part[kGroups][4];
+        uint4v wh[2][kGroups];  // of blocks j and j + 1
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             // the buffer's loads: before the first half nothing was issued after them, before the second the weights
@@ -360,7 +371,7 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
             } else if (c + 1 < chunks) {
                 load_x(c + 1, 0);
             }
-            if (c * kChunk + half * kHalf >= nb) break;
+            if (idle || c * kChunk + half * kHalf >= nb) continue;
             half8v x[2][2];
             float4v p[2][kGroups];
             auto read = [&](int to, int step) {
@@ -378,16 +389,16 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
             if (half == 0)
 #pragma unroll
                 for (int q = 0; q < kGroups; ++q) {
-                    wh[q].x = nibble_pair<0>(w[q][0], k1024);
-                    wh[q].y = nibble_pair<1>(w[q][0], k1024);
-                    wh[q].z = nibble_pair<2>(w[q][0], k1024);
-                    wh[q].w = nibble_pair<3>(w[q][0], k1024);
+                    wh[0][q].x = nibble_pair<0>(w[q][0], k1024);
+                    wh[0][q].y = nibble_pair<1>(w[q][0], k1024);
+                    wh[0][q].z = nibble_pair<2>(w[q][0], k1024);
+                    wh[0][q].w = nibble_pair<3>(w[q][0], k1024);
                 }
 #pragma unroll
             for (int step = 0; step < kHalf * NT; ++step) {  // block step / NT, token group step % NT
                 const int now = step & 1, t = step % NT, j = half * kHalf + step / NT;
                 if (step + 1 < kHalf * NT) read(now ^ 1, step + 1);
-                auto weights = [&](int q) { return __builtin_bit_cast(half8v, wh[q]); };
+                auto weights = [&](int q) { return __builtin_bit_cast(half8v, wh[j & 1][q]); };
 #pragma unroll
                 for (int q = 0; q < kGroups; ++q) {
                     p[now][q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[now][0], weights(q), float4v{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
@@ -404,20 +415,17 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
                     if (j + 1 < kChunk)
 #pragma unroll
                         for (int n = t * kGroups / NT; n < (t + 1) * kGroups / NT; ++n) {
-                            if (q == 0) part[n][0] = nibble_pair<0>(w[n][j + 1], k1024);
-                            if (q == 1) part[n][1] = nibble_pair<1>(w[n][j + 1], k1024);
-                            if (q == 2) part[n][2] = nibble_pair<2>(w[n][j + 1], k1024);
-                            if (q == 3) part[n][3] = nibble_pair<3>(w[n][j + 1], k1024);
+                            if (q == 0) wh[(j + 1) & 1][n].x = nibble_pair<0>(w[n][j + 1], k1024);
+                            if (q == 1) wh[(j + 1) & 1][n].y = nibble_pair<1>(w[n][j + 1], k1024);
+                            if (q == 2) wh[(j + 1) & 1][n].z = nibble_pair<2>(w[n][j + 1], k1024);
+                            if (q == 3) wh[(j + 1) & 1][n].w = nibble_pair<3>(w[n][j + 1], k1024);
                         }
                     if (j + 1 < kChunk)
 #pragma unroll
-                        for (int n = t * kGroups / NT; n < (t + 1) * kGroups / NT; ++n) pin(part[n][q]);
+                        for (int n = t * kGroups / NT; n < (t + 1) * kGroups / NT; ++n) pin(wh[(j + 1) & 1][n]);
                     pin(p[now][q]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                if (t == NT - 1 && j + 1 < kChunk)
-#pragma unroll
-                    for (int q = 0; q < kGroups; ++q) wh[q] = uint4v{part[q][0], part[q][1], part[q][2], part[q][3]};
             }
 #pragma unroll
             for (int q = 0; q < kGroups; ++q) add((kHalf * NT - 1) & 1, q, kHalf * NT - 1);
@@ -445,7 +453,7 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
         }
 }
 
-template <bool DOWN, bool ODD>
+template <bool DOWN, int AT_ONCE>
 __global__ __launch_bounds__(64 * kWaves, 2) void moe_tile_kernel(ExpertArgs a, const Tile *__restrict__ tiles,
                                                                   const uint8_t *__restrict__ xp,
                                                                   const float *__restrict__ xscale, int row_wgs)
@@ -469,10 +477,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_tile_kernel(ExpertArgs a, 
     __syncthreads();
     const int chunk_rows = ((blockIdx.x >> 3) - turn * row_wgs) * kWaves * wave_rows<DOWN>();
     switch ((tile.count + 15) / 16) {
-    case 1: tile_product<DOWN, ODD, 1>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
-    case 2: tile_product<DOWN, ODD, 2>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
-    case 3: tile_product<DOWN, ODD, 3>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
-    default: tile_product<DOWN, ODD, 4>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
+    case 1: tile_product<DOWN, AT_ONCE, 1>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
+    case 2: tile_product<DOWN, AT_ONCE, 2>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
+    case 3: tile_product<DOWN, AT_ONCE, 3>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
+    default: tile_product<DOWN, AT_ONCE, 4>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
     }
 }
 
@@ -1102,12 +1110,14 @@ int launch_tiles(mrml_hip_ctx *ctx, const ExpertArgs &a, int most, const Tile *t
     const int64_t grid = (int64_t)(most + 7) / 8 * 8 * row_wgs;
     REQUIRE(ctx, grid <= INT32_MAX, "moe: batch * k = %d assignments of %d rows are too many for one call", a.batch * a.k,
             a.rows);
-    if (a.cols / 32 % 2)
-        hipLaunchKernelGGL((moe_tile_kernel<DOWN, true>), dim3((uint32_t)grid), dim3(64 * kWaves), 0, ctx->stream, a, tiles, xp,
-                           xscale, row_wgs);
-    else
-        hipLaunchKernelGGL((moe_tile_kernel<DOWN, false>), dim3((uint32_t)grid), dim3(64 * kWaves), 0, ctx->stream, a, tiles, xp,
-                           xscale, row_wgs);
+    const int nb = a.cols / 32;
+#define TILES(AT_ONCE)                                                                                                \
+    hipLaunchKernelGGL((moe_tile_kernel<DOWN, AT_ONCE>), dim3((uint32_t)grid), dim3(64 * kWaves), 0, ctx->stream, a, tiles, \
+                       xp, xscale, row_wgs)
+    if (nb % 2 == 0 && nb >= kChunk) TILES(4);
+    else if (nb % 2 == 0) TILES(2);
+    else TILES(1);
+#undef TILES
     return check_launch(ctx, "moe_tile_kernel");
 }
 
