@@ -36,7 +36,7 @@ struct Tile {
     int expert, first, count, pad;  // places first .. first + count of the order
 };
 
-constexpr int kTileRows = 16, kTileGroups = 4;  // rows of a group, groups of a tile at most
+constexpr int kTileRows = 16, kTileGroups = 6;  // rows of a group, groups of a tile at most
 
 // Tiles that a call can have.
 int max_tiles(const ExpertArgs &a)
@@ -266,9 +266,9 @@ constexpr int kTilePart = kHalf * kTileGroups * 2048;  // bytes of a buffer: [bl
 // Bound by the issue of vector instructions: with two waves a SIMD an MFMA takes 20 cycles, with two FMAs beside it 22, with
 // four 31, and there are 4.5 here, two of them the blocks' FMAs.  So the order is written out, a product of one token group
 // beside the additions of the last one and a part of the next block's halves.  (Left to the compiler the two were one after
-// the other for the most part.)  1501 tokens, 128 experts of 704 x 2816, eight a token: gate and up 270 us, 350 TFLOP/s; down
-// about 145.  Tiles of up to 96 tokens, which take a block's halves apart less often, spill registers around the counted
-// waits.  AT_ONCE: scales of a row read together, as its blocks' number allows.
+// the other for the most part.)  1501 tokens, 128 experts of 704 x 2816, eight a token: gate and up 228 us, 420 TFLOP/s; down
+// about 130.  With tiles of up to 64 tokens, which take a block's halves apart more often, 13 and 4 us more; with a request
+// for each group's scales 21 and 10 more.  AT_ONCE: scales of a row read together, as its blocks' number allows.
 // (pin: a value is formed in its place, which sched_barrier alone does not see to.)
 template <class T>
 __device__ __forceinline__ void pin(T &x)
@@ -480,7 +480,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_tile_kernel(ExpertArgs a, 
     case 1: tile_product<DOWN, AT_ONCE, 1>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
     case 2: tile_product<DOWN, AT_ONCE, 2>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
     case 3: tile_product<DOWN, AT_ONCE, 3>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
-    default: tile_product<DOWN, AT_ONCE, 4>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
+    case 4: tile_product<DOWN, AT_ONCE, 4>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
+    case 5: tile_product<DOWN, AT_ONCE, 5>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
+    default: tile_product<DOWN, AT_ONCE, 6>(a, tile, chunk_rows, xp, lds, s_as, s_scale); break;
     }
 }
 
