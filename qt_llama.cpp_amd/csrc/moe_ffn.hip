@@ -1106,16 +1106,21 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(ExpertArgs a, const fl
 }
 
 template <bool DOWN>
+int row_wgs(const ExpertArgs &a)  // workgroups of a tile
+{
+    return (a.rows + kWaves * wave_rows<DOWN>() - 1) / (kWaves * wave_rows<DOWN>());
+}
+
+template <bool DOWN>
 int launch_tiles(mrml_hip_ctx *ctx, const ExpertArgs &a, int most, const Tile *tiles, const uint8_t *xp, const float *xscale)
 {
-    const int row_wgs = (a.rows + kWaves * wave_rows<DOWN>() - 1) / (kWaves * wave_rows<DOWN>());
-    const int64_t grid = (int64_t)(most + 7) / 8 * 8 * row_wgs;
+    const int64_t grid = (int64_t)(most + 7) / 8 * 8 * row_wgs<DOWN>(a);
     REQUIRE(ctx, grid <= INT32_MAX, "moe: batch * k = %d assignments of %d rows are too many for one call", a.batch * a.k,
             a.rows);
     const int nb = a.cols / 32;
 #define TILES(AT_ONCE)                                                                                                \
     hipLaunchKernelGGL((moe_tile_kernel<DOWN, AT_ONCE>), dim3((uint32_t)grid), dim3(64 * kWaves), 0, ctx->stream, a, tiles, \
-                       xp, xscale, row_wgs)
+                       xp, xscale, row_wgs<DOWN>(a))
     if (nb % 2 == 0 && nb >= kChunk) TILES(4);
     else if (nb % 2 == 0) TILES(2);
     else TILES(1);
@@ -1144,13 +1149,18 @@ int launch_down_one(mrml_hip_ctx *ctx, const ExpertArgs &a)
     return check_launch(ctx, "moe_down_one_kernel");
 }
 
-// Few tokens an expert on average.  Streamed / in tiles, 128 experts of 704 x 2816, eight a token: gate and up 64 tokens 59 /
-// 110 us, 192 100 / 132, 384 152 / 157 (eight experts, two a token: 96 tokens 28 / 55); down 64 54 / 57, 128 68 / 68, 192
-// 77 / 71.
+// Few tokens an expert on average, or, for gate and up, so few tiles that they would leave CUs without any, where a pass over
+// the weights for every 16 tokens is still less than a tile's whole row of blocks one after the other.
+// Streamed / in tiles, k experts a token of E of 704 x 2816, gate and up: E = 128, k = 8: 64 tokens 59 / 95 us, 192 99 / 118,
+// 256 119 / 122, 320 134 / 125; E = 32, k = 4 (256 tokens: 256 workgroups): 256 tokens 60 / 73, 400 82 / 70; E = 8, k = 2: 96
+// tokens 28 / 47, 400 53 / 73.  Down, E = 128, k = 8: 40 tokens 41 / 49, 96 58 / 58, 160 66 / 62; E = 8, k = 2: 32 22 / 18.
 template <bool DOWN>
 bool streams(const ExpertArgs &a)
 {
-    return a.batch * a.k <= (DOWN ? 8 : 24) * a.n_experts && a.cols / 32 <= kStreamBlocks;  // n * cols < 2^26
+    const int n = a.batch * a.k;
+    if (a.cols / 32 > kStreamBlocks) return false;
+    if (n <= (DOWN ? 6 : 16) * a.n_experts) return true;
+    return !DOWN && n <= 100 * a.n_experts && (int64_t)max_tiles(a) * row_wgs<DOWN>(a) <= 256;  // n * cols < 2^27
 }
 
 template <bool DOWN>

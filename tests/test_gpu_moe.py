@@ -287,7 +287,10 @@ SHAPES = [(1, 1, 1, 1, 32, "even"), (4, 2, 1, 17, 64, "even"), (3, 3, 2, 5, 96, 
           (40, 32, 3, 20, 64, "even"), (33, 32, 60, 18, 96, "even"), (8, 2, 110, 65, 1056, "holes"),
           (4, 2, 14, 33, 4096, "even"), (3, 2, 130, 33, 4096, "even"), (512, 8, 40, 5, 64, "even"),
           (4, 4, 4, 30, 4064, "holes"), (2, 1, 400, 9, 32, "even"), (16, 2, 20, 40, 704, "even"),
-          (16, 2, 20, 88, 992, "holes"), (6, 3, 30, 8, 32, "skew"), (6, 3, 30, 24, 224, "even"), (20, 4, 9, 200, 160, "even")]
+          (16, 2, 20, 88, 992, "holes"), (6, 3, 30, 8, 32, "skew"), (6, 3, 30, 24, 224, "even"), (20, 4, 9, 200, 160, "even"),
+          (1, 1, 130, 70, 96, "even"), (1, 1, 130, 33, 64, "even"), (1, 1, 101, 40, 704, "even"), (1, 1, 180, 150, 160, "even"),
+          (4, 2, 260, 129, 352, "skew"), (4, 2, 300, 47, 416, "holes"), (3, 2, 250, 257, 192, "one"), (2, 1, 40, 20, 4160, "even"),
+          (2, 1, 33, 130, 4224, "skew"), (8, 4, 210, 31, 128, "even"), (30, 4, 140, 1100, 32, "skew")]
 
 
 @pytest.mark.parametrize("activation", [0, 1])
@@ -336,7 +339,7 @@ def test_down(backend, dev, orc, synth, e, k, n, rows, cols, how):
     assert (got[(ids < 0).all(1)] == 0).all()
 
 
-@pytest.mark.parametrize("n", [1, 3, 40, 150])
+@pytest.mark.parametrize("n", [1, 3, 40, 150, 250])
 def test_products_of_very_uneven_activations(backend, dev, orc, synth, n):
     """Blocks from 1e-9 to 1e6 in one row, rows of zeros, weights with zero scales: exact where Q8_0 is."""
     e, k, rows, cols = 4, 2, 40, 512
@@ -356,7 +359,7 @@ def test_products_of_very_uneven_activations(backend, dev, orc, synth, n):
     assert (off <= 1).all(), off.max()
 
 
-@pytest.mark.parametrize("n", [1, 20, 100])
+@pytest.mark.parametrize("n", [1, 20, 100, 200])
 def test_products_keep_rows_that_are_not_finite_apart(backend, dev, synth, n):
     """Blocks whose scale passes f16, infinities among them, give values that are not finite in their token's rows
     alone."""
@@ -381,7 +384,7 @@ def test_products_keep_rows_that_are_not_finite_apart(backend, dev, synth, n):
         assert np.array_equal(got[rest], a[rest])
 
 
-@pytest.mark.parametrize("n", [8, 30, 130])
+@pytest.mark.parametrize("n", [8, 30, 130, 250])
 def test_bad_ids_and_orders_are_left_out_and_reported(backend, dev, synth, n):
     e, k, rows, cols = 4, 2, 24, 64
     rng = synth.rng_for(9)
@@ -507,7 +510,7 @@ class Layer:
         return [self.b[name].numpy() for name in names]
 
 
-@pytest.mark.parametrize("n", [1, 2, 19, 150])
+@pytest.mark.parametrize("n", [1, 2, 19, 150, 450])
 def test_layer(backend, dev, orc, synth, n):
     """Each step of the layer against 64 bits on the values that it was given."""
     L = Layer(backend, dev, synth, n, seed=n)
@@ -529,7 +532,7 @@ def test_layer(backend, dev, orc, synth, n):
     assert np.array_equal(bits(h2), bits(want_h2)) and np.array_equal(bits(xn2), bits(want_xn2))
 
 
-@pytest.mark.parametrize("n", [1, 30, 140])
+@pytest.mark.parametrize("n", [1, 30, 140, 450])
 def test_layer_captured(backend, dev, synth, n):
     """A graph of the layer replayed over new inputs, with eager work of another size between: the eager bits each time."""
     a, b = Layer(backend, dev, synth, n, seed=50 + n), Layer(backend, dev, synth, 2 * n + 1, seed=60)
