@@ -264,10 +264,10 @@ constexpr int kTilePart = kHalf * kTileGroups * 2048;  // bytes of a buffer: [bl
 // buffer while the two in the other are multiplied; a step's weights are on their way for two of those.
 //
 // Bound by the issue of vector instructions: with two waves a SIMD an MFMA takes 20 cycles, with two FMAs beside it 22, with
-// four 31, and there are 4.5 here, two of them the blocks' FMAs.  So the order is written out, a product of one token group
+// four 31, and there are 4 here, two of them the blocks' FMAs.  So the order is written out, a product of one token group
 // beside the additions of the last one and a part of the next block's halves.  (Left to the compiler the two were one after
-// the other for the most part.)  1501 tokens, 128 experts of 704 x 2816, eight a token: gate and up 228 us, 420 TFLOP/s; down
-// about 130.  With tiles of up to 64 tokens, which take a block's halves apart more often, 13 and 4 us more; with a request
+// the other for the most part.)  1501 tokens, 128 experts of 704 x 2816, eight a token: gate and up 222 us, 429 TFLOP/s; down
+// about 122.  With tiles of up to 64 tokens, which take a block's halves apart more often, 13 and 4 us more; with a request
 // for each group's scales 21 and 10 more.  AT_ONCE: scales of a row read together, as its blocks' number allows.
 // (pin: a value is formed in its place, which sched_barrier alone does not see to.)
 template <class T>
