@@ -64,7 +64,9 @@ __device__ __forceinline__ double sq_f64(float4 a)
     return ((double)a.x * a.x + (double)a.y * a.y) + ((double)a.z * a.z + (double)a.w * a.w);
 }
 
-// One workgroup a row, CH float4 a thread.
+// One workgroup a row, CH float4 a thread: each value is read once, and waits in registers for the sums of its row.  The sums
+// are f64, so that their order leaves no trace in the f32 scale, nor in the quants behind it.  1900 rows of 2304 with a pack:
+// 15.9 us, 4.7 TB/s, bound by its bytes; one row: 4.8, a launch and the latencies of a load and two sums.
 template <int CH, int THREADS>
 __global__ __launch_bounds__(THREADS) void residual_norm_rows_kernel(const float *t, const float *__restrict__ w_post,
                                                                  const float *h, float *h_out,
@@ -272,6 +274,8 @@ __device__ __forceinline__ int wave_first(uint64_t key, int id)
     return __ffsll((unsigned long long)lanes) - 1;
 }
 
+// (32008 ids of 256 experts, 32 workgroups: 8.4 us, most of it the counting, an addition in LDS for every id in every
+// workgroup; one workgroup an expert that looks through all ids twice took 73.)
 // The plan of places [lo, hi) of n ids, by a workgroup of whole waves, at most 16: counts of every expert, before lo and
 // in all, give where its run goes on; then, blockDim.x ids at a time, a place is its run's end, the ids of the same
 // expert in lower waves and those in lower lanes.  Additions to the counters are whole numbers, so their order does not
@@ -364,7 +368,9 @@ __global__ __launch_bounds__(1024) void moe_plan_kernel(const int32_t *__restric
     plan_range(ids, starts, order, n_experts, n, lo, min(lo + per, n), sh);
 }
 
-// One wave a token; lane l holds the experts l, l + 64, ...  Scores, values and their sums are f64, so that the choice
+// One wave a token; lane l holds the experts l, l + 64, ...  Bound by f64 exponentials and divisions where all tokens' waves
+// are there at once (4001 tokens, 256 experts, 8 groups: 13.3 us), else by the chain of a token's maxima (one token and its
+// plan: 5.6 to 6.1 us; with shuffles of f64 values and a launch of its own for the plan 9.7).  Scores, values and their sums are f64, so that the choice
 // does not hang on how a score was rounded.  PLAN: the only workgroup, which goes on to the plan.
 template <int V, bool PLAN>
 __global__ __launch_bounds__(PLAN ? 1024 : 256) void moe_route_kernel(RouteArgs a)
