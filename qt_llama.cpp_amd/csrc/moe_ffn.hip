@@ -569,7 +569,7 @@ typedef int int4v __attribute__((ext_vector_type(4)));
 template <int AT_ONCE>
 __device__ __forceinline__ uint4 load_scales(const uint8_t *ws, uint32_t row_at, int b, int nb)
 {
-    auto at = [&](int i) { return ws + (row_at + min(i, nb - AT_ONCE)) * 2ull; };
+    auto at = [&](int i) { return ws + (row_at + min(i, nb - AT_ONCE)) * 2u; };
     auto one = [&](int i) { return *reinterpret_cast<const uint32_t *>(at(i)); };
     auto two = [&](int i) { return *reinterpret_cast<const uint2 *>(at(i)); };
     auto half = [&](int i) {
@@ -618,7 +618,7 @@ __device__ __forceinline__ void stream_pass(const ExpertArgs &a, int expert, int
         const int b = min(c * kStep + lb, nb - 1);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-            wv[k][h] = load_stream16(reinterpret_cast<const uint4 *>(w + (row_at(u, h * 8 + lr) + b) * 16ull));
+            wv[k][h] = load_stream16(reinterpret_cast<const uint4 *>(w + (row_at(u, h * 8 + lr) + b) * 16u));
     };
     auto load_scale = [&](int u, int c) {  // lane (g, i): of row i, the blocks of step c + g
         sv = load_scales<AT_ONCE>(matrix(u) + blocks * 16 + first_block * 2, row_at(u, i), (c + g) * kStep, nb);
@@ -730,7 +730,7 @@ __device__ __forceinline__ void stream_whole(const ExpertArgs &a, int expert, in
 #pragma unroll
         for (int k = 0; k < kWholeLoads; ++k)
             if (k * 64 < 16 * nb)
-                wv[k] = load_stream16(reinterpret_cast<const uint4 *>(quants) + min(at + k * 64 + lane, last));
+                wv[k] = load_stream16(reinterpret_cast<const uint4 *>(quants + min(at + k * 64 + lane, last) * 16u));
     };
     const size_t total = (size_t)(DOWN ? a.batch * a.k : a.batch) * nb;
     stream_stage<V>(a.xpack, total, nb, s_row, count, lds, scales, [&]() {
@@ -826,7 +826,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void moe_stream_kernel(ExpertArgs a
     }
     mrml_xsum::lds_barrier();
     if (j < n && !plan_ok(a, j)) moe_fault(a.faults);
-    const int e = s_tile[0], from = s_tile[1], tokens_here = s_tile[2];
+    const int e = __builtin_amdgcn_readfirstlane(s_tile[0]), from = __builtin_amdgcn_readfirstlane(s_tile[1]);
+    const int tokens_here = __builtin_amdgcn_readfirstlane(s_tile[2]);
     if (tokens_here == 0) return;
     if (tid < kStreamTokens) {
         const int o = tid < tokens_here ? a.order[from + tid] : -1;
