@@ -307,12 +307,16 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
     struct __attribute__((packed, aligned(4))) Pair {  // eight bytes from a multiple of four
         uint32_t x, y;
     };
-    // quants: of a block of row i of every group; scales: lane row g has the group g's, which saves requests
-    Pair sv;
+    // quants: of a block of row i of every group; scales: lane row g has the group g's, which saves requests.  AT_ONCE = 1:
+    // four loads of 16 bits, which stay apart until the chunk's turn.
+    uint32_t sv[AT_ONCE == 1 ? 4 : 2];
     static_assert(kGroups == 4, "a lane row a group");
     const uint8_t *ws = a.w[DOWN ? 0 : g >> 1] + blocks * 16 +
                         (first_block + (uint32_t)min(r0 + (DOWN ? g : g & 1) * 16 + i, a.rows - 1) * nb) * 2;
-    auto load_w = [&](int c) {  // kLoadsW loads
+    // kLoadsW loads whatever c is, for the wait that counts them: places behind the row's last block are clamped, and what
+    // was read there is dropped by chunk_scales (a load left out by a branch let that wait pass before the activations
+    // were there).
+    auto load_w = [&](int c) {
         const uint32_t b = min(c * kChunk + g, nb - 1);
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) {
@@ -322,13 +326,25 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
             // (an offset of less than 2^32 from an address that all lanes share)
             wv[q] = *reinterpret_cast<const uint4 *>(w + (at_row + b) * 16u);
         }
-        auto one = [&](int at) { return (uint32_t)*reinterpret_cast<const uint16_t *>(ws + min(at, nb - 1) * 2); };
-        auto two = [&](int at) {
-            if (AT_ONCE == 2) return *reinterpret_cast<const uint32_t *>(ws + min(at, nb - 2) * 2);
-            return one(at) | (at + 1 < nb ? one(at + 1) << 16 : 0u);  // the block behind the last counts nothing
-        };
-        if (AT_ONCE == 4) sv = *reinterpret_cast<const Pair *>(ws + min(c * kChunk, nb - kChunk) * 2);
-        else sv = {two(c * kChunk), two(c * kChunk + 2)};
+        if constexpr (AT_ONCE == 4) {
+            const Pair s = *reinterpret_cast<const Pair *>(ws + min(c * kChunk, nb - kChunk) * 2);
+            sv[0] = s.x;
+            sv[1] = s.y;
+        } else if constexpr (AT_ONCE == 2) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) sv[h] = *reinterpret_cast<const uint32_t *>(ws + min(c * kChunk + h * 2, nb - 2) * 2);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sv[j] = *reinterpret_cast<const uint16_t *>(ws + min(c * kChunk + j, nb - 1) * 2);
+        }
+    };
+    // Scales of blocks 2 half and 2 half + 1 of chunk c, whose loads were the last; 0 behind the row's last block, where a
+    // half has one before it.
+    auto chunk_scales = [&](int c, int half) {
+        // a row's last two come with the two before
+        if constexpr (AT_ONCE == 4) return half == 0 && c * kChunk + 2 != nb ? sv[0] : sv[1];
+        else if constexpr (AT_ONCE == 2) return sv[half];
+        else return sv[half * 2] | (c * kChunk + half * 2 + 1 < nb ? sv[half * 2 + 1] << 16 : 0u);
     };
     float4v acc[kGroups][NT];
 #pragma unroll
@@ -346,8 +362,8 @@ __device__ __forceinline__ void tile_product(const ExpertArgs &a, const Tile &ti
         uint32_t w[kGroups][4];
         half4v d[kGroups];
         uint32_t scales[2][4];
-        spread(AT_ONCE == 4 && c * kChunk + 2 == nb ? sv.y : sv.x, scales[0]);  // a row's last two come with the two before
-        spread(sv.y, scales[1]);
+        spread(chunk_scales(c, 0), scales[0]);
+        spread(chunk_scales(c, 1), scales[1]);
 #pragma unroll
         for (int q = 0; q < kGroups; ++q) {
             w[q][0] = wv[q].x;

@@ -339,6 +339,39 @@ def test_down(backend, dev, orc, synth, e, k, n, rows, cols, how):
     assert (got[(ids < 0).all(1)] == 0).all()
 
 
+def padded(backend, dev, raw, rows, cols, to):
+    """A Q4_0 matrix with blocks of zeros behind every row."""
+    b = np.frombuffer(np.ascontiguousarray(raw).tobytes(), np.uint8).reshape(rows, cols // 32, 18)
+    return backend.HipBuffer.from_gguf(dev, np.pad(b, ((0, 0), (0, (to - cols) // 32), (0, 0))).reshape(-1), backend.Q4_0,
+                                       rows, to)
+
+
+@pytest.mark.parametrize("nb,to", [(5, 6), (5, 8), (7, 8), (9, 10), (13, 16), (15, 16), (129, 130), (131, 132)])
+def test_tiles_of_odd_rows(backend, dev, synth, nb, to):
+    """Tiles of one to six token groups over rows with an odd number of blocks: to the bit what the same rows give with
+    zeros up to an even one, whose scales and weights are read by other loads."""
+    rows, cols, wide = 77, nb * 32, to * 32
+    rng = synth.rng_for(nb + to)
+    counts = [16, 32, 48, 64, 80, 96, 700]  # of the experts; so many that they are not streamed
+    e, n = len(counts), sum(counts)
+    ids = rng.permutation(np.repeat(np.arange(e), counts)).astype(np.int32)[:, None]
+    plan = planned(backend, dev, ids, e)
+    raw = [synth.q4_0_matrix(rng, e * rows, cols) for _ in range(3)]
+    x = rng.standard_normal((n, cols)).astype(np.float32)
+    weights = up(backend, dev, rng.uniform(-1, 1, (n, 1)).astype(np.float32))
+    got = []
+    for c in (cols, wide):
+        w = [padded(backend, dev, r, e * rows, cols, c) for r in raw]
+        xb = up(backend, dev, np.pad(x, ((0, 0), (0, c - cols))))
+        act, y = (up(backend, dev, np.full(n * rows, 7.0, np.float32)) for _ in range(2))
+        dev.moe_gate_up_q4_0(w[0], w[1], xb, *plan, act, e, rows, c, n, 1)
+        dev.moe_down_q4_0(w[2], xb, plan[0], weights, plan[1], plan[2], y, e, rows, c, n, 1)
+        dev.sync()
+        got.append((act.numpy(), y.numpy()))
+    for a, b in zip(*got):
+        assert np.isfinite(a).all() and np.array_equal(bits(a), bits(b))
+
+
 @pytest.mark.parametrize("n", [1, 3, 40, 150, 250])
 def test_products_of_very_uneven_activations(backend, dev, orc, synth, n):
     """Blocks from 1e-9 to 1e6 in one row, rows of zeros, weights with zero scales: exact where Q8_0 is."""
