@@ -807,7 +807,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void moe_stream_kernel(ExpertArgs a
     __shared__ int s_as[kStreamTokens], s_row[kStreamTokens], s_tile[3], s_ends[kWaves];
     __shared__ float s_weight[kStreamTokens];
     const int n = a.batch * a.k, tid = threadIdx.x;
-    const int j = (blockIdx.y * gridDim.x + blockIdx.x) * 64 * kWaves + tid;
+    // (in 64 bits: 2^24 workgroups are within the limits)
+    const uint64_t j = ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * (64 * kWaves) + tid;
     if (tid == 0) s_tile[2] = 0;
     // tiles of the experts of each thread, and before them
     static_assert(kMaxExperts == 2 * 64 * kWaves, "two experts a thread");
@@ -841,7 +842,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void moe_stream_kernel(ExpertArgs a
         at += tiles;
     }
     mrml_xsum::lds_barrier();
-    if (j < n && !plan_ok(a, j)) moe_fault(a.faults);
+    if (j < (uint32_t)n && !plan_ok(a, (int)j)) moe_fault(a.faults);
     const int e = __builtin_amdgcn_readfirstlane(s_tile[0]), from = __builtin_amdgcn_readfirstlane(s_tile[1]);
     const int tokens_here = __builtin_amdgcn_readfirstlane(s_tile[2]);
     if (tokens_here == 0) return;

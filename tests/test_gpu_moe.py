@@ -503,6 +503,33 @@ def test_refusals(backend, dev):
     dev.sync()
 
 
+def test_stream_of_more_threads_than_32_bits_count(backend, dev, orc, synth):
+    """600 assignments, 512 experts of 2^20 rows: 9.6 million workgroups of 256 threads, an output past 2 GiB."""
+    e, rows, cols, n = 512, 1 << 20, 32, 600
+    rng = synth.rng_for(31)
+    quants, base = rng.integers(0, 256, rows * 16, np.uint8), rng.uniform(0.01, 0.02, rows).astype(np.float16)
+    w, first = backend.HipBuffer.alloc(dev, e * rows * 18, np.uint8), up(backend, dev, quants)
+    lib, ctx = dev.lib, dev.ctx
+    for i in range(e):  # the same quants, scales of their own
+        assert lib.mrml_hip_memcpy_d2d_async(ctx, w.ptr + i * rows * 16, first.ptr, rows * 16) == 0
+        scales = base * np.float16(1 << i % 5)
+        assert lib.mrml_hip_memcpy_h2d(ctx, w.ptr + e * rows * 16 + i * rows * 2, scales.ctypes.data, rows * 2) == 0
+    x = rng.standard_normal((n, cols)).astype(np.float32)
+    ids = rng.integers(0, e, (n, 1)).astype(np.int32)
+    act = backend.HipBuffer.alloc(dev, n * rows)
+    dev.moe_gate_up_q4_0(w, w, up(backend, dev, x), *planned(backend, dev, ids, e), act, e, rows, cols, n, 1)
+    dev.sync()
+    some = np.r_[0:40, rows // 2:rows // 2 + 40, rows - 40:rows]
+    q = quants.reshape(rows, 16)[some]
+    q = np.concatenate([q & 15, q >> 4], 1).astype(np.float64) - 8.0
+    xq, got = mm.q8_0_values(orc, x), np.empty(rows, np.float32)
+    for a in (0, 1, 299, 511, 512, 598, 599):
+        assert lib.mrml_hip_memcpy_d2h(ctx, got.ctypes.data, act.ptr + a * rows * 4, rows * 4) == 0
+        wa = (q * base[some].astype(np.float64)[:, None] * (1 << ids[a, 0] % 5))[None]
+        want, bound = mm.gate_up(wa, wa, xq[a:a + 1], np.zeros((1, 1), np.int32), 1, mm.GEGLU)
+        assert (np.abs(got[some] - want[0]) <= bound[0]).all(), a
+
+
 # ---- the layer -----------------------------------------------------------------------------------
 
 class Layer:
