@@ -1131,11 +1131,15 @@ int row_wgs(const ExpertArgs &a)  // workgroups of a tile
 }
 
 template <bool DOWN>
+int64_t tile_grid(const ExpertArgs &a, int most)
+{
+    return (int64_t)(most + 7) / 8 * 8 * row_wgs<DOWN>(a);
+}
+
+template <bool DOWN>
 int launch_tiles(mrml_hip_ctx *ctx, const ExpertArgs &a, int most, const Tile *tiles, const uint8_t *xp, const float *xscale)
 {
-    const int64_t grid = (int64_t)(most + 7) / 8 * 8 * row_wgs<DOWN>(a);
-    REQUIRE(ctx, grid <= INT32_MAX, "moe: batch * k = %d assignments of %d rows are too many for one call", a.batch * a.k,
-            a.rows);
+    const int64_t grid = tile_grid<DOWN>(a, most);
     const int nb = a.cols / 32;
 #define TILES(AT_ONCE)                                                                                                \
     hipLaunchKernelGGL((moe_tile_kernel<DOWN, AT_ONCE>), dim3((uint32_t)grid), dim3(64 * kWaves), 0, ctx->stream, a, tiles, \
@@ -1219,6 +1223,9 @@ template <bool DOWN>
 int launch_product(mrml_hip_ctx *ctx, const ExpertArgs &a)
 {
     const int most = max_tiles(a), nb = a.cols / 32, n = a.batch * a.k, rows = DOWN ? n : a.batch;
+    // a launch has less than 2^32 threads
+    REQUIRE(ctx, tile_grid<DOWN>(a, most) * 64 * kWaves <= UINT32_MAX, "moe: batch * k = %d assignments of %d rows are too "
+            "many for one call", n, a.rows);
     const size_t list = align_up((size_t)(1 + most) * sizeof(Tile), 256), scales = align_up((size_t)rows * 4, 256);
     const size_t packed = (size_t)rows * nb * kXBlock, part = DOWN ? (size_t)n * a.rows * 4 : 0;
     uint8_t *ws = (uint8_t *)workspace(ctx, list + scales + packed + part);

@@ -503,6 +503,20 @@ def test_refusals(backend, dev):
     dev.sync()
 
 
+def test_more_tiles_than_a_launch_holds_are_refused(backend, dev):
+    """Before anything is launched or allocated: of such outputs, of terabytes, only the place is looked at."""
+    b = [backend.HipBuffer.alloc(dev, 1 << 8) for _ in range(6)]
+    p, out, before = [x.ptr for x in b], 1 << 50, dev.workspace_bytes()
+    for e in (1, 512):
+        sizes = (e, 1 << 20, 32, 1 << 19, 1)
+        for fn in (lambda: dev.moe_gate_up_q4_0(*p, out, *sizes), lambda: dev.moe_down_q4_0(*p, out, *sizes)):
+            with pytest.raises(backend.HipError, match="too many for one call") as err:
+                fn()
+            assert err.value.status == -1
+    assert dev.workspace_bytes() == before
+    dev.sync()
+
+
 def test_stream_of_more_threads_than_32_bits_count(backend, dev, orc, synth):
     """600 assignments, 512 experts of 2^20 rows: 9.6 million workgroups of 256 threads, an output past 2 GiB."""
     e, rows, cols, n = 512, 1 << 20, 32, 600
