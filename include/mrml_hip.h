@@ -625,9 +625,11 @@ int mrml_hip_attention_paged(mrml_hip_ctx *ctx, const float *d_q, int32_t q_stri
  * GGUF tensor as it stands: expert e's rows begin at row e * rows).  Nothing goes
  * through the host, so the calls can be captured and replayed (run them once
  * before, or reserve the workspace).  Ids, starts and orders are read from device
- * memory; where they do not agree with each other or lead outside the experts or
- * the batch, that is left out, and the next mrml_hip_sync fails with
- * MRML_HIP_E_INVALID.  Limits: at most 512 experts,
+ * memory.  Where they do not agree with each other or lead outside the experts or
+ * the batch, the next mrml_hip_sync fails with MRML_HIP_E_INVALID, and what is not
+ * named is left out: an assignment takes part if its expert's run of the order
+ * has it.  A run that does not ascend may leave out more of its own, starts that
+ * do not ascend from 0 to at most batch * k all.  Limits: at most 512 experts,
  * 32 experts a token, batch * k at most 2^20, cols a multiple of 32 up to 32768,
  * an expert's matrix below 4 GiB of quants.
  * Outputs share no memory with other arguments unless it says so. */
@@ -682,8 +684,8 @@ int mrml_hip_moe_route(mrml_hip_ctx *ctx, const float *d_logits, const float *d_
  * exactly, the blocks' sums in f32 in an order that depends on the batch: within
  * 1e-5 of mrml_hip_gemm_q4_0 and mrml_hip_geglu relative to the largest output.
  * d_x [batch][cols], d_act [batch * k][rows].  d_ids, d_starts and d_order as
- * mrml_hip_moe_route gives them; rows of assignments without an expert are left
- * as they were.  A row of d_x with a block whose scale passes f16 (magnitudes
+ * mrml_hip_moe_route gives them; rows of assignments without an expert, or left out,
+ * stay as they were.  A row of d_x with a block whose scale passes f16 (magnitudes
  * above 127 * 65504, infinities) gives values that are not finite. */
 enum { MRML_HIP_MOE_GEGLU = 0, MRML_HIP_MOE_SWIGLU = 1 };
 int mrml_hip_moe_gate_up_q4_0(mrml_hip_ctx *ctx, const void *d_w_gate, const void *d_w_up, const float *d_x,
@@ -699,8 +701,8 @@ int mrml_hip_moe_gate_up_q4_0_q8(mrml_hip_ctx *ctx, const void *d_w_gate, const 
 /* The experts' down product (kernels.rs:1711-1821) summed over a token's experts
  * in the order of its slots:
  *   d_y[t][r] = sum_s d_weights[t][s] * sum_c Wd[e][r][c] Q8_0(d_act[t * k + s])[c]
- * with the arithmetic of the products above.  Slots without an expert add
- * nothing; a token without any gives zeros.  d_act [batch * k][cols], d_y
+ * with the arithmetic of the products above.  Slots without an expert, or left
+ * out, add nothing; a token without any gives zeros.  d_act [batch * k][cols], d_y
  * [batch][rows].  Uses the workspace. */
 int mrml_hip_moe_down_q4_0(mrml_hip_ctx *ctx, const void *d_w_down, const float *d_act, const int32_t *d_ids,
                            const float *d_weights, const int32_t *d_starts, const int32_t *d_order, float *d_y,

@@ -714,7 +714,7 @@ int mrml_hip_moe_gate_up_q4_0(mrml_hip_ctx *ctx, const void *w_gate, const void 
 {
     CTX_GUARD(ctx);
     return gate_up(ctx, "moe_gate_up_q4_0",
-                   {{(const uint8_t *)w_gate, (const uint8_t *)w_up}, x, nullptr, ids, starts, order, nullptr, act,
+                   {{(const uint8_t *)w_gate, (const uint8_t *)w_up}, x, nullptr, ids, starts, order, nullptr, act, nullptr,
                     ctx->d_moe_faults, n_experts, rows, cols, batch, k, activation});
 }
 
@@ -726,7 +726,7 @@ int mrml_hip_moe_gate_up_q4_0_q8(mrml_hip_ctx *ctx, const void *w_gate, const vo
     CTX_GUARD(ctx);
     return gate_up(ctx, "moe_gate_up_q4_0_q8",
                    {{(const uint8_t *)w_gate, (const uint8_t *)w_up}, nullptr, (const uint8_t *)xpack, ids, starts, order,
-                    nullptr, act, ctx->d_moe_faults, n_experts, rows, cols, batch, k, activation});
+                    nullptr, act, nullptr, ctx->d_moe_faults, n_experts, rows, cols, batch, k, activation});
 }
 
 int mrml_hip_moe_down_q4_0(mrml_hip_ctx *ctx, const void *w_down, const float *act, const int32_t *ids,
@@ -734,8 +734,8 @@ int mrml_hip_moe_down_q4_0(mrml_hip_ctx *ctx, const void *w_down, const float *a
                            int32_t n_experts, int32_t rows, int32_t cols, int32_t batch, int32_t k)
 {
     CTX_GUARD(ctx);
-    const ExpertArgs a{{(const uint8_t *)w_down, nullptr}, act, nullptr, ids, starts, order, weights, y, ctx->d_moe_faults,
-                       n_experts, rows, cols, batch, k, 0};
+    const ExpertArgs a{{(const uint8_t *)w_down, nullptr}, act, nullptr, ids, starts, order, weights, y, nullptr,
+                       ctx->d_moe_faults, n_experts, rows, cols, batch, k, 0};
     if (int rc = product_ok(ctx, "moe_down_q4_0", a, true)) return rc;
     return launch_moe_down(ctx, a);
 }

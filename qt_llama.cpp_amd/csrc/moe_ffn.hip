@@ -45,12 +45,12 @@ int max_tiles(const ExpertArgs &a)
     return std::min(n, n / (kTileRows * kTileGroups) + std::min(a.n_experts, n));
 }
 
-// One workgroup that lists the tiles: tiles[0].expert of them behind tiles[0]; then one thread an assignment that checks
-// the plan (check_wgs workgroups), then WAVES waves a row.  A row of f32 of up to WAVES * CH * 256 values is read once and
-// stays in registers; CH = 0 reads it twice.
+// One workgroup that lists the tiles: tiles[0].expert of them behind tiles[0], none for starts that do not ascend; then one
+// thread an assignment that checks the plan (check_wgs workgroups), then WAVES waves a row.  A row of f32 of up to
+// WAVES * CH * 256 values is read once and stays in registers; CH = 0 reads it twice.
 template <bool PACKED, int WAVES, int CH>
 __global__ __launch_bounds__(256) void moe_pack_kernel(ExpertArgs a, int rows, int check_wgs, uint8_t *__restrict__ xp,
-                                                       float *__restrict__ xscale, Tile *__restrict__ tiles, int most)
+                                                       float *__restrict__ xscale, Tile *__restrict__ tiles)
 {
     const int nb = a.cols / 32, n = a.batch * a.k;
     if (blockIdx.x == 0) {
@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void moe_pack_kernel(ExpertArgs a, int rows, i
         }
         // tiles of each size (in groups, less one), then where they begin: the largest first
         if (tid < kTileGroups) sizes[tid] = 0;
-        __syncthreads();
+        const bool bad = __syncthreads_or(!starts_ok(a, tid, 256));
         auto each = [&](auto f) {
             for (int v = 0; v < 2; ++v) {
                 int from = first[v], left = count[v];
@@ -92,19 +92,24 @@ __global__ __launch_bounds__(256) void moe_pack_kernel(ExpertArgs a, int rows, i
                 sizes[k] = at;
                 at += c;
             }
-            tiles[0] = {min(at, most), 0, 0, 0};
+            tiles[0] = {bad ? 0 : at, 0, 0, 0};
         }
         __syncthreads();
-        // (equal sizes in any order: no tile's result depends on its place; runs that overlap could ask for more than `most`)
+        if (bad) return;
+        // (equal sizes in any order: no tile's result depends on its place; runs that do not overlap ask for no more than `most`)
         each([&](const Tile &t, int size) {
             const int at = atomicAdd(&sizes[size], 1);
-            if (at < most) tiles[1 + at] = t;
+            tiles[1 + at] = t;
         });
         return;
     }
     if ((int)blockIdx.x <= check_wgs) {
         const int j = (blockIdx.x - 1) * 256 + threadIdx.x;
-        if (j < n && !plan_ok(a, j)) moe_fault(a.faults);
+        const bool bad = __syncthreads_or(!starts_ok(a, threadIdx.x, 256));
+        if (j >= n) return;
+        const bool named = plan_names(a, j);
+        if (a.named) a.named[j] = named && !bad;
+        if (bad || !plan_ok(a, j, named)) moe_fault(a.faults);
         return;
     }
     constexpr int T = WAVES * 64;  // threads a row
@@ -486,7 +491,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_tile_kernel(ExpertArgs a, 
     if (threadIdx.x < kTileGroups * 16) {
         const int j = tile.first + (int)threadIdx.x;
         const int o = (int)threadIdx.x < tile.count ? a.order[j] : -1;
-        const bool ok = o >= 0 && o < n;
+        const bool ok = o >= 0 && o < n && a.ids[o] == tile.expert;
         s_as[threadIdx.x] = ok ? o : -1;
         s_scale[threadIdx.x] = ok ? xscale[DOWN ? o : o / a.k] * (DOWN ? a.weights[o] : 1.0f) : 0.0f;
     }
@@ -804,20 +809,23 @@ template <bool DOWN, int AT_ONCE>
 __global__ __launch_bounds__(64 * kWaves, 4) void moe_stream_kernel(ExpertArgs a, int tokens)
 {
     extern __shared__ __align__(16) uint8_t lds[];
-    __shared__ int s_as[kStreamTokens], s_row[kStreamTokens], s_tile[3], s_ends[kWaves];
+    __shared__ int s_as[kStreamTokens], s_row[kStreamTokens], s_tile[3], s_ends[kWaves], s_bad[kWaves];
     __shared__ float s_weight[kStreamTokens];
     const int n = a.batch * a.k, tid = threadIdx.x;
-    // (in 64 bits: 2^24 workgroups are within the limits)
-    const uint64_t j = ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * (64 * kWaves) + tid;
+    // The assignment and place that this thread looks at, from the last workgroup on, as the last ones mostly have no tile.
+    // (In 64 bits: 2^24 workgroups are within the limits.)
+    const uint64_t j = ((uint64_t)(gridDim.y - 1 - blockIdx.y) * gridDim.x + blockIdx.x) * (64 * kWaves) + tid;
     if (tid == 0) s_tile[2] = 0;
     // tiles of the experts of each thread, and before them
     static_assert(kMaxExperts == 2 * 64 * kWaves, "two experts a thread");
     int first[2], count[2], mine = 0;
+    bool ok = a.starts[0] == 0;
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
         const int e = 2 * tid + v;
-        const int s0 = e < a.n_experts ? min(max(a.starts[e], 0), n) : 0;
-        const int s1 = e < a.n_experts ? min(max(a.starts[e + 1], s0), n) : 0;
+        const int r0 = e < a.n_experts ? a.starts[e] : 0, r1 = e < a.n_experts ? a.starts[e + 1] : 0;
+        ok = ok && r0 <= r1 && r1 <= n;
+        const int s0 = min(max(r0, 0), n), s1 = min(max(r1, s0), n);
         first[v] = s0;
         count[v] = s1 - s0;
         mine += (count[v] + tokens - 1) / tokens;
@@ -827,14 +835,20 @@ __global__ __launch_bounds__(64 * kWaves, 4) void moe_stream_kernel(ExpertArgs a
         const int before = __shfl_up(ends, m, 64);
         if ((tid & 63) >= m) ends += before;
     }
-    if ((tid & 63) == 63) s_ends[tid >> 6] = ends;
+    const bool wave_bad = __any(!ok);
+    if ((tid & 63) == 63) {
+        s_ends[tid >> 6] = ends;
+        s_bad[tid >> 6] = wave_bad;
+    }
     mrml_xsum::lds_barrier();
+    // starts that do not ascend from 0 to at most n: everything is left out
+    const bool bad = s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3];
     int at = ends - mine;
     for (int w = 0; w < (tid >> 6); ++w) at += s_ends[w];
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
         const int tiles = (count[v] + tokens - 1) / tokens, t = (int)blockIdx.y - at;
-        if (t >= 0 && t < tiles) {
+        if (!bad && t >= 0 && t < tiles) {
             s_tile[0] = 2 * tid + v;
             s_tile[1] = first[v] + t * tokens;
             s_tile[2] = min(tokens, count[v] - t * tokens);
@@ -842,16 +856,20 @@ __global__ __launch_bounds__(64 * kWaves, 4) void moe_stream_kernel(ExpertArgs a
         at += tiles;
     }
     mrml_xsum::lds_barrier();
-    if (j < (uint32_t)n && !plan_ok(a, (int)j)) moe_fault(a.faults);
+    if (j < (uint32_t)n) {
+        const bool named = plan_names(a, (int)j);
+        if (DOWN) a.named[j] = named && !bad;
+        if (bad || !plan_ok(a, (int)j, named)) moe_fault(a.faults);
+    }
     const int e = __builtin_amdgcn_readfirstlane(s_tile[0]), from = __builtin_amdgcn_readfirstlane(s_tile[1]);
     const int tokens_here = __builtin_amdgcn_readfirstlane(s_tile[2]);
     if (tokens_here == 0) return;
     if (tid < kStreamTokens) {
         const int o = tid < tokens_here ? a.order[from + tid] : -1;
-        const bool ok = o >= 0 && o < n;
-        s_as[tid] = ok ? o : -1;
-        s_row[tid] = ok ? (DOWN ? o : o / a.k) : 0;
-        s_weight[tid] = DOWN && ok ? a.weights[o] : 0.0f;
+        const bool there = o >= 0 && o < n && a.ids[o] == e;
+        s_as[tid] = there ? o : -1;
+        s_row[tid] = there ? (DOWN ? o : o / a.k) : 0;
+        s_weight[tid] = DOWN && there ? a.weights[o] : 0.0f;
     }
     mrml_xsum::lds_barrier();
 #define PASS(V)                                                                                          \
@@ -865,8 +883,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void moe_stream_kernel(ExpertArgs a
 
 // ---- a handful of assignments ------------------------------------------------------------
 
-// Each assignment by itself, in one launch, from the activations as they come (a launch to quantise and one for the lists
-// would take as long as the products).  The block sums are the matvecs' (v_dot8 on raw weight words and split-nibble
+// Each assignment that is named (moe.h) by itself, in one launch, from the activations as they come (a launch to quantise
+// and one for the lists would take as long as the products).  The block sums are the matvecs' (v_dot8 on raw weight words and split-nibble
 // activations): lane (r, b) = (lane / 8, lane % 8) has block 8 c + b of row r of 8 in step c, a load of 128 bytes a row.
 //  A unit's scales are read as one run of memory into LDS of the wave's own (read where they are needed they
 // are as many requests as the weights).  What it comes to is a few microseconds of latencies one after the other and the
@@ -1012,6 +1030,18 @@ struct DotUnit {
     }
 };
 
+// Whether an assignment of expert e is named, of a handful: asked for behind first loads, answered at the end.
+struct Named {
+    int place = -1, lo = 0, hi = 0;
+    __device__ __forceinline__ void ask(const ExpertArgs &a, int e, int lane)
+    {
+        if (lane < a.batch * a.k) place = a.order[lane];
+        lo = a.starts[e];
+        hi = a.starts[e + 1];
+    }
+    __device__ __forceinline__ bool yes(int as, int lane) const { return __any(place == as && lane >= lo && lane < hi); }
+};
+
 // One assignment (blockIdx.y) and 8 rows of gate and of up, each by two waves that have half of the blocks; four waves more
 // quantise the token.
 constexpr int kPutWaves = 4, kGetWaves = 4;
@@ -1019,9 +1049,12 @@ __global__ __launch_bounds__(64 * (kPutWaves + kGetWaves)) void moe_gate_up_one_
 {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ float part[kGetWaves][kGateRows];
-    const int n = a.batch * a.k, tid = threadIdx.x, lane = tid & 63, nb = a.cols / 32, as = blockIdx.y;
+    __shared__ int s_named;
+    const int tid = threadIdx.x, lane = tid & 63, nb = a.cols / 32, as = blockIdx.y;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), row0 = blockIdx.x * kGateRows;
     const DotToken token(lds, nb);
+    const int e = a.ids[as];
+    const bool there = e >= 0 && e < a.n_experts;
     if (wave < kPutWaves) {
         const size_t t = as / a.k;
         if (a.xpack) {
@@ -1032,13 +1065,17 @@ __global__ __launch_bounds__(64 * (kPutWaves + kGetWaves)) void moe_gate_up_one_
             dot_quantize(a.x + t * a.cols, nb, tid, 64 * kPutWaves, token, []() {});
         }
         mrml_xsum::lds_barrier();
+        if (wave == 0) {  // while the others sum
+            Named named;
+            if (there) named.ask(a, e, lane);
+            const bool yes = named.yes(as, lane);
+            if (lane == 0) s_named = yes;
+        }
         mrml_xsum::lds_barrier();
-        const int j = (blockIdx.y * gridDim.x + blockIdx.x) * 64 * kPutWaves + tid;
-        if (j < n && !plan_ok(a, j)) moe_fault(a.faults);
+        if (blockIdx.x + blockIdx.y == 0) check_few(a, tid, 64 * kPutWaves);
         return;
     }
-    const int e = a.ids[as], w = wave - kPutWaves;
-    const bool there = e >= 0 && e < a.n_experts;
+    const int w = wave - kPutWaves;
     const int steps = there ? (nb + kStep - 1) / kStep : 0, half = (steps + 1) / 2;
     const int c0 = (w & 1) * half, c1 = min(c0 + half, steps);
     uint16_t *scales = reinterpret_cast<uint16_t *>(lds + dot_token_bytes(nb) + w * dot_scales_bytes(nb, kGateRows));
@@ -1054,7 +1091,7 @@ __global__ __launch_bounds__(64 * (kPutWaves + kGetWaves)) void moe_gate_up_one_
     if ((lane & 7) == 0) part[w][lane >> 3] = v[0];
     mrml_xsum::lds_barrier();
     const int r = tid - 64 * kPutWaves;
-    if (r < kGateRows && row0 + r < a.rows && there)
+    if (r < kGateRows && row0 + r < a.rows && s_named)
         a.out[(size_t)as * a.rows + row0 + r] = gated(part[0][r] + part[1][r], part[2][r] + part[3][r], a.activation);
 }
 
@@ -1064,16 +1101,21 @@ __global__ __launch_bounds__(64 * kDownWaves) void moe_down_one_kernel(ExpertArg
 {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ float part[kMaxTopK][kDownRows];
-    const int n = a.batch * a.k, tid = threadIdx.x, lane = tid & 63, nb = a.cols / 32, t = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 63, nb = a.cols / 32, t = blockIdx.y;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int row0 = blockIdx.x * kDownRows, steps = (nb + kStep - 1) / kStep;
     uint8_t *mine = lds + wave * (dot_token_bytes(nb) + dot_scales_bytes(nb, kDownRows));
     const DotToken token(mine, nb);
+    if (blockIdx.x + 1 == gridDim.x) {  // no rows: the first checks the plan (behind the rows of one that has some: 0.8 us)
+        if (blockIdx.y == 0) check_few(a, tid, 64 * kDownWaves);
+        return;
+    }
     uint16_t *scales = reinterpret_cast<uint16_t *>(mine + dot_token_bytes(nb));
     for (int s = wave; s < a.k; s += kDownWaves) {
         const int as = t * a.k + s, e = a.ids[as];
         const bool there = e >= 0 && e < a.n_experts;
         const float weight = there ? a.weights[as] : 0.0f;
+        Named named;
         float v[2] = {0.0f, 0.0f};
         if (there) {
             DotUnit<2> unit(a, 0, e, row0, nb);
@@ -1082,13 +1124,15 @@ __global__ __launch_bounds__(64 * kDownWaves) void moe_down_one_kernel(ExpertArg
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k)
                     if (k < steps) unit.load(k, nb, k, lane);
+                named.ask(a, e, lane);
             });
             unit.store_scales(nb, lane, scales);
             unit.sum(nb, 0, steps, lane, scales, token, v);
         }
+        const bool in = named.yes(as, lane);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-            if ((lane & 7) == 0) part[s][h * 8 + (lane >> 3)] = there ? v[h] * weight : 0.0f;
+            if ((lane & 7) == 0) part[s][h * 8 + (lane >> 3)] = in ? v[h] * weight : 0.0f;
     }
     mrml_xsum::lds_barrier();
     if (tid < kDownRows && row0 + tid < a.rows) {
@@ -1096,14 +1140,12 @@ __global__ __launch_bounds__(64 * kDownWaves) void moe_down_one_kernel(ExpertArg
         for (int s = 0; s < a.k; ++s) y += part[s][tid];
         a.out[(size_t)t * a.rows + row0 + tid] = y;
     }
-    const int j = (blockIdx.y * gridDim.x + blockIdx.x) * 64 * kDownWaves + tid;
-    if (j < n && !plan_ok(a, j)) moe_fault(a.faults);
 }
 
-// y = the sum of a token's weighted products in the order of its slots; VEC values a thread, eight slots' loads at once.
-// Bound by its bytes: 1501 tokens of eight slots, 2816 rows: 24 us for 152 MB, some of them still in a cache.
+// y = the sum of a token's weighted products (a.out) in the order of its slots, of those that were formed (a.named); VEC
+// values a thread, eight slots' loads at once.  Bound by its bytes: 1501 tokens of eight slots, 2816 rows: 24 us for 152 MB, some of them still in a cache.
 template <int VEC>
-__global__ __launch_bounds__(256) void moe_combine_kernel(ExpertArgs a, const float *__restrict__ part, float *__restrict__ y)
+__global__ __launch_bounds__(256) void moe_combine_kernel(ExpertArgs a, float *__restrict__ y)
 {
     const int t = blockIdx.x, r = (blockIdx.y * 256 + threadIdx.x) * VEC;
     if (r >= a.rows) return;
@@ -1113,10 +1155,9 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(ExpertArgs a, const fl
         vec v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int as = t * a.k + min(i0 + i, a.k - 1), e = a.ids[as];
-            const bool there = i0 + i < a.k && e >= 0 && e < a.n_experts;
+            const int as = t * a.k + min(i0 + i, a.k - 1);
             v[i] = 0.0f;
-            if (there) v[i] = *reinterpret_cast<const vec *>(part + (size_t)as * a.rows + r);
+            if (i0 + i < a.k && a.named[as]) v[i] = *reinterpret_cast<const vec *>(a.out + (size_t)as * a.rows + r);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) s += v[i];
@@ -1167,7 +1208,7 @@ int launch_down_one(mrml_hip_ctx *ctx, const ExpertArgs &a)
 {
     const int nb = a.cols / 32;
     const size_t lds = kDownWaves * (dot_token_bytes(nb) + dot_scales_bytes(nb, kDownRows));
-    hipLaunchKernelGGL(moe_down_one_kernel, dim3((a.rows + kDownRows - 1) / kDownRows, a.batch), dim3(64 * kDownWaves), lds,
+    hipLaunchKernelGGL(moe_down_one_kernel, dim3((a.rows + kDownRows - 1) / kDownRows + 1, a.batch), dim3(64 * kDownWaves), lds,
                        ctx->stream, a);
     return check_launch(ctx, "moe_down_one_kernel");
 }
@@ -1207,14 +1248,12 @@ int launch_stream(mrml_hip_ctx *ctx, const ExpertArgs &a)
     return check_launch(ctx, "moe_stream_kernel");
 }
 
-int launch_combine(mrml_hip_ctx *ctx, const ExpertArgs &a, const float *part)
+int launch_combine(mrml_hip_ctx *ctx, const ExpertArgs &a, float *y)
 {
     if (a.rows % 4 == 0)
-        hipLaunchKernelGGL(moe_combine_kernel<4>, dim3(a.batch, (a.rows / 4 + 255) / 256), dim3(256), 0, ctx->stream, a,
-                           part, a.out);
+        hipLaunchKernelGGL(moe_combine_kernel<4>, dim3(a.batch, (a.rows / 4 + 255) / 256), dim3(256), 0, ctx->stream, a, y);
     else
-        hipLaunchKernelGGL(moe_combine_kernel<1>, dim3(a.batch, (a.rows + 255) / 256), dim3(256), 0, ctx->stream, a, part,
-                           a.out);
+        hipLaunchKernelGGL(moe_combine_kernel<1>, dim3(a.batch, (a.rows + 255) / 256), dim3(256), 0, ctx->stream, a, y);
     return check_launch(ctx, "moe_combine_kernel");
 }
 
@@ -1227,8 +1266,8 @@ int launch_product(mrml_hip_ctx *ctx, const ExpertArgs &a)
     REQUIRE(ctx, tile_grid<DOWN>(a, most) * 64 * kWaves <= UINT32_MAX, "moe: batch * k = %d assignments of %d rows are too "
             "many for one call", n, a.rows);
     const size_t list = align_up((size_t)(1 + most) * sizeof(Tile), 256), scales = align_up((size_t)rows * 4, 256);
-    const size_t packed = (size_t)rows * nb * kXBlock, part = DOWN ? (size_t)n * a.rows * 4 : 0;
-    uint8_t *ws = (uint8_t *)workspace(ctx, list + scales + packed + part);
+    const size_t packed = (size_t)rows * nb * kXBlock, part = DOWN ? align_up((size_t)n * a.rows * 4, 16) : 0;
+    uint8_t *ws = (uint8_t *)workspace(ctx, list + scales + packed + part + (DOWN ? (size_t)n * 4 : 0));
     if (!ws) return MRML_HIP_E_ALLOC;
     Tile *tiles = (Tile *)ws;
     float *xscale = (float *)(ws + list);
@@ -1237,9 +1276,10 @@ int launch_product(mrml_hip_ctx *ctx, const ExpertArgs &a)
     // wave a row 16)
     const int check_wgs = (n + 255) / 256, waves = a.cols <= 1024 ? 1 : 4;
     const dim3 grid(1 + check_wgs + (rows * waves + 3) / 4), block(256);
+    ExpertArgs p = a;
+    if (DOWN) p.named = (int32_t *)(xp + packed + part);
 #define PACK(...)                                                                                             \
-    hipLaunchKernelGGL((moe_pack_kernel<__VA_ARGS__>), grid, block, 0, ctx->stream, a, rows, check_wgs, xp, xscale, tiles, \
-                       most)
+    hipLaunchKernelGGL((moe_pack_kernel<__VA_ARGS__>), grid, block, 0, ctx->stream, p, rows, check_wgs, xp, xscale, tiles)
     if (a.xpack && waves == 1) PACK(true, 1, 0);
     else if (a.xpack) PACK(true, 4, 0);
     else if (waves == 1) PACK(false, 1, 4);
@@ -1247,10 +1287,9 @@ int launch_product(mrml_hip_ctx *ctx, const ExpertArgs &a)
     else PACK(false, 4, 0);
 #undef PACK
     if (int rc = check_launch(ctx, "moe_pack_kernel")) return rc;
-    ExpertArgs p = a;
     if (DOWN) p.out = (float *)(xp + packed);
     if (int rc = launch_tiles<DOWN>(ctx, p, most, tiles, xp, xscale)) return rc;
-    return DOWN ? launch_combine(ctx, a, p.out) : MRML_HIP_OK;
+    return DOWN ? launch_combine(ctx, p, a.out) : MRML_HIP_OK;
 }
 
 }  // namespace
@@ -1274,15 +1313,16 @@ int launch_moe_down(mrml_hip_ctx *ctx, const ExpertArgs &a)
     if (one_by_one(a)) return launch_down_one(ctx, a);
     if (!streams<true>(a)) return launch_product<true>(ctx, a);
     const int n = a.batch * a.k;
-    const size_t part = align_up((size_t)n * a.rows * 4, 16);
-    uint8_t *ws = (uint8_t *)workspace(ctx, part + act_pack_bytes(n * (a.cols / 32)));
+    const size_t part = align_up((size_t)n * a.rows * 4, 16), pack = align_up(act_pack_bytes(n * (a.cols / 32)), 16);
+    uint8_t *ws = (uint8_t *)workspace(ctx, part + pack + (size_t)n * 4);
     if (!ws) return MRML_HIP_E_ALLOC;
     if (int rc = launch_quantize_q8_0(ctx, a.x, nullptr, ws + part, n * a.cols)) return rc;
     ExpertArgs p = a;
     p.xpack = ws + part;
     p.out = (float *)ws;
+    p.named = (int32_t *)(ws + part + pack);
     if (int rc = launch_stream<true>(ctx, p)) return rc;
-    return launch_combine(ctx, a, p.out);
+    return launch_combine(ctx, p, a.out);
 }
 
 }  // namespace mrml

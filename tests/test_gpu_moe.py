@@ -451,6 +451,93 @@ def test_bad_ids_and_orders_are_left_out_and_reported(backend, dev, synth, n):
     dev.sync()
 
 
+def plans_that_do_not_agree(ids, e):
+    """(what, starts, order, whether the starts ascend) for valid ids."""
+    starts, order = mm.plan(ids, e)
+    end = starts[-1]
+    run = int(np.argmax(np.diff(starts)))  # the longest
+    at = starts[run]
+    assert starts[run + 1] - at >= 3
+
+    def changed(**places):
+        o = order.copy()
+        for place, value in places.items():
+            o[int(place[1:])] = value
+        return o
+
+    yield "one twice, one nowhere", starts, changed(**{f"p{at + 1}": order[at]}), True
+    yield "nothing named", np.zeros_like(starts), np.full_like(order, -1), True
+    short = starts.copy()
+    short[np.flatnonzero(starts == end)] = end - 1
+    yield "the last one missing", short, changed(**{f"p{end - 1}": -1}), True
+    yield "a hole in a run", starts, changed(**{f"p{at + 1}": -1}), True
+    other = starts[run + 1] % end  # a place of another run
+    yield "two in each other's run", starts, changed(**{f"p{at}": order[other], f"p{other}": order[at]}), True
+    moved = starts.copy()
+    moved[run + 1] = moved[run]
+    yield "a run in the next one's", moved, order, True
+    moved = starts.copy()
+    moved[1], moved[2] = end, 0
+    yield "starts that fall", moved, order, False
+    moved = starts.copy()
+    moved[0] = 1
+    yield "not from 0 on", moved, order, False
+
+
+@pytest.mark.parametrize("n", [8, 11, 30, 130, 250])
+def test_what_a_plan_does_not_name_is_left_out(backend, dev, synth, n):
+    """Assignments that are nowhere, twice, or in another expert's run: reported, the others as they should be, and what
+    earlier calls left in the workspace (NaN here) in no output."""
+    e, k, rows, cols = 4, 2, 40, 96
+    rng = synth.rng_for(n + 1)
+    gu, dn = Experts(backend, dev, synth, 3, e, rows, cols, 2), Experts(backend, dev, synth, 4, e, cols, 64)
+    x = up(backend, dev, rng.standard_normal((n, cols)).astype(np.float32))
+    act64 = up(backend, dev, rng.standard_normal((n * k, 64)).astype(np.float32))
+    weights, nans = (up(backend, dev, a) for a in (rng.uniform(0.1, 1, (n, k)).astype(np.float32),
+                                                   np.full((n, k), np.nan, np.float32)))
+    ids = some_ids(rng, n, e, k, "even")
+
+    def both(ids, starts, order):
+        good = planned(backend, dev, some_ids(rng, n, e, k, "even"), e)
+        out, y = (up(backend, dev, np.full(c, 7.0, np.float32)) for c in (n * k * rows, n * cols))
+        dev.moe_down_q4_0(dn.dev[0], act64, good[0], nans, good[1], good[2], y, e, cols, 64, n, k)
+        dev.sync()
+        assert np.isnan(y.numpy()).all()
+        b = [up(backend, dev, np.asarray(a, np.int32).reshape(-1)) for a in (ids, starts, order)]
+        dev.moe_gate_up_q4_0(*gu.dev, x, *b, out, e, rows, cols, n, k)
+        yield out
+        dev.moe_down_q4_0(dn.dev[0], act64, b[0], weights, b[1], b[2], y, e, cols, 64, n, k)
+        yield y
+
+    def right(ids):
+        out, y = both(ids, *mm.plan(ids, e))
+        dev.sync()
+        return out.numpy().reshape(n * k, rows), y.numpy().reshape(n, cols)
+
+    whole = right(ids)
+    slots = [right(np.where(np.arange(k) == s, ids, -1).astype(np.int32))[1] for s in range(k)]
+    for what, starts, order, ascend in plans_that_do_not_agree(ids, e):
+        got = []
+        for b in both(ids, starts, order):
+            with pytest.raises(backend.HipError, match="expert ops"):
+                dev.sync()
+            got.append(b.numpy())
+        runs = [order[max(starts[j], 0):max(starts[j + 1], 0)] for j in range(e)]
+        flat = ids.reshape(-1)
+        named = np.array([i in runs[j] for i, j in enumerate(flat)])
+        sure = named & ascend & np.array([(np.diff(runs[j]) > 0).all() for j in flat])
+        # gate and up: what is named, or (starts that fall) nothing of it
+        act = bits(got[0].reshape(n * k, rows))
+        done, left = (act == bits(whole[0])).all(1), (act == bits(np.full(rows, 7.0))).all(1)
+        assert (done | left).all() and not done[~named].any() and (not ascend or done[named].all()), what
+        # down: the sum of each token's sure slots, with or without the named ones
+        y, named, sure = got[1].reshape(n, cols), named.reshape(n, k), sure.reshape(n, k)
+        for t in range(n):
+            some = [np.zeros(cols, np.float32), slots[0][t], slots[1][t], whole[1][t]]  # of no slot, 0, 1, both
+            may = [u for u in range(4) if all(sure[t, s] <= (u >> s & 1) <= named[t, s] for s in range(k))]
+            assert any(np.array_equal(y[t], some[u]) for u in may), (what, t, may)
+
+
 # ---- refusals --------------------------------------------------------------------------------
 
 def test_refusals(backend, dev):
