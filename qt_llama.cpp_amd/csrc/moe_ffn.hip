@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "any_bytes.h"
 #include "moe.h"
 #include "exact_sum.h"
 
@@ -571,7 +572,7 @@ __device__ __forceinline__ void stream_stage(const uint8_t *pack, size_t total, 
         for (int k = 0; k < kStageAhead; ++k) {
             if (tt[k] >= count) continue;
             const int b = cc[k] >> 1, h = cc[k] & 1;
-            uint32_t *dst = reinterpret_cast<uint32_t *>(lds + b * stream_block(V) + tt[k] * 8 + h * 4);
+            Any32 *dst = reinterpret_cast<Any32 *>(lds + b * stream_block(V) + tt[k] * 8 + h * 4);
             dst[0] = q[k].x;
             dst[4 * V * 2] = q[k].y;
             dst[8 * V * 2] = q[k].z;
@@ -624,12 +625,12 @@ __device__ __forceinline__ void stream_pass(const ExpertArgs &a, int expert, int
     // the row's eight: both the writes and the reads (word g of one block of row i) go to all banks.
     const int lr = lane >> 3, lb = lane & 7;
     uint4 *put[2];
-    const uint32_t *get[kStep];
+    const Any32 *get[kStep];
 #pragma unroll
     for (int h = 0; h < 2; ++h) put[h] = reinterpret_cast<uint4 *>(bounce) + (h * 8 + lr) * 8 + (lb ^ lr ^ h);
 #pragma unroll
     for (int j = 0; j < kStep; ++j)
-        get[j] = reinterpret_cast<const uint32_t *>(bounce) + (i * 8 + (j ^ (i & 7) ^ (i >> 3))) * 4 + g;
+        get[j] = reinterpret_cast<const Any32 *>(bounce) + (i * 8 + (j ^ (i & 7) ^ (i >> 3))) * 4 + g;
     uint4 wv[kAhead][2], sv;
     // unit u's rows of this lane: of the quants (two), and of the scales
     auto matrix = [&](int u) { return a.w[DOWN ? 0 : u]; };
@@ -688,7 +689,7 @@ __device__ __forceinline__ void stream_pass(const ExpertArgs &a, int expert, int
                         const uint32_t y = *get[4 * h + j] ^ 0x88888888u;
                         const uint64_t both = (uint64_t)(y & 0xF0F0F0F0u) << 32 | ((y << 4) & 0xF0F0F0F0u);
                         const int4v p = __builtin_amdgcn_mfma_i32_16x16x32_i8(
-                            *reinterpret_cast<const long *>(x + (4 * h + j) * stream_block(V)), (long)both,
+                            *reinterpret_cast<const Any64 *>(x + (4 * h + j) * stream_block(V)), (long)both,
                             int4v{0, 0, 0, 0}, 0, 0, 0);
                         const float dw = f16_bits_to_f32(d[k][2 * h + (j >> 1)] >> (j & 1) * 16 & 0xffffu);
 #pragma unroll
@@ -723,8 +724,6 @@ template <bool DOWN, int V>
 __device__ __forceinline__ void stream_whole(const ExpertArgs &a, int expert, int count, uint8_t *lds, const int *s_as,
                                              const int *s_row, const float *s_weight)
 {
-    typedef uint16_t Half __attribute__((may_alias));
-    typedef uint32_t Word __attribute__((may_alias));
     constexpr int kUnits = stream_units<DOWN>(), kRows = DOWN ? 16 * kUnits : 16;  // rows of a wave
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
     const int nb = a.cols / 32, r0 = (blockIdx.x * kWaves + wave) * kRows;
@@ -767,11 +766,11 @@ __device__ __forceinline__ void stream_whole(const ExpertArgs &a, int expert, in
         __builtin_amdgcn_wave_barrier();
         if (unit + 1 < units) load(unit + 1);
         auto block = [&](int b, const float4v (&s)[V], int j) {
-            const uint32_t y = *reinterpret_cast<const Word *>(get + (b + j) * 16) ^ 0x88888888u;
+            const uint32_t y = *reinterpret_cast<const Any32 *>(get + (b + j) * 16) ^ 0x88888888u;
             const uint64_t both = (uint64_t)(y & 0xF0F0F0F0u) << 32 | ((y << 4) & 0xF0F0F0F0u);
             const int4v p = __builtin_amdgcn_mfma_i32_16x16x32_i8(
-                *reinterpret_cast<const long *>(xa + (b + j) * stream_block(V)), (long)both, int4v{0, 0, 0, 0}, 0, 0, 0);
-            const float dw = f16_bits_to_f32(*reinterpret_cast<const Half *>(half_at + (b + j) * 2));
+                *reinterpret_cast<const Any64 *>(xa + (b + j) * stream_block(V)), (long)both, int4v{0, 0, 0, 0}, 0, 0, 0);
+            const float dw = f16_bits_to_f32(*reinterpret_cast<const Any16 *>(half_at + (b + j) * 2));
 #pragma unroll
             for (int v = 0; v < V; ++v) acc[v] = __builtin_fmaf((float)p[v], dw * s[v][j], acc[v]);
         };
@@ -935,7 +934,7 @@ __device__ __forceinline__ void dot_quantize(const float *x, int nb, int tid, in
             const uint32_t q = q8_0_block8x4(v[k], dbits, sum);
             const uint32_t w = q8_split8(q, l, sum);
             if (c < n4) {
-                reinterpret_cast<uint32_t *>(t.x)[c] = w;
+                reinterpret_cast<Any32 *>(t.x)[c] = w;
                 if (l == 0) t.dc[c >> 3] = make_float2(f16_bits_to_f32(dbits), __builtin_bit_cast(float, sum));
             }
         }
@@ -972,7 +971,7 @@ struct DotUnit {
         for (int k = 0; k < kScales; ++k)
             if (k * 64 < nb * H) sv[k] = reinterpret_cast<const uint4 *>(src)[min(k * 64 + lane, halves(nb) / 8 - 1)];
     }
-    __device__ __forceinline__ void store_scales(int nb, int lane, uint16_t *lds) const
+    __device__ __forceinline__ void store_scales(int nb, int lane, Any16 *lds) const
     {
         if (wide) {
 #pragma unroll
@@ -994,7 +993,7 @@ struct DotUnit {
     }
 
     // Steps c0 .. c1, whose first kAhead are on the way: the sums of rows lane / 8 + 8 h, in all lanes of a row.
-    __device__ __forceinline__ void sum(int nb, int c0, int c1, int lane, const uint16_t *scales, const DotToken &x,
+    __device__ __forceinline__ void sum(int nb, int c0, int c1, int lane, const Any16 *scales, const DotToken &x,
                                         float (&acc)[H])
     {
 #pragma unroll
@@ -1078,7 +1077,7 @@ __global__ __launch_bounds__(64 * (kPutWaves + kGetWaves)) void moe_gate_up_one_
     const int w = wave - kPutWaves;
     const int steps = there ? (nb + kStep - 1) / kStep : 0, half = (steps + 1) / 2;
     const int c0 = (w & 1) * half, c1 = min(c0 + half, steps);
-    uint16_t *scales = reinterpret_cast<uint16_t *>(lds + dot_token_bytes(nb) + w * dot_scales_bytes(nb, kGateRows));
+    Any16 *scales = reinterpret_cast<Any16 *>(lds + dot_token_bytes(nb) + w * dot_scales_bytes(nb, kGateRows));
     DotUnit<1> unit(a, w >> 1, there ? e : 0, row0, nb);
     if (c0 < c1) unit.load_scales(nb, lane);
 #pragma unroll
@@ -1110,7 +1109,7 @@ __global__ __launch_bounds__(64 * kDownWaves) void moe_down_one_kernel(ExpertArg
         if (blockIdx.y == 0) check_few(a, tid, 64 * kDownWaves);
         return;
     }
-    uint16_t *scales = reinterpret_cast<uint16_t *>(mine + dot_token_bytes(nb));
+    Any16 *scales = reinterpret_cast<Any16 *>(mine + dot_token_bytes(nb));
     for (int s = wave; s < a.k; s += kDownWaves) {
         const int as = t * a.k + s, e = a.ids[as];
         const bool there = e >= 0 && e < a.n_experts;

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+from pathlib import Path
+
 import numpy as np
 import pytest
 
@@ -16,6 +18,15 @@ def test_null_context_is_refused(backend):
     for fn in (lib.mrml_hip_moe_gate_up_q4_0, lib.mrml_hip_moe_gate_up_q4_0_q8):
         assert fn(None, None, None, None, None, None, None, None, 4, 8, 32, 1, 1, 0) == -1
     assert lib.mrml_hip_moe_down_q4_0(None, None, None, None, None, None, None, None, 4, 8, 32, 1, 1) == -1
+
+
+def test_lds_words_may_name_any_object():
+    """moe_ffn.hip writes quants and scales to LDS in words of one width and reads them in another: through any_bytes.h's
+    types, so that the compiler keeps their order.  Plain 16, 32 and 64 bit words are of global memory alone."""
+    s = (Path(__file__).resolve().parents[1] / "qt_llama.cpp_amd/csrc/moe_ffn.hip").read_text()
+    for line in s[s.index("// ---- few tokens an expert"):s.index("// y = the sum of a token's weighted")].splitlines():
+        if any(plain in line for plain in ("uint16_t *", "uint32_t *", "long *", "int64_t *")):
+            assert "*>(at(i))" in line or "*>(ws)" in line, line
 
 
 def test_model_route_ties_and_masks():
