@@ -62,6 +62,14 @@ def test_residual_norm(backend, dev, orc, synth, dim, batch, norm_t):
         assert np.abs(one.numpy() - xn[-1]).max() <= (dim + 8) * mm.U * 3 * np.abs(xn[-1]).max()
 
 
+@pytest.mark.parametrize("norm_t", [False, True])
+@pytest.mark.parametrize("dim,batch", [(96, 300), (1024, 257), (1056, 258), (2304, 300), (2848, 257), (4096, 290), (8192, 260),
+                                       (8224, 257), (12288, 259)])
+def test_residual_norm_of_many_rows(backend, dev, orc, synth, dim, batch, norm_t):
+    """More than 256 rows: 256 threads a row, of one to twelve chunks."""
+    test_residual_norm(backend, dev, orc, synth, dim, batch, norm_t)
+
+
 def test_residual_norm_in_place_and_without_parts(backend, dev, synth):
     """h_out = h and xn = t, no weights, no outputs but h: each the bits of the call with everything apart."""
     batch, dim = 6, 352
@@ -337,6 +345,25 @@ def test_down(backend, dev, orc, synth, e, k, n, rows, cols, how):
     off = np.abs(got - want) / bound
     assert (off <= 1).all(), off.max()
     assert (got[(ids < 0).all(1)] == 0).all()
+
+
+# Forms that the sizes above leave out: streams whose scales come four at once (rows of 36, 44 blocks; odd numbers of rows of
+# 12), down's streams of more than four tokens an expert in each of their forms, rows of 1025 to 4096 values in tiles.
+MORE_SHAPES = [(8, 2, 20, 33, 1152, "even"), (16, 2, 40, 31, 384, "holes"), (16, 2, 20, 17, 1408, "even"),
+               (10, 5, 11, 40, 96, "even"), (10, 5, 11, 31, 96, "even"), (10, 5, 11, 31, 96, "one"),
+               (10, 5, 11, 33, 192, "skew"), (10, 5, 11, 48, 256, "one"), (10, 5, 11, 150, 704, "skew"),
+               (10, 5, 11, 270, 1152, "skew"), (2, 2, 220, 24, 2816, "even"), (2, 2, 220, 24, 2848, "holes")]
+
+
+@pytest.mark.parametrize("activation", [0, 1])
+@pytest.mark.parametrize("e,k,n,rows,cols,how", MORE_SHAPES)
+def test_gate_up_in_more_forms(backend, dev, orc, synth, e, k, n, rows, cols, how, activation):
+    test_gate_up(backend, dev, orc, synth, e, k, n, rows, cols, how, activation)
+
+
+@pytest.mark.parametrize("e,k,n,rows,cols,how", MORE_SHAPES)
+def test_down_in_more_forms(backend, dev, orc, synth, e, k, n, rows, cols, how):
+    test_down(backend, dev, orc, synth, e, k, n, rows, cols, how)
 
 
 def padded(backend, dev, raw, rows, cols, to):
