@@ -680,9 +680,11 @@ int mrml_hip_moe_route(mrml_hip_ctx *ctx, const float *d_logits, const float *d_
  * activation, for every assignment a = t * k + s with expert e = d_ids[t][s]:
  *   d_act[a][r] = f(sum_c Wg[e][r][c] q[t][c]) * sum_c Wu[e][r][c] q[t][c]
  * where q is Q8_0(d_x[t]) as in every Q4_0 product here, and f is gelu_tanh
- * (MRML_HIP_MOE_GEGLU) or silu (MRML_HIP_MOE_SWIGLU).  Each block of 32 is summed
- * exactly, the blocks' sums in f32 in an order that depends on the batch: within
- * 1e-5 of mrml_hip_gemm_q4_0 and mrml_hip_geglu relative to the largest output.
+ * (MRML_HIP_MOE_GEGLU) or silu (MRML_HIP_MOE_SWIGLU).  A block of 32 is summed in
+ * whole numbers or, for many tokens an expert, in f32, where a value whose block's
+ * scale is below 2^-21 of its row's largest is off by up to 2^-32 of that one; the
+ * blocks' sums are f32 in an order that depends on the batch.  Within 1e-5 of
+ * mrml_hip_gemm_q4_0 and mrml_hip_geglu relative to the largest output.
  * d_x [batch][cols], d_act [batch * k][rows].  d_ids, d_starts and d_order as
  * mrml_hip_moe_route gives them; rows of assignments without an expert, or left out,
  * stay as they were.  A row of d_x with a block whose scale passes f16 (magnitudes

@@ -1,13 +1,16 @@
 // moe_ffn.hip -- the experts' products of a mixture-of-experts layer.
 //
 // y[row] = sum over blocks b of dw_b * (sum over the block's 32 of (q - 8) * x),
-// with x = da_b * a the Q8_0 values of an activation row.  x has 18 significant
-// bits and is split into two halves, hi + lo, exactly (after a power of two per
-// row that keeps both in range), q - 8 is a half as it stands, so a block's sum is
-// two f16 MFMAs whose f32 result only has to be multiplied by dw and added: one
-// FMA an output and block.  (The int8 product gives a whole number that takes a
-// conversion, a product of the two scales and an FMA: three vector instructions
-// for one, and those are what bounds the tiles.)
+// with x = da_b * a the Q8_0 values of an activation row.  For few tokens the inner
+// sum is one of whole numbers, exact, and takes a conversion, a product of the two
+// scales and an FMA behind it.  In the tiles, which vector instructions bound, it
+// is two f16 MFMAs whose f32 result only has to be multiplied by dw and added: one
+// FMA an output and block.  There q - 8 is a half as it stands, and x, after a power of
+// two per row that puts the largest scale at 2^7 .. 2^8, is split into two halves,
+// hi + lo.  x has at most 11 + 7 significant bits and lo is a multiple of 2^-24, so
+// the split is exact for blocks whose scale is no less than 2^-21 of the row's
+// largest; below that x is off by at most 2^-25, 2^-32 of the row's largest scale.  The
+// 32 products are exact, their sum may need 11 + 15 bits and is rounded to f32's 24.
 
 #include <algorithm>
 #include <type_traits>

@@ -419,6 +419,33 @@ def test_products_of_very_uneven_activations(backend, dev, orc, synth, n):
     assert (off <= 1).all(), off.max()
 
 
+@pytest.mark.parametrize("n", [12, 24, 300])
+def test_products_of_blocks_far_below_the_largest(backend, dev, orc, synth, n):
+    """Rows whose largest block the weights leave out (q - 8 = 0), so that only blocks with scales 2^-27 of its remain.  In
+    whole numbers nothing is lost; in tiles (n = 300) each value is off by at most 2^-32 of the row's largest scale."""
+    e, rows, cols = 4, 40, 96
+    rng = synth.rng_for(n)
+    raw = synth.q4_0_matrix(rng, e * rows, cols).reshape(-1, 3, 18)
+    raw[:, 0, 2:] = 0x88
+    w = backend.HipBuffer.from_gguf(dev, raw.reshape(-1), backend.Q4_0, e * rows, cols)
+    values = mm.q4_0_values(raw, e * rows, cols).reshape(e, rows, cols)
+    x = rng.standard_normal((n, cols)).astype(np.float32)
+    x[:, :32] *= 127 * 2.0 ** 14 / np.abs(x[:, :32]).max(1, keepdims=True)
+    x[:, 32:] *= 127 * 2.0 ** -13 / np.abs(x[:, 32:]).max(1, keepdims=True)
+    ids, weights = some_ids(rng, n, e, 1, "even"), np.ones((n, 1), np.float32)
+    want, bound = mm.down(values, mm.q8_0_values(orc, x), ids, weights, 1)
+    if n == 300:
+        bound += np.abs(values[ids[:, 0], :, 32:]).sum(2) * 2.0 ** -32 * 2.0 ** 14
+    else:
+        assert bound.max() < 1e-6  # the largest block counts nothing here: its weights are zeros
+    y = backend.HipBuffer.alloc(dev, n * rows)
+    bid, starts, order = planned(backend, dev, ids, e)
+    dev.moe_down_q4_0(w, up(backend, dev, x), bid, up(backend, dev, weights), starts, order, y, e, rows, cols, n, 1)
+    dev.sync()
+    off = np.abs(y.numpy().reshape(n, rows) - want) / bound
+    assert (off <= 1).all(), off.max()
+
+
 @pytest.mark.parametrize("n", [1, 20, 100, 200])
 def test_products_keep_rows_that_are_not_finite_apart(backend, dev, synth, n):
     """Blocks whose scale passes f16, infinities among them, give values that are not finite in their token's rows
