@@ -155,10 +155,10 @@ __global__ __launch_bounds__(256) void moe_logits_kernel(const float *__restrict
 // instruction therefore go through LDS, each wave through a part of its own (no barrier), 16-byte column c of row r at
 // c ^ r % 8 so that the rows of a read lie in different banks.  A lane reads 16 bytes: component j of a row's lanes are
 // the columns that MFMA j takes, of x and w alike.
-// 1999 tokens, 128 experts of 2816 columns: 17.6 us (one wave a token and expert: 173), against 9.2 that f32 MFMA takes
+// 1999 tokens, 128 experts of 2816 columns: 17.9 us (one wave a token and expert: 173), against 9.2 that f32 MFMA takes
 // for them and 4.7 for the bytes; the loads' way through L1 and LDS, about as long again, hides behind the MFMA only in part.
-// T = 2 reads half as much a product; T = 1 fills the chip with fewer tokens.  128 experts, T = 1 / 2: 64 tokens 6.5 / 16.7
-// us, 512 7.9 / 17.5, 1024 12.5 / 18.0, 1999 22.4 / 19.5.
+// T = 2 reads half as much a product; T = 1 fills the chip with fewer tokens.  128 experts, T = 1 / 2: 64 tokens 6.7 / 16.9
+// us, 512 6.9 / 17.5, 1024 11.7 / 17.5, 1999 20.9 / 17.9; 512 experts: 256 13.7 / 17.8, 512 26.3 / 18.1, 1999 94.4 / 65.0.
 template <int T>
 __global__ __launch_bounds__(512) void moe_logits_tile_kernel(const float *__restrict__ x, const float *__restrict__ w,
                                                               float *__restrict__ logits, int n_experts, int cols,
@@ -274,7 +274,7 @@ __device__ __forceinline__ int wave_first(uint64_t key, int id)
     return __ffsll((unsigned long long)lanes) - 1;
 }
 
-// (32008 ids of 256 experts, 32 workgroups: 8.4 us, most of it the counting, an addition in LDS for every id in every
+// (32008 ids of 256 experts, 32 workgroups: 8.4 to 8.8 us, most of it the counting, an addition in LDS for every id in every
 // workgroup; one workgroup an expert that looks through all ids twice took 73.)
 // The plan of places [lo, hi) of n ids, by a workgroup of whole waves, at most 16: counts of every expert, before lo and
 // in all, give where its run goes on; then, blockDim.x ids at a time, a place is its run's end, the ids of the same
@@ -369,9 +369,10 @@ __global__ __launch_bounds__(1024) void moe_plan_kernel(const int32_t *__restric
 }
 
 // One wave a token; lane l holds the experts l, l + 64, ...  Bound by f64 exponentials and divisions where all tokens' waves
-// are there at once (4001 tokens, 256 experts, 8 groups: 13.3 us), else by the chain of a token's maxima (one token and its
-// plan: 5.6 to 6.1 us; with shuffles of f64 values and a launch of its own for the plan 9.7).  Scores, values and their sums are f64, so that the choice
-// does not hang on how a score was rounded.  PLAN: the only workgroup, which goes on to the plan.
+// are there at once (4001 tokens, 256 experts, 8 groups: 12.6 to 13.3 us), else by the chain of a token's maxima (one token and its
+// plan: 5.6 to 6.1 us; with shuffles of f64 values and a launch of its own for the plan 9.7).  Scores, values and their
+// sums are f64, so that the choice does not hang on how a score was rounded.  PLAN: the only workgroup, which goes on to
+// the plan.
 template <int V, bool PLAN>
 __global__ __launch_bounds__(PLAN ? 1024 : 256) void moe_route_kernel(RouteArgs a)
 {
@@ -526,7 +527,9 @@ int launch_residual_norm_rows(mrml_hip_ctx *ctx, const float *t, const float *w_
 int launch_moe_logits(mrml_hip_ctx *ctx, const float *x, const float *w, float *logits, int n_experts, int cols,
                       int batch)
 {
-    // 128 experts, one wave each / tiles: 16 tokens 5.7 / 6.2 us, 40 6.0 / 6.3, 64 8.8 / 6.5
+    // One wave each / tiles: 128 experts, 16 tokens 5.3 / 6.5 us, 40 5.6 / 6.6, 64 7.0 / 6.7; 32 experts, 64 tokens 4.4 / 6.4.
+    // A wave each reads the whole matrix for each token, so the line is late for more experts: 256, 24 tokens 6.0 / 6.6, 40 10.8
+    // / 6.7; 512, 4 tokens 5.8 / 6.8, 8 8.3 / 6.9, 40 16.7 / 7.4.
     if (batch <= 40) {
         hipLaunchKernelGGL(moe_logits_kernel, dim3(batch, (n_experts + 3) / 4), dim3(256), 0, ctx->stream, x, w, logits,
                            n_experts, cols, batch);

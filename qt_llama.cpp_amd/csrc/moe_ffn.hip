@@ -277,7 +277,9 @@ constexpr int kTilePart = kHalf * kTileGroups * 2048;  // bytes of a buffer: [bl
 // beside the additions of the last one and a part of the next block's halves.  (Left to the compiler the two were one after
 // the other for the most part.)  1501 tokens, 128 experts of 704 x 2816, eight a token: gate and up 222 us, 429 TFLOP/s; down
 // about 122.  With tiles of up to 64 tokens, which take a block's halves apart more often, 13 and 4 us more; with a request
-// for each group's scales 21 and 10 more.  AT_ONCE: scales of a row read together, as its blocks' number allows.
+// for each group's scales 21 and 10 more.  AT_ONCE: scales of a row read together, as its blocks' number allows.  Whole
+// calls, gate and up of 2816, 2848, 2880, 2912 columns 240, 284, 255, 291 us: odd numbers of blocks have a request a scale,
+// and a last step of one or three blocks.
 // (pin: a value is formed in its place, which sched_barrier alone does not see to.)
 template <class T>
 __device__ __forceinline__ void pin(T &x)
@@ -514,13 +516,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_tile_kernel(ExpertArgs a, 
 // ---- few tokens an expert -------------------------------------------------------------
 
 // Bound by the stream of weights (40 tokens, eight of 128 experts of 704 x 2816 each: 91 are asked for, 203 MB for gate and
-// up in 38 to 46 us): one workgroup for a run of rows and up to 16 tokens of one expert.  The activations come quantised (a launch before; every workgroup quantising its own took 10 us of 57 for 40 tokens) and are
-// put in LDS by every workgroup; a wave has kUnits runs of 16 rows one after the other, whose
-// weights go from memory to registers kAhead steps ahead and without a barrier, 128 bytes of a row at once (a stream of 64
-// bytes a row reaches 4.9 TB/s here, of 128 bytes 6.1), and through 2 KB of LDS of the wave's own to the lanes that need
-// them.  The block sums are int8 MFMA: 16 (q - 8) is a byte after one xor, a shift and two ands, half of what a half of it
-// takes, and an int8 activation is a quarter of hi and lo.  Token t is row 4 (t & 3) + t / 4 of the MFMA, so that a lane's
-// V results are its tokens' and up to 4 V tokens fold V values a lane and not four.
+// up in 38 to 46 us): one workgroup for a run of rows and up to 16 tokens of one expert.  The activations come quantised (a
+// launch before; every workgroup quantising its own took 10 us of 57 for 40 tokens) and are put in LDS by every workgroup;
+// a wave has kUnits runs of 16 rows one after the other, whose weights go from memory to registers kAhead steps ahead and
+// without a barrier, 128 bytes of a row at once (a stream of 64 bytes a row reaches 4.9 TB/s here, of 128 bytes 6.1), and
+// through 2 KB of LDS of the wave's own to the lanes that need them.  The block sums are int8 MFMA: 16 (q - 8) is a byte
+// after one xor, a shift and two ands, half of what a half of it takes, and an int8 activation is a quarter of hi and lo.
+// Token t is row 4 (t & 3) + t / 4 of the MFMA, so that a lane's V results are its tokens' and up to 4 V tokens fold V
+// values a lane and not four.
 constexpr int kStreamBlocks = 128;  // of a row at most: they are all in LDS
 constexpr int kStreamTokens = 16;   // a workgroup at most
 constexpr int kStep = 8;            // blocks of a row at once
@@ -590,7 +593,8 @@ __device__ __forceinline__ void stream_stage(const uint8_t *pack, size_t total, 
 typedef int int4v __attribute__((ext_vector_type(4)));
 
 // Eight scales of a row from block b on, read eight, four, two or one at a time as the blocks in a row align them; behind
-// the row's last block any.
+// the row's last block any.  (One at a time takes registers that the kernel does not have: 16 of gate and up's and 12 of
+// down's lie in scratch.)
 template <int AT_ONCE>
 __device__ __forceinline__ uint4 load_scales(const uint8_t *ws, uint32_t row_at, int b, int nb)
 {
@@ -886,8 +890,9 @@ __global__ __launch_bounds__(64 * kWaves, 4) void moe_stream_kernel(ExpertArgs a
 // ---- a handful of assignments ------------------------------------------------------------
 
 // Each assignment that is named (moe.h) by itself, in one launch, from the activations as they come (a launch to quantise
-// and one for the lists would take as long as the products).  The block sums are the matvecs' (v_dot8 on raw weight words and split-nibble
-// activations): lane (r, b) = (lane / 8, lane % 8) has block 8 c + b of row r of 8 in step c, a load of 128 bytes a row.
+// and one for the lists would take as long as the products).  The block sums are the matvecs' (v_dot8 on raw weight words
+// and split-nibble activations): lane (r, b) = (lane / 8, lane % 8) has block 8 c + b of row r of 8 in step c, a load of
+// 128 bytes a row.
 //  A unit's scales are read as one run of memory into LDS of the wave's own (read where they are needed they
 // are as many requests as the weights).  What it comes to is a few microseconds of latencies one after the other and the
 // rate at which a CU takes loads, so:
@@ -895,6 +900,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void moe_stream_kernel(ExpertArgs a
 //    352 workgroups of 16 rows, two on some CUs and one on others, 9.4 us; 704 of 8 rows, three or two, see below);
 //  - waves of their own quantise: a CU takes 1.5 to 4 us to accept the loads of its weights, and a wave that issues those
 //    first cannot quantise meanwhile.
+// A trip to memory stands before the weights' loads all the same: the compiler keeps the first piece of a unit's scales
+// (DotUnit::sv) in scratch, 32 bytes a lane, and waits for it before it goes on; down's kernel waits for the activations with it.
 constexpr int kGateRows = 8, kDownRows = 16;  // of a workgroup
 
 __host__ __device__ constexpr size_t dot_scales_bytes(int nb, int rows) { return (size_t)nb * rows * 2; }  // of a wave
@@ -1145,7 +1152,8 @@ __global__ __launch_bounds__(64 * kDownWaves) void moe_down_one_kernel(ExpertArg
 }
 
 // y = the sum of a token's weighted products (a.out) in the order of its slots, of those that were formed (a.named); VEC
-// values a thread, eight slots' loads at once.  Bound by its bytes: 1501 tokens of eight slots, 2816 rows: 24 us for 152 MB, some of them still in a cache.
+// values a thread, eight slots' loads at once.  Bound by its bytes: 1501 tokens of eight slots, 2816 rows: 24 us for 152
+// MB, some of them still in a cache.
 template <int VEC>
 __global__ __launch_bounds__(256) void moe_combine_kernel(ExpertArgs a, float *__restrict__ y)
 {
@@ -1194,7 +1202,13 @@ int launch_tiles(mrml_hip_ctx *ctx, const ExpertArgs &a, int most, const Tile *t
     return check_launch(ctx, "moe_tile_kernel");
 }
 
-// A handful of assignments: each by itself, from the activations as they come.
+// A handful of assignments: each by itself, from the activations as they come.  So / streamed or in tiles, experts of 704 x
+// 2816 (down: 2816 x 704), in us: 128 experts, eight a token, 1, 2, 3 tokens: gate and up 7.0 / 17.4, 11.3 / 17.6, 15.1 / 17.9,
+// down 6.8 / 15.9, 12.2 / 15.9, 17.6 / 16.0; eight experts, two a token, 4, 8, 12 tokens: gate and up 6.6 / 17.2, 10.1 /
+// 17.9, 13.5 / 19.9, down 11.8 / 15.1, 22.6 / 16.0, 33.0 / 17.6.  The line looks at the number of assignments alone.  It is
+// late where an expert's matrices are read once for each of several tokens and take longer than the other forms' launches:
+// down of one expert, 4, 8, 16 tokens 10.2 / 15.4, 20.1 / 15.5, 37.5 / 15.7; gate and up of 14336 x 4096, eight experts,
+// two a token, 1, 4, 8 tokens 29.8 / 27.8, 107 / 60, 208 / 83.
 bool one_by_one(const ExpertArgs &a) { return a.batch * a.k <= 16 && a.cols / 32 <= kStreamBlocks; }
 
 int launch_gate_up_one(mrml_hip_ctx *ctx, const ExpertArgs &a)
@@ -1219,7 +1233,8 @@ int launch_down_one(mrml_hip_ctx *ctx, const ExpertArgs &a)
 // the weights for every 16 tokens is still less than a tile's whole row of blocks one after the other.
 // Streamed / in tiles, k experts a token of E of 704 x 2816, gate and up: E = 128, k = 8: 64 tokens 59 / 95 us, 192 99 / 118,
 // 256 119 / 122, 320 134 / 125; E = 32, k = 4 (256 tokens: 256 workgroups): 256 tokens 60 / 73, 400 82 / 70; E = 8, k = 2: 96
-// tokens 28 / 47, 400 53 / 73.  Down, E = 128, k = 8: 40 tokens 41 / 49, 96 58 / 58, 160 66 / 62; E = 8, k = 2: 32 22 / 18.
+// tokens 28 / 47, 400 49 / 71 (past 100 tokens an expert: 500 52 / 74, 800 73 / 75; E = 2, k = 1: 300 27 / 69).  Down, E =
+// 128, k = 8: 40 tokens 41 / 49, 96 58 / 58, 160 66 / 62; E = 8, k = 2: 32 22 / 18.
 template <bool DOWN>
 bool streams(const ExpertArgs &a)
 {
@@ -1233,7 +1248,10 @@ template <bool DOWN>
 int launch_stream(mrml_hip_ctx *ctx, const ExpertArgs &a)
 {
     const int n = a.batch * a.k, nb = a.cols / 32, rows = 16 * kWaves * (DOWN ? stream_units<DOWN>() : 1);
-    // the tokens of a tile: room for more costs workgroups on a CU
+    // the tokens of a tile: room for more costs workgroups on a CU, fewer of them passes over the weights.  8 / 16, 128
+    // experts, eight a token, 20, 40, 64, 80, 96 tokens, in us: gate and up 36 / 41, 49 / 52, 57 / 60, 62 / 63, 70 / 67; down
+    // 29.1 / 30.1, 39.8 / 37.9, 48.1 / 44.2, 52.2 / 48.0, 58.2 / 52.4.  Eight experts, two a token, 16, 20 tokens: gate and
+    // up 20.1 / 20.3, 20.2 / 21.2; down 17.7 / 18.0, 17.9 / 19.0.
     const int tokens = n <= 4 * a.n_experts ? 8 : kStreamTokens;
     const dim3 grid((a.rows + rows - 1) / rows, std::min(n, n / tokens + a.n_experts));
 #define MOE_STREAM(AT_ONCE, PART)                                                                            \
