@@ -505,6 +505,32 @@ def test_bad_ids_and_orders_are_left_out_and_reported(backend, dev, synth, n):
     dev.sync()
 
 
+@pytest.mark.parametrize("n,off", [(n, off) for n in (1, 3, 7, 40, 300, 2500) for off in ("none", "some", "all")])
+def test_plans_of_the_route_agree(backend, dev, synth, n, off):
+    """What the route writes for tokens with few experts or none left is a plan that the products take without a word."""
+    e, k, rows, cols = 16, 4, 24, 64
+    rng = synth.rng_for(n)
+    gu, dn = Experts(backend, dev, synth, 5, e, rows, cols, 2), Experts(backend, dev, synth, 6, e, cols, 32)
+    logits = rng.standard_normal((n, e)).astype(np.float32)
+    if off == "all":
+        logits[:] = -np.inf
+    elif off == "some":
+        logits[rng.random((n, e)) < 0.5] = -np.inf
+        logits[::3] = np.nan
+        logits[1::4, 2:] = -np.inf
+    r = Route(backend, dev, logits, None, k)
+    r.call()
+    x, act32 = (up(backend, dev, rng.standard_normal(s).astype(np.float32)) for s in ((n, cols), (n * k, 32)))
+    out, y = (up(backend, dev, np.full(c, 7.0, np.float32)) for c in (n * k * rows, n * cols))
+    dev.moe_gate_up_q4_0(*gu.dev, x, r.ids, r.starts, r.order, out, e, rows, cols, n, k)
+    dev.moe_down_q4_0(dn.dev[0], act32, r.ids, r.weights, r.starts, r.order, y, e, cols, 32, n, k)
+    ids = r.got()[0]  # (syncs)
+    out, y = out.numpy().reshape(n * k, rows), y.numpy().reshape(n, cols)
+    assert ((out == 7.0).all(1) == (ids.reshape(-1) < 0)).all()
+    assert ((y == 0).all(1) == (ids < 0).all(1)).all() and np.isfinite(y).all()
+    assert off != "all" or (ids == -1).all()
+
+
 def plans_that_do_not_agree(ids, e):
     """(what, starts, order, whether the starts ascend) for valid ids."""
     starts, order = mm.plan(ids, e)
