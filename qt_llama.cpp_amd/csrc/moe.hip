@@ -369,10 +369,10 @@ __global__ __launch_bounds__(1024) void moe_plan_kernel(const int32_t *__restric
 }
 
 // One wave a token; lane l holds the experts l, l + 64, ...  Bound by f64 exponentials and divisions where all tokens' waves
-// are there at once (4001 tokens, 256 experts, 8 groups: 12.6 to 13.3 us), else by the chain of a token's maxima (one token and its
-// plan: 5.6 to 6.1 us; with shuffles of f64 values and a launch of its own for the plan 9.7).  Scores, values and their
-// sums are f64, so that the choice does not hang on how a score was rounded.  PLAN: the only workgroup, which goes on to
-// the plan.
+// are there at once (4001 tokens, 256 experts, 8 groups: 12.6 to 13.3 us), else by the chain of a token's maxima (one token
+// and its plan: 5.6 to 6.1 us; with shuffles of f64 values and a launch of its own for the plan 9.7).  Scores, values and
+// their sums are f64, so that the choice does not hang on how a score was rounded.  PLAN: the only workgroup, which goes on
+// to the plan.
 template <int V, bool PLAN>
 __global__ __launch_bounds__(PLAN ? 1024 : 256) void moe_route_kernel(RouteArgs a)
 {

@@ -1039,7 +1039,7 @@ struct DotUnit {
     }
 };
 
-// Whether an assignment of expert e is named, of a handful: asked for behind first loads, answered at the end.
+// Whether an assignment of expert e is named, of a handful: asked for early, answered at the end.
 struct Named {
     int place = -1, lo = 0, hi = 0;
     __device__ __forceinline__ void ask(const ExpertArgs &a, int e, int lane)
@@ -1115,8 +1115,11 @@ __global__ __launch_bounds__(64 * kDownWaves) void moe_down_one_kernel(ExpertArg
     const int row0 = blockIdx.x * kDownRows, steps = (nb + kStep - 1) / kStep;
     uint8_t *mine = lds + wave * (dot_token_bytes(nb) + dot_scales_bytes(nb, kDownRows));
     const DotToken token(mine, nb);
-    if (blockIdx.x + 1 == gridDim.x) {  // no rows: the first checks the plan (behind the rows of one that has some: 0.8 us)
-        if (blockIdx.y == 0) check_few(a, tid, 64 * kDownWaves);
+    // No token: the first of these checks the plan.  (Behind the rows of a workgroup that has some it takes 0.8 us of a
+    // call.  In a column of its own it leaves the tokens' workgroups for one row run on different XCDs, which read the
+    // weights again: eight tokens, four experts, two a token 22.5 us, so 20.2.)
+    if (t == a.batch) {
+        if (blockIdx.x == 0) check_few(a, tid, 64 * kDownWaves);
         return;
     }
     Any16 *scales = reinterpret_cast<Any16 *>(mine + dot_token_bytes(nb));
@@ -1127,13 +1130,13 @@ __global__ __launch_bounds__(64 * kDownWaves) void moe_down_one_kernel(ExpertArg
         Named named;
         float v[2] = {0.0f, 0.0f};
         if (there) {
+            named.ask(a, e, lane);
             DotUnit<2> unit(a, 0, e, row0, nb);
             dot_quantize(a.x + (size_t)as * a.cols, nb, lane, 64, token, [&]() {
                 unit.load_scales(nb, lane);
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k)
                     if (k < steps) unit.load(k, nb, k, lane);
-                named.ask(a, e, lane);
             });
             unit.store_scales(nb, lane, scales);
             unit.sum(nb, 0, steps, lane, scales, token, v);
@@ -1204,10 +1207,10 @@ int launch_tiles(mrml_hip_ctx *ctx, const ExpertArgs &a, int most, const Tile *t
 
 // A handful of assignments: each by itself, from the activations as they come.  So / streamed or in tiles, experts of 704 x
 // 2816 (down: 2816 x 704), in us: 128 experts, eight a token, 1, 2, 3 tokens: gate and up 7.0 / 17.4, 11.3 / 17.6, 15.1 / 17.9,
-// down 6.8 / 15.9, 12.2 / 15.9, 17.6 / 16.0; eight experts, two a token, 4, 8, 12 tokens: gate and up 6.6 / 17.2, 10.1 /
-// 17.9, 13.5 / 19.9, down 11.8 / 15.1, 22.6 / 16.0, 33.0 / 17.6.  The line looks at the number of assignments alone.  It is
+// down 6.7 / 15.9, 12.0 / 15.9, 17.7 / 16.0; eight experts, two a token, 4, 8, 12 tokens: gate and up 6.6 / 17.2, 10.1 /
+// 17.9, 13.5 / 19.9, down 11.3 / 15.1, 21.2 / 16.0, 33.0 / 17.6.  The line looks at the number of assignments alone.  It is
 // late where an expert's matrices are read once for each of several tokens and take longer than the other forms' launches:
-// down of one expert, 4, 8, 16 tokens 10.2 / 15.4, 20.1 / 15.5, 37.5 / 15.7; gate and up of 14336 x 4096, eight experts,
+// down of one expert, 4, 8, 16 tokens 10.3 / 15.4, 19.1 / 15.5, 34.7 / 15.7; gate and up of 14336 x 4096, eight experts,
 // two a token, 1, 4, 8 tokens 29.8 / 27.8, 107 / 60, 208 / 83.
 bool one_by_one(const ExpertArgs &a) { return a.batch * a.k <= 16 && a.cols / 32 <= kStreamBlocks; }
 
@@ -1224,7 +1227,7 @@ int launch_down_one(mrml_hip_ctx *ctx, const ExpertArgs &a)
 {
     const int nb = a.cols / 32;
     const size_t lds = kDownWaves * (dot_token_bytes(nb) + dot_scales_bytes(nb, kDownRows));
-    hipLaunchKernelGGL(moe_down_one_kernel, dim3((a.rows + kDownRows - 1) / kDownRows + 1, a.batch), dim3(64 * kDownWaves), lds,
+    hipLaunchKernelGGL(moe_down_one_kernel, dim3((a.rows + kDownRows - 1) / kDownRows, a.batch + 1), dim3(64 * kDownWaves), lds,
                        ctx->stream, a);
     return check_launch(ctx, "moe_down_one_kernel");
 }
